@@ -6,5 +6,5 @@ generators and GGUF encoders (synth) and the build script (build).
 """
 from ._lib import Q8, Q4, Q4K, Q6K, MODE_EXACT, MODE_FAST, F32, F16, BF16  # noqa: F401
 from .backend import (  # noqa: F401
-    BLOCK, NAMES, CheckQuantScales, Context, DeviceBuffer, QuantBackend, QuantWeight, TrhipError, device_count,
+    BLOCK, NAMES, CheckQuantScales, Context, DeviceBuffer, KVCache, QuantBackend, QuantWeight, TrhipError, device_count,
 )

@@ -13,6 +13,7 @@ P = ctypes.c_void_p
 I64 = ctypes.c_int64
 SZ = ctypes.c_size_t
 INT = ctypes.c_int
+F32_T = ctypes.c_float
 
 # (name, restype, argtypes) for every entry point declared in include/trhip.h
 SIGNATURES = [
@@ -59,9 +60,19 @@ SIGNATURES = [
     ("trhip_quantize_q8", INT, [P, P, I64, I64, INT, P, P, P]),
     ("trhip_swiglu", INT, [P, P, I64, I64, P]),
     ("trhip_gemm_q_swiglu", INT, [P, P, P, P, I64, I64, INT]),
+    ("trhip_page_tables", INT, [P, I64, INT, P, P, P, I64, P, I64, P, P, P, I64, P]),
+    ("trhip_kv_append", INT, [P, P, I64, P, P, INT, I64, P]),
+    ("trhip_attn", INT, [P, P, P, I64, P, I64, I64, INT, I64, P, P, P, I64, I64, I64, I64, F32_T]),
+    ("trhip_attn_shared", INT, [P, P, P, I64, P, I64, I64, INT, I64, P, P, P, I64, P, I64, I64, F32_T]),
     ("trhip_rows_plan", INT, [INT, I64, I64, I64, INT, ctypes.POINTER(I64)]),
     ("trhip_set_launch_shape", INT, [P, INT, INT, INT, INT, INT]),
 ]
+
+
+class KV(ctypes.Structure):
+    """trhip_kv"""
+    _fields_ = [("dtype", INT), ("page", INT), ("heads", INT), ("dim", INT), ("pages", I64), ("k", P), ("v", P)]
+
 
 # Status codes and enums (include/trhip.h)
 OK, ERR_INVALID, ERR_OOM, ERR_HIP, ERR_LAUNCH, ERR_UNSUPPORTED, ERR_NO_DEVICE, ERR_BAD_SCALE = range(8)

@@ -208,6 +208,22 @@ def _ptr(x):
     return P(int(x))
 
 
+class KVCache:
+    """A paged key/value cache (trhip_kv): planes k and v of [pages, heads, page, dim] elements (F16 or BF16) in the
+    caller's memory, or allocated here (NewKVCache) and then freed with release()."""
+
+    def __init__(self, dtype, pages, page, heads, dim, k, v):
+        self.dtype, self.pages, self.page, self.heads, self.dim = dtype, int(pages), int(page), int(heads), int(dim)
+        self.k, self.v = k, v
+        self.c = _lib.KV(dtype, self.page, self.heads, self.dim, self.pages, _ptr(k), _ptr(v))
+        self.ref = ctypes.byref(self.c)
+
+    def release(self):
+        for b in (self.k, self.v):
+            if isinstance(b, DeviceBuffer):
+                b.free()
+
+
 class QuantBackend:
     """The quantized-matmul slice of the reference's Backend, on one MI355X context."""
 
@@ -261,6 +277,42 @@ class QuantBackend:
 
     def QuantizeQ8(self, x, M, K, blk, q, d, bs):
         _check(_lib.lib().trhip_quantize_q8(self.ctx.h, _ptr(x), M, K, blk, _ptr(q), _ptr(d), _ptr(bs)), self.ctx.h)
+
+    def NewKVCache(self, dtype, pages, page, heads, dim):
+        """A cache of `pages` pages of `page` keys in device memory of this context; what it holds is unset."""
+        nbytes = max(int(pages) * page * heads * dim * 2, 1)
+        k = self.ctx.alloc(nbytes)
+        try:
+            return KVCache(dtype, pages, page, heads, dim, k, self.ctx.alloc(nbytes))
+        except Exception:
+            k.free()
+            raise
+
+    def PageTables(self, nreq, page, old_len, add_len, free_pages, nfree, table, max_pages, q_start, kv_len, slots, nslots, used):
+        """Page tables, token starts, lengths and slots of a batch from its requests' lengths (trhip_page_tables)."""
+        _check(_lib.lib().trhip_page_tables(self.ctx.h, nreq, page, _ptr(old_len), _ptr(add_len), _ptr(free_pages), nfree,
+                                            _ptr(table), max_pages, _ptr(q_start), _ptr(kv_len), _ptr(slots), nslots, _ptr(used)),
+               self.ctx.h)
+
+    def KVAppend(self, kv, tokens, k, v, ktype, stride, slots):
+        """Key and value rows (ktype: F32, F16, BF16; stride in elements) into the cache's slots (trhip_kv_append)."""
+        _check(_lib.lib().trhip_kv_append(self.ctx.h, kv.ref, tokens, _ptr(k), _ptr(v), ktype, stride, _ptr(slots)), self.ctx.h)
+
+    def Attention(self, kv, q, q_stride, out, out_stride, tokens, heads, nreq, q_start, kv_len, table, max_pages, max_new=0,
+                  window=0, sinks=0, scale=None):
+        """Causal attention of a step's tokens over the cache, with a sliding window and first tokens that stay visible
+        where window > 0 (trhip_attn). scale: dim ** -0.5 unless given."""
+        scale = kv.dim ** -0.5 if scale is None else scale
+        _check(_lib.lib().trhip_attn(self.ctx.h, kv.ref, _ptr(q), q_stride, _ptr(out), out_stride, tokens, heads, nreq,
+                                     _ptr(q_start), _ptr(kv_len), _ptr(table), max_pages, max_new, window, sinks, scale), self.ctx.h)
+
+    def AttentionShared(self, kv, q, q_stride, out, out_stride, tokens, heads, nreq, q_start, kv_len, table, max_pages,
+                        prefix_pages, prefix_len, max_new=0, scale=None):
+        """Attention for a batch whose requests share their first prefix_len keys (trhip_attn_shared)."""
+        scale = kv.dim ** -0.5 if scale is None else scale
+        _check(_lib.lib().trhip_attn_shared(self.ctx.h, kv.ref, _ptr(q), q_stride, _ptr(out), out_stride, tokens, heads, nreq,
+                                            _ptr(q_start), _ptr(kv_len), _ptr(table), max_pages, _ptr(prefix_pages), prefix_len,
+                                            max_new, scale), self.ctx.h)
 
     def close(self):
         self.ctx.close()

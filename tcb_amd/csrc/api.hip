@@ -266,6 +266,45 @@ template <class F> void for_ranges(size_t n, int T, F &&fn) {
     HostPool::get().run(T, range);
 }
 
+constexpr int64_t kMaxInt = 0x7FFFFFFF;
+
+bool bad_page(int page) { return page < 16 || page > 4096 || (page & (page - 1)) != 0; }
+
+int check_kv(trhip_ctx *ctx, const trhip_kv *kv, const char *what) {
+    auto bad = [&](int code, const char *why) { return fail(ctx, code, std::string(what) + ": " + why); };
+    if (!kv) return bad(TRHIP_ERR_INVALID, "null cache");
+    if (kv->dtype != TRHIP_F16 && kv->dtype != TRHIP_BF16) return bad(TRHIP_ERR_UNSUPPORTED, "the cache must be f16 or bf16");
+    if (bad_page(kv->page)) return bad(TRHIP_ERR_INVALID, "the page must be a power of two, 16 to 4096");
+    if (kv->dim < 8 || kv->dim > 256 || kv->dim % 8 != 0) return bad(TRHIP_ERR_UNSUPPORTED, "the head size must be a multiple of 8 up to 256");
+    if (kv->heads < 1 || kv->heads > 65536 || kv->pages < 0 || kv->pages > kMaxInt || (int64_t)kv->pages * kv->page > kMaxInt)
+        return bad(TRHIP_ERR_INVALID, "bad head or page count");
+    if (kv->pages > 0 && (!kv->k || !kv->v)) return bad(TRHIP_ERR_INVALID, "null cache planes");
+    if (reinterpret_cast<uintptr_t>(kv->k) % 16 || reinterpret_cast<uintptr_t>(kv->v) % 16)
+        return bad(TRHIP_ERR_INVALID, "the cache planes must be 16-byte aligned");
+    return TRHIP_OK;
+}
+
+// trhip_attn and trhip_attn_shared: checks, then the launch.
+int attention(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c, const char *what) {
+    const int st = check_kv(ctx, kv, what);
+    if (st != TRHIP_OK) return st;
+    auto bad = [&](const char *why) { return fail(ctx, TRHIP_ERR_INVALID, std::string(what) + ": " + why); };
+    if (c.tokens < 0 || c.nreq < 0 || c.max_pages < 0 || c.max_new < 0 || c.window < 0 || c.sinks < 0 || c.prefix_len < 0)
+        return bad("negative size");
+    if (c.heads < 1 || c.heads % kv->heads != 0) return bad("the heads must be a multiple of the cache's");
+    if (!(c.scale > 0.0f) || c.scale > 1e30f) return bad("the scale must be positive and finite");
+    if (c.tokens == 0 || c.nreq == 0) return TRHIP_OK;
+    if (c.nreq > kMaxInt || c.max_pages > kMaxInt || c.max_pages * kv->page > kMaxInt || c.window > kMaxInt || c.sinks > kMaxInt ||
+        c.prefix_len > kMaxInt - 4096 || c.tokens > kMaxInt / c.heads)
+        return bad("size past 2^31 - 1");
+    if (!c.q || !c.out || !c.q_start || !c.kv_len || (c.max_pages > 0 && !c.table) || (c.prefix_len > 0 && !c.prefix_table))
+        return bad("null pointer");
+    if (reinterpret_cast<uintptr_t>(c.q) % 2 || reinterpret_cast<uintptr_t>(c.out) % 2) return bad("q or out is not aligned to its type");
+    if (c.q_stride < (int64_t)c.heads * kv->dim || c.out_stride < (int64_t)c.heads * kv->dim) return bad("rows overlap");
+    DevGuard g(ctx);
+    return launch_attn(ctx, kv, c);
+}
+
 // Threads for host passes over `bytes` bytes: one below 4 MiB, where starting threads costs more than it saves.
 int host_threads(size_t bytes) { return bytes < ((size_t)4 << 20) ? 1 : kHostThreads; }
 
@@ -1037,6 +1076,60 @@ int trhip_gemm_q_swiglu(trhip_ctx *ctx, const trhip_wstore *w, const float *x, f
         return launch_gemm_rows_fast(ctx, w, 0, w->N, x, gu, M, false, out);
     if ((st = trhip_gemm_q(ctx, w, 0, w->N, x, gu, M, K, 0, mode)) != TRHIP_OK) return st;
     return launch_swiglu(ctx, gu, M, I, out);
+}
+
+int trhip_page_tables(trhip_ctx *ctx, int64_t nreq, int page, const int32_t *old_len, const int32_t *add_len,
+                      const int32_t *free_pages, int64_t nfree, int32_t *table, int64_t max_pages, int32_t *q_start,
+                      int32_t *kv_len, int32_t *slots, int64_t nslots, int32_t *used) {
+    if (!ctx) return TRHIP_ERR_INVALID;
+    if (nreq < 0 || nfree < 0 || max_pages < 0 || nslots < 0) return fail(ctx, TRHIP_ERR_INVALID, "page_tables: negative size");
+    if (bad_page(page)) return fail(ctx, TRHIP_ERR_INVALID, "page_tables: the page must be a power of two, 16 to 4096");
+    if (nreq > kMaxInt || nfree > kMaxInt || max_pages > kMaxInt || nslots > kMaxInt)
+        return fail(ctx, TRHIP_ERR_INVALID, "page_tables: size past 2^31 - 1");
+    if (!q_start || !used || (nslots > 0 && !slots) || (nfree > 0 && !free_pages) ||
+        (nreq > 0 && (!old_len || !add_len || !kv_len || (max_pages > 0 && !table))))
+        return fail(ctx, TRHIP_ERR_INVALID, "page_tables: null pointer");
+    if (nreq > 0 && (kv_len == old_len || kv_len == add_len || q_start == old_len || q_start == add_len))
+        return fail(ctx, TRHIP_ERR_INVALID, "page_tables: the lengths are read while kv_len and q_start are written");
+    DevGuard g(ctx);
+    return launch_page_tables(ctx, nreq, page, old_len, add_len, free_pages, nfree, table, max_pages, q_start, kv_len, slots, nslots,
+                              used);
+}
+
+int trhip_kv_append(trhip_ctx *ctx, const trhip_kv *kv, int64_t tokens, const void *k, const void *v, int type,
+                    int64_t stride, const int32_t *slots) {
+    if (!ctx) return TRHIP_ERR_INVALID;
+    const int st = check_kv(ctx, kv, "kv_append");
+    if (st != TRHIP_OK) return st;
+    if (tokens < 0) return fail(ctx, TRHIP_ERR_INVALID, "kv_append: negative size");
+    if (type != TRHIP_F32 && type != TRHIP_F16 && type != TRHIP_BF16) return fail(ctx, TRHIP_ERR_INVALID, "kv_append: bad element type");
+    if (tokens == 0) return TRHIP_OK;
+    if (!k || !v || !slots) return fail(ctx, TRHIP_ERR_INVALID, "kv_append: null pointer");
+    if (stride < (int64_t)kv->heads * kv->dim) return fail(ctx, TRHIP_ERR_INVALID, "kv_append: rows overlap");
+    const uintptr_t e = type == TRHIP_F32 ? 4 : 2;
+    if (reinterpret_cast<uintptr_t>(k) % e || reinterpret_cast<uintptr_t>(v) % e)
+        return fail(ctx, TRHIP_ERR_INVALID, "kv_append: k or v is not aligned to its type");
+    DevGuard g(ctx);
+    return launch_kv_append(ctx, kv, tokens, k, v, type, stride, slots);
+}
+
+int trhip_attn(trhip_ctx *ctx, const trhip_kv *kv, const void *q, int64_t q_stride, void *out, int64_t out_stride,
+               int64_t tokens, int heads, int64_t nreq, const int32_t *q_start, const int32_t *kv_len,
+               const int32_t *table, int64_t max_pages, int64_t max_new, int64_t window, int64_t sinks, float scale) {
+    if (!ctx) return TRHIP_ERR_INVALID;
+    AttnCall c = {q, out, q_stride, out_stride, tokens, heads, nreq, q_start, kv_len, table, max_pages, max_new, nullptr, 0, window,
+                  sinks, scale};
+    return attention(ctx, kv, c, "attn");
+}
+
+int trhip_attn_shared(trhip_ctx *ctx, const trhip_kv *kv, const void *q, int64_t q_stride, void *out, int64_t out_stride,
+                      int64_t tokens, int heads, int64_t nreq, const int32_t *q_start, const int32_t *kv_len,
+                      const int32_t *table, int64_t max_pages, const int32_t *prefix_pages, int64_t prefix_len,
+                      int64_t max_new, float scale) {
+    if (!ctx) return TRHIP_ERR_INVALID;
+    AttnCall c = {q, out, q_stride, out_stride, tokens, heads, nreq, q_start, kv_len, table, max_pages, max_new, prefix_pages,
+                  prefix_len, 0, 0, scale};
+    return attention(ctx, kv, c, "attn_shared");
 }
 
 int trhip_quantize_q8(trhip_ctx *ctx, const float *x, int64_t M, int64_t K, int blk, int8_t *q, float *d,

@@ -1,0 +1,538 @@
+// attn_common.hpp -- what the attention kernels over a paged cache share (attn.hip, attn_rows.hip): their arguments, how
+// a batch's rows and keys are cut into work items, the masks, and the product of one block of keys with a tile of rows.
+//
+// Rows. The q_heads / kv_heads = G heads that read one kv head are rows of one matrix product: row r of a request's kv
+// head h is token r / G, head h G + r % G, so a single token brings G rows and a prompt nq G.
+//
+// One block: S^T = K Q^T and O^T += V^T P^T on 32x32x16 matrix instructions (fp32 accumulators). In the accumulator of
+// S^T lane l holds query l % 32 and the keys 8 g + 4 (l / 32) + r (g, r < 4) in register 4 g + r, so a query's maximum and
+// sum are taken over a lane's registers and one exchange between the wave's halves, and rescaling O^T is one multiplier a
+// lane. Registers 8 b .. 8 b + 7, rounded to 16 bits, are the second operand of the product over keys 16 b .. 16 b + 15 as
+// they stand: its contraction runs over the keys in that register order, and the V^T operand is read in the same order
+// (two transposing LDS reads of four keys x sixteen dimensions each). P never leaves its lane.
+//
+// LDS rows hold their 16-byte chunks in the order chunk ^ swz(row), which spreads both reads (a column of sixteen rows,
+// and four rows x 32 bytes) over all banks; the copies into LDS place a lane's chunk by choosing which chunk it fetches.
+#pragma once
+
+#include "trhip_internal.hpp"
+
+namespace trhip {
+
+struct AttnArgs {
+    const uint16_t *q;
+    uint16_t *out;
+    int64_t q_stride, out_stride;  // elements between tokens
+    const uint8_t *k, *v;          // cache planes [page][kv head][page rows][dim]
+    int64_t page_bytes, npages;
+    int head_bytes, page_log2;
+    const int *table;
+    int64_t max_pages;
+    const int *q_start, *kv_len;
+    const int *prefix_table;  // shared prefix: pages of its prefix_len keys (0: none)
+    int64_t prefix_pages;
+    int prefix_len, prefix_splits;
+    float *prefix_part;  // [split][token][head] partial results of the prefix: DP sums, maximum, sum
+    int nreq, tokens, heads, kv_heads, group, dim;
+    int window, sinks;  // window 0: none
+    float scale;        // softmax scale times log2 e
+    int q_aligned, out_aligned;  // 16- and 8-byte aligned rows
+    int target;         // work items that fill the device
+    int row_lo, row_hi; // requests of row_lo < rows <= row_hi are this launch's
+    int split_ok;       // keys may be split (partials and arrival counters are there)
+    float *part;        // [item][tile row]: DP sums, then maximum and sum of each row
+    uint32_t *arrivals;
+};
+
+namespace {
+
+typedef __bf16 a8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 a8h __attribute__((ext_vector_type(8)));
+typedef float a16f __attribute__((ext_vector_type(16)));
+typedef short a4s __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uni64(int64_t v) {
+    return (int64_t)(((uint64_t)(uint32_t)uni((int)(v >> 32)) << 32) | (uint32_t)uni((int)v));
+}
+// Wave-uniform int from memory no kernel writes while this one runs: a scalar load (not held up by, and not waiting
+// for, the copies into LDS).
+__device__ __forceinline__ int sload(const int *p, int64_t i) {
+    typedef const __attribute__((address_space(4))) int *cp;
+    return ((cp)(uintptr_t)p)[i];
+}
+
+template <int DP> __device__ __forceinline__ int swz(int row) {
+    return DP == 64 ? 2 * ((row >> 1) & 3) | ((row >> 3) & 1) : 2 * (row & 7) | ((row >> 3) & 1);
+}
+
+template <bool BF> __device__ __forceinline__ a16f mma(uint4 a, uint4 b, a16f c) {
+    if constexpr (BF)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(a8bf, a), __builtin_bit_cast(a8bf, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(a8h, a), __builtin_bit_cast(a8h, b), c, 0, 0, 0);
+}
+
+// Two floats rounded to nearest even, packed.
+template <bool BF> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (BF) {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, (b2){(__bf16)a, (__bf16)b});
+    } else {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, (h2){(_Float16)a, (_Float16)b});
+    }
+}
+template <bool BF> __device__ __forceinline__ float wide_lo(uint32_t v) {
+    if constexpr (BF) return __uint_as_float(v << 16);
+    else return (float)__builtin_bit_cast(_Float16, (uint16_t)v);
+}
+template <bool BF> __device__ __forceinline__ float wide_hi(uint32_t v) {
+    if constexpr (BF) return __uint_as_float(v & 0xFFFF0000u);
+    else return (float)__builtin_bit_cast(_Float16, (uint16_t)(v >> 16));
+}
+
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The same lane of the other half wave: max / sum of both.
+__device__ __forceinline__ float half_max(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+    typedef uint32_t v4 __attribute__((ext_vector_type(4)));
+    typedef const __attribute__((address_space(3))) v4 *lp;
+    return __builtin_bit_cast(uint4, *(lp)a);
+}
+__device__ __forceinline__ uint2 lds8(uint32_t a) {
+    typedef uint32_t v2 __attribute__((ext_vector_type(2)));
+    typedef const __attribute__((address_space(3))) v2 *lp;
+    return __builtin_bit_cast(uint2, *(lp)a);
+}
+__device__ __forceinline__ uint2 lds_tr(uint32_t a) {
+    typedef __attribute__((address_space(3))) a4s *lp;
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)a));
+}
+
+// ---- work items --------------------------------------------------------------------------------------------------------
+
+// The keys a tile of rows reads, in blocks of BK: blocks [0, ns) hold the first tokens that stay visible, blocks
+// [w0, w0 + nw) the window (all of the cache without one).
+struct Span {
+    int ns, w0, nw;
+    __device__ __forceinline__ int count() const { return ns + nw; }
+    __device__ __forceinline__ int block(int i) const { return i < ns ? i : w0 + (i - ns); }
+};
+// hi: last visible key of the tile's last token (-1: none), lo: first key of its first token's window
+template <int BK> __device__ __forceinline__ Span span_of(int hi, int lo, int sinks) {
+    Span s = {0, 0, 0};
+    if (hi < 0) return s;
+    s.w0 = lo / BK;
+    s.nw = hi / BK + 1 - s.w0;
+    const int e = sinks < hi + 1 ? sinks : hi + 1;
+    s.ns = (e + BK - 1) / BK;
+    if (s.ns >= s.w0) {  // no gap: one run from block 0
+        s.nw += s.w0;
+        s.w0 = 0;
+        s.ns = 0;
+    }
+    return s;
+}
+
+struct Item {
+    int req, tile, split, nsplit, head;
+    int q0, nq, kv;  // the request's first token row, new tokens, keys
+    int first;       // item number of the tile's split 0
+};
+
+struct ReqShape {
+    int q0, nq, kv, tiles, nb;
+};
+template <int TR, int BK> __device__ __forceinline__ ReqShape shape_of(const AttnArgs &p, int i) {
+    ReqShape s = {0, 0, 0, 0, 0};
+    if (i >= p.nreq) return s;
+    int a = p.q_start[i], b = p.q_start[i + 1], kv = p.kv_len[i];
+    a = a < 0 ? 0 : a > p.tokens ? p.tokens : a;
+    b = b < a ? a : b > p.tokens ? p.tokens : b;
+    const int64_t cap = p.max_pages << p.page_log2;
+    kv = kv < 0 ? 0 : (int64_t)kv > cap ? (int)cap : kv;
+    s.q0 = a;
+    s.nq = b - a;
+    s.kv = kv;
+    const int rows = s.nq * p.group;
+    if (rows <= p.row_lo || rows > p.row_hi) return s;
+    s.tiles = (rows + TR - 1) / TR;
+    int keys = kv;
+    if (p.window > 0) {
+        const int64_t most = (int64_t)p.window + p.sinks + TR + 2 * BK;
+        keys = (int64_t)keys > most ? (int)most : keys;
+    }
+    s.nb = (keys + BK - 1) / BK;
+    return s;
+}
+
+// Which tile of rows and which piece of its keys workgroup wg takes; every wave finds out for itself (no barrier). The
+// pieces are as long as it takes for about p.target items in all, and no shorter than p's least; a request's tiles are all
+// cut into the same number of pieces. Items are numbered head fastest, then piece, tile (the last tokens of a prompt, whose rows read most keys,
+// first), request. False: no item left.
+template <int TR, int BK, int CMIN> __device__ __forceinline__ bool find_item(const AttnArgs &p, int wg, Item &it) {
+    it = Item{0, 0, 0, 1, 0, 0, 0, 0, 0};
+    const int lane = threadIdx.x & 63, x = wg / p.kv_heads;
+    ReqShape s = shape_of<TR, BK>(p, lane);
+    int piece = 0x40000000;
+    if (p.split_ok) {
+        int64_t sum = (int64_t)s.tiles * s.nb;
+        for (int base = 64; base < p.nreq; base += 64) {
+            const ReqShape t = shape_of<TR, BK>(p, base + lane);
+            sum += (int64_t)t.tiles * t.nb;
+        }
+#pragma unroll
+        for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+        sum = uni64(sum) * p.kv_heads;
+        const int64_t c = (sum + p.target - 1) / p.target;
+        piece = c < CMIN ? CMIN : c > 0x40000000 ? 0x40000000 : (int)c;
+    }
+    int before = 0;
+    bool found = false;
+    for (int base = 0; base < p.nreq; base += 64) {
+        if (base) s = shape_of<TR, BK>(p, base + lane);
+        const int ns = s.nb <= piece ? 1 : (s.nb + piece - 1) / piece;
+        const int n = s.tiles * ns;
+        int incl = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int u = __shfl_up(incl, o);
+            if (lane >= o) incl += u;
+        }
+        if (!found) {
+            const uint64_t m = __ballot(before + incl > x);
+            if (m) {
+                const int src = __builtin_ctzll(m);
+                it.req = base + src;
+                it.q0 = __builtin_amdgcn_readlane(s.q0, src);
+                it.nq = __builtin_amdgcn_readlane(s.nq, src);
+                it.kv = __builtin_amdgcn_readlane(s.kv, src);
+                it.nsplit = __builtin_amdgcn_readlane(ns, src);
+                const int start = before + __builtin_amdgcn_readlane(incl - n, src), at = x - start;
+                const int t = at / it.nsplit, tiles = __builtin_amdgcn_readlane(s.tiles, src);
+                it.split = at - t * it.nsplit;
+                it.tile = tiles - 1 - t;
+                it.head = wg - x * p.kv_heads;
+                it.first = (x - it.split) * p.kv_heads + it.head;
+                found = true;
+            }
+        }
+        before += __builtin_amdgcn_readlane(incl, 63);
+    }
+    it.req = uni(it.req), it.tile = uni(it.tile), it.split = uni(it.split), it.nsplit = uni(it.nsplit), it.head = uni(it.head);
+    it.q0 = uni(it.q0), it.nq = uni(it.nq), it.kv = uni(it.kv), it.first = uni(it.first);
+    // starts that are not in order could name more items than there are workgroups: then nothing is done
+    return found && (int64_t)before * p.kv_heads <= (int64_t)gridDim.x;
+}
+
+// ---- a tile's rows and masks -------------------------------------------------------------------------------------------
+
+// What the rows of a tile (or of a wave's share of one) see. Per lane: the row's last visible key and the first of its
+// window; per wave: the extremes over all rows.
+struct Rows {
+    int hi, lo;                          // this lane's row
+    int hi_min, hi_max, lo_min, lo_max;  // over the rows
+    int sinks;
+};
+
+// Rows r0 .. r0 + n - 1 (n >= 1) of a request with nq new tokens and kv keys; lane's row r0 + lane % 32 (clamped to the last).
+__device__ __forceinline__ Rows rows_of(const AttnArgs &p, int r0, int n, int nq, int kv) {
+    Rows w;
+    const int row = r0 + ((int)(threadIdx.x & 31) < n ? (int)(threadIdx.x & 31) : n - 1);
+    const int t0 = r0 / p.group, t1 = (r0 + n - 1) / p.group, t = row / p.group, first = kv - nq;
+    auto low = [&](int hi) { return p.window > 0 && hi >= p.window ? hi - p.window + 1 : 0; };
+    w.hi = first + t;
+    w.lo = low(w.hi);
+    w.hi_min = uni(first + t0);
+    w.hi_max = uni(first + t1);
+    w.lo_min = uni(low(first + t0));
+    w.lo_max = uni(low(first + t1));
+    w.sinks = p.sinks;
+    return w;
+}
+
+// Sixteen rows of keys (or values) from token t, t a multiple of 16: the LDS copies of one wave. Rows past hi, rows
+// hidden from every row of the tile (between the first tokens and the window) and chunks past dim are zeros, whatever the
+// cache holds there; page numbers out of range read as zeros.
+struct Piece16 {
+    dma_rsrc k, v;
+    int ha, hb;  // hidden rows [ha, hb)
+};
+__device__ __forceinline__ Piece16 piece16(const AttnArgs &p, const int *table, int head, int t, int hi, int lo, int sinks) {
+    Piece16 s;
+    int cnt = hi + 1 - t;
+    cnt = cnt < 0 ? 0 : cnt > 16 ? 16 : cnt;
+    s.ha = sinks - t < 0 ? 0 : sinks - t;
+    s.hb = lo - t > 16 ? 16 : lo - t;
+    if (s.ha == 0 && s.hb >= 16) cnt = 0;
+    int64_t page = 0;
+    if (cnt > 0) page = sload(table, t >> p.page_log2);
+    if ((uint64_t)page >= (uint64_t)p.npages) {
+        page = 0;
+        cnt = 0;
+    }
+    const int64_t off = uni64(page * p.page_bytes + (int64_t)head * p.head_bytes + (int64_t)((t & ((1 << p.page_log2) - 1)) * p.dim * 2));
+    const uint32_t bytes = (uint32_t)uni(cnt * p.dim * 2);
+    s.k = dma_desc(p.k + off, bytes);
+    s.v = dma_desc(p.v + off, bytes);
+    return s;
+}
+// Per-lane byte offsets of instruction i's chunks (16 * DP / 512 instructions a piece).
+template <int DP> struct Lanes16 {
+    static constexpr int N = DP / 32, CH = DP / 8, RPI = 64 / CH;
+    uint32_t voff[N];
+    int row;  // row of instruction 0
+    __device__ __forceinline__ void init(int dim) {
+        const int lane = threadIdx.x & 63;
+        row = lane / CH;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int r = row + i * RPI, c = (lane % CH) ^ swz<DP>(r);
+            voff[i] = 8 * c < dim ? (uint32_t)(r * dim * 2 + c * 16) : 0x80000000u;
+        }
+    }
+    __device__ __forceinline__ void copy(dma_rsrc d, uint32_t dst, int ha, int hb) const {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            uint32_t o = voff[i];
+            if (hb > ha) o = (uint32_t)(row + i * RPI - ha) < (uint32_t)(hb - ha) ? 0x80000000u : o;
+            dma16(d, dst + i * 1024, o, 0);
+        }
+    }
+};
+
+// Q^T operands of this lane's row (element 16 s + 8 (lane / 32) + i in q[s]); zeros for rows past the tile's and past dim.
+template <int DP> __device__ __forceinline__ void load_q(const AttnArgs &p, uint4 (&q)[DP / 16], int q0, int r0, int n, int head) {
+    const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+    const int row = r0 + (r < n ? r : 0), t = row / p.group, g = row - t * p.group;
+    const uint16_t *src = p.q + (int64_t)(q0 + t) * p.q_stride + (int64_t)(head * p.group + g) * p.dim;
+#pragma unroll
+    for (int s = 0; s < DP / 16; s++) {
+        const int d = 16 * s + 8 * h;
+        q[s] = make_uint4(0, 0, 0, 0);
+        if (r < n && d < p.dim) {
+            if (p.q_aligned) {
+                q[s] = *reinterpret_cast<const uint4 *>(src + d);
+            } else {
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[i] = (uint32_t)src[d + 2 * i] | ((uint32_t)src[d + 2 * i + 1] << 16);
+                q[s] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+    }
+}
+
+// ---- one block of keys -------------------------------------------------------------------------------------------------
+
+template <int DP> struct Acc {
+    a16f o[DP / 32];
+    float m, l;  // running maximum of the scores; this lane's share of the sum (its half of the keys)
+    __device__ __forceinline__ void init() {
+#pragma unroll
+        for (int i = 0; i < DP / 32; i++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[i][r] = 0.0f;
+        m = -__builtin_inff();
+        l = 0.0f;
+    }
+};
+
+// S^T of 32 keys at LDS address k.
+template <int DP, bool BF> __device__ __forceinline__ a16f scores(uint32_t k, const uint4 (&q)[DP / 16]) {
+    const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+    const uint32_t a = k + r * (2 * DP) + ((h ^ swz<DP>(r)) << 4);
+    a16f s = {};
+#pragma unroll
+    for (int i = 0; i < DP / 16; i++) s = mma<BF>(lds16(a ^ (i << 5)), q[i], s);
+    return s;
+}
+
+// Scores of keys a row does not see become -Inf. t: the block's first key.
+__device__ __forceinline__ void mask(a16f &s, const Rows &w, int t) {
+    const int b = t + 4 * ((threadIdx.x >> 5) & 1), dh = w.hi - b, dl = w.lo - b, ds = w.sinks - b;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        const int e = 8 * (i >> 2) + (i & 3);
+        s[i] = e <= dh && (e >= dl || e < ds) ? s[i] : -__builtin_inff();
+    }
+}
+// Whether every row sees all of keys t .. t + n - 1.
+__device__ __forceinline__ bool all_see(const Rows &w, int t, int n) {
+    return t + n - 1 <= w.hi_min && (t >= w.lo_max || t + n <= w.sinks);
+}
+
+// Whether 32 rows of values at LDS address v hold an infinity or a NaN (exponent all ones).
+template <int DP, bool BF> __device__ __forceinline__ bool odd_values(uint32_t v) {
+    constexpr uint32_t E = BF ? 0x7F807F80u : 0x7C007C00u, U = BF ? 0x00800080u : 0x04000400u;
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < DP / 16; i++) {
+        const uint4 x = lds16(v + i * 1024 + (threadIdx.x & 63) * 16);
+        any |= ((x.x & E) + U) | ((x.y & E) + U) | ((x.z & E) + U) | ((x.w & E) + U);
+    }
+    return __any((any & 0x80008000u) != 0);
+}
+
+// O^T += V^T P^T key by key in fp32, a key's values reaching only the rows that see it: for blocks where some rows see
+// a key that others do not and some value is not finite (0 times it would reach every row of the tile).
+template <int DP, bool BF>
+__device__ __attribute__((noinline)) void values_one_by_one(a16f (&o)[DP / 32], const a16f &pr, uint32_t v, int hi, int lo, int sinks, int t) {
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+#pragma unroll 1
+    for (int k = 0; k < 32; k++) {
+        const int reg = 4 * (k >> 3) + (k & 3);
+        float x = pr[0];
+#pragma unroll
+        for (int i = 1; i < 16; i++) x = reg == i ? pr[i] : x;
+        x = __shfl(x, (lane & 31) + 32 * ((k >> 2) & 1));
+        const int j = t + k;
+        const bool see = j <= hi && (j >= lo || j < sinks);
+#pragma unroll
+        for (int b = 0; b < DP / 32; b++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const uint2 w = lds8(v + k * (2 * DP) + (((4 * b + g) ^ swz<DP>(k)) << 4) + 8 * h);
+                const float e[4] = {wide_lo<BF>(w.x), wide_hi<BF>(w.x), wide_lo<BF>(w.y), wide_hi<BF>(w.y)};
+#pragma unroll
+                for (int r = 0; r < 4; r++) o[b][4 * g + r] = see ? fmaf(x, e[r], o[b][4 * g + r]) : o[b][4 * g + r];
+            }
+    }
+}
+
+// O^T += V^T P^T of 32 keys at LDS address v, P in 16 bits; TWO: in two terms (what the first rounding drops is the
+// second), so that P's rounding does not show beside the output's.
+template <int DP, bool BF, bool TWO> __device__ __forceinline__ void values(a16f (&o)[DP / 32], const a16f &pr, uint32_t v) {
+    const int lane = threadIdx.x & 63, i = lane & 15, h = lane >> 5;
+    const int row = 4 * h + (i >> 2), c = 2 * ((lane >> 4) & 1) + ((i >> 1) & 1);
+    const uint32_t a = v + row * (2 * DP) + ((c ^ swz<DP>(row)) << 4) + 8 * (i & 1);
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float x = pr[8 * b + 2 * j], y = pr[8 * b + 2 * j + 1];
+            hi[j] = pack2<BF>(x, y);
+            if (TWO) lo[j] = pack2<BF>(x - wide_lo<BF>(hi[j]), y - wide_hi<BF>(hi[j]));
+        }
+        const uint4 ph = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+#pragma unroll
+        for (int d = 0; d < DP / 32; d++) {
+            const uint32_t at = (a ^ (d << 6)) + b * 32 * DP;
+            const uint2 x = lds_tr(at), y = lds_tr((at ^ 16) + 16 * DP);
+            const uint4 vt = make_uint4(x.x, x.y, y.x, y.y);
+            o[d] = mma<BF>(vt, ph, o[d]);
+            if (TWO) o[d] = mma<BF>(vt, make_uint4(lo[0], lo[1], lo[2], lo[3]), o[d]);
+        }
+    }
+}
+
+// The running softmax's step over NB blocks of 32 scores: the new maximum, O^T and the sum rescaled to it, scores
+// replaced by exp2(scale (s - m)). A row that has seen nothing keeps m = -Inf and adds nothing.
+template <int DP, int NB> __device__ __forceinline__ void softmax_step(Acc<DP> &A, a16f (&s)[NB], float scale) {
+    float x = s[0][0];
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) x = fmaxf(x, s[b][i]);
+    const float m = fmaxf(A.m, half_max(x));
+    if (__any(m > A.m)) {
+        const float a = m > A.m ? exp2_hw((A.m - m) * scale) : 1.0f;  // A.m = -Inf: 0
+        A.l *= a;
+#pragma unroll
+        for (int d = 0; d < DP / 32; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) A.o[d][i] *= a;
+        A.m = m;
+    }
+    const float mu = m == -__builtin_inff() ? 0.0f : m, ms = mu * scale;
+    // One fused step an element. The rounding of ms is the same factor in every weight and cancels, as long as it is
+    // small: where scores are past 2^20 the difference is taken first.
+    const bool far = __any(fabsf(ms) > 1048576.0f);
+    float l = 0.0f;
+    if (far) {
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[b][i] = (s[b][i] - mu) * scale;
+    } else {
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[b][i] = fmaf(s[b][i], scale, -ms);
+    }
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            s[b][i] = exp2_hw(s[b][i]);
+            l += s[b][i];
+        }
+    A.l += l;
+}
+
+// ---- results -----------------------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ void agent_store(float *p, float a, float b) {
+    const uint64_t v = (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32);
+    __hip_atomic_store(reinterpret_cast<uint64_t *>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 agent_load(const float *p) {
+    const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+
+// Four finished outputs of row `row` (of the request's kv head) from dimension d; l: the row's sum. A row whose mask
+// leaves nothing (hi < 0) is 0; a sum of 0 over visible keys is the formula's 0 / 0.
+template <bool BF> __device__ __forceinline__ void put4(const AttnArgs &p, int q0, int row, int head, int d, const float (&o)[4], float l, bool sees) {
+    if (d >= p.dim) return;
+    const int t = row / p.group, g = row - t * p.group;
+    uint16_t *dst = p.out + (int64_t)(q0 + t) * p.out_stride + (int64_t)(head * p.group + g) * p.dim + d;
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) y[i] = sees ? o[i] / l : 0.0f;
+    const uint2 w = make_uint2(pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3]));
+    if (p.out_aligned) {
+        *reinterpret_cast<uint2 *>(dst) = w;
+    } else {
+        dst[0] = (uint16_t)w.x;
+        dst[1] = (uint16_t)(w.x >> 16);
+        dst[2] = (uint16_t)w.y;
+        dst[3] = (uint16_t)(w.y >> 16);
+    }
+}
+
+// A sum over partial results of one row: the largest maximum so far, sums relative to it.
+struct Join {
+    float m, l, o[4], scale;
+    __device__ __forceinline__ void init(float s) {
+        scale = s;
+        m = -__builtin_inff();
+        l = o[0] = o[1] = o[2] = o[3] = 0.0f;
+    }
+    __device__ __forceinline__ void add(float pm, float pl, float a, float b, float c, float d) {
+        const float n = fmaxf(m, pm);
+        const float x = m == n ? 1.0f : exp2_hw((m - n) * scale), y = pm == n ? 1.0f : exp2_hw((pm - n) * scale);
+        l = l * x + pl * y;
+        o[0] = o[0] * x + a * y;
+        o[1] = o[1] * x + b * y;
+        o[2] = o[2] * x + c * y;
+        o[3] = o[3] * x + d * y;
+        m = n;
+    }
+};
+
+}  // namespace
+}  // namespace trhip

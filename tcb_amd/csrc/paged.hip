@@ -1,0 +1,207 @@
+// paged.hip -- the bookkeeping of a paged key/value cache: the page tables of a batch, built from its requests' lengths,
+// and the append of new key and value rows.
+#include "trhip_internal.hpp"
+
+namespace trhip {
+namespace {
+
+// Page tables. Request i holds old_i keys and brings add_i: have_i = ceil(old_i / page) pages it has, need_i =
+// ceil((old_i + add_i) / page); the grow_i = need_i - have_i fresh ones are free[base_i ...], base the running sum of
+// grow. One launch: every workgroup makes the running sums for itself (12 bytes a request, cached) and then writes its
+// 4 x THREADS slots; the tables' fresh entries, lengths and starts are dealt over the workgroups by request. A slot's page is
+// read from the table only where it was there before, else from the free list, so no workgroup waits for another's entries.
+// What bounds it is latency: the lengths, the scan, one dependent read (4.x us for sixteen requests).
+__device__ __forceinline__ int clamp31(int64_t v) { return v > 0x7FFFFFFF ? 0x7FFFFFFF : (int)v; }
+
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void page_tables_kernel(int nreq, int page_log2, const int *__restrict__ old_len,
+                                                              const int *__restrict__ add_len, const int *__restrict__ free_list,
+                                                              int64_t nfree, int *table, int64_t max_pages,
+                                                              int *__restrict__ q_start, int *__restrict__ kv_len,
+                                                              int *__restrict__ slots, int64_t nslots, int *__restrict__ used) {
+    constexpr int WAVES = THREADS / 64, PER = 4;
+    __shared__ int s_start[THREADS + 1], s_old[THREADS], s_base[THREADS];
+    __shared__ int64_t s_wave[2][WAVES];
+    __shared__ int s_used[WAVES];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int64_t page = (int64_t)1 << page_log2, first = (int64_t)blockIdx.x * (PER * THREADS);
+    int64_t tok0 = 0, base0 = 0;  // sums over the chunks of requests before this one
+    int most = 0;
+    int out[PER];
+#pragma unroll
+    for (int u = 0; u < PER; u++) out[u] = -1;
+    for (int c = 0; c < nreq; c += THREADS) {
+        const int i = c + tid;
+        int64_t old = 0, add = 0;
+        if (i < nreq) {
+            old = old_len[i];
+            add = add_len[i];
+            old = old < 0 ? 0 : old;
+            add = add < 0 ? 0 : add;
+        }
+        const int64_t have = (old + page - 1) >> page_log2, need = (old + add + page - 1) >> page_log2;
+        const int64_t grow = need <= max_pages ? need - have : 0;
+        int64_t st = add, sg = grow;  // inclusive sums over the wave
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int64_t a = __shfl_up(st, o), b = __shfl_up(sg, o);
+            if (lane >= o) {
+                st += a;
+                sg += b;
+            }
+        }
+        __syncthreads();  // the chunk before has been used
+        if (lane == 63) {
+            s_wave[0][w] = st;
+            s_wave[1][w] = sg;
+        }
+        __syncthreads();
+        int64_t bt = tok0, bg = base0, tt = 0, tg = 0;
+#pragma unroll
+        for (int k = 0; k < WAVES; k++) {
+            if (k < w) {
+                bt += s_wave[0][k];
+                bg += s_wave[1][k];
+            }
+            tt += s_wave[0][k];
+            tg += s_wave[1][k];
+        }
+        const int64_t start = bt + st - add, base = bg + sg - grow;
+        const bool fits = need <= max_pages && (grow == 0 || base + grow <= nfree);
+        if (i < nreq && fits && base + grow > most) most = (int)(base + grow);
+        s_start[tid] = clamp31(start);
+        s_old[tid] = fits ? (int)old : -1;
+        s_base[tid] = clamp31(base);
+        if (tid == THREADS - 1) s_start[THREADS] = clamp31(start + add);
+        // this workgroup's share of the requests' own outputs
+        if (i < nreq && (int)((unsigned)(c / THREADS) % gridDim.x) == (int)blockIdx.x) {
+            kv_len[i] = clamp31(old + (fits ? add : 0));
+            q_start[i + 1] = clamp31(start + add);
+            if (i == 0) q_start[0] = 0;
+        }
+        __syncthreads();
+        const int cnt = nreq - c < THREADS ? nreq - c : THREADS;
+        for (int k = (int)blockIdx.x * WAVES + w; k < cnt; k += (int)gridDim.x * WAVES) {  // a wave writes a request's fresh entries
+            const int o = s_old[k];
+            if (o < 0) continue;
+            const int64_t h = ((int64_t)o + page - 1) >> page_log2;
+            const int64_t e = ((int64_t)o + (s_start[k + 1] - s_start[k]) + page - 1) >> page_log2;
+            for (int64_t j = h + lane; j < e; j += 64) table[(c + k) * max_pages + j] = free_list[s_base[k] + (j - h)];
+        }
+        if (first < tok0 + tt && first + PER * THREADS > tok0) {
+#pragma unroll
+            for (int u = 0; u < PER; u++) {
+                const int64_t t = first + u * THREADS + tid;
+                if (t < tok0 || t >= tok0 + tt || t >= nslots) continue;
+                int lo = 0, hi = cnt;  // the last request that starts at or before t
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (s_start[mid] <= (int)t) lo = mid;
+                    else hi = mid;
+                }
+                const int o = s_old[lo];
+                if (o < 0) continue;
+                const int64_t pos = (int64_t)o + (t - s_start[lo]), pi = pos >> page_log2, h = ((int64_t)o + page - 1) >> page_log2;
+                int64_t pg = 0;
+                if (pi < h) pg = table[(c + lo) * max_pages + pi];
+                else pg = free_list[s_base[lo] + (pi - h)];
+                out[u] = (int)((pg << page_log2) + (pos & (page - 1)));
+            }
+        }
+        tok0 += tt;
+        base0 += tg;
+    }
+#pragma unroll
+    for (int u = 0; u < PER; u++) {
+        const int64_t t = first + u * THREADS + tid;
+        if (t < nslots) slots[t] = out[u];
+    }
+    if (blockIdx.x == 0) {
+#pragma unroll
+        for (int o = 32; o; o >>= 1) {
+            const int v = __shfl_xor(most, o);
+            most = v > most ? v : most;
+        }
+        if (lane == 0) s_used[w] = most;
+        __syncthreads();
+        if (tid == 0) {
+            for (int k = 1; k < WAVES; k++) most = s_used[k] > most ? s_used[k] : most;
+            *used = most;
+            if (nreq == 0) q_start[0] = 0;
+        }
+    }
+}
+
+// Cache append: eight elements a thread, rounded to the cache's type (nearest even) where the source's is another.
+__device__ __forceinline__ uint4 take8(const void *src, int64_t at, int io, int dtype, bool wide) {
+    uint32_t h[8];
+    if (io == TRHIP_F32) {
+        const float *s = static_cast<const float *>(src) + at;
+        float f[8];
+        if (wide) {
+            *reinterpret_cast<float4 *>(f) = *reinterpret_cast<const float4 *>(s);
+            *reinterpret_cast<float4 *>(f + 4) = *reinterpret_cast<const float4 *>(s + 4);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) f[i] = s[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) h[i] = f32_to_h16(f[i], dtype);
+    } else {
+        const uint16_t *s = static_cast<const uint16_t *>(src) + at;
+        if (io == dtype && wide) return *reinterpret_cast<const uint4 *>(s);
+#pragma unroll
+        for (int i = 0; i < 8; i++) h[i] = io == dtype ? (uint32_t)s[i] : f32_to_h16(h16_to_f32(s[i], io), dtype);
+    }
+    return make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
+}
+__global__ __launch_bounds__(256) void kv_append_kernel(uint16_t *__restrict__ kc, uint16_t *__restrict__ vc, int dtype, int page_log2,
+                                                        int64_t places, int heads, int dim, int64_t tokens, const void *__restrict__ k,
+                                                        const void *__restrict__ v, int io, int64_t stride,
+                                                        const int *__restrict__ slots, int wide) {
+    const int row = heads * dim / 8, per = 2 * row;  // eights of a token: k's, then v's
+    const int64_t total = tokens * per, step = (int64_t)gridDim.x * blockDim.x;
+    for (int64_t x = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; x < total; x += step) {
+        const int64_t t = x / per;
+        const int c = (int)(x - t * per), e = c < row ? c : c - row;
+        const int64_t slot = slots[t];
+        if ((uint64_t)slot >= (uint64_t)places) continue;
+        const int head = 8 * e / dim, d = 8 * e - head * dim;
+        const int64_t pg = slot >> page_log2, in = slot & ((1 << page_log2) - 1);
+        const uint4 y = take8(c < row ? k : v, t * stride + 8 * e, io, dtype, wide);
+        *reinterpret_cast<uint4 *>((c < row ? kc : vc) + (((pg * heads + head) << page_log2) + in) * dim + d) = y;
+    }
+}
+
+}  // namespace
+
+int launch_page_tables(trhip_ctx *ctx, int64_t nreq, int page, const int *old_len, const int *add_len, const int *free_list,
+                       int64_t nfree, int *table, int64_t max_pages, int *q_start, int *kv_len, int *slots, int64_t nslots,
+                       int *used) {
+    const int lg = __builtin_ctz((unsigned)page);
+    const int64_t threads = nreq <= 256 ? 256 : 1024, grid = nslots > 0 ? (nslots + 4 * threads - 1) / (4 * threads) : 1;
+    if (grid >= ((int64_t)1 << 31)) return fail(ctx, TRHIP_ERR_INVALID, "page_tables: too many slots");
+    if (threads == 256)
+        hipLaunchKernelGGL(page_tables_kernel<256>, dim3((unsigned)grid), dim3(256), 0, ctx->stream, (int)nreq, lg, old_len, add_len,
+                           free_list, nfree, table, max_pages, q_start, kv_len, slots, nslots, used);
+    else
+        hipLaunchKernelGGL(page_tables_kernel<1024>, dim3((unsigned)grid), dim3(1024), 0, ctx->stream, (int)nreq, lg, old_len, add_len,
+                           free_list, nfree, table, max_pages, q_start, kv_len, slots, nslots, used);
+    return launch_check(ctx, "page_tables");
+}
+
+int launch_kv_append(trhip_ctx *ctx, const trhip_kv *kv, int64_t tokens, const void *k, const void *v, int io, int64_t stride,
+                     const int *slots) {
+    const int64_t esize = io == TRHIP_F32 ? 4 : 2;
+    const int wide = reinterpret_cast<uintptr_t>(k) % 16 == 0 && reinterpret_cast<uintptr_t>(v) % 16 == 0 && stride * esize % 16 == 0;
+    const int64_t total = tokens * (kv->heads * kv->dim / 4);
+    int64_t blocks = (total + 255) / 256;
+    const int64_t cap = (int64_t)(ctx->sm_count > 0 ? ctx->sm_count : 256) * 16;
+    if (blocks > cap) blocks = cap;
+    hipLaunchKernelGGL(kv_append_kernel, dim3((unsigned)blocks), dim3(256), 0, ctx->stream, static_cast<uint16_t *>(kv->k),
+                       static_cast<uint16_t *>(kv->v), kv->dtype, __builtin_ctz((unsigned)kv->page), kv->pages * kv->page, kv->heads,
+                       kv->dim, tokens, k, v, io, stride, slots, wide);
+    return launch_check(ctx, "kv_append");
+}
+
+}  // namespace trhip

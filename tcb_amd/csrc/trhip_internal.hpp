@@ -480,4 +480,23 @@ int launch_actq4_mfma(trhip_ctx *ctx, const trhip_wstore *w, int64_t row0, int64
 int launch_actq(trhip_ctx *ctx, const trhip_wstore *w, int64_t row0, int64_t N, const float *x, float *c,
                 int64_t M, bool acc, const int8_t *q, const float *d, const int16_t *bs, const uint8_t *bad,
                 const uint16_t *sj, bool fast);
+// The paged key/value cache (paged.hip) and the attention over it (attn.hip); arguments as the entry points check them.
+int launch_page_tables(trhip_ctx *ctx, int64_t nreq, int page, const int *old_len, const int *add_len, const int *free_list,
+                       int64_t nfree, int *table, int64_t max_pages, int *q_start, int *kv_len, int *slots, int64_t nslots,
+                       int *used);
+int launch_kv_append(trhip_ctx *ctx, const trhip_kv *kv, int64_t tokens, const void *k, const void *v, int io, int64_t stride,
+                     const int *slots);
+struct AttnCall {
+    const void *q;
+    void *out;
+    int64_t q_stride, out_stride, tokens;
+    int heads;
+    int64_t nreq;
+    const int *q_start, *kv_len, *table;
+    int64_t max_pages, max_new;
+    const int *prefix_table;  // prefix_len 0: none
+    int64_t prefix_len, window, sinks;
+    float scale;
+};
+int launch_attn(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c);
 }  // namespace trhip
