@@ -389,7 +389,7 @@ template <int DP, bool BF> __device__ __forceinline__ bool odd_values(uint32_t v
 // O^T += V^T P^T key by key in fp32, a key's values reaching only the rows that see it: for blocks where some rows see
 // a key that others do not and some value is not finite (0 times it would reach every row of the tile).
 template <int DP, bool BF>
-__device__ __attribute__((noinline)) void values_one_by_one(a16f (&o)[DP / 32], const a16f &pr, uint32_t v, int hi, int lo, int sinks, int t) {
+__device__ __forceinline__ void values_one_by_one(a16f (&o)[DP / 32], const a16f &pr, uint32_t v, int hi, int lo, int sinks, int t) {
     const int lane = threadIdx.x & 63, h = lane >> 5;
 #pragma unroll 1
     for (int k = 0; k < 32; k++) {
@@ -401,7 +401,8 @@ __device__ __attribute__((noinline)) void values_one_by_one(a16f (&o)[DP / 32], 
         const int j = t + k;
         const bool see = j <= hi && (j >= lo || j < sinks);
 #pragma unroll
-        for (int b = 0; b < DP / 32; b++)
+        for (int b = 0; b < DP / 32; b++) {
+            __builtin_amdgcn_sched_barrier(0);  // a rare path: few registers rather than many reads in flight
 #pragma unroll
             for (int g = 0; g < 4; g++) {
                 const uint2 w = lds8(v + k * (2 * DP) + (((4 * b + g) ^ swz<DP>(k)) << 4) + 8 * h);
@@ -409,6 +410,7 @@ __device__ __attribute__((noinline)) void values_one_by_one(a16f (&o)[DP / 32], 
 #pragma unroll
                 for (int r = 0; r < 4; r++) o[b][4 * g + r] = see ? fmaf(x, e[r], o[b][4 * g + r]) : o[b][4 * g + r];
             }
+        }
     }
 }
 
