@@ -15,7 +15,7 @@ LIB = os.path.join(HERE, "libtrhip.so")
 
 SOURCES = ["api.hip", "wstore.hip", "gemv.hip", "gemv_fast.hip", "gemm_rows.hip", "actq.hip", "actq_mfma.hip",
            "swiglu.hip", "probe.hip", "prefill.hip", "actqw.hip", "rows16.hip", "actq4.hip", "fastg.hip",
-           "io16.hip", "paged.hip", "attn.hip"]
+           "io16.hip", "paged.hip", "attn.hip", "attn_rows.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # -ffp-contract=off: no multiply-add is fused unless written as fmaf (bit-exact rounding order).
@@ -23,6 +23,9 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-ffp-contract=off",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
          "-Wall", "-Wno-unused-function", "-Wno-unused-variable"]
+# attn_rows.hip: matrix instructions take their accumulators in architectural registers where they fit. A wave there uses over
+# 256 registers, and the compiler's default then keeps every accumulator in the other file, a move away from the softmax.
+FILE_FLAGS = {"attn_rows.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def _run(cmd):
@@ -37,7 +40,7 @@ def build_lib(jobs=None):
 
     def compile_one(src):
         obj = os.path.join(OBJ, src.replace(".hip", ".o"))
-        _run([HIPCC] + FLAGS + ["-c", os.path.join(CSRC, src), "-o", obj])
+        _run([HIPCC] + FLAGS + FILE_FLAGS.get(src, []) + ["-c", os.path.join(CSRC, src), "-o", obj])
         return obj
 
     with ThreadPoolExecutor(max_workers=jobs or min(8, len(SOURCES))) as ex:

@@ -24,58 +24,6 @@ template <int DP> struct TokLds {
     static constexpr int BYTES = kTokWaves * (WAVE + 32 * 8) + 16;
 };
 
-// Joins nsplit pieces of a row (agent-coherent loads: other workgroups of this launch wrote them) and the prefix's (an earlier launch).
-template <int DP, int TR, bool BF>
-__device__ __forceinline__ void join_tile(const AttnArgs &p, const Item &it, int r0, int n, int threads) {
-    constexpr int ST = DP + 2;
-    for (int idx = threadIdx.x; idx < n * (DP / 4); idx += threads) {
-        const int r = idx / (DP / 4), d = (idx - r * (DP / 4)) * 4, row = r0 + r, t = row / p.group;
-        if (d >= p.dim) continue;
-        Join j;
-        j.init(p.scale);
-        const float *src = p.part + ((int64_t)it.first * TR + r) * ST;
-        const int64_t step = (int64_t)p.kv_heads * TR * ST;
-        for (int s0 = 0; s0 < it.nsplit; s0 += 4) {
-            float2 a[4], b[4], ml[4];
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const float *x = src + (s0 + u < it.nsplit ? s0 + u : s0) * step;
-                a[u] = agent_load(x + d);
-                b[u] = agent_load(x + d + 2);
-                ml[u] = agent_load(x + DP);
-            }
-#pragma unroll
-            for (int u = 0; u < 4; u++)
-                if (s0 + u < it.nsplit) j.add(ml[u].x, ml[u].y, a[u].x, a[u].y, b[u].x, b[u].y);
-        }
-        const float *pre = p.prefix_part + ((int64_t)(it.q0 + t) * p.heads + it.head * p.group + (row - t * p.group)) * ST;
-        for (int s = 0; s < p.prefix_splits; s++) {
-            const float *x = pre + (int64_t)s * p.tokens * p.heads * ST;
-            const float2 a = *reinterpret_cast<const float2 *>(x + d), b = *reinterpret_cast<const float2 *>(x + d + 2);
-            const float2 ml = *reinterpret_cast<const float2 *>(x + DP);
-            j.add(ml.x, ml.y, a.x, a.y, b.x, b.y);
-        }
-        put4<BF>(p, it.q0, row, it.head, d, j.o, j.l, p.prefix_splits > 0 || it.kv - it.nq + t >= 0);
-    }
-}
-
-// Partial results are written: whether this workgroup is the last of its tile's pieces.
-__device__ __forceinline__ bool last_piece(const AttnArgs &p, const Item &it, int *flag) {
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    __builtin_amdgcn_s_waitcnt(0);  // this thread's stores have completed
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    __syncthreads();
-    if (it.nsplit == 1) return true;
-    if (threadIdx.x == 0) {
-        const bool last = __hip_atomic_fetch_add(&p.arrivals[it.first], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-                          (uint32_t)(it.nsplit - 1);
-        if (last) __hip_atomic_store(&p.arrivals[it.first], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        *flag = last;
-    }
-    __syncthreads();
-    return *flag != 0;
-}
-
 // PREFIX: rows are all tokens' and keys the shared prefix's; results go to prefix_part.
 template <int DP, bool BF, bool PREFIX> __global__ __launch_bounds__(64 * kTokWaves) void attn_tokens(const AttnArgs p) {
     using L = TokLds<DP>;
@@ -92,7 +40,7 @@ template <int DP, bool BF, bool PREFIX> __global__ __launch_bounds__(64 * kTokWa
         it.nsplit = p.prefix_splits;
         it.q0 = 0;
         it.nq = p.tokens;
-        it.kv = it.first = 0;
+        it.kv = it.slot = it.counter = 0;
         table = p.prefix_table;
         keys = p.prefix_len;
     } else {
@@ -172,7 +120,7 @@ template <int DP, bool BF, bool PREFIX> __global__ __launch_bounds__(64 * kTokWa
             for (int g = 0; g < 4; g++)
                 *reinterpret_cast<float4 *>(mine + r * L::OSTRIDE + 32 * d + 8 * g + 4 * h) =
                     make_float4(A.o[d][4 * g], A.o[d][4 * g + 1], A.o[d][4 * g + 2], A.o[d][4 * g + 3]);
-        if (h == 0) ml[w * 32 + r] = make_float2(A.m, l);
+        if (h == 0) ml[w * 32 + r] = make_float2(A.m * p.scale, l);
     }
     __syncthreads();
     const bool direct = !PREFIX && it.nsplit == 1 && p.prefix_splits == 0;
@@ -180,7 +128,7 @@ template <int DP, bool BF, bool PREFIX> __global__ __launch_bounds__(64 * kTokWa
         const int r = idx / (DP / 4), d = (idx - r * (DP / 4)) * 4, row = r0 + r, t = row / p.group;
         if (d >= p.dim) continue;
         Join j;
-        j.init(p.scale);
+        j.init();
 #pragma unroll
         for (int u = 0; u < kTokWaves; u++) {
             const float4 o = *reinterpret_cast<const float4 *>(reinterpret_cast<const char *>(smem) + u * L::WAVE +
@@ -196,7 +144,7 @@ template <int DP, bool BF, bool PREFIX> __global__ __launch_bounds__(64 * kTokWa
             *reinterpret_cast<float2 *>(dst + d + 2) = make_float2(j.o[2], j.o[3]);
             if (d == 0) *reinterpret_cast<float2 *>(dst + DP) = make_float2(j.m, j.l);
         } else {
-            float *dst = p.part + ((int64_t)wg * kTokRows + r) * (DP + 2);
+            float *dst = p.part + ((int64_t)it.slot * kTokRows + r) * (DP + 2);
             agent_store(dst + d, j.o[0], j.o[1]);
             agent_store(dst + d + 2, j.o[2], j.o[3]);
             if (d == 0) agent_store(dst + DP, j.m, j.l);
@@ -219,6 +167,20 @@ template <bool PREFIX> int launch_tokens(trhip_ctx *ctx, const AttnArgs &p, int 
     if (dp == 64) return bf ? launch_tokens<64, true, PREFIX>(ctx, p, grid) : launch_tokens<64, false, PREFIX>(ctx, p, grid);
     if (dp == 128) return bf ? launch_tokens<128, true, PREFIX>(ctx, p, grid) : launch_tokens<128, false, PREFIX>(ctx, p, grid);
     return bf ? launch_tokens<256, true, PREFIX>(ctx, p, grid) : launch_tokens<256, false, PREFIX>(ctx, p, grid);
+}
+
+// The launch's workgroups: as many items as a batch of these sizes can have (find_item), whatever its lengths are.
+int64_t plan_items(AttnArgs &p, const AttnCall &c, int tile_rows, int block, int least) {
+    const int64_t tiles = (c.tokens * p.group / tile_rows + c.nreq) * p.kv_heads;
+    const int64_t blocks = ((c.max_pages << p.page_log2) + block - 1) / block, most = tiles * ((blocks + least - 1) / least + 1);
+    int64_t k = (2 * tiles + p.target - 1) / p.target;
+    p.rounds = (int)(k < kMostRounds ? k : kMostRounds);
+    p.part_slots = p.rounds * p.target;
+    if (tiles > trhip_ctx::kArrivalSlots && c.prefix_len > 0) p.rounds = 0;  // behind a prefix every tile has a place: too many for counters
+    int64_t items = p.part_slots < most ? p.part_slots : most;
+    if (tiles > items) items = tiles;
+    if (c.prefix_len > 0) p.part_slots = (int)items;
+    return items;
 }
 
 }  // namespace
@@ -254,38 +216,52 @@ int launch_attn(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c) {
     p.scale = c.scale * 1.44269504088896341f;
     p.q_aligned = (reinterpret_cast<uintptr_t>(c.q) % 16 == 0) && c.q_stride % 8 == 0;
     p.out_aligned = (reinterpret_cast<uintptr_t>(c.out) % 8 == 0) && c.out_stride % 4 == 0;
-    p.target = 2 * (ctx->sm_count > 0 ? ctx->sm_count : 256);
-    p.row_lo = 0;
-    p.row_hi = 0x7FFFFFFF;
     p.arrivals = ctx->arrivals;
-    // workgroups: every tile of rows once, and as many again as pieces may be cut (find_item)
-    const int64_t rows = c.tokens * p.group, tiles = rows / kTokRows + c.nreq;
-    int64_t grid = tiles * p.kv_heads;
-    p.split_ok = grid + p.target + p.kv_heads <= trhip_ctx::kArrivalSlots;
-    if (p.split_ok) grid += p.target + p.kv_heads;
-    if (grid >= ((int64_t)1 << 31)) return fail(ctx, TRHIP_ERR_INVALID, "attention: too many rows");
-    const int64_t ptiles = (rows + kTokRows - 1) / kTokRows;
-    if (p.prefix_len > 0) {
-        const int64_t nb = (p.prefix_len + kTokBlock - 1) / kTokBlock, items = ptiles * p.kv_heads;
-        int64_t s = (p.target + items - 1) / items;
-        if (s > (nb + kTokWaves - 1) / kTokWaves) s = (nb + kTokWaves - 1) / kTokWaves;
-        const int64_t piece = (nb + s - 1) / s;
-        p.prefix_splits = (int)((nb + piece - 1) / piece);
+    const int cus = ctx->sm_count > 0 ? ctx->sm_count : 256;
+    const int64_t rows = c.tokens * p.group;
+    // Requests of up to kTokRows rows go to attn_tokens, longer ones to attn_rows; which there are is known only from
+    // the hint, so both are launched unless it (or the sizes) rules one out. Each takes the requests of its own length, or
+    // all of them when it is alone.
+    const int64_t most_rows = (c.max_new < c.tokens ? c.max_new : c.tokens) * p.group;
+    const bool tokens_alone = most_rows <= kTokRows, rows_alone = !tokens_alone && c.tokens == c.nreq * c.max_new;
+    AttnArgs pt = p, pr = p;
+    pt.target = cus * (dp == 64 ? 2 : 1);
+    pt.row_lo = 0;
+    pt.row_hi = tokens_alone ? 0x7FFFFFFF : kTokRows;
+    pr.target = cus;
+    pr.row_lo = rows_alone ? 0 : kTokRows;
+    pr.row_hi = 0x7FFFFFFF;
+    const int tr = attn_rows_tile(dp), br = attn_rows_block(dp);
+    const int64_t grid_t = plan_items(pt, c, kTokRows, kTokBlock, kTokWaves), grid_r = plan_items(pr, c, tr, br, 4);
+    if (grid_t >= ((int64_t)1 << 31) || grid_r >= ((int64_t)1 << 31)) return fail(ctx, TRHIP_ERR_INVALID, "attention: too many rows");
+    const int64_t part_t = rows_alone ? 0 : (int64_t)pt.part_slots * kTokRows, part_r = tokens_alone ? 0 : (int64_t)pr.part_slots * tr;
+    const int64_t part = (part_t > part_r ? part_t : part_r) * (dp + 2);
+    // the prefix: all tokens' rows are one tall product, its keys cut to fill the device
+    const bool tall = rows > kTokRows;
+    const int ptr = tall ? tr : kTokRows, pbk = tall ? br : kTokBlock;
+    const int64_t ptiles = (rows + ptr - 1) / ptr;
+    int splits = 0;
+    if (c.prefix_len > 0) {
+        const int64_t nb = (c.prefix_len + pbk - 1) / pbk, items = ptiles * p.kv_heads;
+        const int64_t piece = piece_blocks(items * nb, items, tall ? pr.target : pt.target, kMostRounds, 4);
+        splits = piece >= nb ? 1 : (int)((nb + piece - 1) / piece);
     }
-    const bool parts = p.split_ok || p.prefix_splits > 0;
-    const int64_t part = parts ? grid * kTokRows * (dp + 2) : 0;
-    const int64_t pre = (int64_t)p.prefix_splits * c.tokens * c.heads * (dp + 2);
-    if (part + pre > 0) {
-        int st = TRHIP_OK;
-        p.part = static_cast<float *>(workspace(ctx, (size_t)(part + pre) * sizeof(float), &st));
-        if (!p.part) return st;
-        p.prefix_part = p.part + part;
+    int st = TRHIP_OK;
+    float *ws = static_cast<float *>(workspace(ctx, (size_t)(part + (int64_t)splits * c.tokens * c.heads * (dp + 2)) * sizeof(float), &st));
+    if (!ws) return st;
+    for (AttnArgs *a : {&pt, &pr}) {
+        a->part = ws;
+        a->prefix_part = ws + part;
+        a->prefix_splits = splits;
     }
-    if (p.prefix_len > 0) {
-        const int st = launch_tokens<true>(ctx, p, dp, bf, ptiles * p.prefix_splits * p.kv_heads);
+    if (splits > 0) {
+        const int64_t grid = ptiles * splits * p.kv_heads;
+        st = tall ? launch_attn_rows(ctx, pr, dp, bf, true, grid) : launch_tokens<true>(ctx, pt, dp, bf, grid);
         if (st != TRHIP_OK) return st;
     }
-    return launch_tokens<false>(ctx, p, dp, bf, grid);
+    if (!rows_alone) st = launch_tokens<false>(ctx, pt, dp, bf, grid_t);
+    if (st == TRHIP_OK && !tokens_alone) st = launch_attn_rows(ctx, pr, dp, bf, false, grid_r);
+    return st;
 }
 
 }  // namespace trhip

@@ -32,15 +32,15 @@ struct AttnArgs {
     const int *prefix_table;  // shared prefix: pages of its prefix_len keys (0: none)
     int64_t prefix_pages;
     int prefix_len, prefix_splits;
-    float *prefix_part;  // [split][token][head] partial results of the prefix: DP sums, maximum, sum
+    float *prefix_part;  // [split][token][head] partial results of the prefix: DP sums, reference, sum
     int nreq, tokens, heads, kv_heads, group, dim;
     int window, sinks;  // window 0: none
     float scale;        // softmax scale times log2 e
     int q_aligned, out_aligned;  // 16- and 8-byte aligned rows
-    int target;         // work items that fill the device
+    int target, rounds; // workgroups at a time, and how often at most
     int row_lo, row_hi; // requests of row_lo < rows <= row_hi are this launch's
-    int split_ok;       // keys may be split (partials and arrival counters are there)
-    float *part;        // [item][tile row]: DP sums, then maximum and sum of each row
+    int part_slots;     // places for the pieces of tiles that are cut (of all tiles behind a prefix), each with an arrival counter
+    float *part;        // [place][tile row]: DP sums, then reference (log2 units) and sum of each row
     uint32_t *arrivals;
 };
 
@@ -90,6 +90,17 @@ template <bool BF> __device__ __forceinline__ float wide_lo(uint32_t v) {
 template <bool BF> __device__ __forceinline__ float wide_hi(uint32_t v) {
     if constexpr (BF) return __uint_as_float(v & 0xFFFF0000u);
     else return (float)__builtin_bit_cast(_Float16, (uint16_t)(v >> 16));
+}
+
+// c plus both halves of v: the sum of two rounded weights in one instruction.
+template <bool BF> __device__ __forceinline__ float add2(uint32_t v, float c) {
+    if constexpr (BF) {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, v), __builtin_bit_cast(b2, 0x3F803F80u), c, false);
+    } else {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, v), __builtin_bit_cast(h2, 0x3C003C00u), c, false);
+    }
 }
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -149,7 +160,8 @@ template <int BK> __device__ __forceinline__ Span span_of(int hi, int lo, int si
 struct Item {
     int req, tile, split, nsplit, head;
     int q0, nq, kv;  // the request's first token row, new tokens, keys
-    int first;       // item number of the tile's split 0
+    int slot;        // its partial result's place (a tile's pieces are kv_heads apart), if it writes one
+    int counter;     // place of the tile's piece 0: its arrival counter
 };
 
 struct ReqShape {
@@ -178,38 +190,61 @@ template <int TR, int BK> __device__ __forceinline__ ReqShape shape_of(const Att
     return s;
 }
 
-// Which tile of rows and which piece of its keys workgroup wg takes; every wave finds out for itself (no barrier). The
-// pieces are as long as it takes for about p.target items in all, and no shorter than p's least; a request's tiles are all
-// cut into the same number of pieces. Items are numbered head fastest, then piece, tile (the last tokens of a prompt, whose rows read most keys,
+// How many blocks a piece of a tile's keys has. n tiles of `sum` blocks in all run on `target` workgroups at a time. Pieces
+// of at most c blocks are at most sum / c + n; with c = sum / (k target - n) they fill at most k rounds, which last about
+// k (c + o), o the blocks' worth of starting and joining a piece. Taken: the k up to `rounds` for which that is least: one
+// round of few long tiles, several where tiles of all lengths have to be dealt out. No more than k target pieces in all.
+constexpr int kMostRounds = 6;
+__host__ __device__ inline int piece_blocks(int64_t sum, int64_t n, int target, int rounds, int least) {
+    float best = 3e38f;
+    int64_t c = 0x40000000;
+    for (int k = 1; k <= rounds; k++) {
+        const int64_t room = (int64_t)k * target - n;
+        if (room <= 0) continue;
+        int64_t x = (sum + room - 1) / room;
+        x = x < least ? least : x;
+        const float t = (float)k * ((float)x + (float)least);
+        if (t < best) {
+            best = t;
+            c = x;
+        }
+    }
+    return c > 0x40000000 ? 0x40000000 : (int)c;
+}
+
+// Which tile of rows and which piece of its keys workgroup wg takes; every wave finds out for itself (no barrier). A
+// request's tiles are all cut into the same number of pieces (piece_blocks). Items are numbered head fastest, then piece, tile (the last tokens of a prompt, whose rows read most keys,
 // first), request. False: no item left.
 template <int TR, int BK, int CMIN> __device__ __forceinline__ bool find_item(const AttnArgs &p, int wg, Item &it) {
-    it = Item{0, 0, 0, 1, 0, 0, 0, 0, 0};
+    it = Item{0, 0, 0, 1, 0, 0, 0, 0, 0, 0};
     const int lane = threadIdx.x & 63, x = wg / p.kv_heads;
     ReqShape s = shape_of<TR, BK>(p, lane);
-    int piece = 0x40000000;
-    if (p.split_ok) {
-        int64_t sum = (int64_t)s.tiles * s.nb;
-        for (int base = 64; base < p.nreq; base += 64) {
-            const ReqShape t = shape_of<TR, BK>(p, base + lane);
-            sum += (int64_t)t.tiles * t.nb;
-        }
-#pragma unroll
-        for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-        sum = uni64(sum) * p.kv_heads;
-        const int64_t c = (sum + p.target - 1) / p.target;
-        piece = c < CMIN ? CMIN : c > 0x40000000 ? 0x40000000 : (int)c;
+    int64_t sum = (int64_t)s.tiles * s.nb, tiles = s.tiles;
+    for (int base = 64; base < p.nreq; base += 64) {
+        const ReqShape t = shape_of<TR, BK>(p, base + lane);
+        sum += (int64_t)t.tiles * t.nb;
+        tiles += t.tiles;
     }
-    int before = 0;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+        sum += __shfl_xor(sum, o);
+        tiles += __shfl_xor(tiles, o);
+    }
+    const int piece = piece_blocks(uni64(sum) * p.kv_heads, uni64(tiles) * p.kv_heads, p.target, p.rounds, CMIN);
+    int before = 0, parts = 0;
     bool found = false;
     for (int base = 0; base < p.nreq; base += 64) {
         if (base) s = shape_of<TR, BK>(p, base + lane);
         const int ns = s.nb <= piece ? 1 : (s.nb + piece - 1) / piece;
-        const int n = s.tiles * ns;
-        int incl = n;
+        const int n = s.tiles * ns, np = ns > 1 || p.prefix_splits > 0 ? n : 0;
+        int incl = n, inclp = np;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
-            const int u = __shfl_up(incl, o);
-            if (lane >= o) incl += u;
+            const int u = __shfl_up(incl, o), v = __shfl_up(inclp, o);
+            if (lane >= o) {
+                incl += u;
+                inclp += v;
+            }
         }
         if (!found) {
             const uint64_t m = __ballot(before + incl > x);
@@ -225,16 +260,18 @@ template <int TR, int BK, int CMIN> __device__ __forceinline__ bool find_item(co
                 it.split = at - t * it.nsplit;
                 it.tile = tiles - 1 - t;
                 it.head = wg - x * p.kv_heads;
-                it.first = (x - it.split) * p.kv_heads + it.head;
+                it.slot = (parts + __builtin_amdgcn_readlane(inclp - np, src) + at) * p.kv_heads + it.head;
+                it.counter = it.slot - it.split * p.kv_heads;
                 found = true;
             }
         }
         before += __builtin_amdgcn_readlane(incl, 63);
+        parts += __builtin_amdgcn_readlane(inclp, 63);
     }
     it.req = uni(it.req), it.tile = uni(it.tile), it.split = uni(it.split), it.nsplit = uni(it.nsplit), it.head = uni(it.head);
-    it.q0 = uni(it.q0), it.nq = uni(it.nq), it.kv = uni(it.kv), it.first = uni(it.first);
+    it.q0 = uni(it.q0), it.nq = uni(it.nq), it.kv = uni(it.kv), it.slot = uni(it.slot), it.counter = uni(it.counter);
     // starts that are not in order could name more items than there are workgroups: then nothing is done
-    return found && (int64_t)before * p.kv_heads <= (int64_t)gridDim.x;
+    return found && (int64_t)before * p.kv_heads <= (int64_t)gridDim.x && parts * p.kv_heads <= p.part_slots;
 }
 
 // ---- a tile's rows and masks -------------------------------------------------------------------------------------------
@@ -516,17 +553,16 @@ template <bool BF> __device__ __forceinline__ void put4(const AttnArgs &p, int q
     }
 }
 
-// A sum over partial results of one row: the largest maximum so far, sums relative to it.
+// A sum over partial results of one row: the largest reference so far (in units of log2), sums relative to it.
 struct Join {
-    float m, l, o[4], scale;
-    __device__ __forceinline__ void init(float s) {
-        scale = s;
+    float m, l, o[4];
+    __device__ __forceinline__ void init() {
         m = -__builtin_inff();
         l = o[0] = o[1] = o[2] = o[3] = 0.0f;
     }
     __device__ __forceinline__ void add(float pm, float pl, float a, float b, float c, float d) {
         const float n = fmaxf(m, pm);
-        const float x = m == n ? 1.0f : exp2_hw((m - n) * scale), y = pm == n ? 1.0f : exp2_hw((pm - n) * scale);
+        const float x = m == n ? 1.0f : exp2_hw(m - n), y = pm == n ? 1.0f : exp2_hw(pm - n);
         l = l * x + pl * y;
         o[0] = o[0] * x + a * y;
         o[1] = o[1] * x + b * y;
@@ -536,5 +572,63 @@ struct Join {
     }
 };
 
+// Joins nsplit pieces of a row (agent-coherent loads: other workgroups of this launch wrote them) and the prefix's (an earlier launch).
+template <int DP, int TR, bool BF>
+__device__ __forceinline__ void join_tile(const AttnArgs &p, const Item &it, int r0, int n, int threads) {
+    constexpr int ST = DP + 2;
+    for (int idx = threadIdx.x; idx < n * (DP / 4); idx += threads) {
+        const int r = idx / (DP / 4), d = (idx - r * (DP / 4)) * 4, row = r0 + r, t = row / p.group;
+        if (d >= p.dim) continue;
+        Join j;
+        j.init();
+        const float *src = p.part + ((int64_t)it.counter * TR + r) * ST;
+        const int64_t step = (int64_t)p.kv_heads * TR * ST;
+        for (int s0 = 0; s0 < it.nsplit; s0 += 4) {
+            float2 a[4], b[4], ml[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const float *x = src + (s0 + u < it.nsplit ? s0 + u : s0) * step;
+                a[u] = agent_load(x + d);
+                b[u] = agent_load(x + d + 2);
+                ml[u] = agent_load(x + DP);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (s0 + u < it.nsplit) j.add(ml[u].x, ml[u].y, a[u].x, a[u].y, b[u].x, b[u].y);
+        }
+        const float *pre = p.prefix_part + ((int64_t)(it.q0 + t) * p.heads + it.head * p.group + (row - t * p.group)) * ST;
+        for (int s = 0; s < p.prefix_splits; s++) {
+            const float *x = pre + (int64_t)s * p.tokens * p.heads * ST;
+            const float2 a = *reinterpret_cast<const float2 *>(x + d), b = *reinterpret_cast<const float2 *>(x + d + 2);
+            const float2 ml = *reinterpret_cast<const float2 *>(x + DP);
+            j.add(ml.x, ml.y, a.x, a.y, b.x, b.y);
+        }
+        put4<BF>(p, it.q0, row, it.head, d, j.o, j.l, p.prefix_splits > 0 || it.kv - it.nq + t >= 0);
+    }
+}
+
+// Partial results are written: whether this workgroup is the last of its tile's pieces.
+__device__ __forceinline__ bool last_piece(const AttnArgs &p, const Item &it, int *flag) {
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0);  // this thread's stores have completed
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __syncthreads();
+    if (it.nsplit == 1) return true;
+    if (threadIdx.x == 0) {
+        const bool last = __hip_atomic_fetch_add(&p.arrivals[it.counter], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+                          (uint32_t)(it.nsplit - 1);
+        if (last) __hip_atomic_store(&p.arrivals[it.counter], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *flag = last;
+    }
+    __syncthreads();
+    return *flag != 0;
+}
+
 }  // namespace
+
+// attn_rows.hip: rows of a tile and keys of a block, and the launch.
+int attn_rows_tile(int dp);
+int attn_rows_block(int dp);
+int launch_attn_rows(trhip_ctx *ctx, const AttnArgs &p, int dp, bool bf, bool prefix, int64_t grid);
+
 }  // namespace trhip
