@@ -13,7 +13,7 @@
 namespace trhip {
 namespace {
 
-constexpr int kTokRows = 32, kTokBlock = 32, kTokWaves = 4;
+constexpr int kTokRows = 32, kTokBlock = 32, kTokWaves = 4, kTokOver = 6;
 
 template <int DP> struct TokLds {
     static constexpr int SLOT = 32 * DP * 2;  // 32 keys or values
@@ -44,7 +44,7 @@ template <int DP, bool BF, bool PREFIX> __global__ __launch_bounds__(64 * kTokWa
         table = p.prefix_table;
         keys = p.prefix_len;
     } else {
-        if (!find_item<kTokRows, kTokBlock, kTokWaves>(p, wg, it)) return;
+        if (!find_item<kTokRows, kTokBlock, kTokWaves, kTokOver>(p, wg, it)) return;
         table = p.table + (int64_t)it.req * p.max_pages;
         keys = it.kv;
     }
@@ -171,7 +171,9 @@ template <bool PREFIX> int launch_tokens(trhip_ctx *ctx, const AttnArgs &p, int 
 
 // The launch's workgroups: as many items as a batch of these sizes can have (find_item), whatever its lengths are.
 int64_t plan_items(AttnArgs &p, const AttnCall &c, int tile_rows, int block, int least) {
-    const int64_t tiles = (c.tokens * p.group / tile_rows + c.nreq) * p.kv_heads;
+    int64_t tiles = c.tokens * p.group / tile_rows + c.nreq;
+    if (p.row_hi <= tile_rows && tiles > c.nreq) tiles = c.nreq;
+    tiles *= p.kv_heads;
     const int64_t blocks = ((c.max_pages << p.page_log2) + block - 1) / block, most = tiles * ((blocks + least - 1) / least + 1);
     int64_t k = (2 * tiles + p.target - 1) / p.target;
     p.rounds = (int)(k < kMostRounds ? k : kMostRounds);
@@ -243,7 +245,7 @@ int launch_attn(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c) {
     int splits = 0;
     if (c.prefix_len > 0) {
         const int64_t nb = (c.prefix_len + pbk - 1) / pbk, items = ptiles * p.kv_heads;
-        const int64_t piece = piece_blocks(items * nb, items, tall ? pr.target : pt.target, kMostRounds, 4);
+        const int64_t piece = piece_blocks(items * nb, items, (int)nb, tall ? pr.target : pt.target, kMostRounds, 4, tall ? kRowsOver : kTokOver);
         splits = piece >= nb ? 1 : (int)((nb + piece - 1) / piece);
     }
     int st = TRHIP_OK;

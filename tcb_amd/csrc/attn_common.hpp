@@ -190,47 +190,66 @@ template <int TR, int BK> __device__ __forceinline__ ReqShape shape_of(const Att
     return s;
 }
 
-// How many blocks a piece of a tile's keys has. n tiles of `sum` blocks in all run on `target` workgroups at a time. Pieces
-// of at most c blocks are at most sum / c + n; with c = sum / (k target - n) they fill at most k rounds, which last about
-// k (c + o), o the blocks' worth of starting and joining a piece. Taken: the k up to `rounds` for which that is least: one
-// round of few long tiles, several where tiles of all lengths have to be dealt out. No more than k target pieces in all.
+// How many blocks a piece of a tile's keys has: n tiles of `sum` blocks in all, the longest of `most`, on `target` workgroups
+// at a time; starting a piece, writing its result and joining it take as long as `over` blocks. Pieces of at most c
+// blocks are at most sum / c + n. Estimated, in blocks, and the least taken:
+//   whole tiles       most, where all run at once; else sum / target and half the longest
+//   one round         c + over, c = sum / (target - n) (all pieces at once), where n < target
+//   dealt out         (sum + over (sum / c + n)) / target + c + over, least at c = sqrt(over sum / target)
+// Never more than rounds * target pieces.
 constexpr int kMostRounds = 6;
-__host__ __device__ inline int piece_blocks(int64_t sum, int64_t n, int target, int rounds, int least) {
-    float best = 3e38f;
-    int64_t c = 0x40000000;
-    for (int k = 1; k <= rounds; k++) {
-        const int64_t room = (int64_t)k * target - n;
-        if (room <= 0) continue;
-        int64_t x = (sum + room - 1) / room;
-        x = x < least ? least : x;
-        const float t = (float)k * ((float)x + (float)least);
-        if (t < best) {
-            best = t;
-            c = x;
+constexpr int kRowsOver = 10;  // attn_rows
+__host__ __device__ inline int piece_blocks(int64_t sum, int64_t n, int most, int target, int rounds, int least, int over) {
+    constexpr int kWhole = 0x40000000;
+    const float s = (float)sum, t = (float)target;
+    float best = n <= target ? (float)most : s / t + 0.5f * (float)most;
+    int64_t piece = kWhole;
+    if (rounds > 0 && n < target) {
+        int64_t c = (sum + target - n - 1) / (target - n);
+        c = c < least ? least : c;
+        if ((float)(c + over) < best) {
+            best = (float)(c + over);
+            piece = c;
         }
     }
-    return c > 0x40000000 ? 0x40000000 : (int)c;
+    const int64_t room = (int64_t)rounds * target - n;
+    if (room > 0) {
+        int64_t c = (int64_t)sqrtf((float)over * s / t);
+        const int64_t low = (sum + room - 1) / room;
+        c = c < low ? low : c;
+        c = c < least ? least : c;
+        const float e = (s + (float)over * (s / (float)c + (float)n)) / t + (float)(c + over);
+        if (e < best) {
+            best = e;
+            piece = c;
+        }
+    }
+    return piece >= most || piece > kWhole ? kWhole : (int)piece;
 }
 
 // Which tile of rows and which piece of its keys workgroup wg takes; every wave finds out for itself (no barrier). A
 // request's tiles are all cut into the same number of pieces (piece_blocks). Items are numbered head fastest, then piece, tile (the last tokens of a prompt, whose rows read most keys,
 // first), request. False: no item left.
-template <int TR, int BK, int CMIN> __device__ __forceinline__ bool find_item(const AttnArgs &p, int wg, Item &it) {
+template <int TR, int BK, int CMIN, int OVER> __device__ __forceinline__ bool find_item(const AttnArgs &p, int wg, Item &it) {
     it = Item{0, 0, 0, 1, 0, 0, 0, 0, 0, 0};
     const int lane = threadIdx.x & 63, x = wg / p.kv_heads;
     ReqShape s = shape_of<TR, BK>(p, lane);
     int64_t sum = (int64_t)s.tiles * s.nb, tiles = s.tiles;
+    int most = s.nb;
     for (int base = 64; base < p.nreq; base += 64) {
         const ReqShape t = shape_of<TR, BK>(p, base + lane);
         sum += (int64_t)t.tiles * t.nb;
         tiles += t.tiles;
+        most = t.nb > most ? t.nb : most;
     }
 #pragma unroll
     for (int o = 32; o; o >>= 1) {
         sum += __shfl_xor(sum, o);
         tiles += __shfl_xor(tiles, o);
+        const int m = __shfl_xor(most, o);
+        most = m > most ? m : most;
     }
-    const int piece = piece_blocks(uni64(sum) * p.kv_heads, uni64(tiles) * p.kv_heads, p.target, p.rounds, CMIN);
+    const int piece = piece_blocks(uni64(sum) * p.kv_heads, uni64(tiles) * p.kv_heads, uni(most), p.target, p.rounds, CMIN, OVER);
     int before = 0, parts = 0;
     bool found = false;
     for (int base = 0; base < p.nreq; base += 64) {

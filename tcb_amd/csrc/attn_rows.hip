@@ -74,7 +74,7 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::WAVES / 4) v
         table = p.prefix_table;
         keys = p.prefix_len;
     } else {
-        if (!find_item<L::TR, BK, 4>(p, blockIdx.x, it)) return;
+        if (!find_item<L::TR, BK, 4, kRowsOver>(p, blockIdx.x, it)) return;
         table = p.table + (int64_t)it.req * p.max_pages;
         keys = it.kv;
     }
