@@ -1,17 +1,18 @@
 // attn_rows.hip -- attention over a paged cache for many rows: prompts, and a shared prefix under a batch's tokens.
 //
 // A workgroup takes a tile of 32 rows a wave (attn_common.hpp) and goes through its keys in blocks of BK that its waves copy
-// into LDS together. What bounds it are the matrix instructions and the LDS reads that feed them (a KB an instruction: at
-// full rate both are busy all the time); the softmax's instructions have to run under them. So the loop is skewed: step j multiplies K of
-// block j + 1 and V of block j - 1 while it takes the exponentials of block j, three independent pieces of work in one run
-// of instructions, and two waves share a SIMD.
+// into LDS together. What bounds it are the matrix instructions and, nearly as much, the softmax's instructions, which
+// have to run under them. Blocks that every row sees whole are taken in a skewed loop: step j multiplies K of block j + 1 and V of
+// block j - 1 while it takes the exponentials of block j, three independent pieces of work in one run of instructions, and two
+// waves share a SIMD. Blocks with a mask go through a plain step. The two are loops of their own: with masks as branches of one loop the
+// compiler copied O^T between registers at every join, a third of the loop's instructions.
 //
-// The softmax's reference (what is subtracted from a row's scores) is a whole power of two, raised only when a step's
+// The softmax's reference (what is subtracted from a row's scores) is a whole power of two, raised only when a block's
 // maximum exceeds it by more than 2^8: then the sums, O^T and the pending weights are multiplied by a power of two, exactly.
-// The weights stay below 2^9, inside f16 and bf16, and lose no precision to a reference that is a little low. They are rounded
-// to 16 bits for the product with V, and the row's sum is taken of the rounded ones, so that a lone key's rounding cancels wholly and
-// many keys' averages out. Steps with a mask, and all steps of rows that see fewer than kFewKeys keys, add the second term of
-// each weight (what the rounding dropped): there the result is as near as with weights in fp32.
+// The weights stay below 2^9, inside f16 and bf16, and lose no precision to a reference that is a little low. In the skewed
+// loop they are rounded to 16 bits for the product with V, and the row's sum is taken of the rounded ones, so that many keys'
+// rounding averages out. The plain step, which all blocks of rows that see fewer than kFewKeys keys take, multiplies a second
+// term of each weight (what the rounding dropped): as near as with weights in fp32.
 #include "attn_common.hpp"
 
 namespace trhip {
@@ -26,8 +27,7 @@ template <int DP> struct RowsShape {
     static constexpr int SLOTS = 3;                // blocks of each in LDS
     static constexpr int PI = DP / 64;             // copies a wave makes of a block: eight rows
     static constexpr int ZERO = 2 * SLOTS * TILE;  // a block of zeros behind the rings
-    static constexpr int LOW = ZERO + TILE;        // second terms of a step's weights, 32 NT bytes a lane
-    static constexpr int BYTES = LOW + THREADS * 32 * NT + 16;
+    static constexpr int BYTES = ZERO + TILE + 16;
 };
 
 // A wave's share of a block: eight rows of a sixteen-row piece, from row `r0` of it.
@@ -123,7 +123,6 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::WAVES / 4) v
     // lane parts of the operands' addresses
     const int kr = lane & 31, vi = lane & 15, vr = 4 * h + (vi >> 2), vc = 2 * ((lane >> 4) & 1) + ((vi >> 1) & 1);
     const uint32_t ka = kr * (2 * DP) + ((h ^ swz<DP>(kr)) << 4), va = vr * (2 * DP) + ((vc ^ swz<DP>(vr)) << 4) + 8 * (vi & 1);
-    const uint32_t low = ring + L::LOW + tid * 16;
     constexpr int NK = DP / 16, NV = DP / 16;
 
     auto maximum = [&](const a16f (&x)[NT]) {
@@ -144,154 +143,154 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::WAVES / 4) v
         const int c = i / (DP / 32), t = c / 2, e = 4 * (c & 1);
         return make_uint4(x[t][e], x[t][e + 1], x[t][e + 2], x[t][e + 3]);
     };
-    const bool few = !PREFIX && (all.hi_min + 1 < kFewKeys || (p.window > 0 && p.window < kFewKeys));
-    bool was_fine = false;  // the step before left second terms in LDS
-    int t_before = 0;
-    // The pending weights' product where it is not an ordinary one. Returns the address of V for the ordinary product.
-    auto pending = [&](uint32_t at) -> uint32_t {
-        if (!was_fine) return at;
-        if (mixed) {
-            bool odd = false;
-#pragma unroll
-            for (int t = 0; t < NT; t++) odd = odd || odd_values<DP, BF>(at + t * 64 * DP);
-            if (odd) {  // an infinity or a NaN that not all rows see: key by key, zeros in V's place
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    a16f x;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        x[2 * i] = wide_lo<BF>(pk[t][i]);
-                        x[2 * i + 1] = wide_hi<BF>(pk[t][i]);
-                    }
-                    values_one_by_one<DP, BF>(o, x, at + t * 64 * DP, rw.hi, rw.lo, rw.sinks, t_before + 32 * t);
-                }
-                return ring + L::ZERO;
-            }
-        }
-#pragma unroll
-        for (int c = 0; c < 2 * NT; c++) {
-            const uint4 lo = lds16(low + c * 16 * L::THREADS);
-#pragma unroll
-            for (int d = 0; d < DP / 32; d++) o[d] = mma<BF>(v_frag(at, c * (DP / 32) + d), lo, o[d]);
-        }
-        return at;
-    };
-
-    Piece16 c0 = piece_of(0), c1 = piece_of(1), c2 = piece_of(2);
-    copy_k(c0, 0);
-    copy_k(c1, 1);
-    copy_k(c2, 2);
-    copy_v(c0, 0);
-    wait_vmcnt(3 * L::PI);
-    lds_barrier();
-#pragma unroll
-    for (int i = 0; i < NT * NK; i++) s[i / NK] = mma<BF>(k_frag(ring, i), q[i % NK], i % NK == 0 ? a16f{} : s[i / NK]);
-    top = maximum(s);
-    int k1 = 1, v1 = 2;  // ring places of K of block j + 1 and V of block j - 1
-    for (int j = 0; j < nb; j++) {
-        wait_vmcnt(2 * L::PI);
-        lds_barrier();  // keys of block j + 1 and values of j - 1 are there, and what the next copies replace has been read
-        {
-            const Piece16 c3 = piece_of(j + 3);
-            copy_k(c3, k1 + 2 >= L::SLOTS ? k1 + 2 - L::SLOTS : k1 + 2);
-            copy_v(c1, v1 + 2 >= L::SLOTS ? v1 + 2 - L::SLOTS : v1 + 2);
-            c1 = c2, c2 = c3;
-        }
-        const uint32_t kat = ring + k1 * L::TILE, vat = pending(j > 0 ? ring + (L::SLOTS + v1) * L::TILE : ring + L::ZERO);
-        // rare: masks, a raised reference, scores too large for a fused step
-        const int t0 = key_of(j);
-        const bool see = all_see(rw, t0, BK);
-        if (!see) {
-#pragma unroll
-            for (int t = 0; t < NT; t++) mask(s[t], rw, t0 + 32 * t);
-            top = maximum(s);
-        }
+    // Raises the reference to a block's maxima where they exceed it by more than 2^8; returns minus the reference for the
+    // exponentials' fused step (0 where scores x were too large for it and have been made relative here).
+    auto refer = [&](a16f (&x)[NT], bool weights) -> float {
         top = half_max(top);
         if (__any(top * p.scale > ms + 8.0f)) {
-            const float y = top * p.scale, x = fabsf(y) > 1048576.0f ? y : ceilf(y);
-            if (x > ms + 8.0f) {
-                const float a = exp2_hw(ms - x);  // from -Inf: 0
-                ms = x;
-                mf = top;
-                l *= a;
+            const float y = top * p.scale, r = fabsf(y) > 1048576.0f ? y : ceilf(y);
+            const bool up = r > ms + 8.0f;
+            const float a = up ? exp2_hw(ms - r) : 1.0f;  // from -Inf: 0
+            ms = up ? r : ms;
+            mf = up ? top : mf;
+            l *= a;
 #pragma unroll
-                for (int d = 0; d < DP / 32; d++)
+            for (int d = 0; d < DP / 32; d++)
 #pragma unroll
-                    for (int i = 0; i < 16; i++) o[d][i] *= a;
+                for (int i = 0; i < 16; i++) o[d][i] *= a;
+            if (weights) {
 #pragma unroll
                 for (int t = 0; t < NT; t++)
 #pragma unroll
                     for (int i = 0; i < 8; i++) pk[t][i] = pack2<BF>(wide_lo<BF>(pk[t][i]) * a, wide_hi<BF>(pk[t][i]) * a);
             }
         }
-        float neg = ms == -__builtin_inff() ? 0.0f : -ms;
-        if (__any(fabsf(neg) > 1048576.0f)) {
-            const bool far = fabsf(neg) > 1048576.0f;
+        const float neg = ms == -__builtin_inff() ? 0.0f : -ms;
+        const bool far = fabsf(neg) > 1048576.0f;
+        if (__any(far)) {
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) s[t][i] -= far ? mf : 0.0f;
-            neg = far ? 0.0f : neg;
+                for (int i = 0; i < 16; i++) x[t][i] -= far ? mf : 0.0f;
         }
-        was_fine = !see || few;
-        t_before = t0;
-        if (was_fine) {  // second terms, to LDS until the next step
-            // (the scale is hidden, or the compiler would move the exponentials of the run below to before this branch)
-            const float scale = __uint_as_float(opaque(__float_as_uint(p.scale)));
+        return far ? 0.0f : neg;
+    };
+
+    // Blocks [f0, f1) are seen whole by every row of the tile.
+    const int at0 = sp.ns - sp.w0 - b0;
+    int f0 = at0 + (all.lo_max + BK - 1) / BK, f1 = at0 + (all.hi_min + 1) / BK;
+    f0 = f0 < 0 ? 0 : f0;
+    f1 = f1 > nb ? nb : f1;
+    if (f1 < f0 + 2 || all.hi_min + 1 < kFewKeys || (p.window > 0 && p.window < kFewKeys)) f0 = f1 = nb;
+
+    // Copies run ahead of step j by K of block j + 3 and V of block j + 1.
+    Piece16 c1 = piece_of(1), c2 = piece_of(2);
+    {
+        const Piece16 c0 = piece_of(0);
+        copy_k(c0, 0);
+        copy_k(c1, 1);
+        copy_k(c2, 2);
+        copy_v(c0, 0);
+    }
+    int k0 = 0;  // ring place of block j, keys and values
+    auto next = [&](int k) { return k + 1 == L::SLOTS ? 0 : k + 1; };
+    auto ahead = [&](int j) {
+        const Piece16 c3 = piece_of(j + 3);
+        copy_v(c1, next(k0));
+        copy_k(c3, k0);
+        c1 = c2, c2 = c3;
+    };
+    auto plain = [&](int j) {
+        wait_vmcnt(0);
+        lds_barrier();
+        const uint32_t kat = ring + k0 * L::TILE, vat = ring + (L::SLOTS + k0) * L::TILE;
 #pragma unroll
-            for (int c = 0; c < 2 * NT; c++) {
-                uint32_t r[4];
+        for (int i = 0; i < NT * NK; i++) s[i / NK] = mma<BF>(k_frag(kat, i), q[i % NK], i % NK == 0 ? a16f{} : s[i / NK]);
+        lds_barrier();  // the keys have been read
+        ahead(j);
+        const int t0 = key_of(j);
+        const bool see = all_see(rw, t0, BK);
+        if (!see) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int e = 8 * (c & 1) + 2 * i;
-                    const float x = exp2_hw(fmaf(s[c / 2][e], scale, neg)), y = exp2_hw(fmaf(s[c / 2][e + 1], scale, neg));
-                    const uint32_t u = pack2<BF>(x, y);
-                    r[i] = pack2<BF>(x - wide_lo<BF>(u), y - wide_hi<BF>(u));
-                    l = add2<BF>(r[i], l);
-                }
-                smem[(L::LOW + c * 16 * L::THREADS) / 16 + tid] = make_uint4(r[0], r[1], r[2], r[3]);
-            }
+            for (int t = 0; t < NT; t++) mask(s[t], rw, t0 + 32 * t);
         }
-        // three independent runs, dealt over one another: products with K, exponentials, products with V
-        a16f sn[NT];
-        uint32_t pn[NT][8];
-        float sum = 0.0f;
-        constexpr int M = NT * (NK + NV), NW = 8 * NT, AHEAD = 3;  // products, pairs of weights, operands read ahead
-        uint4 f[AHEAD + 1];
-        auto frag = [&](int i) { return i < NT * NK ? k_frag(kat, i) : v_frag(vat, i - NT * NK); };
-#pragma unroll
-        for (int i = 0; i < AHEAD; i++) f[i] = frag(i);
-#pragma unroll
-        for (int i = 0; i < M; i++) {
-            if (i + AHEAD < M) f[(i + AHEAD) % (AHEAD + 1)] = frag(i + AHEAD);
-            const uint4 a = f[i % (AHEAD + 1)];
-            if (i < NT * NK) sn[i / NK] = mma<BF>(a, q[i % NK], i % NK == 0 ? a16f{} : sn[i / NK]);
-            else o[(i - NT * NK) % (DP / 32)] = mma<BF>(a, p_frag(pk, i - NT * NK), o[(i - NT * NK) % (DP / 32)]);
-#pragma unroll
-            for (int e = i * NW / M; e < (i + 1) * NW / M; e++) {
-                const int t = e >> 3, k = e & 7;
-                pn[t][k] = pack2<BF>(exp2_hw(fmaf(s[t][2 * k], p.scale, neg)), exp2_hw(fmaf(s[t][2 * k + 1], p.scale, neg)));
-                sum = add2<BF>(pn[t][k], sum);  // of the rounded weights
-            }
-        }
-        l += sum;
-        top = maximum(sn);
+        top = maximum(s);
+        const float neg = refer(s, false);
+        bool odd = false;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            s[t] = sn[t];
 #pragma unroll
-            for (int i = 0; i < 8; i++) pk[t][i] = pn[t][i];
+            for (int i = 0; i < 16; i++) {
+                s[t][i] = exp2_hw(fmaf(s[t][i], p.scale, neg));
+                l += s[t][i];
+            }
+            if (!see && mixed) odd = odd || odd_values<DP, BF>(vat + t * 64 * DP);
         }
-        k1 = k1 + 1 == L::SLOTS ? 0 : k1 + 1;
-        v1 = v1 + 1 == L::SLOTS ? 0 : v1 + 1;
-    }
-    wait_vmcnt(0);
-    lds_barrier();
-    if (nb > 0) {
-        const uint32_t vat = pending(ring + (L::SLOTS + v1) * L::TILE);
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            if (odd) values_one_by_one<DP, BF>(o, s[t], vat + t * 64 * DP, rw.hi, rw.lo, rw.sinks, t0 + 32 * t);
+            else values<DP, BF, true>(o, s[t], vat + t * 64 * DP);
+        }
+        k0 = next(k0);
+    };
+    int j = 0;
+    for (; j < f0; j++) plain(j);
+    if (j < f1) {
+        wait_vmcnt(2 * L::PI);
+        lds_barrier();
+        {
+            const uint32_t kat = ring + k0 * L::TILE;
+#pragma unroll
+            for (int i = 0; i < NT * NK; i++) s[i / NK] = mma<BF>(k_frag(kat, i), q[i % NK], i % NK == 0 ? a16f{} : s[i / NK]);
+        }
+        top = maximum(s);
+        uint32_t vat = ring + L::ZERO;  // V of block j - 1
+        for (; j < f1; j++) {
+            wait_vmcnt(2 * L::PI);
+            lds_barrier();  // keys of block j + 1 and values of j - 1 are there, and what the next copies replace has been read
+            ahead(j);
+            const uint32_t kat = ring + next(k0) * L::TILE;
+            const float neg = refer(s, true);
+            // three independent runs, dealt over one another: products with K, exponentials, products with V
+            a16f sn[NT];
+            uint32_t pn[NT][8];
+            float sum = 0.0f;
+            constexpr int M = NT * (NK + NV), NW = 8 * NT, AHEAD = 3;  // products, pairs of weights, operands read ahead
+            uint4 f[AHEAD + 1];
+            auto frag = [&](int i) { return i < NT * NK ? k_frag(kat, i) : v_frag(vat, i - NT * NK); };
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) f[i] = frag(i);
+#pragma unroll
+            for (int i = 0; i < M; i++) {
+                if (i + AHEAD < M) f[(i + AHEAD) % (AHEAD + 1)] = frag(i + AHEAD);
+                const uint4 a = f[i % (AHEAD + 1)];
+                if (i < NT * NK) sn[i / NK] = mma<BF>(a, q[i % NK], i % NK == 0 ? a16f{} : sn[i / NK]);
+                else o[(i - NT * NK) % (DP / 32)] = mma<BF>(a, p_frag(pk, i - NT * NK), o[(i - NT * NK) % (DP / 32)]);
+#pragma unroll
+                for (int e = i * NW / M; e < (i + 1) * NW / M; e++) {
+                    const int t = e >> 3, k = e & 7;
+                    pn[t][k] = pack2<BF>(exp2_hw(fmaf(s[t][2 * k], p.scale, neg)), exp2_hw(fmaf(s[t][2 * k + 1], p.scale, neg)));
+                    sum = add2<BF>(pn[t][k], sum);  // of the rounded weights
+                }
+            }
+            l += sum;
+            top = maximum(sn);
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                s[t] = sn[t];
+#pragma unroll
+                for (int i = 0; i < 8; i++) pk[t][i] = pn[t][i];
+            }
+            vat = ring + (L::SLOTS + k0) * L::TILE;
+            k0 = next(k0);
+        }
+        wait_vmcnt(0);
+        lds_barrier();
 #pragma unroll
         for (int i = 0; i < NT * NV; i++) o[i % (DP / 32)] = mma<BF>(v_frag(vat, i), p_frag(pk, i), o[i % (DP / 32)]);
     }
+    for (; j < nb; j++) plain(j);
+    wait_vmcnt(0);
 
     const bool direct = !PREFIX && it.nsplit == 1 && p.prefix_splits == 0;
     const float sum = half_sum(l);
