@@ -67,7 +67,7 @@ template <int DP, bool BF, bool PREFIX> __global__ __launch_bounds__(64 * kTokWa
     auto pieces = [&](int b, Piece16 (&s)[2]) {  // past the last block: nothing but zeros
         const int t = b < b1 ? key_of(b) : 0, hi = b < b1 ? rw.hi_max : -1;
 #pragma unroll
-        for (int i = 0; i < 2; i++) s[i] = piece16(p, table, it.head, t + 16 * i, hi, rw.lo_min, rw.sinks);
+        for (int i = 0; i < 2; i++) s[i] = piece16(p, page16(p, table, t + 16 * i, hi), it.head, t + 16 * i, hi, rw.lo_min, rw.sinks);
     };
     auto copy_k = [&](const Piece16 (&s)[2], int slot) {
 #pragma unroll
@@ -230,7 +230,7 @@ int launch_attn(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c) {
     pt.target = cus * (dp == 64 ? 2 : 1);
     pt.row_lo = 0;
     pt.row_hi = tokens_alone ? 0x7FFFFFFF : kTokRows;
-    pr.target = cus;
+    pr.target = cus * attn_rows_per_cu(dp);
     pr.row_lo = rows_alone ? 0 : kTokRows;
     pr.row_hi = 0x7FFFFFFF;
     const int tr = attn_rows_tile(dp), br = attn_rows_block(dp);

@@ -12,7 +12,7 @@
 // (two transposing LDS reads of four keys x sixteen dimensions each). P never leaves its lane.
 //
 // LDS rows hold their 16-byte chunks in the order chunk ^ swz(row), which spreads both reads (a column of sixteen rows,
-// and four rows x 32 bytes) over all banks; the copies into LDS place a lane's chunk by choosing which chunk it fetches.
+// and four rows x 64 bytes) over all banks; the copies into LDS place a lane's chunk by choosing which chunk it fetches.
 #pragma once
 
 #include "trhip_internal.hpp"
@@ -63,7 +63,7 @@ __device__ __forceinline__ int sload(const int *p, int64_t i) {
 }
 
 template <int DP> __device__ __forceinline__ int swz(int row) {
-    return DP == 64 ? 2 * ((row >> 1) & 3) | ((row >> 3) & 1) : 2 * (row & 7) | ((row >> 3) & 1);
+    return DP == 64 ? 4 * ((row >> 1) & 1) | ((row >> 2) & 3) : 4 * (row & 3) | ((row >> 2) & 3);
 }
 
 template <bool BF> __device__ __forceinline__ a16f mma(uint4 a, uint4 b, a16f c) {
@@ -326,20 +326,21 @@ struct Piece16 {
     dma_rsrc k, v;
     int ha, hb;  // hidden rows [ha, hb)
 };
-__device__ __forceinline__ Piece16 piece16(const AttnArgs &p, const int *table, int head, int t, int hi, int lo, int sinks) {
+__device__ __forceinline__ int page16(const AttnArgs &p, const int *table, int t, int hi) {
+    return t <= hi ? sload(table, t >> p.page_log2) : 0;
+}
+__device__ __forceinline__ Piece16 piece16(const AttnArgs &p, int page, int head, int t, int hi, int lo, int sinks) {
     Piece16 s;
     int cnt = hi + 1 - t;
     cnt = cnt < 0 ? 0 : cnt > 16 ? 16 : cnt;
     s.ha = sinks - t < 0 ? 0 : sinks - t;
     s.hb = lo - t > 16 ? 16 : lo - t;
     if (s.ha == 0 && s.hb >= 16) cnt = 0;
-    int64_t page = 0;
-    if (cnt > 0) page = sload(table, t >> p.page_log2);
-    if ((uint64_t)page >= (uint64_t)p.npages) {
+    if ((uint32_t)page >= (uint32_t)p.npages) {
         page = 0;
         cnt = 0;
     }
-    const int64_t off = uni64(page * p.page_bytes + (int64_t)head * p.head_bytes + (int64_t)((t & ((1 << p.page_log2) - 1)) * p.dim * 2));
+    const int64_t off = uni64((int64_t)page * p.page_bytes + (int64_t)head * p.head_bytes + (int64_t)((t & ((1 << p.page_log2) - 1)) * p.dim * 2));
     const uint32_t bytes = (uint32_t)uni(cnt * p.dim * 2);
     s.k = dma_desc(p.k + off, bytes);
     s.v = dma_desc(p.v + off, bytes);
@@ -489,7 +490,7 @@ template <int DP, bool BF, bool TWO> __device__ __forceinline__ void values(a16f
 #pragma unroll
         for (int d = 0; d < DP / 32; d++) {
             const uint32_t at = (a ^ (d << 6)) + b * 32 * DP;
-            const uint2 x = lds_tr(at), y = lds_tr((at ^ 16) + 16 * DP);
+            const uint2 x = lds_tr(at), y = lds_tr((at ^ 32) + 16 * DP);
             const uint4 vt = make_uint4(x.x, x.y, y.x, y.y);
             o[d] = mma<BF>(vt, ph, o[d]);
             if (TWO) o[d] = mma<BF>(vt, make_uint4(lo[0], lo[1], lo[2], lo[3]), o[d]);
@@ -646,6 +647,7 @@ __device__ __forceinline__ bool last_piece(const AttnArgs &p, const Item &it, in
 }  // namespace
 
 // attn_rows.hip: rows of a tile and keys of a block, and the launch.
+int attn_rows_per_cu(int dp);
 int attn_rows_tile(int dp);
 int attn_rows_block(int dp);
 int launch_attn_rows(trhip_ctx *ctx, const AttnArgs &p, int dp, bool bf, bool prefix, int64_t grid);

@@ -20,14 +20,16 @@ namespace {
 
 constexpr int kFewKeys = 128;
 
+template <int V> struct Const {
+    static constexpr int value = V;
+};
+
 template <int DP> struct RowsShape {
     static constexpr int WAVES = DP == 256 ? 4 : 8, BK = DP == 256 ? 32 : 64, NT = BK / 32;  // two waves a SIMD where the registers allow
     static constexpr int THREADS = 64 * WAVES, TR = 32 * WAVES;
     static constexpr int TILE = BK * DP * 2;       // bytes of a block's keys or values
-    static constexpr int SLOTS = 3;                // blocks of each in LDS
     static constexpr int PI = DP / 64;             // copies a wave makes of a block: eight rows
-    static constexpr int ZERO = 2 * SLOTS * TILE;  // a block of zeros behind the rings
-    static constexpr int BYTES = ZERO + TILE + 16;
+    static constexpr int BYTES = 4 * TILE + 16;  // two blocks of each are in LDS
 };
 
 // A wave's share of a block: eight rows of a sixteen-row piece, from row `r0` of it.
@@ -44,13 +46,14 @@ template <int DP> struct Share {
             voff[i] = 8 * c < dim ? (uint32_t)(r * dim * 2 + c * 16) : 0x80000000u;
         }
     }
+    __device__ __forceinline__ void copy_one(dma_rsrc d, uint32_t dst, int i, int ha, int hb) const {
+        uint32_t o = voff[i];
+        if (hb > ha) o = (uint32_t)(row + i * RPI - ha) < (uint32_t)(hb - ha) ? 0x80000000u : o;
+        dma16(d, dst + i * 1024, o, 0);
+    }
     __device__ __forceinline__ void copy(dma_rsrc d, uint32_t dst, int ha, int hb) const {
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            uint32_t o = voff[i];
-            if (hb > ha) o = (uint32_t)(row + i * RPI - ha) < (uint32_t)(hb - ha) ? 0x80000000u : o;
-            dma16(d, dst + i * 1024, o, 0);
-        }
+        for (int i = 0; i < N; i++) copy_one(d, dst, i, ha, hb);
     }
 };
 
@@ -97,17 +100,21 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::WAVES / 4) v
     Share<DP> share;
     share.init(p.dim, 8 * (w & 1));
     const int prow = 16 * (w >> 1);  // its piece's first row in a block
-    for (int i = tid; i < L::TILE / 16; i += L::THREADS) smem[L::ZERO / 16 + i] = make_uint4(0, 0, 0, 0);
 
     uint4 q[DP / 16];
     load_q<DP>(p, q, it.q0, wn > 0 ? r0 + wr : r0, wn, it.head);
     auto key_of = [&](int j) { return BK * sp.block(b0 + j); };
-    auto piece_of = [&](int j) {  // past the last block: zeros
-        return piece16(p, table, it.head, (j < nb ? key_of(j) : 0) + prow, j < nb ? all.hi_max : -1, all.lo_min, all.sinks);
+    // Block j's piece of this wave; past the last block: zeros. The page's number is fetched a step before it is used.
+    auto page_of = [&](int j) { return j < nb ? page16(p, table, key_of(j) + prow, all.hi_max) : 0; };
+    auto piece_of = [&](int j, int page) {
+        return piece16(p, page, it.head, (j < nb ? key_of(j) : 0) + prow, j < nb ? all.hi_max : -1, all.lo_min, all.sinks);
     };
-    const uint32_t dst = ring + w * (16 * DP);
-    auto copy_k = [&](const Piece16 &s, int slot) { share.copy(s.k, dst + slot * L::TILE, s.ha, s.hb); };
-    auto copy_v = [&](const Piece16 &s, int slot) { share.copy(s.v, dst + (L::SLOTS + slot) * L::TILE, s.ha, s.hb); };
+    // block j's places: keys at k_at, values at v_at
+    auto k_at = [&](int j) { return ring + (j & 1) * L::TILE; };
+    auto v_at = [&](int j) { return ring + (2 + (j & 1)) * L::TILE; };
+    const uint32_t mine = w * (16 * DP);
+    auto copy_k = [&](const Piece16 &c, int j) { share.copy(c.k, k_at(j) + mine, c.ha, c.hb); };
+    auto copy_v = [&](const Piece16 &c, int j) { share.copy(c.v, v_at(j) + mine, c.ha, c.hb); };
 
     a16f o[DP / 32], s[NT];
     uint32_t pk[NT][8];  // weights of the block before, two a register, in the order of its score registers
@@ -133,47 +140,47 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::WAVES / 4) v
             for (int i = 0; i < 16; i++) m = fmaxf(m, x[t][i]);
         return m;
     };
-    auto k_frag = [&](uint32_t base, int i) { return lds16(base + (ka ^ ((i % NK) << 5)) + (i / NK) * 64 * DP); };
-    auto v_frag = [&](uint32_t base, int i) {
+    auto k_frag = [&](uint32_t at, int i) { return lds16(ring + (ka ^ ((i / NT) << 5)) + (at + (i % NT) * 64 * DP)); };  // the NT sums in turn
+    auto v_frag = [&](uint32_t at, int i) {
         const int d = i % (DP / 32), c = i / (DP / 32);  // dimensions 32 d ..., keys 16 c ...
-        const uint2 x = lds_tr(base + (va ^ (d << 6)) + c * 32 * DP), y = lds_tr(base + (va ^ (d << 6) ^ 16) + c * 32 * DP + 16 * DP);
+        const uint2 x = lds_tr(ring + (va ^ (d << 6)) + (at + c * 32 * DP)), y = lds_tr(ring + (va ^ (d << 6) ^ 32) + (at + c * 32 * DP + 16 * DP));
         return make_uint4(x.x, x.y, y.x, y.y);
     };
     auto p_frag = [&](const uint32_t (&x)[NT][8], int i) {
         const int c = i / (DP / 32), t = c / 2, e = 4 * (c & 1);
         return make_uint4(x[t][e], x[t][e + 1], x[t][e + 2], x[t][e + 3]);
     };
-    // Raises the reference to a block's maxima where they exceed it by more than 2^8; returns minus the reference for the
-    // exponentials' fused step (0 where scores x were too large for it and have been made relative here).
-    auto refer = [&](a16f (&x)[NT], bool weights) -> float {
-        top = half_max(top);
-        if (__any(top * p.scale > ms + 8.0f)) {
-            const float y = top * p.scale, r = fabsf(y) > 1048576.0f ? y : ceilf(y);
-            const bool up = r > ms + 8.0f;
-            const float a = up ? exp2_hw(ms - r) : 1.0f;  // from -Inf: 0
-            ms = up ? r : ms;
-            mf = up ? top : mf;
-            l *= a;
+    // The reference: raised to a block's maximum where that exceeds it by more than 2^8. neg: minus the reference, for the
+    // exponentials' fused step; 0 where scores are too large for that (far) and are made relative first.
+    float neg = 0.0f;
+    bool far = false;
+    auto raise = [&](uint32_t (&pk)[NT][8], bool weights) {
+        const float y = top * p.scale, r = fabsf(y) > 1048576.0f ? y : ceilf(y);
+        const bool up = r > ms + 8.0f;
+        const float a = up ? exp2_hw(ms - r) : 1.0f;  // from -Inf: 0
+        ms = up ? r : ms;
+        mf = up ? top : mf;
+        l *= a;
 #pragma unroll
-            for (int d = 0; d < DP / 32; d++)
+        for (int d = 0; d < DP / 32; d++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) o[d][i] *= a;
-            if (weights) {
+            for (int i = 0; i < 16; i++) o[d][i] *= a;
+        if (weights) {
 #pragma unroll
-                for (int t = 0; t < NT; t++)
+            for (int t = 0; t < NT; t++)
 #pragma unroll
-                    for (int i = 0; i < 8; i++) pk[t][i] = pack2<BF>(wide_lo<BF>(pk[t][i]) * a, wide_hi<BF>(pk[t][i]) * a);
-            }
+                for (int i = 0; i < 8; i++) pk[t][i] = pack2<BF>(wide_lo<BF>(pk[t][i]) * a, wide_hi<BF>(pk[t][i]) * a);
         }
-        const float neg = ms == -__builtin_inff() ? 0.0f : -ms;
-        const bool far = fabsf(neg) > 1048576.0f;
+        far = fabsf(ms) > 1048576.0f && ms != -__builtin_inff();
+        neg = far || ms == -__builtin_inff() ? 0.0f : -ms;
+    };
+    auto relative = [&](a16f (&x)[NT]) {
         if (__any(far)) {
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) x[t][i] -= far ? mf : 0.0f;
         }
-        return far ? 0.0f : neg;
     };
 
     // Blocks [f0, f1) are seen whole by every row of the tile.
@@ -181,41 +188,34 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::WAVES / 4) v
     int f0 = at0 + (all.lo_max + BK - 1) / BK, f1 = at0 + (all.hi_min + 1) / BK;
     f0 = f0 < 0 ? 0 : f0;
     f1 = f1 > nb ? nb : f1;
+    f0 += f0 & 1;  // pairs of blocks, the first even: places in LDS are constants in the loop
+    f1 -= (f1 - f0) & 1;
     if (f1 < f0 + 2 || all.hi_min + 1 < kFewKeys || (p.window > 0 && p.window < kFewKeys)) f0 = f1 = nb;
 
-    // Copies run ahead of step j by K of block j + 3 and V of block j + 1.
-    Piece16 c1 = piece_of(1), c2 = piece_of(2);
-    {
-        const Piece16 c0 = piece_of(0);
-        copy_k(c0, 0);
-        copy_k(c1, 1);
-        copy_k(c2, 2);
-        copy_v(c0, 0);
-    }
-    int k0 = 0;  // ring place of block j, keys and values
-    auto next = [&](int k) { return k + 1 == L::SLOTS ? 0 : k + 1; };
-    auto ahead = [&](int j) {
-        const Piece16 c3 = piece_of(j + 3);
-        copy_v(c1, next(k0));
-        copy_k(c3, k0);
-        c1 = c2, c2 = c3;
+    auto qk = [&](a16f (&x)[NT], int place) {
+#pragma unroll
+        for (int i = 0; i < NT * NK; i++) x[i % NT] = mma<BF>(k_frag(place * L::TILE, i), q[i / NT], i < NT ? a16f{} : x[i % NT]);
     };
     auto plain = [&](int j) {
+        const int page = page_of(j + 1);
         wait_vmcnt(0);
-        lds_barrier();
-        const uint32_t kat = ring + k0 * L::TILE, vat = ring + (L::SLOTS + k0) * L::TILE;
-#pragma unroll
-        for (int i = 0; i < NT * NK; i++) s[i / NK] = mma<BF>(k_frag(kat, i), q[i % NK], i % NK == 0 ? a16f{} : s[i / NK]);
-        lds_barrier();  // the keys have been read
-        ahead(j);
+        lds_barrier();  // block j is there, and block j - 1 has been read
+        {
+            const Piece16 c = piece_of(j + 1, page);
+            copy_k(c, j + 1);
+            copy_v(c, j + 1);
+        }
+        qk(s, j & 1);
+        const uint32_t vat = v_at(j);
         const int t0 = key_of(j);
         const bool see = all_see(rw, t0, BK);
         if (!see) {
 #pragma unroll
             for (int t = 0; t < NT; t++) mask(s[t], rw, t0 + 32 * t);
         }
-        top = maximum(s);
-        const float neg = refer(s, false);
+        top = half_max(maximum(s));
+        if (__any(top * p.scale > ms + 8.0f)) raise(pk, false);
+        relative(s);
         bool odd = false;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
@@ -231,63 +231,86 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::WAVES / 4) v
             if (odd) values_one_by_one<DP, BF>(o, s[t], vat + t * 64 * DP, rw.hi, rw.lo, rw.sinks, t0 + 32 * t);
             else values<DP, BF, true>(o, s[t], vat + t * 64 * DP);
         }
-        k0 = next(k0);
     };
+    {
+        const Piece16 c = piece_of(0, page_of(0));
+        copy_k(c, 0);
+        copy_v(c, 0);
+    }
     int j = 0;
     for (; j < f0; j++) plain(j);
     if (j < f1) {
-        wait_vmcnt(2 * L::PI);
+        Piece16 c0 = piece_of(j, page_of(j)), c1 = piece_of(j + 1, page_of(j + 1));
+        int page2 = page_of(j + 2);
+        wait_vmcnt(0);
         lds_barrier();
-        {
-            const uint32_t kat = ring + k0 * L::TILE;
-#pragma unroll
-            for (int i = 0; i < NT * NK; i++) s[i / NK] = mma<BF>(k_frag(kat, i), q[i % NK], i % NK == 0 ? a16f{} : s[i / NK]);
-        }
-        top = maximum(s);
-        uint32_t vat = ring + L::ZERO;  // V of block j - 1
-        for (; j < f1; j++) {
-            wait_vmcnt(2 * L::PI);
-            lds_barrier();  // keys of block j + 1 and values of j - 1 are there, and what the next copies replace has been read
-            ahead(j);
-            const uint32_t kat = ring + next(k0) * L::TILE;
-            const float neg = refer(s, true);
-            // three independent runs, dealt over one another: products with K, exponentials, products with V
-            a16f sn[NT];
-            uint32_t pn[NT][8];
-            float sum = 0.0f;
+        // no weights are pending: zeros in the place of block j - 1's values
+        for (int i = tid; i < L::TILE / 16; i += L::THREADS) smem[3 * L::TILE / 16 + i] = make_uint4(0, 0, 0, 0);
+        copy_k(c1, 1);
+        qk(s, 0);
+        top = half_max(maximum(s));
+        bool higher = top * p.scale > ms + 8.0f;
+        a16f s1[NT];
+        uint32_t p1[NT][8];
+        // Step j, P = j % 2: scores x, weights y of block j - 1; leaves the next scores in xn, this block's weights in yn.
+        auto step = [&](auto P, a16f (&x)[NT], a16f (&xn)[NT], uint32_t (&y)[NT][8], uint32_t (&yn)[NT][8]) {
+            constexpr int here = decltype(P)::value, there = 1 - here;
+            const int page3 = page_of(j + 3);
+            wait_vmcnt(0);
+            lds_barrier();  // keys of block j + 1 and values of j - 1 are there; keys of j and values of j - 2 have been read
+            if (__any(higher)) raise(y, true);
+            relative(x);
+            // three independent runs, dealt over one another: products with K, exponentials, products with V; between
+            // them the copies of keys j + 2 and values j, and behind the first the next scores' maximum
+            const Piece16 c2 = piece_of(j + 2, page2);
+            float sum = 0.0f, best = 0.0f;
             constexpr int M = NT * (NK + NV), NW = 8 * NT, AHEAD = 3;  // products, pairs of weights, operands read ahead
             uint4 f[AHEAD + 1];
-            auto frag = [&](int i) { return i < NT * NK ? k_frag(kat, i) : v_frag(vat, i - NT * NK); };
+            auto frag = [&](int i) { return i < NT * NK ? k_frag(there * L::TILE, i) : v_frag((2 + there) * L::TILE, i - NT * NK); };
 #pragma unroll
             for (int i = 0; i < AHEAD; i++) f[i] = frag(i);
 #pragma unroll
             for (int i = 0; i < M; i++) {
                 if (i + AHEAD < M) f[(i + AHEAD) % (AHEAD + 1)] = frag(i + AHEAD);
                 const uint4 a = f[i % (AHEAD + 1)];
-                if (i < NT * NK) sn[i / NK] = mma<BF>(a, q[i % NK], i % NK == 0 ? a16f{} : sn[i / NK]);
-                else o[(i - NT * NK) % (DP / 32)] = mma<BF>(a, p_frag(pk, i - NT * NK), o[(i - NT * NK) % (DP / 32)]);
+                if (i < NT * NK) xn[i % NT] = mma<BF>(a, q[i / NT], i < NT ? a16f{} : xn[i % NT]);
+                else o[(i - NT * NK) % (DP / 32)] = mma<BF>(a, p_frag(y, i - NT * NK), o[(i - NT * NK) % (DP / 32)]);
+                if (i % 2 == 0 && i / 2 < L::PI) share.copy_one(c2.k, ring + here * L::TILE + mine, i / 2, c2.ha, c2.hb);
+                if (i % 2 == 0 && i / 2 >= L::PI && i / 2 < 2 * L::PI) share.copy_one(c0.v, ring + (2 + here) * L::TILE + mine, i / 2 - L::PI, c0.ha, c0.hb);
 #pragma unroll
                 for (int e = i * NW / M; e < (i + 1) * NW / M; e++) {
                     const int t = e >> 3, k = e & 7;
-                    pn[t][k] = pack2<BF>(exp2_hw(fmaf(s[t][2 * k], p.scale, neg)), exp2_hw(fmaf(s[t][2 * k + 1], p.scale, neg)));
-                    sum = add2<BF>(pn[t][k], sum);  // of the rounded weights
+                    const float u = exp2_hw(fmaf(x[t][2 * k], p.scale, neg)), v = exp2_hw(fmaf(x[t][2 * k + 1], p.scale, neg));
+                    yn[t][k] = opaque(pack2<BF>(u, v));  // (made here: the compiler would move it to the next step, where it is used)
+                    sum += u;
+                    sum += v;
+                }
+                const int m0 = NT * NK + 2, m1 = M - 2;  // maxima of pairs [from, to)
+                if (i >= m0 && i < m1) {
+#pragma unroll
+                    for (int e = (i - m0) * 8 * NT / (m1 - m0); e < (i - m0 + 1) * 8 * NT / (m1 - m0); e++) {
+                        const float u = xn[e / 8][2 * (e % 8)], v = xn[e / 8][2 * (e % 8) + 1];
+                        best = e == 0 ? fmaxf(u, v) : fmaxf(fmaxf(best, u), v);
+                    }
+                }
+                if (i == M - 2) {
+                    top = half_max(best);
+                    higher = top * p.scale > ms + 8.0f;
                 }
             }
             l += sum;
-            top = maximum(sn);
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                s[t] = sn[t];
-#pragma unroll
-                for (int i = 0; i < 8; i++) pk[t][i] = pn[t][i];
-            }
-            vat = ring + (L::SLOTS + k0) * L::TILE;
-            k0 = next(k0);
+            c0 = c1, c1 = c2, page2 = page3;
+            j++;
+        };
+        while (j < f1) {
+            step(Const<0>{}, s, s1, pk, p1);
+            step(Const<1>{}, s1, s, p1, pk);
         }
         wait_vmcnt(0);
         lds_barrier();
+        copy_v(c0, 0);
 #pragma unroll
-        for (int i = 0; i < NT * NV; i++) o[i % (DP / 32)] = mma<BF>(v_frag(vat, i), p_frag(pk, i), o[i % (DP / 32)]);
+        for (int i = 0; i < NT * NV; i++) o[i % (DP / 32)] = mma<BF>(v_frag(3 * L::TILE, i), p_frag(pk, i), o[i % (DP / 32)]);
     }
     for (; j < nb; j++) plain(j);
     wait_vmcnt(0);
@@ -322,7 +345,7 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::WAVES / 4) v
         }
     }
     if (direct || PREFIX) return;
-    if (last_piece(p, it, reinterpret_cast<int *>(smem) + (L::BYTES - 16) / 4)) join_tile<DP, L::TR, BF>(p, it, r0, n, L::THREADS);
+    if (last_piece(p, it, reinterpret_cast<int *>(smem) + 4 * L::TILE / 4)) join_tile<DP, L::TR, BF>(p, it, r0, n, L::THREADS);
 }
 
 template <int DP, bool BF, bool PREFIX> int launch_rows(trhip_ctx *ctx, const AttnArgs &p, int64_t grid) {
@@ -335,6 +358,7 @@ template <int DP, bool BF, bool PREFIX> int launch_rows(trhip_ctx *ctx, const At
 
 }  // namespace
 
+int attn_rows_per_cu(int dp) { return 1; }
 int attn_rows_tile(int dp) { return dp == 256 ? RowsShape<256>::TR : RowsShape<128>::TR; }
 int attn_rows_block(int dp) { return dp == 256 ? RowsShape<256>::BK : RowsShape<128>::BK; }
 
