@@ -25,16 +25,18 @@ template <int V> struct Const {
 };
 
 template <int DP> struct RowsShape {
-    static constexpr int WAVES = DP == 256 ? 4 : 8, BK = DP == 256 ? 32 : 64, NT = BK / 32;  // two waves a SIMD where the registers allow
+    static constexpr int WAVES = 4, BK = DP == 256 ? 32 : 64, NT = BK / 32;
+    static constexpr int PER_CU = DP == 256 ? 1 : 2;  // workgroups a CU: by registers
+    static constexpr int SHARE = BK / WAVES;          // rows of a block that a wave copies
     static constexpr int THREADS = 64 * WAVES, TR = 32 * WAVES;
     static constexpr int TILE = BK * DP * 2;       // bytes of a block's keys or values
-    static constexpr int PI = DP / 64;             // copies a wave makes of a block: eight rows
+    static constexpr int PI = SHARE * DP / 512;    // copies a wave makes of a block
     static constexpr int BYTES = 4 * TILE + 16;  // two blocks of each are in LDS
 };
 
-// A wave's share of a block: eight rows of a sixteen-row piece, from row `r0` of it.
+// A wave's share of a block: rows of a sixteen-row piece, from row `r0` of it.
 template <int DP> struct Share {
-    static constexpr int N = DP / 64, CH = DP / 8, RPI = 64 / CH;
+    static constexpr int N = RowsShape<DP>::PI, CH = DP / 8, RPI = 64 / CH;
     uint32_t voff[N];
     int row;
     __device__ __forceinline__ void init(int dim, int r0) {
@@ -58,7 +60,7 @@ template <int DP> struct Share {
 };
 
 template <int DP, bool BF, bool PREFIX>
-__global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::WAVES / 4) void attn_rows(const AttnArgs p) {
+__global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::PER_CU) void attn_rows(const AttnArgs p) {
     using L = RowsShape<DP>;
     constexpr int BK = L::BK, NT = L::NT;
     extern __shared__ __attribute__((aligned(1024))) uint4 smem[];
@@ -98,8 +100,8 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::WAVES / 4) v
 
     const uint32_t ring = lds_addr(smem);
     Share<DP> share;
-    share.init(p.dim, 8 * (w & 1));
-    const int prow = 16 * (w >> 1);  // its piece's first row in a block
+    share.init(p.dim, L::SHARE == 16 ? 0 : 8 * (w & 1));
+    const int prow = L::SHARE == 16 ? 16 * w : 16 * (w >> 1);  // its piece's first row in a block
 
     uint4 q[DP / 16];
     load_q<DP>(p, q, it.q0, wn > 0 ? r0 + wr : r0, wn, it.head);
@@ -112,7 +114,7 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::WAVES / 4) v
     // block j's places: keys at k_at, values at v_at
     auto k_at = [&](int j) { return ring + (j & 1) * L::TILE; };
     auto v_at = [&](int j) { return ring + (2 + (j & 1)) * L::TILE; };
-    const uint32_t mine = w * (16 * DP);
+    const uint32_t mine = w * (L::SHARE * 2 * DP);
     auto copy_k = [&](const Piece16 &c, int j) { share.copy(c.k, k_at(j) + mine, c.ha, c.hb); };
     auto copy_v = [&](const Piece16 &c, int j) { share.copy(c.v, v_at(j) + mine, c.ha, c.hb); };
 
@@ -358,7 +360,7 @@ template <int DP, bool BF, bool PREFIX> int launch_rows(trhip_ctx *ctx, const At
 
 }  // namespace
 
-int attn_rows_per_cu(int dp) { return 1; }
+int attn_rows_per_cu(int dp) { return dp == 256 ? RowsShape<256>::PER_CU : RowsShape<128>::PER_CU; }
 int attn_rows_tile(int dp) { return dp == 256 ? RowsShape<256>::TR : RowsShape<128>::TR; }
 int attn_rows_block(int dp) { return dp == 256 ? RowsShape<256>::BK : RowsShape<128>::BK; }
 
