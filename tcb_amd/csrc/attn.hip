@@ -44,7 +44,9 @@ template <int DP, bool BF, bool PREFIX> __global__ __launch_bounds__(64 * kTokWa
         table = p.prefix_table;
         keys = p.prefix_len;
     } else {
-        if (!find_item<kTokRows, kTokBlock, kTokWaves, kTokOver>(p, wg, it)) return;
+        const bool some = find_item<kTokRows, kTokBlock, kTokWaves, kTokOver>(p, wg, it);
+        leave_count(p, it);
+        if (!some) return;
         table = p.table + (int64_t)it.req * p.max_pages;
         keys = it.kv;
     }
@@ -151,7 +153,57 @@ template <int DP, bool BF, bool PREFIX> __global__ __launch_bounds__(64 * kTokWa
         }
     }
     if (direct || PREFIX) return;
-    if (last_piece(p, it, reinterpret_cast<int *>(ml + kTokWaves * 32))) join_tile<DP, kTokRows, BF>(p, it, r0, n, 64 * kTokWaves);
+    if (p.parts) {
+        leave_place(p, it, r0, n);
+        return;
+    }
+    if (last_piece(p, it, reinterpret_cast<int *>(ml + kTokWaves * 32)))
+        join_tile<DP, kTokRows, BF, kTokWaves>(p, it, r0, n, reinterpret_cast<float *>(smem), kTokWaves * L::WAVE);
+}
+
+// Joins the pieces of a tile's rows, and the shared prefix's: a workgroup for sixteen rows of a place (workgroups of
+// places that hold no tile's first piece end at once).
+template <int DP, bool BF> __global__ __launch_bounds__(256) void attn_join(const AttnArgs p, int tr) {
+    constexpr int ST = DP + 2, AT = 8;
+    if ((int)blockIdx.x >= p.parts[0]) return;
+    const Place t = reinterpret_cast<const Place *>(p.parts + 8)[blockIdx.x];
+    const int g = 16 * blockIdx.y, rows = t.n - g < 16 ? t.n - g : 16;
+    if (t.pieces == 0 || rows <= 0) return;
+    const int64_t step = (int64_t)p.kv_heads * tr * ST, pstep = (int64_t)p.tokens * p.heads * ST;
+    for (int idx = threadIdx.x; idx < rows * (DP / 4); idx += 256) {
+        const int r = idx / (DP / 4), d = (idx - r * (DP / 4)) * 4, row = t.r0 + g + r, tok = row / p.group;
+        if (d >= p.dim) continue;
+        const float *x = p.part + ((int64_t)blockIdx.x * tr + g + r) * ST;
+        const float *pre = p.prefix_part + ((int64_t)(t.q0 + tok) * p.heads + t.head * p.group + (row - tok * p.group)) * ST;
+        Join j;
+        j.init();
+        const int all = t.pieces + p.prefix_splits;
+        for (int s0 = 0; s0 < all; s0 += AT) {
+            float2 a[AT], b[AT], ml[AT];
+#pragma unroll
+            for (int u = 0; u < AT; u++) {
+                const int s = s0 + u < all ? s0 + u : s0;
+                const float *y = s < t.pieces ? x + s * step : pre + (s - t.pieces) * pstep;
+                a[u] = *reinterpret_cast<const float2 *>(y + d);
+                b[u] = *reinterpret_cast<const float2 *>(y + d + 2);
+                ml[u] = *reinterpret_cast<const float2 *>(y + DP);
+            }
+#pragma unroll
+            for (int u = 0; u < AT; u++)
+                if (s0 + u < all) j.add(ml[u].x, ml[u].y, a[u].x, a[u].y, b[u].x, b[u].y);
+        }
+        put4<BF>(p, t.q0, row, t.head, d, j.o, j.l, p.prefix_splits > 0 || t.kv - t.nq + tok >= 0);
+    }
+}
+
+template <int DP, bool BF> int launch_join(trhip_ctx *ctx, const AttnArgs &p, int tr) {
+    hipLaunchKernelGGL((attn_join<DP, BF>), dim3((unsigned)p.part_slots, (unsigned)(tr / 16)), dim3(256), 0, ctx->stream, p, tr);
+    return launch_check(ctx, "attention");
+}
+int launch_join(trhip_ctx *ctx, const AttnArgs &p, int dp, bool bf, int tr) {
+    if (dp == 64) return bf ? launch_join<64, true>(ctx, p, tr) : launch_join<64, false>(ctx, p, tr);
+    if (dp == 128) return bf ? launch_join<128, true>(ctx, p, tr) : launch_join<128, false>(ctx, p, tr);
+    return bf ? launch_join<256, true>(ctx, p, tr) : launch_join<256, false>(ctx, p, tr);
 }
 
 template <int DP, bool BF, bool PREFIX> int launch_tokens(trhip_ctx *ctx, const AttnArgs &p, int64_t grid) {
@@ -169,16 +221,20 @@ template <bool PREFIX> int launch_tokens(trhip_ctx *ctx, const AttnArgs &p, int 
     return bf ? launch_tokens<256, true, PREFIX>(ctx, p, grid) : launch_tokens<256, false, PREFIX>(ctx, p, grid);
 }
 
-// The launch's workgroups: as many items as a batch of these sizes can have (find_item), whatever its lengths are.
-int64_t plan_items(AttnArgs &p, const AttnCall &c, int tile_rows, int block, int least) {
+// Tiles of a batch of these sizes, at most.
+int64_t tiles_of(const AttnArgs &p, const AttnCall &c, int tile_rows) {
     int64_t tiles = c.tokens * p.group / tile_rows + c.nreq;
     if (p.row_hi <= tile_rows && tiles > c.nreq) tiles = c.nreq;
-    tiles *= p.kv_heads;
+    return tiles * p.kv_heads;
+}
+
+// The launch's workgroups: as many items as a batch of these sizes can have (find_item), whatever its lengths are.
+int64_t plan_items(AttnArgs &p, const AttnCall &c, int tile_rows, int block, int least) {
+    const int64_t tiles = tiles_of(p, c, tile_rows);
     const int64_t blocks = ((c.max_pages << p.page_log2) + block - 1) / block, most = tiles * ((blocks + least - 1) / least + 1);
     int64_t k = (2 * tiles + p.target - 1) / p.target;
     p.rounds = (int)(k < kMostRounds ? k : kMostRounds);
     p.part_slots = p.rounds * p.target;
-    if (tiles > trhip_ctx::kArrivalSlots && c.prefix_len > 0) p.rounds = 0;  // behind a prefix every tile has a place: too many for counters
     int64_t items = p.part_slots < most ? p.part_slots : most;
     if (tiles > items) items = tiles;
     if (c.prefix_len > 0) p.part_slots = (int)items;
@@ -236,24 +292,31 @@ int launch_attn(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c) {
     const int tr = attn_rows_tile(dp), br = attn_rows_block(dp);
     const int64_t grid_t = plan_items(pt, c, kTokRows, kTokBlock, kTokWaves), grid_r = plan_items(pr, c, tr, br, 4);
     if (grid_t >= ((int64_t)1 << 31) || grid_r >= ((int64_t)1 << 31)) return fail(ctx, TRHIP_ERR_INVALID, "attention: too many rows");
+    const bool prefix = c.prefix_len > 0;
+    // Pieces of long tiles are joined by a launch of their own (a workgroup that joined a tile of 128 rows alone would take
+    // longer than the pieces); there are none where the tiles fill the device by themselves. A token's few rows are joined
+    // by the last workgroup of their tile, in the same launch, except behind a prefix.
+    const bool cut = !tokens_alone && (prefix || tiles_of(pr, c, tr) < pr.target);
+    if (!cut) pr.rounds = pr.part_slots = 0;
     const int64_t part_t = rows_alone ? 0 : (int64_t)pt.part_slots * kTokRows, part_r = tokens_alone ? 0 : (int64_t)pr.part_slots * tr;
     const int64_t part = (part_t > part_r ? part_t : part_r) * (dp + 2);
+    const int64_t places = 8 + 8 * (int64_t)(pt.part_slots > pr.part_slots ? pt.part_slots : pr.part_slots);
     // the prefix: all tokens' rows are one tall product, its keys cut to fill the device
     const bool tall = rows > kTokRows;
     const int ptr = tall ? tr : kTokRows, pbk = tall ? br : kTokBlock;
     const int64_t ptiles = (rows + ptr - 1) / ptr;
     int splits = 0;
-    if (c.prefix_len > 0) {
+    if (prefix) {
         const int64_t nb = (c.prefix_len + pbk - 1) / pbk, items = ptiles * p.kv_heads;
         const int64_t piece = piece_blocks(items * nb, items, (int)nb, tall ? pr.target : pt.target, kMostRounds, 4, tall ? kRowsOver : kTokOver);
         splits = piece >= nb ? 1 : (int)((nb + piece - 1) / piece);
     }
     int st = TRHIP_OK;
-    float *ws = static_cast<float *>(workspace(ctx, (size_t)(part + (int64_t)splits * c.tokens * c.heads * (dp + 2)) * sizeof(float), &st));
+    float *ws = static_cast<float *>(workspace(ctx, (size_t)(places + part + (int64_t)splits * c.tokens * c.heads * (dp + 2)) * sizeof(float), &st));
     if (!ws) return st;
     for (AttnArgs *a : {&pt, &pr}) {
-        a->part = ws;
-        a->prefix_part = ws + part;
+        a->part = ws + places;
+        a->prefix_part = ws + places + part;
         a->prefix_splits = splits;
     }
     if (splits > 0) {
@@ -261,8 +324,17 @@ int launch_attn(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c) {
         st = tall ? launch_attn_rows(ctx, pr, dp, bf, true, grid) : launch_tokens<true>(ctx, pt, dp, bf, grid);
         if (st != TRHIP_OK) return st;
     }
-    if (!rows_alone) st = launch_tokens<false>(ctx, pt, dp, bf, grid_t);
-    if (st == TRHIP_OK && !tokens_alone) st = launch_attn_rows(ctx, pr, dp, bf, false, grid_r);
+    pt.parts = prefix ? reinterpret_cast<int *>(ws) : nullptr;
+    pr.parts = cut ? reinterpret_cast<int *>(ws) : nullptr;
+    if (!rows_alone) {
+        st = launch_tokens<false>(ctx, pt, dp, bf, grid_t);
+        if (st == TRHIP_OK && prefix) st = launch_join(ctx, pt, dp, bf, kTokRows);
+        if (st != TRHIP_OK) return st;
+    }
+    if (!tokens_alone) {
+        st = launch_attn_rows(ctx, pr, dp, bf, false, grid_r);
+        if (st == TRHIP_OK && cut) st = launch_join(ctx, pr, dp, bf, tr);
+    }
     return st;
 }
 

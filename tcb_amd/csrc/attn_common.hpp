@@ -42,6 +42,7 @@ struct AttnArgs {
     int part_slots;     // places for the pieces of tiles that are cut (of all tiles behind a prefix), each with an arrival counter
     float *part;        // [place][tile row]: DP sums, then reference (log2 units) and sum of each row
     uint32_t *arrivals;
+    int *parts;         // places in use, then for each place what the joining launch needs (Place); nullptr: the last workgroup of a tile joins it
 };
 
 namespace {
@@ -157,11 +158,17 @@ template <int BK> __device__ __forceinline__ Span span_of(int hi, int lo, int si
     return s;
 }
 
+// A place's tile, for the launch that joins its pieces: pieces 0: another place has it.
+struct Place {
+    int pieces, q0, nq, kv, r0, n, head, unused;
+};
+
 struct Item {
     int req, tile, split, nsplit, head;
     int q0, nq, kv;  // the request's first token row, new tokens, keys
     int slot;        // its partial result's place (a tile's pieces are kv_heads apart), if it writes one
     int counter;     // place of the tile's piece 0: its arrival counter
+    int parts;       // places in use by the launch
 };
 
 struct ReqShape {
@@ -231,7 +238,7 @@ __host__ __device__ inline int piece_blocks(int64_t sum, int64_t n, int most, in
 // request's tiles are all cut into the same number of pieces (piece_blocks). Items are numbered head fastest, then piece, tile (the last tokens of a prompt, whose rows read most keys,
 // first), request. False: no item left.
 template <int TR, int BK, int CMIN, int OVER> __device__ __forceinline__ bool find_item(const AttnArgs &p, int wg, Item &it) {
-    it = Item{0, 0, 0, 1, 0, 0, 0, 0, 0, 0};
+    it = Item{0, 0, 0, 1, 0, 0, 0, 0, 0, 0, 0};
     const int lane = threadIdx.x & 63, x = wg / p.kv_heads;
     ReqShape s = shape_of<TR, BK>(p, lane);
     int64_t sum = (int64_t)s.tiles * s.nb, tiles = s.tiles;
@@ -289,8 +296,11 @@ template <int TR, int BK, int CMIN, int OVER> __device__ __forceinline__ bool fi
     }
     it.req = uni(it.req), it.tile = uni(it.tile), it.split = uni(it.split), it.nsplit = uni(it.nsplit), it.head = uni(it.head);
     it.q0 = uni(it.q0), it.nq = uni(it.nq), it.kv = uni(it.kv), it.slot = uni(it.slot), it.counter = uni(it.counter);
+    it.parts = uni(parts) * p.kv_heads;
     // starts that are not in order could name more items than there are workgroups: then nothing is done
-    return found && (int64_t)before * p.kv_heads <= (int64_t)gridDim.x && parts * p.kv_heads <= p.part_slots;
+    const bool fits = (int64_t)before * p.kv_heads <= (int64_t)gridDim.x && (int64_t)parts * p.kv_heads <= p.part_slots;
+    if (!fits) it.parts = 0;
+    return found && fits;
 }
 
 // ---- a tile's rows and masks -------------------------------------------------------------------------------------------
@@ -592,39 +602,63 @@ struct Join {
     }
 };
 
-// Joins nsplit pieces of a row (agent-coherent loads: other workgroups of this launch wrote them) and the prefix's (an earlier launch).
-template <int DP, int TR, bool BF>
-__device__ __forceinline__ void join_tile(const AttnArgs &p, const Item &it, int r0, int n, int threads) {
-    constexpr int ST = DP + 2;
-    for (int idx = threadIdx.x; idx < n * (DP / 4); idx += threads) {
-        const int r = idx / (DP / 4), d = (idx - r * (DP / 4)) * 4, row = r0 + r, t = row / p.group;
-        if (d >= p.dim) continue;
-        Join j;
-        j.init();
-        const float *src = p.part + ((int64_t)it.counter * TR + r) * ST;
-        const int64_t step = (int64_t)p.kv_heads * TR * ST;
-        for (int s0 = 0; s0 < it.nsplit; s0 += 4) {
-            float2 a[4], b[4], ml[4];
+// The last workgroup of a tile joins its pieces (agent-coherent loads: other workgroups of this launch wrote them). The
+// WAVES waves take every WAVES-th piece, eight loads of each in flight, and join their sums in LDS (`room` bytes at `lds`).
+template <int DP, int TR, bool BF, int WAVES>
+__device__ __forceinline__ void join_tile(const AttnArgs &p, const Item &it, int r0, int n, float *lds, int room) {
+    constexpr int ST = DP + 2, AT = 8;
+    const int lane = threadIdx.x & 63, w = uni(threadIdx.x >> 6), items = n * (DP / 4);
+    const int chunk = room / (WAVES * 6 * 4) / 64 * 64;
+    const float *src = p.part + (int64_t)it.counter * TR * ST;
+    const int64_t step = (int64_t)p.kv_heads * TR * ST;
+    for (int c0 = 0; c0 < items; c0 += chunk) {
+        const int cnt = items - c0 < chunk ? items - c0 : chunk;
+        for (int i = lane; i < cnt; i += 64) {
+            const int idx = c0 + i, r = idx / (DP / 4), d = (idx - r * (DP / 4)) * 4;
+            Join j;
+            j.init();
+            const float *x = src + r * ST;
+            for (int s0 = w; s0 < it.nsplit; s0 += AT * WAVES) {
+                float2 a[AT], b[AT], ml[AT];
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const float *x = src + (s0 + u < it.nsplit ? s0 + u : s0) * step;
-                a[u] = agent_load(x + d);
-                b[u] = agent_load(x + d + 2);
-                ml[u] = agent_load(x + DP);
+                for (int u = 0; u < AT; u++) {
+                    const float *y = x + (s0 + u * WAVES < it.nsplit ? s0 + u * WAVES : s0) * step;
+                    a[u] = agent_load(y + d);
+                    b[u] = agent_load(y + d + 2);
+                    ml[u] = agent_load(y + DP);
+                }
+#pragma unroll
+                for (int u = 0; u < AT; u++)
+                    if (s0 + u * WAVES < it.nsplit) j.add(ml[u].x, ml[u].y, a[u].x, a[u].y, b[u].x, b[u].y);
             }
+            float *dst = lds + (w * chunk + i) * 6;
+            dst[0] = j.m, dst[1] = j.l;
 #pragma unroll
-            for (int u = 0; u < 4; u++)
-                if (s0 + u < it.nsplit) j.add(ml[u].x, ml[u].y, a[u].x, a[u].y, b[u].x, b[u].y);
+            for (int k = 0; k < 4; k++) dst[2 + k] = j.o[k];
         }
-        const float *pre = p.prefix_part + ((int64_t)(it.q0 + t) * p.heads + it.head * p.group + (row - t * p.group)) * ST;
-        for (int s = 0; s < p.prefix_splits; s++) {
-            const float *x = pre + (int64_t)s * p.tokens * p.heads * ST;
-            const float2 a = *reinterpret_cast<const float2 *>(x + d), b = *reinterpret_cast<const float2 *>(x + d + 2);
-            const float2 ml = *reinterpret_cast<const float2 *>(x + DP);
-            j.add(ml.x, ml.y, a.x, a.y, b.x, b.y);
+        __syncthreads();
+        for (int i = threadIdx.x; i < cnt; i += 64 * WAVES) {
+            const int idx = c0 + i, r = idx / (DP / 4), d = (idx - r * (DP / 4)) * 4, row = r0 + r;
+            Join j;
+            j.init();
+#pragma unroll
+            for (int u = 0; u < WAVES; u++) {
+                const float *x = lds + (u * chunk + i) * 6;
+                j.add(x[0], x[1], x[2], x[3], x[4], x[5]);
+            }
+            put4<BF>(p, it.q0, row, it.head, d, j.o, j.l, it.kv - it.nq + row / p.group >= 0);
         }
-        put4<BF>(p, it.q0, row, it.head, d, j.o, j.l, p.prefix_splits > 0 || it.kv - it.nq + t >= 0);
+        __syncthreads();
     }
+}
+
+// For the joining launch: this item's place, and (by workgroup 0) how many there are.
+__device__ __forceinline__ void leave_place(const AttnArgs &p, const Item &it, int r0, int n) {
+    if (threadIdx.x == 0)
+        reinterpret_cast<Place *>(p.parts + 8)[it.slot] = Place{it.split == 0 ? it.nsplit : 0, it.q0, it.nq, it.kv, r0, n, it.head, 0};
+}
+__device__ __forceinline__ void leave_count(const AttnArgs &p, const Item &it) {
+    if (p.parts && blockIdx.x == 0 && threadIdx.x == 0) p.parts[0] = it.parts;
 }
 
 // Partial results are written: whether this workgroup is the last of its tile's pieces.
@@ -633,7 +667,6 @@ __device__ __forceinline__ bool last_piece(const AttnArgs &p, const Item &it, in
     __builtin_amdgcn_s_waitcnt(0);  // this thread's stores have completed
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
     __syncthreads();
-    if (it.nsplit == 1) return true;
     if (threadIdx.x == 0) {
         const bool last = __hip_atomic_fetch_add(&p.arrivals[it.counter], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
                           (uint32_t)(it.nsplit - 1);

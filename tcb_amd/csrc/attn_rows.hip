@@ -31,7 +31,7 @@ template <int DP> struct RowsShape {
     static constexpr int THREADS = 64 * WAVES, TR = 32 * WAVES;
     static constexpr int TILE = BK * DP * 2;       // bytes of a block's keys or values
     static constexpr int PI = SHARE * DP / 512;    // copies a wave makes of a block
-    static constexpr int BYTES = 4 * TILE + 16;  // two blocks of each are in LDS
+    static constexpr int BYTES = 4 * TILE;  // two blocks of each are in LDS
 };
 
 // A wave's share of a block: rows of a sixteen-row piece, from row `r0` of it.
@@ -79,7 +79,9 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::PER_CU) void
         table = p.prefix_table;
         keys = p.prefix_len;
     } else {
-        if (!find_item<L::TR, BK, 4, kRowsOver>(p, blockIdx.x, it)) return;
+        const bool some = find_item<L::TR, BK, 4, kRowsOver>(p, blockIdx.x, it);
+        leave_count(p, it);
+        if (!some) return;
         table = p.table + (int64_t)it.req * p.max_pages;
         keys = it.kv;
     }
@@ -333,21 +335,14 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::PER_CU) void
                 const float y[4] = {o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
                 if (direct) {
                     put4<BF>(p, it.q0, row, it.head, at, y, sum, sees);
-                } else if (PREFIX) {
+                } else {
                     *reinterpret_cast<float2 *>(part + at) = make_float2(y[0], y[1]);
                     *reinterpret_cast<float2 *>(part + at + 2) = make_float2(y[2], y[3]);
-                } else {
-                    agent_store(part + at, y[0], y[1]);
-                    agent_store(part + at + 2, y[2], y[3]);
                 }
             }
-        if (!direct && h == 0) {
-            if (PREFIX) *reinterpret_cast<float2 *>(part + DP) = make_float2(ms, sum);
-            else agent_store(part + DP, ms, sum);
-        }
+        if (!direct && h == 0) *reinterpret_cast<float2 *>(part + DP) = make_float2(ms, sum);
     }
-    if (direct || PREFIX) return;
-    if (last_piece(p, it, reinterpret_cast<int *>(smem) + 4 * L::TILE / 4)) join_tile<DP, L::TR, BF>(p, it, r0, n, L::THREADS);
+    if (!direct && !PREFIX) leave_place(p, it, r0, n);
 }
 
 template <int DP, bool BF, bool PREFIX> int launch_rows(trhip_ctx *ctx, const AttnArgs &p, int64_t grid) {
