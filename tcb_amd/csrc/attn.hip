@@ -13,11 +13,11 @@
 namespace trhip {
 namespace {
 
-constexpr int kTokRows = 32, kTokBlock = 32, kTokWaves = 4, kTokOver = 6;
+constexpr int kTokRows = 32, kTokBlock = 32, kTokWaves = 4, kTokLeast = 8, kTokOver = 6;
 
 template <int DP> struct TokLds {
     static constexpr int SLOT = 32 * DP * 2;  // 32 keys or values
-    static constexpr int SLOTS = DP == 64 ? 8 : DP == 128 ? 4 : 2;
+    static constexpr int SLOTS = DP == 64 ? 4 : DP == 128 ? 4 : 2;
     static constexpr int OSTRIDE = DP + 4;  // floats between rows of a wave's results
     static constexpr int RING = SLOT * SLOTS, OUT = 32 * OSTRIDE * 4;
     static constexpr int WAVE = RING > OUT ? RING : OUT;
@@ -44,7 +44,7 @@ template <int DP, bool BF, bool PREFIX> __global__ __launch_bounds__(64 * kTokWa
         table = p.prefix_table;
         keys = p.prefix_len;
     } else {
-        const bool some = find_item<kTokRows, kTokBlock, kTokWaves, kTokOver>(p, wg, it);
+        const bool some = find_item<kTokRows, kTokBlock, kTokLeast, kTokOver>(p, wg, it);
         leave_count(p, it);
         if (!some) return;
         table = p.table + (int64_t)it.req * p.max_pages;
@@ -66,10 +66,15 @@ template <int DP, bool BF, bool PREFIX> __global__ __launch_bounds__(64 * kTokWa
     load_q<DP>(p, q, it.q0, r0, n, it.head);
 
     auto key_of = [&](int b) { return 32 * sp.block(b); };
-    auto pieces = [&](int b, Piece16 (&s)[2]) {  // past the last block: nothing but zeros
+    // Block b's two pages, fetched a step before they are used, and its pieces; past the last block nothing but zeros.
+    auto pages_of = [&](int b) {
         const int t = b < b1 ? key_of(b) : 0, hi = b < b1 ? rw.hi_max : -1;
-#pragma unroll
-        for (int i = 0; i < 2; i++) s[i] = piece16(p, page16(p, table, t + 16 * i, hi), it.head, t + 16 * i, hi, rw.lo_min, rw.sinks);
+        return make_int2(page16(p, table, t, hi), page16(p, table, t + 16, hi));
+    };
+    auto pieces = [&](int b, int2 pages, Piece16 (&s)[2]) {
+        const int t = b < b1 ? key_of(b) : 0, hi = b < b1 ? rw.hi_max : -1;
+        s[0] = piece16(p, pages.x, it.head, t, hi, rw.lo_min, rw.sinks);
+        s[1] = piece16(p, pages.y, it.head, t + 16, hi, rw.lo_min, rw.sinks);
     };
     auto copy_k = [&](const Piece16 (&s)[2], int slot) {
 #pragma unroll
@@ -81,18 +86,23 @@ template <int DP, bool BF, bool PREFIX> __global__ __launch_bounds__(64 * kTokWa
     };
     constexpr int D = L::SLOTS / 2, AHEAD = (L::SLOTS - 1) * (DP / 16);
     Piece16 s[2];
+    int2 pages[D + 1];
+#pragma unroll
+    for (int i = 0; i <= D; i++) pages[i] = pages_of(b0 + w + i * kTokWaves);
 #pragma unroll
     for (int i = 0; i < D; i++) {
-        pieces(b0 + w + i * kTokWaves, s);
+        pieces(b0 + w + i * kTokWaves, pages[i], s);
         copy_k(s, 2 * i);
         copy_v(s, 2 * i + 1);
     }
+    int2 pg = pages[D];
     Acc<DP> A;
     A.init();
     int slot = 0;
     for (int b = b0 + w; b < b1; b += kTokWaves) {
         const int t = key_of(b);
-        pieces(b + D * kTokWaves, s);
+        pieces(b + D * kTokWaves, pg, s);
+        pg = pages_of(b + (D + 1) * kTokWaves);
         wait_vmcnt(AHEAD);
         a16f x[1];
         x[0] = scores<DP, BF>(ring + slot * L::SLOT, q);
@@ -290,7 +300,7 @@ int launch_attn(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c) {
     pr.row_lo = rows_alone ? 0 : kTokRows;
     pr.row_hi = 0x7FFFFFFF;
     const int tr = attn_rows_tile(dp), br = attn_rows_block(dp);
-    const int64_t grid_t = plan_items(pt, c, kTokRows, kTokBlock, kTokWaves), grid_r = plan_items(pr, c, tr, br, 4);
+    const int64_t grid_t = plan_items(pt, c, kTokRows, kTokBlock, kTokLeast), grid_r = plan_items(pr, c, tr, br, 4);
     if (grid_t >= ((int64_t)1 << 31) || grid_r >= ((int64_t)1 << 31)) return fail(ctx, TRHIP_ERR_INVALID, "attention: too many rows");
     const bool prefix = c.prefix_len > 0;
     // Pieces of long tiles are joined by a launch of their own (a workgroup that joined a tile of 128 rows alone would take
@@ -308,7 +318,7 @@ int launch_attn(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c) {
     int splits = 0;
     if (prefix) {
         const int64_t nb = (c.prefix_len + pbk - 1) / pbk, items = ptiles * p.kv_heads;
-        const int64_t piece = piece_blocks(items * nb, items, (int)nb, tall ? pr.target : pt.target, kMostRounds, 4, tall ? kRowsOver : kTokOver);
+        const int64_t piece = piece_blocks((float)items * (float)nb, (int)items, (int)nb, tall ? pr.target : pt.target, kMostRounds, tall ? 4 : kTokLeast, tall ? kRowsOver : kTokOver);
         splits = piece >= nb ? 1 : (int)((nb + piece - 1) / piece);
     }
     int st = TRHIP_OK;

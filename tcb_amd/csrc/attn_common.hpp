@@ -206,32 +206,39 @@ template <int TR, int BK> __device__ __forceinline__ ReqShape shape_of(const Att
 // Never more than rounds * target pieces.
 constexpr int kMostRounds = 6;
 constexpr int kRowsOver = 10;  // attn_rows
-__host__ __device__ inline int piece_blocks(int64_t sum, int64_t n, int most, int target, int rounds, int least, int over) {
+__host__ __device__ inline int piece_blocks(float sum, int n, int most, int target, int rounds, int least, int over) {
     constexpr int kWhole = 0x40000000;
-    const float s = (float)sum, t = (float)target;
-    float best = n <= target ? (float)most : s / t + 0.5f * (float)most;
-    int64_t piece = kWhole;
+    // (sums in floats, made a little larger than they can have been rounded down)
+    const float s = sum * 1.0001f, t = (float)target;
+    float best = n <= target ? (float)most : s / t + 0.5f * (float)most, piece = (float)kWhole;
     if (rounds > 0 && n < target) {
-        int64_t c = (sum + target - n - 1) / (target - n);
-        c = c < least ? least : c;
-        if ((float)(c + over) < best) {
-            best = (float)(c + over);
+        const float c = fmaxf(ceilf(s / (float)(target - n)), (float)least);
+        if (c + (float)over < best) {
+            best = c + (float)over;
             piece = c;
         }
     }
     const int64_t room = (int64_t)rounds * target - n;
     if (room > 0) {
-        int64_t c = (int64_t)sqrtf((float)over * s / t);
-        const int64_t low = (sum + room - 1) / room;
-        c = c < low ? low : c;
-        c = c < least ? least : c;
-        const float e = (s + (float)over * (s / (float)c + (float)n)) / t + (float)(c + over);
-        if (e < best) {
-            best = e;
-            piece = c;
-        }
+        const float c = fmaxf(ceilf(fmaxf(sqrtf((float)over * s / t), s / (float)room)), (float)least);
+        const float e = (s + (float)over * (s / c + (float)n)) / t + c + (float)over;
+        if (e < best) piece = c;
     }
-    return piece >= most || piece > kWhole ? kWhole : (int)piece;
+    return piece >= (float)most ? kWhole : (int)piece;
+}
+
+// Inclusive sums (or maxima) over the wave's lanes in six lane moves.
+template <int CTRL, int ROWS, class T> __device__ __forceinline__ T lane_move(T v, T zero) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, zero), __builtin_bit_cast(int, v), CTRL, ROWS, 0xF, false));
+}
+template <class T, class F> __device__ __forceinline__ T scan64(T v, T zero, F f) {
+    v = f(v, lane_move<0x111, 0xF>(v, zero));  // row_shr 1, 2, 4, 8: within sixteen lanes
+    v = f(v, lane_move<0x112, 0xF>(v, zero));
+    v = f(v, lane_move<0x114, 0xF>(v, zero));
+    v = f(v, lane_move<0x118, 0xF>(v, zero));
+    v = f(v, lane_move<0x142, 0xA>(v, zero));  // row_bcast 15, 31: across them
+    v = f(v, lane_move<0x143, 0xC>(v, zero));
+    return v;
 }
 
 // Which tile of rows and which piece of its keys workgroup wg takes; every wave finds out for itself (no barrier). A
@@ -241,37 +248,26 @@ template <int TR, int BK, int CMIN, int OVER> __device__ __forceinline__ bool fi
     it = Item{0, 0, 0, 1, 0, 0, 0, 0, 0, 0, 0};
     const int lane = threadIdx.x & 63, x = wg / p.kv_heads;
     ReqShape s = shape_of<TR, BK>(p, lane);
-    int64_t sum = (int64_t)s.tiles * s.nb, tiles = s.tiles;
-    int most = s.nb;
+    float sum = (float)s.tiles * (float)s.nb;
+    int tiles = s.tiles, most = s.nb;
     for (int base = 64; base < p.nreq; base += 64) {
         const ReqShape t = shape_of<TR, BK>(p, base + lane);
-        sum += (int64_t)t.tiles * t.nb;
+        sum += (float)t.tiles * (float)t.nb;
         tiles += t.tiles;
         most = t.nb > most ? t.nb : most;
     }
-#pragma unroll
-    for (int o = 32; o; o >>= 1) {
-        sum += __shfl_xor(sum, o);
-        tiles += __shfl_xor(tiles, o);
-        const int m = __shfl_xor(most, o);
-        most = m > most ? m : most;
-    }
-    const int piece = piece_blocks(uni64(sum) * p.kv_heads, uni64(tiles) * p.kv_heads, uni(most), p.target, p.rounds, CMIN, OVER);
+    auto add = [](auto a, auto b) { return a + b; };
+    sum = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scan64(sum, 0.0f, add)), 63));
+    tiles = __builtin_amdgcn_readlane(scan64(tiles, 0, add), 63);
+    most = __builtin_amdgcn_readlane(scan64(most, 0, [](int a, int b) { return a > b ? a : b; }), 63);
+    const int piece = piece_blocks(sum * (float)p.kv_heads, tiles * p.kv_heads, most, p.target, p.rounds, CMIN, OVER);
     int before = 0, parts = 0;
     bool found = false;
     for (int base = 0; base < p.nreq; base += 64) {
         if (base) s = shape_of<TR, BK>(p, base + lane);
         const int ns = s.nb <= piece ? 1 : (s.nb + piece - 1) / piece;
         const int n = s.tiles * ns, np = ns > 1 || p.prefix_splits > 0 ? n : 0;
-        int incl = n, inclp = np;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int u = __shfl_up(incl, o), v = __shfl_up(inclp, o);
-            if (lane >= o) {
-                incl += u;
-                inclp += v;
-            }
-        }
+        const int incl = scan64(n, 0, add), inclp = scan64(np, 0, add);
         if (!found) {
             const uint64_t m = __ballot(before + incl > x);
             if (m) {
@@ -417,13 +413,18 @@ template <int DP> struct Acc {
     }
 };
 
-// S^T of 32 keys at LDS address k.
+// S^T of 32 keys at LDS address k. All operands are read before the first product (the compiler would read each right
+// before its use, an LDS latency a product).
 template <int DP, bool BF> __device__ __forceinline__ a16f scores(uint32_t k, const uint4 (&q)[DP / 16]) {
     const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
     const uint32_t a = k + r * (2 * DP) + ((h ^ swz<DP>(r)) << 4);
+    uint4 f[DP / 16];
+#pragma unroll
+    for (int i = 0; i < DP / 16; i++) f[i] = lds16(a ^ (i << 5));
+    __builtin_amdgcn_sched_barrier(0);
     a16f s = {};
 #pragma unroll
-    for (int i = 0; i < DP / 16; i++) s = mma<BF>(lds16(a ^ (i << 5)), q[i], s);
+    for (int i = 0; i < DP / 16; i++) s = mma<BF>(f[i], q[i], s);
     return s;
 }
 
@@ -487,8 +488,21 @@ template <int DP, bool BF, bool TWO> __device__ __forceinline__ void values(a16f
     const int lane = threadIdx.x & 63, i = lane & 15, h = lane >> 5;
     const int row = 4 * h + (i >> 2), c = 2 * ((lane >> 4) & 1) + ((i >> 1) & 1);
     const uint32_t a = v + row * (2 * DP) + ((c ^ swz<DP>(row)) << 4) + 8 * (i & 1);
+    uint4 f[2][DP / 32];
+    auto read = [&](int b) {
+#pragma unroll
+        for (int d = 0; d < DP / 32; d++) {
+            const uint32_t at = (a ^ (d << 6)) + b * 32 * DP;
+            const uint2 x = lds_tr(at), y = lds_tr((at ^ 32) + 16 * DP);
+            f[b][d] = make_uint4(x.x, x.y, y.x, y.y);
+        }
+    };
+    read(0);
+    if (DP <= 128) read(1);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int b = 0; b < 2; b++) {
+        if (DP > 128 && b == 1) read(1);
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -498,12 +512,10 @@ template <int DP, bool BF, bool TWO> __device__ __forceinline__ void values(a16f
         }
         const uint4 ph = make_uint4(hi[0], hi[1], hi[2], hi[3]);
 #pragma unroll
-        for (int d = 0; d < DP / 32; d++) {
-            const uint32_t at = (a ^ (d << 6)) + b * 32 * DP;
-            const uint2 x = lds_tr(at), y = lds_tr((at ^ 32) + 16 * DP);
-            const uint4 vt = make_uint4(x.x, x.y, y.x, y.y);
-            o[d] = mma<BF>(vt, ph, o[d]);
-            if (TWO) o[d] = mma<BF>(vt, make_uint4(lo[0], lo[1], lo[2], lo[3]), o[d]);
+        for (int d = 0; d < DP / 32; d++) o[d] = mma<BF>(f[b][d], ph, o[d]);
+        if (TWO) {
+#pragma unroll
+            for (int d = 0; d < DP / 32; d++) o[d] = mma<BF>(f[b][d], make_uint4(lo[0], lo[1], lo[2], lo[3]), o[d]);
         }
     }
 }
@@ -569,9 +581,10 @@ template <bool BF> __device__ __forceinline__ void put4(const AttnArgs &p, int q
     if (d >= p.dim) return;
     const int t = row / p.group, g = row - t * p.group;
     uint16_t *dst = p.out + (int64_t)(q0 + t) * p.out_stride + (int64_t)(head * p.group + g) * p.dim + d;
+    const float inv = 1.0f / l;  // one division, an fp32 rounding more
     float y[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) y[i] = sees ? o[i] / l : 0.0f;
+    for (int i = 0; i < 4; i++) y[i] = sees ? o[i] * inv : 0.0f;
     const uint2 w = make_uint2(pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3]));
     if (p.out_aligned) {
         *reinterpret_cast<uint2 *>(dst) = w;
