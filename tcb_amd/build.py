@@ -23,9 +23,11 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-ffp-contract=off",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
          "-Wall", "-Wno-unused-function", "-Wno-unused-variable"]
-# attn_rows.hip: matrix instructions take their accumulators in architectural registers where they fit. A wave there uses over
-# 256 registers, and the compiler's default then keeps every accumulator in the other file, a move away from the softmax.
-FILE_FLAGS = {"attn_rows.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+# attn*.hip: matrix instructions take their accumulators in architectural registers where they fit. The compiler's default
+# for waves of over 256 registers keeps every accumulator in the other file, a move away from the softmax.
+VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
+FILE_FLAGS = {"attn.hip": VGPR_FORM, "attn_rows.hip": VGPR_FORM}
+
 
 
 def _run(cmd):

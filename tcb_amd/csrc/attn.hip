@@ -110,7 +110,7 @@ template <int DP, bool BF, bool PREFIX> __global__ __launch_bounds__(64 * kTokWa
         copy_k(s, slot);
         const bool all = all_see(rw, t, 32);
         if (!all) mask(x[0], rw, t);
-        softmax_step<DP, 1>(A, x, p.scale);
+        softmax_step<DP, 1>(A, x, p.scale, p.slack);
         wait_vmcnt(AHEAD);
         const uint32_t v = ring + (slot + 1) * L::SLOT;
         if (!all && mixed && odd_values<DP, BF>(v)) values_one_by_one<DP, BF>(A.o, x[0], v, rw.hi, rw.lo, rw.sinks, t);
@@ -282,6 +282,7 @@ int launch_attn(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c) {
     p.window = (int)c.window;
     p.sinks = (int)c.sinks;
     p.scale = c.scale * 1.44269504088896341f;
+    p.slack = 8.0f / p.scale;
     p.q_aligned = (reinterpret_cast<uintptr_t>(c.q) % 16 == 0) && c.q_stride % 8 == 0;
     p.out_aligned = (reinterpret_cast<uintptr_t>(c.out) % 8 == 0) && c.out_stride % 4 == 0;
     p.arrivals = ctx->arrivals;

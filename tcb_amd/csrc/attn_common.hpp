@@ -35,7 +35,7 @@ struct AttnArgs {
     float *prefix_part;  // [split][token][head] partial results of the prefix: DP sums, reference, sum
     int nreq, tokens, heads, kv_heads, group, dim;
     int window, sinks;  // window 0: none
-    float scale;        // softmax scale times log2 e
+    float scale, slack; // softmax scale times log2 e; what is 2^8 in units of scores
     int q_aligned, out_aligned;  // 16- and 8-byte aligned rows
     int target, rounds; // workgroups at a time, and how often at most
     int row_lo, row_hi; // requests of row_lo < rows <= row_hi are this launch's
@@ -520,16 +520,19 @@ template <int DP, bool BF, bool TWO> __device__ __forceinline__ void values(a16f
     }
 }
 
-// The running softmax's step over NB blocks of 32 scores: the new maximum, O^T and the sum rescaled to it, scores
-// replaced by exp2(scale (s - m)). A row that has seen nothing keeps m = -Inf and adds nothing.
-template <int DP, int NB> __device__ __forceinline__ void softmax_step(Acc<DP> &A, a16f (&s)[NB], float scale) {
+// The running softmax's step over NB blocks of 32 scores: scores replaced by exp2(scale (s - m)), m the row's reference.
+// It is raised to the largest score so far, and O^T and the sum are rescaled to it, only where that exceeds it by more than
+// 2^8: weights of up to 2^8 cost no precision, rescaling every time a maximum grows cost a quarter of a token step's
+// instructions. A row that has seen nothing keeps m = -Inf and adds nothing.
+template <int DP, int NB> __device__ __forceinline__ void softmax_step(Acc<DP> &A, a16f (&s)[NB], float scale, float slack) {
     float x = s[0][0];
 #pragma unroll
     for (int b = 0; b < NB; b++)
 #pragma unroll
         for (int i = 0; i < 16; i++) x = fmaxf(x, s[b][i]);
-    const float m = fmaxf(A.m, half_max(x));
-    if (__any(m > A.m)) {
+    x = half_max(x);
+    if (__any(x > A.m + slack)) {
+        const float m = x > A.m + slack ? x : A.m;
         const float a = m > A.m ? exp2_hw((A.m - m) * scale) : 1.0f;  // A.m = -Inf: 0
         A.l *= a;
 #pragma unroll
@@ -538,7 +541,7 @@ template <int DP, int NB> __device__ __forceinline__ void softmax_step(Acc<DP> &
             for (int i = 0; i < 16; i++) A.o[d][i] *= a;
         A.m = m;
     }
-    const float mu = m == -__builtin_inff() ? 0.0f : m, ms = mu * scale;
+    const float mu = A.m == -__builtin_inff() ? 0.0f : A.m, ms = mu * scale;
     // One fused step an element. The rounding of ms is the same factor in every weight and cancels, as long as it is
     // small: where scores are past 2^20 the difference is taken first.
     const bool far = __any(fabsf(ms) > 1048576.0f);
