@@ -114,7 +114,7 @@ template <int DP, bool BF, bool PREFIX> __global__ __launch_bounds__(64 * kTokWa
         wait_vmcnt(AHEAD);
         const uint32_t v = ring + (slot + 1) * L::SLOT;
         if (!all && mixed && odd_values<DP, BF>(v)) values_one_by_one<DP, BF>(A.o, x[0], v, rw.hi, rw.lo, rw.sinks, t);
-        else values<DP, BF, true>(A.o, x[0], v);
+        else values<DP, BF, true, true>(A.o, x[0], v);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         copy_v(s, slot + 1);
         slot = slot + 2 == L::SLOTS ? 0 : slot + 2;

@@ -483,8 +483,8 @@ __device__ __forceinline__ void values_one_by_one(a16f (&o)[DP / 32], const a16f
 }
 
 // O^T += V^T P^T of 32 keys at LDS address v, P in 16 bits; TWO: in two terms (what the first rounding drops is the
-// second), so that P's rounding does not show beside the output's.
-template <int DP, bool BF, bool TWO> __device__ __forceinline__ void values(a16f (&o)[DP / 32], const a16f &pr, uint32_t v) {
+// second), so that P's rounding does not show beside the output's. EARLY: operands are read before the products, where there are registers for them.
+template <int DP, bool BF, bool TWO, bool EARLY> __device__ __forceinline__ void values(a16f (&o)[DP / 32], const a16f &pr, uint32_t v) {
     const int lane = threadIdx.x & 63, i = lane & 15, h = lane >> 5;
     const int row = 4 * h + (i >> 2), c = 2 * ((lane >> 4) & 1) + ((i >> 1) & 1);
     const uint32_t a = v + row * (2 * DP) + ((c ^ swz<DP>(row)) << 4) + 8 * (i & 1);
@@ -497,12 +497,14 @@ template <int DP, bool BF, bool TWO> __device__ __forceinline__ void values(a16f
             f[b][d] = make_uint4(x.x, x.y, y.x, y.y);
         }
     };
-    read(0);
-    if (DP <= 128) read(1);
-    __builtin_amdgcn_sched_barrier(0);
+    if (EARLY) {
+        read(0);
+        if (DP <= 128) read(1);
+        __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
     for (int b = 0; b < 2; b++) {
-        if (DP > 128 && b == 1) read(1);
+        if (!EARLY || (DP > 128 && b == 1)) read(b);
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {

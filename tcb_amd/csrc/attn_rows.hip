@@ -26,6 +26,7 @@ template <int V> struct Const {
 
 template <int DP> struct RowsShape {
     static constexpr int WAVES = 4, BK = DP == 256 ? 32 : 64, NT = BK / 32;
+    static constexpr bool SKEW = DP != 256;  // (its accumulators leave no registers for a second block's scores and weights)
     static constexpr int PER_CU = DP == 256 ? 1 : 2;  // workgroups a CU: by registers
     static constexpr int SHARE = BK / WAVES;          // rows of a block that a wave copies
     static constexpr int THREADS = 64 * WAVES, TR = 32 * WAVES;
@@ -194,7 +195,8 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::PER_CU) void
     f1 = f1 > nb ? nb : f1;
     f0 += f0 & 1;  // pairs of blocks, the first even: places in LDS are constants in the loop
     f1 -= (f1 - f0) & 1;
-    if (f1 < f0 + 2 || all.hi_min + 1 < kFewKeys || (p.window > 0 && p.window < kFewKeys)) f0 = f1 = nb;
+    const bool few = all.hi_min + 1 < kFewKeys || (p.window > 0 && p.window < kFewKeys);
+    if (!L::SKEW || f1 < f0 + 2 || few) f0 = f1 = nb;
 
     auto qk = [&](a16f (&x)[NT], int place) {
 #pragma unroll
@@ -233,7 +235,8 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::PER_CU) void
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             if (odd) values_one_by_one<DP, BF>(o, s[t], vat + t * 64 * DP, rw.hi, rw.lo, rw.sinks, t0 + 32 * t);
-            else values<DP, BF, true>(o, s[t], vat + t * 64 * DP);
+            else if (L::SKEW || !see || few) values<DP, BF, true, false>(o, s[t], vat + t * 64 * DP);
+            else values<DP, BF, false, false>(o, s[t], vat + t * 64 * DP);
         }
     };
     {
@@ -243,6 +246,7 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::PER_CU) void
     }
     int j = 0;
     for (; j < f0; j++) plain(j);
+    if constexpr (L::SKEW)
     if (j < f1) {
         Piece16 c0 = piece_of(j, page_of(j)), c1 = piece_of(j + 1, page_of(j + 1));
         int page2 = page_of(j + 2);
