@@ -300,7 +300,7 @@ int launch_attn(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c) {
     pr.target = cus * attn_rows_per_cu(dp);
     pr.row_lo = rows_alone ? 0 : kTokRows;
     pr.row_hi = 0x7FFFFFFF;
-    const int tr = attn_rows_tile(dp), br = attn_rows_block(dp);
+    const int tr = attn_rows_tile(), br = attn_rows_block();
     const int64_t grid_t = plan_items(pt, c, kTokRows, kTokBlock, kTokLeast), grid_r = plan_items(pr, c, tr, br, 4);
     if (grid_t >= ((int64_t)1 << 31) || grid_r >= ((int64_t)1 << 31)) return fail(ctx, TRHIP_ERR_INVALID, "attention: too many rows");
     const bool prefix = c.prefix_len > 0;

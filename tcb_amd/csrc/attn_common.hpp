@@ -366,13 +366,14 @@ template <int DP> struct Lanes16 {
             voff[i] = 8 * c < dim ? (uint32_t)(r * dim * 2 + c * 16) : 0x80000000u;
         }
     }
+    __device__ __forceinline__ void copy_one(dma_rsrc d, uint32_t dst, int i, int ha, int hb) const {
+        uint32_t o = voff[i];
+        if (hb > ha) o = (uint32_t)(row + i * RPI - ha) < (uint32_t)(hb - ha) ? 0x80000000u : o;
+        dma16(d, dst + i * 1024, o, 0);
+    }
     __device__ __forceinline__ void copy(dma_rsrc d, uint32_t dst, int ha, int hb) const {
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            uint32_t o = voff[i];
-            if (hb > ha) o = (uint32_t)(row + i * RPI - ha) < (uint32_t)(hb - ha) ? 0x80000000u : o;
-            dma16(d, dst + i * 1024, o, 0);
-        }
+        for (int i = 0; i < N; i++) copy_one(d, dst, i, ha, hb);
     }
 };
 
@@ -699,8 +700,8 @@ __device__ __forceinline__ bool last_piece(const AttnArgs &p, const Item &it, in
 
 // attn_rows.hip: rows of a tile and keys of a block, and the launch.
 int attn_rows_per_cu(int dp);
-int attn_rows_tile(int dp);
-int attn_rows_block(int dp);
+int attn_rows_tile();
+int attn_rows_block();
 int launch_attn_rows(trhip_ctx *ctx, const AttnArgs &p, int dp, bool bf, bool prefix, int64_t grid);
 
 }  // namespace trhip

@@ -25,39 +25,13 @@ template <int V> struct Const {
 };
 
 template <int DP> struct RowsShape {
-    static constexpr int WAVES = 4, BK = DP == 256 ? 32 : 64, NT = BK / 32;
+    static constexpr int WAVES = 4, BK = 64, NT = BK / 32;
     static constexpr bool SKEW = DP != 256;  // (its accumulators leave no registers for a second block's scores and weights)
     static constexpr int PER_CU = DP == 256 ? 1 : 2;  // workgroups a CU: by registers
-    static constexpr int SHARE = BK / WAVES;          // rows of a block that a wave copies
     static constexpr int THREADS = 64 * WAVES, TR = 32 * WAVES;
     static constexpr int TILE = BK * DP * 2;       // bytes of a block's keys or values
-    static constexpr int PI = SHARE * DP / 512;    // copies a wave makes of a block
+    static constexpr int PI = DP / 32;             // copies a wave makes of a block: a sixteen-row piece
     static constexpr int BYTES = 4 * TILE;  // two blocks of each are in LDS
-};
-
-// A wave's share of a block: rows of a sixteen-row piece, from row `r0` of it.
-template <int DP> struct Share {
-    static constexpr int N = RowsShape<DP>::PI, CH = DP / 8, RPI = 64 / CH;
-    uint32_t voff[N];
-    int row;
-    __device__ __forceinline__ void init(int dim, int r0) {
-        const int lane = threadIdx.x & 63;
-        row = r0 + lane / CH;
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            const int r = row + i * RPI, c = (lane % CH) ^ swz<DP>(r);
-            voff[i] = 8 * c < dim ? (uint32_t)(r * dim * 2 + c * 16) : 0x80000000u;
-        }
-    }
-    __device__ __forceinline__ void copy_one(dma_rsrc d, uint32_t dst, int i, int ha, int hb) const {
-        uint32_t o = voff[i];
-        if (hb > ha) o = (uint32_t)(row + i * RPI - ha) < (uint32_t)(hb - ha) ? 0x80000000u : o;
-        dma16(d, dst + i * 1024, o, 0);
-    }
-    __device__ __forceinline__ void copy(dma_rsrc d, uint32_t dst, int ha, int hb) const {
-#pragma unroll
-        for (int i = 0; i < N; i++) copy_one(d, dst, i, ha, hb);
-    }
 };
 
 template <int DP, bool BF, bool PREFIX>
@@ -102,9 +76,9 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::PER_CU) void
     const int b0 = it.split * piece, left_b = total - b0, nb = left_b < 0 ? 0 : left_b < piece ? left_b : piece;
 
     const uint32_t ring = lds_addr(smem);
-    Share<DP> share;
-    share.init(p.dim, L::SHARE == 16 ? 0 : 8 * (w & 1));
-    const int prow = L::SHARE == 16 ? 16 * w : 16 * (w >> 1);  // its piece's first row in a block
+    Lanes16<DP> share;
+    share.init(p.dim);
+    const int prow = 16 * w;  // its piece's first row in a block
 
     uint4 q[DP / 16];
     load_q<DP>(p, q, it.q0, wn > 0 ? r0 + wr : r0, wn, it.head);
@@ -117,7 +91,7 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::PER_CU) void
     // block j's places: keys at k_at, values at v_at
     auto k_at = [&](int j) { return ring + (j & 1) * L::TILE; };
     auto v_at = [&](int j) { return ring + (2 + (j & 1)) * L::TILE; };
-    const uint32_t mine = w * (L::SHARE * 2 * DP);
+    const uint32_t mine = w * (32 * DP);
     auto copy_k = [&](const Piece16 &c, int j) { share.copy(c.k, k_at(j) + mine, c.ha, c.hb); };
     auto copy_v = [&](const Piece16 &c, int j) { share.copy(c.v, v_at(j) + mine, c.ha, c.hb); };
 
@@ -199,8 +173,20 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::PER_CU) void
     if (!L::SKEW || f1 < f0 + 2 || few) f0 = f1 = nb;
 
     auto qk = [&](a16f (&x)[NT], int place) {
+        if constexpr (L::SKEW) {
 #pragma unroll
-        for (int i = 0; i < NT * NK; i++) x[i % NT] = mma<BF>(k_frag(place * L::TILE, i), q[i / NT], i < NT ? a16f{} : x[i % NT]);
+            for (int i = 0; i < NT * NK; i++) x[i % NT] = mma<BF>(k_frag(place * L::TILE, i), q[i / NT], i < NT ? a16f{} : x[i % NT]);
+        } else {  // alone on its SIMD: operands eight ahead
+            uint4 f[NT * NK];
+#pragma unroll
+            for (int i = 0; i < 8; i++) f[i] = k_frag(place * L::TILE, i);
+#pragma unroll
+            for (int i = 0; i < NT * NK; i++) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (i + 8 < NT * NK) f[i + 8] = k_frag(place * L::TILE, i + 8);
+                x[i % NT] = mma<BF>(f[i], q[i / NT], i < NT ? a16f{} : x[i % NT]);
+            }
+        }
     };
     auto plain = [&](int j) {
         const int page = page_of(j + 1);
@@ -235,8 +221,8 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::PER_CU) void
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             if (odd) values_one_by_one<DP, BF>(o, s[t], vat + t * 64 * DP, rw.hi, rw.lo, rw.sinks, t0 + 32 * t);
-            else if (L::SKEW || !see || few) values<DP, BF, true, false>(o, s[t], vat + t * 64 * DP);
-            else values<DP, BF, false, false>(o, s[t], vat + t * 64 * DP);
+            else if (L::SKEW || !see || few) values<DP, BF, true, !L::SKEW>(o, s[t], vat + t * 64 * DP);
+            else values<DP, BF, false, !L::SKEW>(o, s[t], vat + t * 64 * DP);
         }
     };
     {
@@ -360,8 +346,8 @@ template <int DP, bool BF, bool PREFIX> int launch_rows(trhip_ctx *ctx, const At
 }  // namespace
 
 int attn_rows_per_cu(int dp) { return dp == 256 ? RowsShape<256>::PER_CU : RowsShape<128>::PER_CU; }
-int attn_rows_tile(int dp) { return dp == 256 ? RowsShape<256>::TR : RowsShape<128>::TR; }
-int attn_rows_block(int dp) { return dp == 256 ? RowsShape<256>::BK : RowsShape<128>::BK; }
+int attn_rows_tile() { return RowsShape<128>::TR; }
+int attn_rows_block() { return RowsShape<128>::BK; }
 
 template <bool PREFIX> static int by_type(trhip_ctx *ctx, const AttnArgs &p, int dp, bool bf, int64_t grid) {
     if (dp == 64) return bf ? launch_rows<64, true, PREFIX>(ctx, p, grid) : launch_rows<64, false, PREFIX>(ctx, p, grid);
