@@ -505,7 +505,10 @@ template <int DP, bool BF, bool TWO, bool EARLY> __device__ __forceinline__ void
     }
 #pragma unroll
     for (int b = 0; b < 2; b++) {
-        if (!EARLY || (DP > 128 && b == 1)) read(b);
+        if (!EARLY || (DP > 128 && b == 1)) {
+            read(b);
+            if (!EARLY) __builtin_amdgcn_sched_barrier(0);
+        }
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -703,5 +706,6 @@ int attn_rows_per_cu(int dp);
 int attn_rows_tile();
 int attn_rows_block();
 int launch_attn_rows(trhip_ctx *ctx, const AttnArgs &p, int dp, bool bf, bool prefix, int64_t grid);
+int launch_attn_rows256(trhip_ctx *ctx, const AttnArgs &p, bool bf, bool prefix, int64_t grid);  // attn_rows256.hip
 
 }  // namespace trhip
