@@ -2,10 +2,10 @@
 //
 // A workgroup takes a tile of 32 rows a wave (attn_common.hpp) and goes through its keys in blocks of BK that its waves copy
 // into LDS together. What bounds it are the matrix instructions and, nearly as much, the softmax's instructions, which
-// have to run under them. Blocks that every row sees whole are taken in a skewed loop: step j multiplies K of block j + 1 and V of
+// have to run under them. Blocks are taken in a skewed loop: step j multiplies K of block j + 1 and V of
 // block j - 1 while it takes the exponentials of block j, three independent pieces of work in one run of instructions, and two
-// waves share a SIMD. Blocks with a mask go through a plain step. The two are loops of their own: with masks as branches of one loop the
-// compiler copied O^T between registers at every join, a third of the loop's instructions.
+// waves share a SIMD. Masks only touch the scores there. Rows that see few keys go through a plain step, in a loop of its own: as a
+// branch of the skewed one it made the compiler copy O^T between registers at every join, a third of the instructions.
 //
 // The softmax's reference (what is subtracted from a row's scores) is a whole power of two, raised only when a block's
 // maximum exceeds it by more than 2^8: then the sums, O^T and the pending weights are multiplied by a power of two, exactly.
@@ -33,7 +33,7 @@ template <int DP> struct RowsShape {
     static constexpr int THREADS = 64 * WAVES, TR = 32 * WAVES;
     static constexpr int TILE = BK * DP * 2;       // bytes of a block's keys or values
     static constexpr int PI = DP / 32;             // copies a wave makes of a block: a sixteen-row piece
-    static constexpr int BYTES = 4 * TILE;  // two blocks of each are in LDS
+    static constexpr int BYTES = 4 * TILE + 16;  // two blocks of each are in LDS
 };
 
 template <int DP, bool BF, bool PREFIX>
@@ -164,16 +164,33 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::PER_CU) void
         }
     };
 
-    // Blocks [f0, f1) are seen whole by every row of the tile.
-    const int at0 = sp.ns - sp.w0 - b0;
-    int f0 = at0 + (all.lo_max + BK - 1) / BK, f1 = at0 + (all.hi_min + 1) / BK;
-    f0 = f0 < 0 ? 0 : f0;
-    f1 = f1 > nb ? nb : f1;
-    f0 += f0 & 1;  // pairs of blocks, the first even: places in LDS are constants in the loop
-    f1 -= (f1 - f0) & 1;
+    // Whether a key that some rows see and others do not has a value that is not finite (0 times it would reach all rows): its
+    // tile goes through plain steps, which look out for that. Those keys are the ones behind the first token's last and
+    // before the last token's window, one for each token of the tile.
+    bool odd = false;
+    if (!PREFIX && mixed) {
+        constexpr uint32_t E = BF ? 0x7F807F80u : 0x7C007C00u, U = BF ? 0x00800080u : 0x04000400u;
+        const int chunks = p.dim / 8, n0 = all.hi_max - all.hi_min, n1 = all.lo_max - all.lo_min;
+        uint32_t any = 0;
+        for (int i = tid; i < (n0 + n1) * chunks; i += L::THREADS) {
+            const int k = i / chunks, c = i - k * chunks, t = k < n0 ? all.hi_min + 1 + k : all.lo_min + (k - n0);
+            if (t < 0) continue;
+            const int page = table[t >> p.page_log2];
+            if ((uint32_t)page >= (uint32_t)p.npages) continue;
+            const uint4 x = *reinterpret_cast<const uint4 *>(p.v + (int64_t)page * p.page_bytes + (int64_t)it.head * p.head_bytes +
+                                                             (int64_t)((t & ((1 << p.page_log2) - 1)) * p.dim * 2 + c * 16));
+            any |= ((x.x & E) + U) | ((x.y & E) + U) | ((x.z & E) + U) | ((x.w & E) + U);
+        }
+        int *flag = reinterpret_cast<int *>(smem) + 4 * L::TILE / 4;
+        if (tid == 0) *flag = 0;
+        lds_barrier();
+        if (any & 0x80008000u) *flag = 1;
+        lds_barrier();
+        odd = *flag != 0;
+    }
+    // Blocks go through the skewed loop in pairs (an odd one last through a plain step), except where rows see few keys.
     const bool few = all.hi_min + 1 < kFewKeys || (p.window > 0 && p.window < kFewKeys);
-    if (!L::SKEW || f1 < f0 + 2 || few) f0 = f1 = nb;
-
+    const int pairs = !L::SKEW || few || odd ? 0 : nb & ~1;
     auto qk = [&](a16f (&x)[NT], int place) {
         if constexpr (L::SKEW) {
 #pragma unroll
@@ -210,7 +227,7 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::PER_CU) void
         top = half_max(maximum(s));
         if (__any(top * p.scale > ms + 8.0f)) raise(pk, false);
         relative(s);
-        bool odd = false;
+        bool odd_here = false;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
 #pragma unroll
@@ -218,11 +235,11 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::PER_CU) void
                 s[t][i] = exp2_hw(fmaf(s[t][i], p.scale, neg));
                 l += s[t][i];
             }
-            if (!see && mixed) odd = odd || odd_values<DP, BF>(vat + t * 64 * DP);
+            if (!see && odd) odd_here = odd_here || odd_values<DP, BF>(vat + t * 64 * DP);
         }
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            if (odd) values_one_by_one<DP, BF>(o, s[t], vat + t * 64 * DP, rw.hi, rw.lo, rw.sinks, t0 + 32 * t);
+            if (odd_here) values_one_by_one<DP, BF>(o, s[t], vat + t * 64 * DP, rw.hi, rw.lo, rw.sinks, t0 + 32 * t);
             else if (few || (!L::SKEW && !see)) values<DP, BF, true, false>(o, s[t], vat + t * 64 * DP);
             else values<DP, BF, false, false>(o, s[t], vat + t * 64 * DP);
         }
@@ -233,9 +250,8 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::PER_CU) void
         copy_v(c, 0);
     }
     int j = 0;
-    for (; j < f0; j++) plain(j);
     if constexpr (L::SKEW)
-    if (j < f1) {
+    if (pairs > 0) {
         Piece16 c0 = piece_of(j, page_of(j)), c1 = piece_of(j + 1, page_of(j + 1));
         int page2 = page_of(j + 2);
         wait_vmcnt(0);
@@ -254,6 +270,13 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::PER_CU) void
             const int page3 = page_of(j + 3);
             wait_vmcnt(0);
             lds_barrier();  // keys of block j + 1 and values of j - 1 are there; keys of j and values of j - 2 have been read
+            const int t0 = key_of(j);
+            if (!all_see(rw, t0, BK)) {
+#pragma unroll
+                for (int t = 0; t < NT; t++) mask(x[t], rw, t0 + 32 * t);
+                top = half_max(maximum(x));
+                higher = top * p.scale > ms + 8.0f;
+            }
             if (__any(higher)) raise(y, true);
             relative(x);
             // three independent runs, dealt over one another: products with K, exponentials, products with V; between
@@ -298,7 +321,7 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::PER_CU) void
             c0 = c1, c1 = c2, page2 = page3;
             j++;
         };
-        while (j < f1) {
+        while (j < pairs) {
             step(Const<0>{}, s, s1, pk, p1);
             step(Const<1>{}, s1, s, p1, pk);
         }
