@@ -17,7 +17,7 @@ constexpr int kTokRows = 32, kTokBlock = 32, kTokWaves = 4, kTokLeast = 8, kTokO
 
 template <int DP> struct TokLds {
     static constexpr int SLOT = 32 * DP * 2;  // 32 keys or values
-    static constexpr int SLOTS = DP == 64 ? 4 : DP == 128 ? 4 : 2;
+    static constexpr int SLOTS = 2;
     static constexpr int OSTRIDE = DP + 4;  // floats between rows of a wave's results
     static constexpr int RING = SLOT * SLOTS, OUT = 32 * OSTRIDE * 4;
     static constexpr int WAVE = RING > OUT ? RING : OUT;
@@ -294,7 +294,7 @@ int launch_attn(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c) {
     const int64_t most_rows = (c.max_new < c.tokens ? c.max_new : c.tokens) * p.group;
     const bool tokens_alone = most_rows <= kTokRows, rows_alone = !tokens_alone && c.tokens == c.nreq * c.max_new;
     AttnArgs pt = p, pr = p;
-    pt.target = cus * (dp == 64 ? 2 : 1);
+    pt.target = cus * (dp <= 128 ? 2 : 1);
     pt.row_lo = 0;
     pt.row_hi = tokens_alone ? 0x7FFFFFFF : kTokRows;
     pr.target = cus * attn_rows_per_cu(dp);
