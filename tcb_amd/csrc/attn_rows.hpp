@@ -20,7 +20,7 @@
 namespace trhip {
 namespace {
 
-constexpr int kFewKeys = 128;
+constexpr int kFewKeys = 256;
 
 template <int V> struct Const {
     static constexpr int value = V;

@@ -168,11 +168,115 @@ def test_a_key_reaches_only_the_tokens_that_see_it(backend, dtype, value, plane)
                 assert np.isfinite(got[row, 2:]).all()  # the other kv head
 
 
+def whole(b, window=0, sinks=0, scale=None):
+    """want() on the GPU in float64, for batches too large for the loop: every request's heads as matrix products."""
+    dev, outs, tols = "cuda:0", [], []
+    scale = b.dim ** -0.5 if scale is None else scale
+    for i, (n, m) in enumerate(zip(b.new, b.kv)):
+        pages = [int(x) for x in b.prefix_table[:-(-b.prefix // b.page)]], [int(x) for x in b.table[i, :-(-m // b.page)]]
+        kv = []
+        for plane in (b.k, b.v):
+            parts = [plane[p].to(dev).double().transpose(1, 2).reshape(-1, b.kv_heads, b.dim)[:c] for p, c in zip(pages, (b.prefix, m))]
+            kv.append(torch.cat(parts).repeat_interleave(b.heads // b.kv_heads, 1).transpose(0, 1))
+        q = b.q[b.start[i]:b.start[i + 1]].to(dev).double().transpose(0, 1)
+        s = torch.matmul(q, kv[0].transpose(1, 2).contiguous()) * scale
+        j = torch.arange(b.prefix + m, device=dev) - b.prefix
+        p = (torch.arange(n, device=dev) + m - n).unsqueeze(1)
+        see = (j < 0) | ((j <= p) & ((window == 0) | (j > p - window) | (j < sinks)))
+        e = torch.softmax(s.masked_fill(~see, -float("inf")), 2)
+        o, spread = torch.matmul(e, kv[1]), torch.matmul(e, kv[1].abs())
+        reach = scale * torch.matmul(q.abs(), kv[0].abs().transpose(1, 2).contiguous()).masked_fill(~see, 0).amax(2, keepdim=True)
+        o, spread, reach = (x.transpose(0, 1).cpu().numpy() for x in (o, spread, reach))
+        outs.append(o)
+        tols.append(R.bound(b.dtype, b.dim, m + b.prefix, o, spread, reach))
+    return np.concatenate(outs), np.concatenate(tols)
+
+
+def check_whole(tb, b, window=0, sinks=0, scale=None, **how):
+    got = b.run(tb, window, sinks, scale, **how)
+    want, tol = whole(b, window, sinks, scale)
+    off = np.abs(got - want) - tol
+    assert np.isfinite(got).all()
+    worst = np.unravel_index(np.argmax(off), off.shape)
+    assert off.max() <= 0, "at %s: got %r want %r, allowed %r" % (worst, got[worst], want[worst], tol[worst])
+    return got
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (4, 4, 64), (5, 1, 96), (4, 2, 256), (3, 1, 200)])
+def test_long_prompts(backend, dtype, heads, kv_heads, dim):
+    """Blocks in pairs and an odd one, tiles that end anywhere, a short chunk behind a long history (pieces that are joined)."""
+    for new, kv, page in (([700], [700], 16), ([129, 64, 500], [900, 1500, 513], 32), ([40], [9000], 64), ([33, 1, 200], [5000, 3000, 260], 16)):
+        print(dtype, heads, kv_heads, dim, new, kv, flush=True)
+        b = Batch(dtype, heads, kv_heads, dim, page, new, kv, seed=30)
+        got = check_whole(backend, b)
+        assert np.array_equal(got, b.run(backend))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("window,sinks", [(128, 0), (130, 4), (300, 64), (1000, 1), (257, 700)])
+def test_long_prompts_in_a_window(backend, dtype, window, sinks):
+    for heads, kv_heads, dim in ((8, 2, 128), (4, 4, 64), (2, 1, 256)):
+        print(dtype, window, sinks, dim, flush=True)
+        check_whole(backend, Batch(dtype, heads, kv_heads, dim, 16, [600, 1, 77, 300], [900, 1300, 2000, 300], seed=31), window, sinks)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_a_late_key_reaches_only_the_tokens_that_see_it(backend, dtype, value):
+    """As above for keys far into long prompts: at a block's edge, in its middle, the last, and one that a window passes."""
+    for heads, kv_heads, dim, window, sinks in ((4, 1, 128, 0, 0), (4, 1, 128, 200, 4), (2, 2, 64, 0, 0), (2, 1, 256, 150, 0)):
+        for j in (447, 448, 460, 499, 300):
+            print(dtype, value, dim, window, j, flush=True)
+            b = Batch(dtype, heads, kv_heads, dim, 16, [200, 1], [500, 300], seed=32)
+            clean = b.run(backend, window, sinks)
+            b.v[b.table[0, j // 16], 0, j % 16, 7] = value
+            b.k[b.table[0, j // 16], 0, j % 16, 7] = 1e3
+            got = b.run(backend, window, sinks)
+            g = heads // kv_heads
+            for t in range(200):
+                if R.visible(300 + t, j, window, sinks):
+                    assert not np.isfinite(got[t, :g, 7]).any()
+                    assert np.isfinite(got[t, :g, 8]).all()
+                else:
+                    assert np.abs(got[t, :g] - clean[t, :g]).max() <= 2.0 ** -7 * np.abs(clean[t, :g]).max()
+            assert np.array_equal(got[200], clean[200]) and np.isfinite(got[:, g:]).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_scores_that_grow_along_the_keys(backend, dtype):
+    """References raised again and again, by little and by much, and sharp rows whose last keys hold nearly all weight."""
+    for grow in (0.02, 1.0, 30.0):
+        for new, kv in (([200], [700]), ([1], [700]), ([1], [20000])):
+            b = Batch(dtype, 4, 1, 128, 64, new, kv, seed=33)
+            b.q[:] = b.q.abs()
+            for j in range(kv[0]):
+                b.k[b.table[0, j // 64], 0, j % 64] *= 0.05
+                b.k[b.table[0, j // 64], 0, j % 64] += grow * j / kv[0] * 4
+            check_whole(backend, b)
+
+
+def test_far_scores_in_long_prompts(backend):
+    """Scores past 2^20 in units of log2, of both signs: the differences are taken first; equal ones average."""
+    for x in (-1e30, 1e30, 3e4):
+        b = Batch("bf16", 4, 1, 128, 16, [150], [700], seed=34)
+        b.q[:] = 0
+        b.q[:, :, 0] = 1e30 if abs(x) > 1e20 else 1e3
+        for j in range(700):
+            b.k[b.table[0, j // 16], 0, j % 16] = 0
+            b.k[b.table[0, j // 16], 0, j % 16, 0] = x * (1e-28 if abs(x) > 1e20 else 1)
+        check_whole(backend, b, scale=1.0)
+
+
 def test_rows_that_see_nothing_are_zero(backend):
     """No keys, or fewer than the tokens the request brings: the first tokens sit before key 0."""
     b = Batch("bf16", 4, 2, 64, 16, [1, 5, 70, 2], [0, 3, 40, 2], seed=10)
     got = b.check(backend)
     assert (got[0] == 0).all() and (got[1:3] == 0).all() and (got[6:36] == 0).all() and (got[36] != 0).any()
+    for new, kv in (([300], [200]), ([200, 40], [0, 10])):
+        b = Batch("f16", 4, 1, 128, 16, new, kv, seed=24)
+        got = b.check(backend)
+        assert (got[:new[0] - kv[0]] == 0).all()
 
 
 def test_scores_of_the_lowest_and_highest_values(backend):
@@ -254,6 +358,18 @@ def test_shared_prefix_of_a_large_batch(backend):
     Batch("f16", 8, 2, 128, 32, [1] * 3, [1, 5, 9], 5000, seed=20).check(backend)
     b = Batch("bf16", 8, 2, 128, 32, [2, 1], [1, 0], 100, seed=21)  # tokens without a key of their own: the prefix alone
     b.check(backend)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_long_shared_prefix(backend, dtype, dim):
+    """The prefix's rows fill tiles of their own and its keys are cut; own parts of one token, of several, of a prompt."""
+    for new, kv, prefix in (([1] * 40, [1 + 13 * i % 200 for i in range(40)], 3001), ([3] * 20, [3 + i for i in range(20)], 777),
+                            ([1, 150, 2, 1], [40, 150, 300, 1], 2000), ([2], [70], 4097)):
+        print(dtype, dim, new[:4], prefix, flush=True)
+        b = Batch(dtype, 8, 2, dim, 32, new, kv, prefix, seed=35)
+        got = check_whole(backend, b)
+        assert np.array_equal(got, b.run(backend))
 
 
 def test_shared_prefix_equals_whole_tables(backend):
