@@ -16,7 +16,7 @@ LIB = os.path.join(HERE, "libtrhip.so")
 SOURCES = ["api.hip", "wstore.hip", "gemv.hip", "gemv_fast.hip", "gemm_rows.hip", "actq.hip", "actq_mfma.hip",
            "swiglu.hip", "probe.hip", "prefill.hip", "actqw.hip", "rows16.hip", "actq4.hip", "fastg.hip",
            "io16.hip", "paged.hip", "attn.hip", "attn_rows.hip",
-           "attn_rows256.hip"]
+           "attn_rows256.hip", "attn_two.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # -ffp-contract=off: no multiply-add is fused unless written as fmaf (bit-exact rounding order).

@@ -244,7 +244,7 @@ template <class T, class F> __device__ __forceinline__ T scan64(T v, T zero, F f
 // Which tile of rows and which piece of its keys workgroup wg takes; every wave finds out for itself (no barrier). A
 // request's tiles are all cut into the same number of pieces (piece_blocks). Items are numbered head fastest, then piece, tile (the last tokens of a prompt, whose rows read most keys,
 // first), request. False: no item left.
-template <int TR, int BK, int CMIN, int OVER> __device__ __forceinline__ bool find_item(const AttnArgs &p, int wg, Item &it) {
+template <int TR, int BK, int CMIN, int OVER> __device__ __forceinline__ bool find_item(const AttnArgs &p, int wg, int grid, Item &it) {
     it = Item{0, 0, 0, 1, 0, 0, 0, 0, 0, 0, 0};
     const int lane = threadIdx.x & 63, x = wg / p.kv_heads;
     ReqShape s = shape_of<TR, BK>(p, lane);
@@ -294,7 +294,7 @@ template <int TR, int BK, int CMIN, int OVER> __device__ __forceinline__ bool fi
     it.q0 = uni(it.q0), it.nq = uni(it.nq), it.kv = uni(it.kv), it.slot = uni(it.slot), it.counter = uni(it.counter);
     it.parts = uni(parts) * p.kv_heads;
     // starts that are not in order could name more items than there are workgroups: then nothing is done
-    const bool fits = (int64_t)before * p.kv_heads <= (int64_t)gridDim.x && (int64_t)parts * p.kv_heads <= p.part_slots;
+    const bool fits = (int64_t)before * p.kv_heads <= (int64_t)grid && (int64_t)parts * p.kv_heads <= p.part_slots;
     if (!fits) it.parts = 0;
     return found && fits;
 }
@@ -679,8 +679,8 @@ __device__ __forceinline__ void leave_place(const AttnArgs &p, const Item &it, i
     if (threadIdx.x == 0)
         reinterpret_cast<Place *>(p.parts + 8)[it.slot] = Place{it.split == 0 ? it.nsplit : 0, it.q0, it.nq, it.kv, r0, n, it.head, 0};
 }
-__device__ __forceinline__ void leave_count(const AttnArgs &p, const Item &it) {
-    if (p.parts && blockIdx.x == 0 && threadIdx.x == 0) p.parts[0] = it.parts;
+__device__ __forceinline__ void leave_count(const AttnArgs &p, const Item &it, int wg) {
+    if (p.parts && wg == 0 && threadIdx.x == 0) p.parts[0] = it.parts;
 }
 
 // Partial results are written: whether this workgroup is the last of its tile's pieces.
@@ -701,6 +701,9 @@ __device__ __forceinline__ bool last_piece(const AttnArgs &p, const Item &it, in
 
 }  // namespace
 
+// attn_two.hip: two kinds of work in one launch. a: what `kind` says, on na workgroups; b: few rows, on nb.
+enum class TwoKind { Rows, PrefixRows, PrefixTokens };
+int launch_attn_two(trhip_ctx *ctx, const AttnArgs &a, int na, TwoKind kind, const AttnArgs &b, int nb, int dp, bool bf, int cus);
 // attn_rows.hip: rows of a tile and keys of a block, and the launch.
 int attn_rows_per_cu(int dp);
 int attn_rows_tile();

@@ -36,8 +36,8 @@ template <int DP> struct RowsShape {
     static constexpr int BYTES = 4 * TILE + 16;  // two blocks of each are in LDS
 };
 
-template <int DP, bool BF, bool PREFIX>
-__global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::PER_CU) void attn_rows(const AttnArgs p) {
+// PREFIX: rows are all tokens' and keys the shared prefix's; results go to prefix_part.
+template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_tile(const AttnArgs &p, int wg, int grid) {
     using L = RowsShape<DP>;
     constexpr int BK = L::BK, NT = L::NT;
     extern __shared__ __attribute__((aligned(1024))) uint4 smem[];
@@ -46,8 +46,8 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::PER_CU) void
     const int *table;
     int keys;
     if (PREFIX) {
-        const int x = blockIdx.x / p.kv_heads;
-        it.head = blockIdx.x - x * p.kv_heads;
+        const int x = wg / p.kv_heads;
+        it.head = wg - x * p.kv_heads;
         it.tile = x / p.prefix_splits;
         it.split = x - it.tile * p.prefix_splits;
         it.nsplit = p.prefix_splits;
@@ -56,8 +56,8 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::PER_CU) void
         table = p.prefix_table;
         keys = p.prefix_len;
     } else {
-        const bool some = find_item<L::TR, BK, 4, kRowsOver>(p, blockIdx.x, it);
-        leave_count(p, it);
+        const bool some = find_item<L::TR, BK, 4, kRowsOver>(p, wg, grid, it);
+        leave_count(p, it, wg);
         if (!some) return;
         table = p.table + (int64_t)it.req * p.max_pages;
         keys = it.kv;
@@ -358,6 +358,11 @@ __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::PER_CU) void
         if (!direct && h == 0) *reinterpret_cast<float2 *>(part + DP) = make_float2(ms, sum);
     }
     if (!direct && !PREFIX) leave_place(p, it, r0, n);
+}
+
+template <int DP, bool BF, bool PREFIX>
+__global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::PER_CU) void attn_rows(const AttnArgs p) {
+    rows_of_tile<DP, BF, PREFIX>(p, blockIdx.x, gridDim.x);
 }
 
 template <int DP, bool BF, bool PREFIX> int launch_rows(trhip_ctx *ctx, const AttnArgs &p, int64_t grid) {
