@@ -7,11 +7,24 @@ namespace {
 
 // Page tables. Request i holds old_i keys and brings add_i: have_i = ceil(old_i / page) pages it has, need_i =
 // ceil((old_i + add_i) / page); the grow_i = need_i - have_i fresh ones are free[base_i ...], base the running sum of
-// grow. One launch: every workgroup makes the running sums for itself (12 bytes a request, cached) and then writes its
-// 4 x THREADS slots; the tables' fresh entries, lengths and starts are dealt over the workgroups by request. A slot's page is
-// read from the table only where it was there before, else from the free list, so no workgroup waits for another's entries.
-// What bounds it is latency: the lengths, the scan, one dependent read (4.x us for sixteen requests).
-__device__ __forceinline__ int clamp31(int64_t v) { return v > 0x7FFFFFFF ? 0x7FFFFFFF : (int)v; }
+// grow. One launch: every workgroup makes the running sums for itself (8 bytes a request, cached) and then writes its
+// 4 x THREADS slots, four in a row a thread, whose request it finds by halving; the tables' fresh entries, lengths and starts are
+// dealt over the workgroups by request. A slot's page is read from the table only where it was there before, else from
+// the free list, so no workgroup waits for another's entries. What bounds it is latency: lengths, sums, one dependent read.
+// Sums saturate at 2^32 - 1 (a step of so many tokens has no slots anyway), so their order holds whatever the lengths are.
+__device__ __forceinline__ int clamp31(uint32_t v) { return v > 0x7FFFFFFFu ? 0x7FFFFFFF : (int)v; }
+__device__ __forceinline__ uint32_t sat_add(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t moved(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ uint32_t running_sum(uint32_t v) {  // over the wave's lanes, inclusive
+    v = sat_add(v, moved<0x111, 0xF>(v));  // row_shr 1, 2, 4, 8, then row_bcast 15 and 31
+    v = sat_add(v, moved<0x112, 0xF>(v));
+    v = sat_add(v, moved<0x114, 0xF>(v));
+    v = sat_add(v, moved<0x118, 0xF>(v));
+    v = sat_add(v, moved<0x142, 0xA>(v));
+    return sat_add(v, moved<0x143, 0xC>(v));
+}
 
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void page_tables_kernel(int nreq, int page_log2, const int *__restrict__ old_len,
@@ -20,101 +33,93 @@ __global__ __launch_bounds__(THREADS) void page_tables_kernel(int nreq, int page
                                                               int *__restrict__ q_start, int *__restrict__ kv_len,
                                                               int *__restrict__ slots, int64_t nslots, int *__restrict__ used) {
     constexpr int WAVES = THREADS / 64, PER = 4;
-    __shared__ int s_start[THREADS + 1], s_old[THREADS], s_base[THREADS];
-    __shared__ int64_t s_wave[2][WAVES];
+    __shared__ uint32_t s_start[THREADS], s_base[THREADS], s_grow[THREADS];
+    __shared__ int s_old[THREADS];  // -1: refused
+    __shared__ uint32_t s_wave[2][WAVES];
     __shared__ int s_used[WAVES];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const int64_t page = (int64_t)1 << page_log2, first = (int64_t)blockIdx.x * (PER * THREADS);
-    int64_t tok0 = 0, base0 = 0;  // sums over the chunks of requests before this one
+    const int64_t page = (int64_t)1 << page_log2, first = (int64_t)blockIdx.x * (PER * THREADS), mine = first + PER * tid;
+    uint32_t tok0 = 0, base0 = 0;  // sums over the chunks of requests before this one
     int most = 0;
     int out[PER];
 #pragma unroll
     for (int u = 0; u < PER; u++) out[u] = -1;
     for (int c = 0; c < nreq; c += THREADS) {
         const int i = c + tid;
-        int64_t old = 0, add = 0;
+        int old = 0, add = 0;
         if (i < nreq) {
             old = old_len[i];
             add = add_len[i];
             old = old < 0 ? 0 : old;
             add = add < 0 ? 0 : add;
         }
-        const int64_t have = (old + page - 1) >> page_log2, need = (old + add + page - 1) >> page_log2;
-        const int64_t grow = need <= max_pages ? need - have : 0;
-        int64_t st = add, sg = grow;  // inclusive sums over the wave
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int64_t a = __shfl_up(st, o), b = __shfl_up(sg, o);
-            if (lane >= o) {
-                st += a;
-                sg += b;
-            }
-        }
+        const int64_t have = ((int64_t)old + page - 1) >> page_log2, need = ((int64_t)old + add + page - 1) >> page_log2;
+        const uint32_t grow = need <= max_pages ? (uint32_t)(need - have) : 0;
+        const uint32_t st = running_sum((uint32_t)add), sg = running_sum(grow);
         __syncthreads();  // the chunk before has been used
         if (lane == 63) {
             s_wave[0][w] = st;
             s_wave[1][w] = sg;
         }
         __syncthreads();
-        int64_t bt = tok0, bg = base0, tt = 0, tg = 0;
+        uint32_t bt = tok0, bg = base0, tt = tok0, tg = base0;  // before this wave, after all
 #pragma unroll
         for (int k = 0; k < WAVES; k++) {
-            if (k < w) {
-                bt += s_wave[0][k];
-                bg += s_wave[1][k];
-            }
-            tt += s_wave[0][k];
-            tg += s_wave[1][k];
+            tt = sat_add(tt, s_wave[0][k]);
+            tg = sat_add(tg, s_wave[1][k]);
+            if (k < w) bt = tt, bg = tg;
         }
-        const int64_t start = bt + st - add, base = bg + sg - grow;
-        const bool fits = need <= max_pages && (grow == 0 || base + grow <= nfree);
-        if (i < nreq && fits && base + grow > most) most = (int)(base + grow);
-        s_start[tid] = clamp31(start);
-        s_old[tid] = fits ? (int)old : -1;
-        s_base[tid] = clamp31(base);
-        if (tid == THREADS - 1) s_start[THREADS] = clamp31(start + add);
+        const uint32_t end = sat_add(bt, st), start = end - (uint32_t)add, top = sat_add(bg, sg), base = top - grow;
+        const bool fits = need <= max_pages && (grow == 0 || (int64_t)top <= nfree);
+        if (i < nreq && fits && (int64_t)top > most) most = (int)top;
+        s_start[tid] = start;
+        s_old[tid] = fits ? old : -1;
+        s_base[tid] = base;
+        s_grow[tid] = fits ? grow : 0;
         // this workgroup's share of the requests' own outputs
         if (i < nreq && (int)((unsigned)(c / THREADS) % gridDim.x) == (int)blockIdx.x) {
-            kv_len[i] = clamp31(old + (fits ? add : 0));
-            q_start[i + 1] = clamp31(start + add);
+            kv_len[i] = clamp31((uint32_t)old + (fits ? (uint32_t)add : 0u));
+            q_start[i + 1] = clamp31(end);
             if (i == 0) q_start[0] = 0;
         }
         __syncthreads();
         const int cnt = nreq - c < THREADS ? nreq - c : THREADS;
         for (int k = (int)blockIdx.x * WAVES + w; k < cnt; k += (int)gridDim.x * WAVES) {  // a wave writes a request's fresh entries
-            const int o = s_old[k];
-            if (o < 0) continue;
-            const int64_t h = ((int64_t)o + page - 1) >> page_log2;
-            const int64_t e = ((int64_t)o + (s_start[k + 1] - s_start[k]) + page - 1) >> page_log2;
-            for (int64_t j = h + lane; j < e; j += 64) table[(c + k) * max_pages + j] = free_list[s_base[k] + (j - h)];
+            const uint32_t n = s_grow[k];
+            if (n == 0) continue;
+            int *row = table + (c + k) * max_pages + (((int64_t)s_old[k] + page - 1) >> page_log2);
+            for (uint32_t j = lane; j < n; j += 64) row[j] = free_list[s_base[k] + j];
         }
-        if (first < tok0 + tt && first + PER * THREADS > tok0) {
+        if (first < (int64_t)tt && first + PER * THREADS > (int64_t)tok0) {
+            int lo = 0, hi = cnt;  // the last request that starts at or before this thread's first slot
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if ((int64_t)s_start[mid] <= mine) lo = mid;
+                else hi = mid;
+            }
 #pragma unroll
             for (int u = 0; u < PER; u++) {
-                const int64_t t = first + u * THREADS + tid;
-                if (t < tok0 || t >= tok0 + tt || t >= nslots) continue;
-                int lo = 0, hi = cnt;  // the last request that starts at or before t
-                while (hi - lo > 1) {
-                    const int mid = (lo + hi) >> 1;
-                    if (s_start[mid] <= (int)t) lo = mid;
-                    else hi = mid;
-                }
+                const int64_t t = mine + u;
+                if (t < (int64_t)tok0 || t >= (int64_t)tt || t >= nslots) continue;
+                while (lo + 1 < cnt && (int64_t)s_start[lo + 1] <= t) lo++;
                 const int o = s_old[lo];
                 if (o < 0) continue;
-                const int64_t pos = (int64_t)o + (t - s_start[lo]), pi = pos >> page_log2, h = ((int64_t)o + page - 1) >> page_log2;
+                const int64_t pos = (int64_t)o + (t - (int64_t)s_start[lo]), pi = pos >> page_log2, h = ((int64_t)o + page - 1) >> page_log2;
                 int64_t pg = 0;
                 if (pi < h) pg = table[(c + lo) * max_pages + pi];
                 else pg = free_list[s_base[lo] + (pi - h)];
                 out[u] = (int)((pg << page_log2) + (pos & (page - 1)));
             }
         }
-        tok0 += tt;
-        base0 += tg;
+        tok0 = tt;
+        base0 = tg;
     }
+    if (mine + PER <= nslots && reinterpret_cast<uintptr_t>(slots) % 16 == 0) {
+        *reinterpret_cast<int4 *>(slots + mine) = make_int4(out[0], out[1], out[2], out[3]);
+    } else {
 #pragma unroll
-    for (int u = 0; u < PER; u++) {
-        const int64_t t = first + u * THREADS + tid;
-        if (t < nslots) slots[t] = out[u];
+        for (int u = 0; u < PER; u++)
+            if (mine + u < nslots) slots[mine + u] = out[u];
     }
     if (blockIdx.x == 0) {
 #pragma unroll

@@ -75,6 +75,24 @@ def test_requests_that_do_not_fit(backend):
     check_tables(backend, 16, [5] * 600, [17] * 600, 700, 4)
 
 
+def test_lengths_past_32_bits_together(backend):
+    """Lengths whose sums pass 2^31 and 2^32: those requests do not fit, and what stands before them is served."""
+    for huge in ([2 ** 31 - 1] * 2, [2 ** 31 - 1] * 5, [2 ** 30] * 3):
+        old, add = [7, 3] + [0] * len(huge) + [9], [30, 1] + huge + [5]
+        have = [1, 1] + [0] * len(huge) + [1]
+        table = np.full((len(old), 6), -1, np.int32)
+        table[:, 0] = np.arange(len(old))
+        free = np.arange(100, 120, dtype=np.int32)
+        got = run_tables(backend, 16, old, add, free, table.copy(), 60)
+        want = table.copy()
+        want[0, 1:3] = [100, 101]
+        assert np.array_equal(got[0], want) and got[4][0] == 2
+        assert got[2][:2].tolist() == [37, 4] and got[2][2:-1].tolist() == [0] * len(huge)
+        assert got[1][:3].tolist() == [0, 30, 31] and (np.diff(got[1].astype(np.int64)) >= 0).all()
+        slots = [p % 16 + 16 * [0, 100, 101][p // 16] for p in range(7, 37)] + [16 + 3]
+        assert got[3].tolist() == slots + [-1] * (60 - len(slots))
+
+
 @pytest.mark.parametrize("nslots", [0, 1, 50, 5000])
 def test_slots_shorter_or_longer_than_the_step(backend, nslots):
     check_tables(backend, 16, [3, 50, 0], [40, 1, 70], 30, 10, nslots)
