@@ -144,14 +144,14 @@ int launch_attn(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c) {
     pr.row_lo = rows_alone ? 0 : kTokRows;
     pr.row_hi = 0x7FFFFFFF;
     const int tr = attn_rows_tile(), br = attn_rows_block();
-    const int64_t grid_t = plan_items(pt, c, kTokRows, kTokBlock, kTokLeast), grid_r = plan_items(pr, c, tr, br, 4);
-    if (grid_t >= ((int64_t)1 << 31) || grid_r >= ((int64_t)1 << 31)) return fail(ctx, TRHIP_ERR_INVALID, "attention: too many rows");
     const bool prefix = c.prefix_len > 0;
     // Pieces of long tiles are joined by a launch of their own (a workgroup that joined a tile of 128 rows alone would take
     // longer than the pieces); there are none where the tiles fill the device by themselves. A token's few rows are joined
     // by the last workgroup of their tile, in the same launch, except behind a prefix.
-    const bool cut = !tokens_alone && (prefix || tiles_of(pr, c, tr) < pr.target);
-    if (!cut) pr.rounds = pr.part_slots = 0;
+    const int64_t tiles_r = tiles_of(pr, c, tr);
+    const bool cut = !tokens_alone && (prefix || tiles_r < pr.target);
+    const int64_t grid_t = plan_items(pt, c, kTokRows, kTokBlock, kTokLeast), grid_r = cut ? plan_items(pr, c, tr, br, kRowsLeast) : tiles_r;
+    if (grid_t >= ((int64_t)1 << 31) || grid_r >= ((int64_t)1 << 31)) return fail(ctx, TRHIP_ERR_INVALID, "attention: too many rows");
     const int64_t part_t = rows_alone ? 0 : (int64_t)pt.part_slots * kTokRows, part_r = tokens_alone ? 0 : (int64_t)pr.part_slots * tr;
     const int64_t part = (part_t + part_r) * (dp + 2);
     const int64_t places = 8 + 8 * (int64_t)(pt.part_slots > pr.part_slots ? pt.part_slots : pr.part_slots);
@@ -162,7 +162,7 @@ int launch_attn(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c) {
     int splits = 0;
     if (prefix) {
         const int64_t nb = (c.prefix_len + pbk - 1) / pbk, items = ptiles * p.kv_heads;
-        const int64_t piece = piece_blocks((float)items * (float)nb, (int)items, (int)nb, tall ? pr.target : pt.target, kMostRounds, tall ? 4 : kTokLeast, tall ? kRowsOver : kTokOver);
+        const int64_t piece = piece_blocks((float)items * (float)nb, (int)items, (int)nb, tall ? pr.target : pt.target, kMostRounds, tall ? kRowsLeast : kTokLeast, tall ? kRowsOver : kTokOver);
         splits = piece >= nb ? 1 : (int)((nb + piece - 1) / piece);
     }
     int st = TRHIP_OK;
@@ -177,15 +177,20 @@ int launch_attn(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c) {
     if (grid_p + grid_t + grid_r >= ((int64_t)1 << 30)) return fail(ctx, TRHIP_ERR_INVALID, "attention: too many rows");
     pt.parts = prefix ? reinterpret_cast<int *>(ws) : nullptr;
     pr.parts = cut ? reinterpret_cast<int *>(ws) : nullptr;
-    // Two kinds of work in one launch: the one waits for memory while the other multiplies.
+    // Two kinds of work in one launch: the one waits for memory while the other multiplies. Prompts and tokens take turns in
+    // runs of a workgroup a CU, a prefix goes first (its pieces are the long ones), and so do prompts of three times as many tiles
+    // as there are tokens', which then fill the prompts' last round (8 prompts of up to 901 with a window of 1024 beside 32
+    // tokens: 129 us in turns, 119; 16 prompts of up to 500 beside 16 tokens 120, 113; 2 of up to 4000 beside 32 tokens with up
+    // to 6000 keys 387, 397; but 4 of up to 2000 beside 128 tokens with up to 8000 keys, twice as many tiles, 647, 716).
     const bool two = dp <= 128 && (prefix ? !rows_alone : !tokens_alone && !rows_alone);
     bool rows_left = !tokens_alone, tokens_left = !rows_alone;
     if (two && prefix) {
-        st = launch_attn_two(ctx, tall ? pr : pt, (int)grid_p, tall ? TwoKind::PrefixRows : TwoKind::PrefixTokens, pt, (int)grid_t, dp, bf, cus);
+        st = launch_attn_two(ctx, tall ? pr : pt, (int)grid_p, tall ? TwoKind::PrefixRows : TwoKind::PrefixTokens, pt, (int)grid_t, dp, bf, (int)grid_p);
         if (st == TRHIP_OK) st = launch_join(ctx, pt, dp, bf, kTokRows);
         tokens_left = false;
     } else if (two) {
-        st = launch_attn_two(ctx, pr, (int)grid_r, TwoKind::Rows, pt, (int)grid_t, dp, bf, cus);
+        const bool rows_first = c.tokens * p.group / tr >= 3 * c.nreq;
+        st = launch_attn_two(ctx, pr, (int)grid_r, TwoKind::Rows, pt, (int)grid_t, dp, bf, rows_first ? (int)grid_r : cus);
         if (st == TRHIP_OK && cut) st = launch_join(ctx, pr, dp, bf, tr);
         return st;
     } else if (prefix) {

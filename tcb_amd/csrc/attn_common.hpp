@@ -174,14 +174,23 @@ struct Item {
 struct ReqShape {
     int q0, nq, kv, tiles, nb;
 };
-template <int TR, int BK> __device__ __forceinline__ ReqShape shape_of(const AttnArgs &p, int i) {
+struct ReqLens {
+    int start, end, keys;
+};
+__device__ __forceinline__ ReqLens lens_of(const AttnArgs &p, int i) {
+    ReqLens r = {0, 0, 0};
+    if (i < p.nreq) {
+        r.start = p.q_start[i];
+        r.end = p.q_start[i + 1];
+        r.keys = p.kv_len[i];
+    }
+    return r;
+}
+template <int TR, int BK> __device__ __forceinline__ ReqShape shape_of(const AttnArgs &p, const ReqLens &r) {
     ReqShape s = {0, 0, 0, 0, 0};
-    if (i >= p.nreq) return s;
-    int a = p.q_start[i], b = p.q_start[i + 1], kv = p.kv_len[i];
-    a = a < 0 ? 0 : a > p.tokens ? p.tokens : a;
-    b = b < a ? a : b > p.tokens ? p.tokens : b;
+    const int a = r.start < 0 ? 0 : r.start > p.tokens ? p.tokens : r.start, b = r.end < a ? a : r.end > p.tokens ? p.tokens : r.end;
     const int64_t cap = p.max_pages << p.page_log2;
-    kv = kv < 0 ? 0 : (int64_t)kv > cap ? (int)cap : kv;
+    const int kv = r.keys < 0 ? 0 : (int64_t)r.keys > cap ? (int)cap : r.keys;
     s.q0 = a;
     s.nq = b - a;
     s.kv = kv;
@@ -205,7 +214,7 @@ template <int TR, int BK> __device__ __forceinline__ ReqShape shape_of(const Att
 //   dealt out         (sum + over (sum / c + n)) / target + c + over, least at c = sqrt(over sum / target)
 // Never more than rounds * target pieces.
 constexpr int kMostRounds = 6;
-constexpr int kRowsOver = 10;  // attn_rows
+constexpr int kRowsLeast = 4, kRowsOver = 10;  // attn_rows: blocks of a piece at least, and what one costs beside them
 __host__ __device__ inline int piece_blocks(float sum, int n, int most, int target, int rounds, int least, int over) {
     constexpr int kWhole = 0x40000000;
     // (sums in floats, made a little larger than they can have been rounded down)
@@ -241,35 +250,54 @@ template <class T, class F> __device__ __forceinline__ T scan64(T v, T zero, F f
     return v;
 }
 
-// Which tile of rows and which piece of its keys workgroup wg takes; every wave finds out for itself (no barrier). A
-// request's tiles are all cut into the same number of pieces (piece_blocks). Items are numbered head fastest, then piece, tile (the last tokens of a prompt, whose rows read most keys,
-// first), request. False: no item left.
+struct Plus {
+    __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+    __device__ __forceinline__ int operator()(int a, int b) const { return __builtin_elementwise_add_sat(a, b); }  // (starts out of order)
+};
+
+// Which tile of rows and which piece of its keys workgroup wg takes; every wave finds out for itself (no barrier). A request's
+// tiles are all cut into the same number of pieces (piece_blocks). Items are numbered head fastest, then piece, tile (the last
+// tokens of a prompt, whose rows read most keys, first), request. False: no item left.
 template <int TR, int BK, int CMIN, int OVER> __device__ __forceinline__ bool find_item(const AttnArgs &p, int wg, int grid, Item &it) {
     it = Item{0, 0, 0, 1, 0, 0, 0, 0, 0, 0, 0};
     const int lane = threadIdx.x & 63, x = wg / p.kv_heads;
-    ReqShape s = shape_of<TR, BK>(p, lane);
-    float sum = (float)s.tiles * (float)s.nb;
-    int tiles = s.tiles, most = s.nb;
-    for (int base = 64; base < p.nreq; base += 64) {
-        const ReqShape t = shape_of<TR, BK>(p, base + lane);
-        sum += (float)t.tiles * (float)t.nb;
-        tiles += t.tiles;
-        most = t.nb > most ? t.nb : most;
+    // The lengths of the first 64 READ requests are read at once (each 64 by themselves are a memory latency more: 128 requests
+    // of 1000 keys took 60.5 us so, 58.6 now) and go round in registers, so that the loops stay short: a launch fetches
+    // their instructions anew.
+    constexpr int READ = 4;
+    ReqLens lens[READ] = {};
+    lens[0] = lens_of(p, lane);
+    if (p.nreq > 64) {
+#pragma unroll
+        for (int c = 1; c < READ; c++) lens[c] = lens_of(p, 64 * c + lane);
     }
-    auto add = [](auto a, auto b) { return a + b; };
-    sum = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scan64(sum, 0.0f, add)), 63));
-    tiles = __builtin_amdgcn_readlane(scan64(tiles, 0, add), 63);
+    auto each = [&](auto use) {
+        ReqLens at[READ] = {lens[0], lens[1], lens[2], lens[3]};
+#pragma unroll 1
+        for (int base = 0; base < p.nreq; base += 64) {
+            if (base >= 64 * READ) at[0] = lens_of(p, base + lane);
+            use(shape_of<TR, BK>(p, at[0]), base);
+            at[0] = at[1], at[1] = at[2], at[2] = at[3];
+        }
+    };
+    float sum = 0.0f;
+    int tiles = 0, most = 0;
+    each([&](const ReqShape &t, int) {
+        sum += (float)t.tiles * (float)t.nb;
+        tiles = Plus()(tiles, t.tiles);
+        most = t.nb > most ? t.nb : most;
+    });
+    sum = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scan64(sum, 0.0f, Plus())), 63));
+    tiles = __builtin_amdgcn_readlane(scan64(tiles, 0, Plus()), 63);
     most = __builtin_amdgcn_readlane(scan64(most, 0, [](int a, int b) { return a > b ? a : b; }), 63);
     const int piece = piece_blocks(sum * (float)p.kv_heads, tiles * p.kv_heads, most, p.target, p.rounds, CMIN, OVER);
     int before = 0, parts = 0;
     bool found = false;
-    for (int base = 0; base < p.nreq; base += 64) {
-        if (base) s = shape_of<TR, BK>(p, base + lane);
-        const int ns = s.nb <= piece ? 1 : (s.nb + piece - 1) / piece;
-        const int n = s.tiles * ns, np = ns > 1 || p.prefix_splits > 0 ? n : 0;
-        const int incl = scan64(n, 0, add), inclp = scan64(np, 0, add);
+    each([&](const ReqShape &s, int base) {
+        const int ns = s.nb <= piece ? 1 : (s.nb + piece - 1) / piece, n = s.tiles * ns, np = ns > 1 || p.prefix_splits > 0 ? n : 0;
+        const int incl = scan64(n, 0, Plus()), inclp = scan64(np, 0, Plus());
         if (!found) {
-            const uint64_t m = __ballot(before + incl > x);
+            const uint64_t m = __ballot(Plus()(before, incl) > x);
             if (m) {
                 const int src = __builtin_ctzll(m);
                 it.req = base + src;
@@ -287,9 +315,9 @@ template <int TR, int BK, int CMIN, int OVER> __device__ __forceinline__ bool fi
                 found = true;
             }
         }
-        before += __builtin_amdgcn_readlane(incl, 63);
-        parts += __builtin_amdgcn_readlane(inclp, 63);
-    }
+        before = Plus()(before, __builtin_amdgcn_readlane(incl, 63));
+        parts = Plus()(parts, __builtin_amdgcn_readlane(inclp, 63));
+    });
     it.req = uni(it.req), it.tile = uni(it.tile), it.split = uni(it.split), it.nsplit = uni(it.nsplit), it.head = uni(it.head);
     it.q0 = uni(it.q0), it.nq = uni(it.nq), it.kv = uni(it.kv), it.slot = uni(it.slot), it.counter = uni(it.counter);
     it.parts = uni(parts) * p.kv_heads;
@@ -703,7 +731,7 @@ __device__ __forceinline__ bool last_piece(const AttnArgs &p, const Item &it, in
 
 // attn_two.hip: two kinds of work in one launch. a: what `kind` says, on na workgroups; b: few rows, on nb.
 enum class TwoKind { Rows, PrefixRows, PrefixTokens };
-int launch_attn_two(trhip_ctx *ctx, const AttnArgs &a, int na, TwoKind kind, const AttnArgs &b, int nb, int dp, bool bf, int cus);
+int launch_attn_two(trhip_ctx *ctx, const AttnArgs &a, int na, TwoKind kind, const AttnArgs &b, int nb, int dp, bool bf, int turn);
 // attn_rows.hip: rows of a tile and keys of a block, and the launch.
 int attn_rows_per_cu(int dp);
 int attn_rows_tile();

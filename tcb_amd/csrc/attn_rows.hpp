@@ -56,7 +56,7 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_
         table = p.prefix_table;
         keys = p.prefix_len;
     } else {
-        const bool some = find_item<L::TR, BK, 4, kRowsOver>(p, wg, grid, it);
+        const bool some = find_item<L::TR, BK, kRowsLeast, kRowsOver>(p, wg, grid, it);
         leave_count(p, it, wg);
         if (!some) return;
         table = p.table + (int64_t)it.req * p.max_pages;
@@ -164,6 +164,12 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_
         }
     };
 
+    {
+        const Piece16 c = piece_of(0, page_of(0));
+        copy_k(c, 0);
+        copy_v(c, 0);
+    }
+
     // Whether a key that some rows see and others do not has a value that is not finite (0 times it would reach all rows): its
     // tile goes through plain steps, which look out for that. Those keys are the ones behind the first token's last and
     // before the last token's window, one for each token of the tile.
@@ -244,11 +250,6 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_
             else values<DP, BF, false, false>(o, s[t], vat + t * 64 * DP);
         }
     };
-    {
-        const Piece16 c = piece_of(0, page_of(0));
-        copy_k(c, 0);
-        copy_v(c, 0);
-    }
     int j = 0;
     if constexpr (L::SKEW)
     if (pairs > 0) {

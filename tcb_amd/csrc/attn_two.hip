@@ -44,9 +44,9 @@ int by_kind(trhip_ctx *ctx, const AttnArgs &a, int na, TwoKind kind, const AttnA
 
 }  // namespace
 
-int launch_attn_two(trhip_ctx *ctx, const AttnArgs &a, int na, TwoKind kind, const AttnArgs &b, int nb, int dp, bool bf, int cus) {
-    if (dp == 64) return bf ? by_kind<64, true>(ctx, a, na, kind, b, nb, cus) : by_kind<64, false>(ctx, a, na, kind, b, nb, cus);
-    return bf ? by_kind<128, true>(ctx, a, na, kind, b, nb, cus) : by_kind<128, false>(ctx, a, na, kind, b, nb, cus);
+int launch_attn_two(trhip_ctx *ctx, const AttnArgs &a, int na, TwoKind kind, const AttnArgs &b, int nb, int dp, bool bf, int turn) {
+    if (dp == 64) return bf ? by_kind<64, true>(ctx, a, na, kind, b, nb, turn) : by_kind<64, false>(ctx, a, na, kind, b, nb, turn);
+    return bf ? by_kind<128, true>(ctx, a, na, kind, b, nb, turn) : by_kind<128, false>(ctx, a, na, kind, b, nb, turn);
 }
 
 }  // namespace trhip
