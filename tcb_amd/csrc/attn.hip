@@ -24,7 +24,7 @@ template <int DP, bool BF> __global__ __launch_bounds__(256) void attn_join(cons
     if (t.pieces == 0 || rows <= 0) return;
     const int64_t step = (int64_t)p.kv_heads * tr * ST, pstep = (int64_t)p.tokens * p.heads * ST;
     for (int idx = threadIdx.x; idx < rows * (DP / 4); idx += 256) {
-        const int r = idx / (DP / 4), d = (idx - r * (DP / 4)) * 4, row = t.r0 + g + r, tok = row / p.group;
+        const int r = idx / (DP / 4), d = (idx - r * (DP / 4)) * 4, row = t.r0 + g + r, tok = p.by_group(row);
         if (d >= p.dim) continue;
         const float *x = p.part + ((int64_t)blockIdx.x * tr + g + r) * ST;
         const float *pre = p.prefix_part + ((int64_t)(t.q0 + tok) * p.heads + t.head * p.group + (row - tok * p.group)) * ST;
@@ -126,7 +126,8 @@ int launch_attn(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c) {
     p.sinks = (int)c.sinks;
     p.scale = c.scale * 1.44269504088896341f;
     p.slack = 8.0f / p.scale;
-    p.q_aligned = (reinterpret_cast<uintptr_t>(c.q) % 16 == 0) && c.q_stride % 8 == 0;
+    p.by_group.of(p.group);
+    p.by_heads.of(p.kv_heads);
     p.out_aligned = (reinterpret_cast<uintptr_t>(c.out) % 8 == 0) && c.out_stride % 4 == 0;
     p.arrivals = ctx->arrivals;
     const int cus = ctx->sm_count > 0 ? ctx->sm_count : 256;

@@ -19,6 +19,19 @@
 
 namespace trhip {
 
+// x / d of 0 <= x < 2^31 for a d of the call's, in a few scalar instructions: floor(x m / 2^(31 + s)), 2^s >= d, m = ceil(2^(31 + s) / d).
+// (The excess m d - 2^(31 + s) is below d <= 2^s, so that times x stays below 2^(31 + s).)
+struct Div {
+    uint32_t m;
+    int s;
+    void of(int d) {
+        s = 0;
+        while (((int64_t)1 << s) < d) s++;
+        m = (uint32_t)((((uint64_t)1 << (31 + s)) + (uint64_t)d - 1) / (uint64_t)d);
+    }
+    __device__ __forceinline__ int operator()(int x) const { return (int)(((uint64_t)(uint32_t)x * m) >> (31 + s)); }
+};
+
 struct AttnArgs {
     const uint16_t *q;
     uint16_t *out;
@@ -36,7 +49,8 @@ struct AttnArgs {
     int nreq, tokens, heads, kv_heads, group, dim;
     int window, sinks;  // window 0: none
     float scale, slack; // softmax scale times log2 e; what is 2^8 in units of scores
-    int q_aligned, out_aligned;  // 16- and 8-byte aligned rows
+    int out_aligned;    // 8-byte aligned rows
+    Div by_group, by_heads;  // by group, kv_heads
     int target, rounds; // workgroups at a time, and how often at most
     int row_lo, row_hi; // requests of row_lo < rows <= row_hi are this launch's
     int part_slots;     // places for the pieces of tiles that are cut (of all tiles behind a prefix), each with an arrival counter
@@ -217,11 +231,18 @@ constexpr int kMostRounds = 6;
 constexpr int kRowsLeast = 4, kRowsOver = 10;  // attn_rows: blocks of a piece at least, and what one costs beside them
 __host__ __device__ inline int piece_blocks(float sum, int n, int most, int target, int rounds, int least, int over) {
     constexpr int kWhole = 0x40000000;
-    // (sums in floats, made a little larger than they can have been rounded down)
-    const float s = sum * 1.0001f, t = (float)target;
-    float best = n <= target ? (float)most : s / t + 0.5f * (float)most, piece = (float)kWhole;
+    // (in floats, made a little larger than they can have been rounded down)
+#if defined(__HIP_DEVICE_COMPILE__)
+    auto ratio = [](float a, float b) { return a * __builtin_amdgcn_rcpf(b); };
+    auto root = [](float a) { return __builtin_amdgcn_sqrtf(a); };
+#else
+    auto ratio = [](float a, float b) { return a / b; };
+    auto root = [](float a) { return sqrtf(a); };
+#endif
+    const float s = sum * 1.0001f, each = ratio(s, (float)target);
+    float best = n <= target ? (float)most : each + 0.5f * (float)most, piece = (float)kWhole;
     if (rounds > 0 && n < target) {
-        const float c = fmaxf(ceilf(s / (float)(target - n)), (float)least);
+        const float c = fmaxf(ceilf(ratio(s, (float)(target - n))), (float)least);
         if (c + (float)over < best) {
             best = c + (float)over;
             piece = c;
@@ -229,8 +250,8 @@ __host__ __device__ inline int piece_blocks(float sum, int n, int most, int targ
     }
     const int64_t room = (int64_t)rounds * target - n;
     if (room > 0) {
-        const float c = fmaxf(ceilf(fmaxf(sqrtf((float)over * s / t), s / (float)room)), (float)least);
-        const float e = (s + (float)over * (s / c + (float)n)) / t + c + (float)over;
+        const float c = fmaxf(ceilf(fmaxf(root((float)over * each), ratio(s, (float)room))), (float)least);
+        const float e = each + ratio((float)over * (ratio(s, c) + (float)n), (float)target) + c + (float)over;
         if (e < best) piece = c;
     }
     return piece >= (float)most ? kWhole : (int)piece;
@@ -255,12 +276,21 @@ struct Plus {
     __device__ __forceinline__ int operator()(int a, int b) const { return __builtin_elementwise_add_sat(a, b); }  // (starts out of order)
 };
 
+// ceil(nb / piece); a batch has few thousand pieces at most (piece_blocks), so a quotient in floats is one off at most.
+__device__ __forceinline__ int pieces_of(int nb, int piece) {
+    const int x = nb + piece - 1;
+    int q = (int)((float)x * __builtin_amdgcn_rcpf((float)piece));
+    const int r = x - q * piece;
+    q = r < 0 ? q - 1 : r >= piece ? q + 1 : q;
+    return nb <= piece ? 1 : q;
+}
+
 // Which tile of rows and which piece of its keys workgroup wg takes; every wave finds out for itself (no barrier). A request's
 // tiles are all cut into the same number of pieces (piece_blocks). Items are numbered head fastest, then piece, tile (the last
 // tokens of a prompt, whose rows read most keys, first), request. False: no item left.
 template <int TR, int BK, int CMIN, int OVER> __device__ __forceinline__ bool find_item(const AttnArgs &p, int wg, int grid, Item &it) {
     it = Item{0, 0, 0, 1, 0, 0, 0, 0, 0, 0, 0};
-    const int lane = threadIdx.x & 63, x = wg / p.kv_heads;
+    const int lane = threadIdx.x & 63, x = p.by_heads(wg);
     // The lengths of the first 64 READ requests are read at once (each 64 by themselves are a memory latency more: 128 requests
     // of 1000 keys took 60.5 us so, 58.6 now) and go round in registers, so that the loops stay short: a launch fetches
     // their instructions anew.
@@ -294,7 +324,7 @@ template <int TR, int BK, int CMIN, int OVER> __device__ __forceinline__ bool fi
     int before = 0, parts = 0;
     bool found = false;
     each([&](const ReqShape &s, int base) {
-        const int ns = s.nb <= piece ? 1 : (s.nb + piece - 1) / piece, n = s.tiles * ns, np = ns > 1 || p.prefix_splits > 0 ? n : 0;
+        const int ns = pieces_of(s.nb, piece), n = s.tiles * ns, np = ns > 1 || p.prefix_splits > 0 ? n : 0;
         const int incl = scan64(n, 0, Plus()), inclp = scan64(np, 0, Plus());
         if (!found) {
             const uint64_t m = __ballot(Plus()(before, incl) > x);
@@ -306,7 +336,7 @@ template <int TR, int BK, int CMIN, int OVER> __device__ __forceinline__ bool fi
                 it.kv = __builtin_amdgcn_readlane(s.kv, src);
                 it.nsplit = __builtin_amdgcn_readlane(ns, src);
                 const int start = before + __builtin_amdgcn_readlane(incl - n, src), at = x - start;
-                const int t = at / it.nsplit, tiles = __builtin_amdgcn_readlane(s.tiles, src);
+                const int t = it.nsplit == 1 ? at : at / it.nsplit, tiles = __builtin_amdgcn_readlane(s.tiles, src);
                 it.split = at - t * it.nsplit;
                 it.tile = tiles - 1 - t;
                 it.head = wg - x * p.kv_heads;
@@ -341,7 +371,7 @@ struct Rows {
 __device__ __forceinline__ Rows rows_of(const AttnArgs &p, int r0, int n, int nq, int kv) {
     Rows w;
     const int row = r0 + ((int)(threadIdx.x & 31) < n ? (int)(threadIdx.x & 31) : n - 1);
-    const int t0 = r0 / p.group, t1 = (r0 + n - 1) / p.group, t = row / p.group, first = kv - nq;
+    const int t0 = p.by_group(r0), t1 = p.by_group(r0 + n - 1), t = p.by_group(row), first = kv - nq;
     auto low = [&](int hi) { return p.window > 0 && hi >= p.window ? hi - p.window + 1 : 0; };
     w.hi = first + t;
     w.lo = low(w.hi);
@@ -405,25 +435,25 @@ template <int DP> struct Lanes16 {
     }
 };
 
-// Q^T operands of this lane's row (element 16 s + 8 (lane / 32) + i in q[s]); zeros for rows past the tile's and past dim.
+// Q^T operands of this lane's row (element 16 s + 8 (lane / 32) + i in q[s]), zeros past dim. Lanes past the tile's rows
+// take its first.
 template <int DP> __device__ __forceinline__ void load_q(const AttnArgs &p, uint4 (&q)[DP / 16], int q0, int r0, int n, int head) {
     const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
-    const int row = r0 + (r < n ? r : 0), t = row / p.group, g = row - t * p.group;
-    const uint16_t *src = p.q + (int64_t)(q0 + t) * p.q_stride + (int64_t)(head * p.group + g) * p.dim;
+    const int row = r0 + (r < n ? r : 0), t = p.by_group(row), g = row - t * p.group;
+    const uint16_t *src = p.q + (int64_t)(q0 + t) * p.q_stride + (int64_t)(head * p.group + g) * p.dim + 8 * h;
+    auto read = [&](int d) {
+        uint4 w;
+        __builtin_memcpy(&w, src + d, 16);  // (rows need be aligned to their type only)
+        return w;
+    };
+    if (p.dim == DP) {
 #pragma unroll
-    for (int s = 0; s < DP / 16; s++) {
-        const int d = 16 * s + 8 * h;
-        q[s] = make_uint4(0, 0, 0, 0);
-        if (r < n && d < p.dim) {
-            if (p.q_aligned) {
-                q[s] = *reinterpret_cast<const uint4 *>(src + d);
-            } else {
-                uint32_t w[4];
+        for (int s = 0; s < DP / 16; s++) q[s] = read(16 * s);
+    } else {
 #pragma unroll
-                for (int i = 0; i < 4; i++) w[i] = (uint32_t)src[d + 2 * i] | ((uint32_t)src[d + 2 * i + 1] << 16);
-                q[s] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-        }
+        for (int s = 0; s < DP / 16; s++) q[s] = read(16 * s + 8 * h < p.dim ? 16 * s : -8 * h);
+#pragma unroll
+        for (int s = 0; s < DP / 16; s++) q[s] = 16 * s + 8 * h < p.dim ? q[s] : make_uint4(0, 0, 0, 0);
     }
 }
 
@@ -616,7 +646,7 @@ __device__ __forceinline__ float2 agent_load(const float *p) {
 // leaves nothing (hi < 0) is 0; a sum of 0 over visible keys is the formula's 0 / 0.
 template <bool BF> __device__ __forceinline__ void put4(const AttnArgs &p, int q0, int row, int head, int d, const float (&o)[4], float l, bool sees) {
     if (d >= p.dim) return;
-    const int t = row / p.group, g = row - t * p.group;
+    const int t = p.by_group(row), g = row - t * p.group;
     uint16_t *dst = p.out + (int64_t)(q0 + t) * p.out_stride + (int64_t)(head * p.group + g) * p.dim + d;
     const float inv = 1.0f / l;  // one division, an fp32 rounding more
     float y[4];
@@ -696,7 +726,7 @@ __device__ __forceinline__ void join_tile(const AttnArgs &p, const Item &it, int
                 const float *x = lds + (u * chunk + i) * 6;
                 j.add(x[0], x[1], x[2], x[3], x[4], x[5]);
             }
-            put4<BF>(p, it.q0, row, it.head, d, j.o, j.l, it.kv - it.nq + row / p.group >= 0);
+            put4<BF>(p, it.q0, row, it.head, d, j.o, j.l, it.kv - it.nq + p.by_group(row) >= 0);
         }
         __syncthreads();
     }

@@ -46,7 +46,7 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_
     const int *table;
     int keys;
     if (PREFIX) {
-        const int x = wg / p.kv_heads;
+        const int x = p.by_heads(wg);
         it.head = wg - x * p.kv_heads;
         it.tile = x / p.prefix_splits;
         it.split = x - it.tile * p.prefix_splits;
@@ -74,7 +74,7 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_
     }
     const bool mixed = all.hi_min != all.hi_max || all.lo_min != all.lo_max;
     const Span sp = span_of<BK>(all.hi_max, all.lo_min, all.sinks);
-    const int total = sp.count(), piece = (total + it.nsplit - 1) / it.nsplit;
+    const int total = sp.count(), piece = it.nsplit == 1 ? total : (total + it.nsplit - 1) / it.nsplit;
     const int b0 = it.split * piece, left_b = total - b0, nb = left_b < 0 ? 0 : left_b < piece ? left_b : piece;
 
     const uint32_t ring = lds_addr(smem);
@@ -338,7 +338,7 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_
     const bool direct = !PREFIX && it.nsplit == 1 && p.prefix_splits == 0;
     const float sum = half_sum(l);
     if ((lane & 31) < wn) {
-        const int r = wr + (lane & 31), row = r0 + r, t = row / p.group;
+        const int r = wr + (lane & 31), row = r0 + r, t = p.by_group(row);
         float *part = PREFIX ? p.prefix_part + ((int64_t)it.split * p.tokens * p.heads + (int64_t)t * p.heads + it.head * p.group +
                                                 (row - t * p.group)) * (DP + 2)
                              : p.part + ((int64_t)it.slot * L::TR + r) * (DP + 2);

@@ -31,7 +31,7 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void tokens_o
     const int *table;
     int keys;
     if (PREFIX) {
-        const int x = wg / p.kv_heads;
+        const int x = p.by_heads(wg);
         it.head = wg - x * p.kv_heads;
         it.tile = x / p.prefix_splits;
         it.split = x - it.tile * p.prefix_splits;
@@ -53,7 +53,7 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void tokens_o
     if (PREFIX) rw = {keys - 1, 0, keys - 1, keys - 1, 0, 0, 0};
     else rw = rows_of(p, r0, n, it.nq, keys);
     const Span sp = span_of<kTokBlock>(rw.hi_max, rw.lo_min, rw.sinks);
-    const int nb = sp.count(), piece = (nb + it.nsplit - 1) / it.nsplit;
+    const int nb = sp.count(), piece = it.nsplit == 1 ? nb : (nb + it.nsplit - 1) / it.nsplit;
     const int b0 = it.split * piece, b1 = b0 + piece < nb ? b0 + piece : nb;
     const bool mixed = rw.hi_min != rw.hi_max || rw.lo_min != rw.lo_max;  // some rows see keys that others do not
 
@@ -135,7 +135,7 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void tokens_o
     __syncthreads();
     const bool direct = !PREFIX && it.nsplit == 1 && p.prefix_splits == 0;
     for (int idx = tid; idx < n * (DP / 4); idx += 64 * kTokWaves) {
-        const int r = idx / (DP / 4), d = (idx - r * (DP / 4)) * 4, row = r0 + r, t = row / p.group;
+        const int r = idx / (DP / 4), d = (idx - r * (DP / 4)) * 4, row = r0 + r, t = p.by_group(row);
         if (d >= p.dim) continue;
         Join j;
         j.init();
