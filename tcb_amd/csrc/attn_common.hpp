@@ -81,7 +81,7 @@ template <int DP> __device__ __forceinline__ int swz(int row) {
     return DP == 64 ? 4 * ((row >> 1) & 1) | ((row >> 2) & 3) : 4 * (row & 3) | ((row >> 2) & 3);
 }
 
-template <bool BF> __device__ __forceinline__ a16f mma(uint4 a, uint4 b, a16f c) {
+template <bool BF, class A, class B> __device__ __forceinline__ a16f mma(A a, B b, a16f c) {
     if constexpr (BF)
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(a8bf, a), __builtin_bit_cast(a8bf, b), c, 0, 0, 0);
     else
@@ -132,10 +132,10 @@ __device__ __forceinline__ float half_sum(float x) {
     return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
 
-__device__ __forceinline__ uint4 lds16(uint32_t a) {
-    typedef uint32_t v4 __attribute__((ext_vector_type(4)));
-    typedef const __attribute__((address_space(3))) v4 *lp;
-    return __builtin_bit_cast(uint4, *(lp)a);
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));  // (a uint4's members would be read two by two)
+__device__ __forceinline__ u32x4 lds16(uint32_t a) {
+    typedef const __attribute__((address_space(3))) u32x4 *lp;
+    return *(lp)a;
 }
 __device__ __forceinline__ uint2 lds8(uint32_t a) {
     typedef uint32_t v2 __attribute__((ext_vector_type(2)));
@@ -477,7 +477,7 @@ template <int DP> struct Acc {
 template <int DP, bool BF> __device__ __forceinline__ a16f scores(uint32_t k, const uint4 (&q)[DP / 16]) {
     const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
     const uint32_t a = k + r * (2 * DP) + ((h ^ swz<DP>(r)) << 4);
-    uint4 f[DP / 16];
+    u32x4 f[DP / 16];
 #pragma unroll
     for (int i = 0; i < DP / 16; i++) f[i] = lds16(a ^ (i << 5));
     __builtin_amdgcn_sched_barrier(0);
@@ -507,7 +507,7 @@ template <int DP, bool BF> __device__ __forceinline__ bool odd_values(uint32_t v
     uint32_t any = 0;
 #pragma unroll
     for (int i = 0; i < DP / 16; i++) {
-        const uint4 x = lds16(v + i * 1024 + (threadIdx.x & 63) * 16);
+        const u32x4 x = lds16(v + i * 1024 + (threadIdx.x & 63) * 16);
         any |= ((x.x & E) + U) | ((x.y & E) + U) | ((x.z & E) + U) | ((x.w & E) + U);
     }
     return __any((any & 0x80008000u) != 0);

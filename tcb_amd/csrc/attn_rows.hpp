@@ -125,7 +125,7 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_
     auto v_frag = [&](uint32_t at, int i) {
         const int d = i % (DP / 32), c = i / (DP / 32);  // dimensions 32 d ..., keys 16 c ...
         const uint2 x = lds_tr(ring + (va ^ (d << 6)) + (at + c * 32 * DP)), y = lds_tr(ring + (va ^ (d << 6) ^ 32) + (at + c * 32 * DP + 16 * DP));
-        return make_uint4(x.x, x.y, y.x, y.y);
+        return (u32x4){x.x, x.y, y.x, y.y};
     };
     auto p_frag = [&](const uint32_t (&x)[NT][8], int i) {
         const int c = i / (DP / 32), t = c / 2, e = 4 * (c & 1);
@@ -202,7 +202,7 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_
 #pragma unroll
             for (int i = 0; i < NT * NK; i++) x[i % NT] = mma<BF>(k_frag(place * L::TILE, i), q[i / NT], i < NT ? a16f{} : x[i % NT]);
         } else {  // alone on its SIMD: operands eight ahead
-            uint4 f[NT * NK];
+            u32x4 f[NT * NK];
 #pragma unroll
             for (int i = 0; i < 8; i++) f[i] = k_frag(place * L::TILE, i);
 #pragma unroll
@@ -285,14 +285,14 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_
             const Piece16 c2 = piece_of(j + 2, page2);
             float sum = 0.0f, best = 0.0f;
             constexpr int M = NT * (NK + NV), NW = 8 * NT, AHEAD = 3;  // products, pairs of weights, operands read ahead
-            uint4 f[AHEAD + 1];
+            u32x4 f[AHEAD + 1];
             auto frag = [&](int i) { return i < NT * NK ? k_frag(there * L::TILE, i) : v_frag((2 + there) * L::TILE, i - NT * NK); };
 #pragma unroll
             for (int i = 0; i < AHEAD; i++) f[i] = frag(i);
 #pragma unroll
             for (int i = 0; i < M; i++) {
                 if (i + AHEAD < M) f[(i + AHEAD) % (AHEAD + 1)] = frag(i + AHEAD);
-                const uint4 a = f[i % (AHEAD + 1)];
+                const u32x4 a = f[i % (AHEAD + 1)];
                 if (i < NT * NK) xn[i % NT] = mma<BF>(a, q[i / NT], i < NT ? a16f{} : xn[i % NT]);
                 else o[(i - NT * NK) % (DP / 32)] = mma<BF>(a, p_frag(y, i - NT * NK), o[(i - NT * NK) % (DP / 32)]);
                 if (i % 2 == 0 && i / 2 < L::PI) share.copy_one(c2.k, ring + here * L::TILE + mine, i / 2, c2.ha, c2.hb);
