@@ -383,23 +383,21 @@ __device__ __forceinline__ Rows rows_of(const AttnArgs &p, int r0, int n, int nq
     return w;
 }
 
-// Sixteen rows of keys (or values) from token t, t a multiple of 16: the LDS copies of one wave. Rows past hi, rows
-// hidden from every row of the tile (between the first tokens and the window) and chunks past dim are zeros, whatever the
-// cache holds there; page numbers out of range read as zeros.
-struct Piece16 {
-    dma_rsrc k, v;
-    int ha, hb;  // hidden rows [ha, hb)
-};
+// Sixteen rows of keys (or values) from token t, t a multiple of 16, for the LDS copies of one wave: the page they lie in, if a
+// row sees them, and the descriptors. Rows past hi, pieces that no row of the tile sees (between the first tokens and the
+// window) and chunks past dim become zeros, whatever the cache holds there, and so do pages out of range. A piece that
+// the window's start or the first tokens' end divides comes whole.
 __device__ __forceinline__ int page16(const AttnArgs &p, const int *table, int t, int hi) {
     return t <= hi ? sload(table, t >> p.page_log2) : 0;
 }
+struct Piece16 {
+    dma_rsrc k, v;
+};
 __device__ __forceinline__ Piece16 piece16(const AttnArgs &p, int page, int head, int t, int hi, int lo, int sinks) {
     Piece16 s;
     int cnt = hi + 1 - t;
     cnt = cnt < 0 ? 0 : cnt > 16 ? 16 : cnt;
-    s.ha = sinks - t < 0 ? 0 : sinks - t;
-    s.hb = lo - t > 16 ? 16 : lo - t;
-    if (s.ha == 0 && s.hb >= 16) cnt = 0;
+    if (sinks <= t && lo >= t + 16) cnt = 0;
     if ((uint32_t)page >= (uint32_t)p.npages) {
         page = 0;
         cnt = 0;
@@ -414,24 +412,18 @@ __device__ __forceinline__ Piece16 piece16(const AttnArgs &p, int page, int head
 template <int DP> struct Lanes16 {
     static constexpr int N = DP / 32, CH = DP / 8, RPI = 64 / CH;
     uint32_t voff[N];
-    int row;  // row of instruction 0
     __device__ __forceinline__ void init(int dim) {
         const int lane = threadIdx.x & 63;
-        row = lane / CH;
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            const int r = row + i * RPI, c = (lane % CH) ^ swz<DP>(r);
+            const int r = lane / CH + i * RPI, c = (lane % CH) ^ swz<DP>(r);
             voff[i] = 8 * c < dim ? (uint32_t)(r * dim * 2 + c * 16) : 0x80000000u;
         }
     }
-    __device__ __forceinline__ void copy_one(dma_rsrc d, uint32_t dst, int i, int ha, int hb) const {
-        uint32_t o = voff[i];
-        if (hb > ha) o = (uint32_t)(row + i * RPI - ha) < (uint32_t)(hb - ha) ? 0x80000000u : o;
-        dma16(d, dst + i * 1024, o, 0);
-    }
-    __device__ __forceinline__ void copy(dma_rsrc d, uint32_t dst, int ha, int hb) const {
+    __device__ __forceinline__ void copy_one(dma_rsrc d, uint32_t dst, int i) const { dma16(d, dst + i * 1024, voff[i], 0); }
+    __device__ __forceinline__ void copy(dma_rsrc d, uint32_t dst) const {
 #pragma unroll
-        for (int i = 0; i < N; i++) copy_one(d, dst, i, ha, hb);
+        for (int i = 0; i < N; i++) copy_one(d, dst, i);
     }
 };
 

@@ -94,8 +94,8 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_
     auto k_at = [&](int j) { return ring + (j & 1) * L::TILE; };
     auto v_at = [&](int j) { return ring + (2 + (j & 1)) * L::TILE; };
     const uint32_t mine = w * (32 * DP);
-    auto copy_k = [&](const Piece16 &c, int j) { share.copy(c.k, k_at(j) + mine, c.ha, c.hb); };
-    auto copy_v = [&](const Piece16 &c, int j) { share.copy(c.v, v_at(j) + mine, c.ha, c.hb); };
+    auto copy_k = [&](const Piece16 &c, int j) { share.copy(c.k, k_at(j) + mine); };
+    auto copy_v = [&](const Piece16 &c, int j) { share.copy(c.v, v_at(j) + mine); };
 
     a16f o[DP / 32], s[NT];
     uint32_t pk[NT][8];  // weights of the block before, two a register, in the order of its score registers
@@ -170,16 +170,21 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_
         copy_v(c, 0);
     }
 
-    // Whether a key that some rows see and others do not has a value that is not finite (0 times it would reach all rows): its
-    // tile goes through plain steps, which look out for that. Those keys are the ones behind the first token's last and
-    // before the last token's window, one for each token of the tile.
+    // Whether a key that some rows see and others do not, or one that none sees in a piece of sixteen that some see, has a value
+    // that is not finite (0 times it would reach all rows): its tile goes through plain steps, which look out for that. Those
+    // keys are the ones behind the first token's last and before the last token's window, one for each token of the
+    // tile, and up to fifteen before the window and behind the first tokens.
     bool odd = false;
-    if (!PREFIX && mixed) {
+    const bool gap = all.lo_min > all.sinks;
+    if (!PREFIX && (mixed || gap)) {
         constexpr uint32_t E = BF ? 0x7F807F80u : 0x7C007C00u, U = BF ? 0x00800080u : 0x04000400u;
-        const int chunks = p.dim / 8, n0 = all.hi_max - all.hi_min, n1 = all.lo_max - all.lo_min;
+        const int l0 = gap ? (all.lo_min & ~15) < all.sinks ? all.sinks : all.lo_min & ~15 : all.lo_min;
+        const uint32_t e0 = ((uint32_t)all.sinks + 15) & ~15u;
+        const int e1 = e0 < (uint32_t)l0 ? (int)e0 : l0;
+        const int chunks = p.dim / 8, n0 = all.hi_max - all.hi_min, n1 = all.lo_max - l0, n2 = gap ? e1 - all.sinks : 0;
         uint32_t any = 0;
-        for (int i = tid; i < (n0 + n1) * chunks; i += L::THREADS) {
-            const int k = i / chunks, c = i - k * chunks, t = k < n0 ? all.hi_min + 1 + k : all.lo_min + (k - n0);
+        for (int i = tid; i < (n0 + n1 + n2) * chunks; i += L::THREADS) {
+            const int k = i / chunks, c = i - k * chunks, t = k < n0 ? all.hi_min + 1 + k : k < n0 + n1 ? l0 + (k - n0) : all.sinks + (k - n0 - n1);
             if (t < 0) continue;
             const int page = table[t >> p.page_log2];
             if ((uint32_t)page >= (uint32_t)p.npages) continue;
@@ -291,12 +296,13 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_
             for (int i = 0; i < AHEAD; i++) f[i] = frag(i);
 #pragma unroll
             for (int i = 0; i < M; i++) {
+                __builtin_amdgcn_sched_barrier(0);  // in this order: the compiler would read operands late and add up last
                 if (i + AHEAD < M) f[(i + AHEAD) % (AHEAD + 1)] = frag(i + AHEAD);
                 const u32x4 a = f[i % (AHEAD + 1)];
                 if (i < NT * NK) xn[i % NT] = mma<BF>(a, q[i / NT], i < NT ? a16f{} : xn[i % NT]);
                 else o[(i - NT * NK) % (DP / 32)] = mma<BF>(a, p_frag(y, i - NT * NK), o[(i - NT * NK) % (DP / 32)]);
-                if (i % 2 == 0 && i / 2 < L::PI) share.copy_one(c2.k, ring + here * L::TILE + mine, i / 2, c2.ha, c2.hb);
-                if (i % 2 == 0 && i / 2 >= L::PI && i / 2 < 2 * L::PI) share.copy_one(c0.v, ring + (2 + here) * L::TILE + mine, i / 2 - L::PI, c0.ha, c0.hb);
+                if (i % 2 == 0 && i / 2 < L::PI) share.copy_one(c2.k, ring + here * L::TILE + mine, i / 2);
+                if (i % 2 == 0 && i / 2 >= L::PI && i / 2 < 2 * L::PI) share.copy_one(c0.v, ring + (2 + here) * L::TILE + mine, i / 2 - L::PI);
 #pragma unroll
                 for (int e = i * NW / M; e < (i + 1) * NW / M; e++) {
                     const int t = e >> 3, k = e & 7;
@@ -304,6 +310,7 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_
                     yn[t][k] = opaque(pack2<BF>(u, v));  // (made here: the compiler would move it to the next step, where it is used)
                     sum += u;
                     sum += v;
+                    asm("" : "+v"(sum));  // (likewise)
                 }
                 const int m0 = NT * NK + 2, m1 = M - 2;  // maxima of pairs [from, to)
                 if (i >= m0 && i < m1) {

@@ -55,7 +55,8 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void tokens_o
     const Span sp = span_of<kTokBlock>(rw.hi_max, rw.lo_min, rw.sinks);
     const int nb = sp.count(), piece = it.nsplit == 1 ? nb : (nb + it.nsplit - 1) / it.nsplit;
     const int b0 = it.split * piece, b1 = b0 + piece < nb ? b0 + piece : nb;
-    const bool mixed = rw.hi_min != rw.hi_max || rw.lo_min != rw.lo_max;  // some rows see keys that others do not
+    // some rows see keys that others do not, or keys that none sees are copied with those before or behind them
+    const bool mixed = rw.hi_min != rw.hi_max || rw.lo_min != rw.lo_max || rw.lo_min > rw.sinks;
 
     const uint32_t ring = lds_addr(smem) + w * L::WAVE;
     Lanes16<DP> lanes;
@@ -76,11 +77,11 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void tokens_o
     };
     auto copy_k = [&](const Piece16 (&s)[2], int slot) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) lanes.copy(s[i].k, ring + slot * L::SLOT + i * (L::SLOT / 2), s[i].ha, s[i].hb);
+        for (int i = 0; i < 2; i++) lanes.copy(s[i].k, ring + slot * L::SLOT + i * (L::SLOT / 2));
     };
     auto copy_v = [&](const Piece16 (&s)[2], int slot) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) lanes.copy(s[i].v, ring + slot * L::SLOT + i * (L::SLOT / 2), s[i].ha, s[i].hb);
+        for (int i = 0; i < 2; i++) lanes.copy(s[i].v, ring + slot * L::SLOT + i * (L::SLOT / 2));
     };
     constexpr int D = L::SLOTS / 2, AHEAD = (L::SLOTS - 1) * (DP / 16);
     Piece16 s[2];

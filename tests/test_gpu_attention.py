@@ -222,6 +222,26 @@ def test_long_prompts_in_a_window(backend, dtype, window, sinks):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("window,sinks", [(20, 0), (37, 3), (64, 16), (300, 5), (513, 40)])
+def test_keys_that_no_token_sees(backend, dtype, window, sinks):
+    """Bad keys and values everywhere between the first tokens and the window of a request's first new token: next to the seen
+    ones in a piece, a page and a block."""
+    for heads, kv_heads, dim in ((4, 1, 128), (4, 2, 64), (33, 1, 128), (2, 1, 256)):
+        for new, kv in (([1, 1, 2, 1], [600, 561, 577, 900]), ([1, 60, 130, 300], [700, 641, 800, 1200])):
+            print(dtype, window, sinks, heads, dim, new, flush=True)
+            b = Batch(dtype, heads, kv_heads, dim, 32, new, kv, seed=33)
+            want, tol = whole(b, window, sinks)
+            for i, (n, m) in enumerate(zip(new, kv)):
+                for j in range(sinks, m - n - window + 1):
+                    page, row = b.table[i, j // 32], j % 32
+                    b.k[page, :, row] = float("nan")
+                    b.v[page, :, row] = float("inf") if j % 2 else float("nan")
+            got = b.run(backend, window, sinks)
+            assert np.isfinite(got).all()
+            assert (np.abs(got - want) <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("value", [float("nan"), float("inf")])
 def test_a_late_key_reaches_only_the_tokens_that_see_it(backend, dtype, value):
     """As above for keys far into long prompts: at a block's edge, in its middle, the last, and one that a window passes."""
