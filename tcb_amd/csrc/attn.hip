@@ -74,18 +74,24 @@ template <bool PREFIX> int launch_tokens(trhip_ctx *ctx, const AttnArgs &p, int 
     return bf ? launch_tokens<256, true, PREFIX>(ctx, p, grid) : launch_tokens<256, false, PREFIX>(ctx, p, grid);
 }
 
+constexpr int kAnyRows = 0x7FFFFFFF;
+
 // Tiles of a batch of these sizes, at most.
 int64_t tiles_of(const AttnArgs &p, const AttnCall &c, int tile_rows) {
     int64_t tiles = c.tokens * p.group / tile_rows + c.nreq;
-    if (p.row_hi <= tile_rows && tiles > c.nreq) tiles = c.nreq;
+    if (p.row_hi != kAnyRows) {
+        const int64_t few = (p.row_hi + tile_rows - 1) / tile_rows * c.nreq;
+        tiles = tiles < few ? tiles : few;
+    }
     return tiles * p.kv_heads;
 }
 
-// The launch's workgroups: as many items as a batch of these sizes can have (find_item), whatever its lengths are.
+// The launch's workgroups: as many items as a batch of these sizes can have (find_item), whatever its lengths are. The rounds
+// that pieces may take go by the tiles there will be: a tile a request beside longer ones.
 int64_t plan_items(AttnArgs &p, const AttnCall &c, int tile_rows, int block, int least) {
-    const int64_t tiles = tiles_of(p, c, tile_rows);
+    const int64_t tiles = tiles_of(p, c, tile_rows), one = c.nreq * p.kv_heads, usual = p.row_hi != kAnyRows && one < tiles ? one : tiles;
     const int64_t blocks = ((c.max_pages << p.page_log2) + block - 1) / block, most = tiles * ((blocks + least - 1) / least + 1);
-    int64_t k = (2 * tiles + p.target - 1) / p.target;
+    const int64_t k = (2 * usual + p.target - 1) / p.target;
     p.rounds = (int)(k < kMostRounds ? k : kMostRounds);
     p.part_slots = p.rounds * p.target;
     int64_t items = p.part_slots < most ? p.part_slots : most;
@@ -132,18 +138,19 @@ int launch_attn(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c) {
     p.arrivals = ctx->arrivals;
     const int cus = ctx->sm_count > 0 ? ctx->sm_count : 256;
     const int64_t rows = c.tokens * p.group;
-    // Requests of up to kTokRows rows go to attn_tokens, longer ones to attn_rows; which there are is known only from
-    // the hint, so both are launched unless it (or the sizes) rules one out. Each takes the requests of its own length, or
-    // all of them when it is alone.
+    // Requests of up to kTokMost rows go to attn_tokens, longer ones to attn_rows, which multiplies 128 rows whatever there are:
+    // 64 requests of up to 12 tokens over 2000 keys, 4 heads a kv head, took 72.6 us there, 63.9 here; of up to 24 tokens (96 rows)
+    // 79.6 and 80.4. Which there are is known only from the hint, so both are launched unless it (or the sizes) rules one
+    // out. Each takes the requests of its own length, or all of them when it is alone.
     const int64_t most_rows = (c.max_new < c.tokens ? c.max_new : c.tokens) * p.group;
-    const bool tokens_alone = most_rows <= kTokRows, rows_alone = !tokens_alone && c.tokens == c.nreq * c.max_new;
+    const bool tokens_alone = most_rows <= kTokMost, rows_alone = !tokens_alone && c.tokens == c.nreq * c.max_new;
     AttnArgs pt = p, pr = p;
     pt.target = cus * (dp <= 128 ? 2 : 1);
     pt.row_lo = 0;
-    pt.row_hi = tokens_alone ? 0x7FFFFFFF : kTokRows;
+    pt.row_hi = tokens_alone ? kAnyRows : kTokMost;
     pr.target = cus * attn_rows_per_cu(dp);
-    pr.row_lo = rows_alone ? 0 : kTokRows;
-    pr.row_hi = 0x7FFFFFFF;
+    pr.row_lo = rows_alone ? 0 : kTokMost;
+    pr.row_hi = kAnyRows;
     const int tr = attn_rows_tile(), br = attn_rows_block();
     const bool prefix = c.prefix_len > 0;
     // Pieces of long tiles are joined by a launch of their own (a workgroup that joined a tile of 128 rows alone would take
@@ -157,7 +164,7 @@ int launch_attn(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c) {
     const int64_t part = (part_t + part_r) * (dp + 2);
     const int64_t places = 8 + 8 * (int64_t)(pt.part_slots > pr.part_slots ? pt.part_slots : pr.part_slots);
     // the prefix: all tokens' rows are one tall product, its keys cut to fill the device
-    const bool tall = rows > kTokRows;
+    const bool tall = rows > kTokMost;  // (24 tokens of 4 heads behind 20000 keys: 40.8 us as rows, 35.5)
     const int ptr = tall ? tr : kTokRows, pbk = tall ? br : kTokBlock;
     const int64_t ptiles = (rows + ptr - 1) / ptr;
     int splits = 0;

@@ -228,7 +228,7 @@ template <int TR, int BK> __device__ __forceinline__ ReqShape shape_of(const Att
 //   dealt out         (sum + over (sum / c + n)) / target + c + over, least at c = sqrt(over sum / target)
 // Never more than rounds * target pieces.
 constexpr int kMostRounds = 6;
-constexpr int kRowsLeast = 4, kRowsOver = 10;  // attn_rows: blocks of a piece at least, and what one costs beside them
+constexpr int kRowsLeast = 4, kRowsOver = 20;  // attn_rows: blocks of a piece at least, and what one costs beside them
 __host__ __device__ inline int piece_blocks(float sum, int n, int most, int target, int rounds, int least, int over) {
     constexpr int kWhole = 0x40000000;
     // (in floats, made a little larger than they can have been rounded down)

@@ -11,7 +11,7 @@
 namespace trhip {
 namespace {
 
-constexpr int kTokRows = 32, kTokBlock = 32, kTokWaves = 4, kTokLeast = 8, kTokOver = 6;
+constexpr int kTokMost = 96, kTokRows = 32, kTokBlock = 32, kTokWaves = 4, kTokLeast = 8, kTokOver = 6;
 
 template <int DP> struct TokLds {
     static constexpr int SLOT = 32 * DP * 2;  // 32 keys or values
