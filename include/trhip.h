@@ -260,8 +260,8 @@ int trhip_kv_append(trhip_ctx *ctx, const trhip_kv *kv, int64_t tokens, const vo
  *               p - window < j or j < sinks (window 0: no window, every j <= p)
  * Key j lies in page table[i, j / page]; pages that no token sees are not read, so their entries may hold anything. What the cache
  * holds where a token's mask hides it never reaches that token, NaN and Inf included; a token that sees no key gets zeros. Products and sums are in
- * fp32 (matrix cores), the weights e_j are rounded to the cache's type for the product with v where a request brings many tokens,
- * and out is rounded once. Results do not depend on the order in which workgroups run. Entries out of range read as
+ * fp32 (matrix cores); where a request brings more than 96 rows (tokens times heads / kv->heads) and its tokens see 256 keys and
+ * more, the weights e_j are rounded to the cache's type for the product with v; out is rounded once. Results do not depend on the order in which workgroups run. Entries out of range read as
  * keys and values of 0; kv_len is cut to max_pages * page. max_new: the largest q_start[i + 1] - q_start[i], a hint: a smaller
  * value costs speed, not correctness. Tokens outside every request keep their rows of out. */
 int trhip_attn(trhip_ctx *ctx, const trhip_kv *kv, const void *q, int64_t q_stride, void *out, int64_t out_stride,

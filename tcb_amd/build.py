@@ -15,8 +15,7 @@ LIB = os.path.join(HERE, "libtrhip.so")
 
 SOURCES = ["api.hip", "wstore.hip", "gemv.hip", "gemv_fast.hip", "gemm_rows.hip", "actq.hip", "actq_mfma.hip",
            "swiglu.hip", "probe.hip", "prefill.hip", "actqw.hip", "rows16.hip", "actq4.hip", "fastg.hip",
-           "io16.hip", "paged.hip", "attn.hip", "attn_rows.hip",
-           "attn_rows256.hip", "attn_two.hip"]
+           "io16.hip", "paged.hip", "attn.hip", "attn_rows.hip", "attn_rows256.hip", "attn_two.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # -ffp-contract=off: no multiply-add is fused unless written as fmaf (bit-exact rounding order).
@@ -24,11 +23,11 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-ffp-contract=off",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
          "-Wall", "-Wno-unused-function", "-Wno-unused-variable"]
-# attn.hip, attn_rows256.hip: matrix instructions take their accumulators in architectural registers where they fit. The compiler's default
-# for waves of over 256 registers keeps every accumulator in the other file, a move away from the softmax.
+# attn.hip, attn_rows256.hip: matrix instructions take their accumulators in architectural registers where they fit. The
+# compiler's default for waves of over 256 registers keeps every accumulator in the other file, a move away from the softmax
+# (one token x 300 keys 11.6 -> 10.6 us, 39 requests of heads of 256 130 -> 71).
 VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
 FILE_FLAGS = {"attn.hip": VGPR_FORM, "attn_rows256.hip": VGPR_FORM}
-
 
 
 def _run(cmd):

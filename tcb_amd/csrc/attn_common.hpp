@@ -1,5 +1,6 @@
-// attn_common.hpp -- what the attention kernels over a paged cache share (attn.hip, attn_rows.hip): their arguments, how
-// a batch's rows and keys are cut into work items, the masks, and the product of one block of keys with a tile of rows.
+// attn_common.hpp -- what the attention kernels over a paged cache share (attn_tokens.hpp, attn_rows.hpp, and attn.hip, which
+// plans a call): their arguments, how a batch's rows and keys are cut into work items, the masks, the copies into LDS, and the
+// product of one block of keys with a tile of rows.
 //
 // Rows. The q_heads / kv_heads = G heads that read one kv head are rows of one matrix product: row r of a request's kv
 // head h is token r / G, head h G + r % G, so a single token brings G rows and a prompt nq G.
@@ -12,7 +13,8 @@
 // (two transposing LDS reads of four keys x sixteen dimensions each). P never leaves its lane.
 //
 // LDS rows hold their 16-byte chunks in the order chunk ^ swz(row), which spreads both reads (a column of sixteen rows,
-// and four rows x 64 bytes) over all banks; the copies into LDS place a lane's chunk by choosing which chunk it fetches.
+// and four rows x 64 bytes) over all banks (measured: no conflict in either); the copies into LDS place a lane's chunk by
+// choosing which chunk it fetches.
 #pragma once
 
 #include "trhip_internal.hpp"
@@ -105,17 +107,6 @@ template <bool BF> __device__ __forceinline__ float wide_lo(uint32_t v) {
 template <bool BF> __device__ __forceinline__ float wide_hi(uint32_t v) {
     if constexpr (BF) return __uint_as_float(v & 0xFFFF0000u);
     else return (float)__builtin_bit_cast(_Float16, (uint16_t)(v >> 16));
-}
-
-// c plus both halves of v: the sum of two rounded weights in one instruction.
-template <bool BF> __device__ __forceinline__ float add2(uint32_t v, float c) {
-    if constexpr (BF) {
-        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, v), __builtin_bit_cast(b2, 0x3F803F80u), c, false);
-    } else {
-        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-        return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, v), __builtin_bit_cast(h2, 0x3C003C00u), c, false);
-    }
 }
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -226,7 +217,11 @@ template <int TR, int BK> __device__ __forceinline__ ReqShape shape_of(const Att
 //   whole tiles       most, where all run at once; else sum / target and half the longest
 //   one round         c + over, c = sum / (target - n) (all pieces at once), where n < target
 //   dealt out         (sum + over (sum / c + n)) / target + c + over, least at c = sqrt(over sum / target)
-// Never more than rounds * target pieces.
+// Never more than rounds * target pieces, and none of under `least` blocks.
+// Measured, in us, at these constants and at others: kMostRounds 6 (64 tokens of up to 8192 keys 203; 2: 219); kTokLeast 8, two
+// blocks a wave (one token x 4096 keys 13.7; 4: 14.8, 16: 15.2); kTokOver 6 (64 requests of up to 12 tokens 72.6; 3: 78.0;
+// 12: the same); kRowsOver 20 (6 prompts of up to 300 tokens 30.1; 10: 34.4); kRowsLeast 4 (2 and
+// 8 the same).
 constexpr int kMostRounds = 6;
 constexpr int kRowsLeast = 4, kRowsOver = 20;  // attn_rows: blocks of a piece at least, and what one costs beside them
 __host__ __device__ inline int piece_blocks(float sum, int n, int most, int target, int rounds, int least, int over) {
