@@ -239,39 +239,44 @@ typedef struct trhip_kv {
  *   slots[t] = the slot of the step's token t (tokens in request order), -1 from the last one up to nslots
  *   used[0] = pages taken
  * A request that does not fit its table (max_pages) or the free pages left is refused alone: none of its pages are
- * taken, its slots are -1, kv_len[i] = old_len[i], and its tokens keep their places in q_start. (Pages it could not have still count against the
- * requests after it.) Tokens past nslots get no slot. kv_len and q_start must not be old_len or add_len. */
+ * taken, its slots are -1, kv_len[i] = old_len[i], and its tokens keep their places in q_start. (Pages it could
+ * not have still count against the requests after it.) Tokens past nslots get no slot. kv_len and q_start must not
+ * be old_len or add_len. */
 int trhip_page_tables(trhip_ctx *ctx, int64_t nreq, int page, const int32_t *old_len, const int32_t *add_len,
                       const int32_t *free_pages, int64_t nfree, int32_t *table, int64_t max_pages, int32_t *q_start,
                       int32_t *kv_len, int32_t *slots, int64_t nslots, int32_t *used);
 
-/* Key and value rows of `tokens` tokens into the cache: rows k + t * stride and v + t * stride of heads * dim elements
- * each (type: TRHIP_F32, TRHIP_F16 or TRHIP_BF16; stride in elements, so they may lie inside a merged q/k/v product's
- * rows), rounded to the cache's type as trhip_gemm_q_typed rounds, to slot slots[t]. A slot below 0 or past the cache is skipped. Two tokens
- * with the same slot leave either's row. */
+/* Key and value rows of `tokens` tokens into the cache: rows k + t * stride and v + t * stride of heads * dim
+ * elements each (type: TRHIP_F32, TRHIP_F16 or TRHIP_BF16; stride in elements, so they may lie inside a merged
+ * q/k/v product's rows), rounded to the cache's type as trhip_gemm_q_typed rounds, to slot slots[t]. A slot below
+ * 0 or past the cache is skipped. Two tokens with the same slot leave elements of either's row. */
 int trhip_kv_append(trhip_ctx *ctx, const trhip_kv *kv, int64_t tokens, const void *k, const void *v, int type,
                     int64_t stride, const int32_t *slots);
 
-/* Attention of a step's tokens over the cache, causal, in the cache's type (q and out: rows of heads * dim elements,
- * q_stride and out_stride elements apart; out must not overlap q or the cache). Request i owns tokens q_start[i] <= t <
- * q_start[i + 1] (in order, none past `tokens`) and keys 0 <= j < kv_len[i], its own tokens' included: they are the
- * last ones, so token t sits at p = kv_len[i] - q_start[i + 1] + t. Query head a reads kv head a / (heads / kv->heads):
+/* Attention of a step's tokens over the cache, causal, in the cache's type (q and out: rows of heads * dim
+ * elements, q_stride and out_stride elements apart; out must not overlap q or the cache). Request i owns tokens
+ * q_start[i] <= t < q_start[i + 1] (in order, none past `tokens`) and keys 0 <= j < kv_len[i], its own tokens'
+ * included: they are the last ones, so token t sits at p = kv_len[i] - q_start[i + 1] + t. Query head a reads kv
+ * head a / (heads / kv->heads):
  *   out[t, a] = sum_j e_j v_j / sum_j e_j, e_j = exp(scale * q.k_j - max), over j <= p with
  *               p - window < j or j < sinks (window 0: no window, every j <= p)
- * Key j lies in page table[i, j / page]; pages that no token sees are not read, so their entries may hold anything. What the cache
- * holds where a token's mask hides it never reaches that token, NaN and Inf included; a token that sees no key gets zeros. Products and sums are in
- * fp32 (matrix cores); where a request brings more than 96 rows (tokens times heads / kv->heads) and its tokens see 256 keys and
- * more, the weights e_j are rounded to the cache's type for the product with v; out is rounded once. Results do not depend on the order in which workgroups run. Entries out of range read as
- * keys and values of 0; kv_len is cut to max_pages * page. max_new: the largest q_start[i + 1] - q_start[i], a hint: a smaller
- * value costs speed, not correctness. Tokens outside every request keep their rows of out. */
+ * Key j lies in page table[i, j / page]; pages that no token sees are not read, so their entries may hold
+ * anything. What the cache holds where a token's mask hides it never reaches that token, NaN and Inf included; a
+ * token that sees no key gets zeros. Products and sums are in fp32 (matrix cores); where a request brings more
+ * than 96 rows (tokens times heads / kv->heads) and its tokens see 256 keys and more, the weights e_j are rounded
+ * to the cache's type for the product with v; out is rounded once. Results do not depend on the order in which
+ * workgroups run. Entries out of range read as keys and values of 0; kv_len is cut to max_pages * page. max_new:
+ * the largest q_start[i + 1] - q_start[i], a hint: a smaller value costs speed, not correctness. Tokens outside
+ * every request keep their rows of out. */
 int trhip_attn(trhip_ctx *ctx, const trhip_kv *kv, const void *q, int64_t q_stride, void *out, int64_t out_stride,
                int64_t tokens, int heads, int64_t nreq, const int32_t *q_start, const int32_t *kv_len,
                const int32_t *table, int64_t max_pages, int64_t max_new, int64_t window, int64_t sinks, float scale);
 
-/* trhip_attn for a batch whose requests share their first prefix_len keys (a system prompt, one document, samples of
- * one prompt): those lie in pages prefix_pages[0 ...] and are read once for all requests, as one product with every token's
- * rows, instead of once a request. kv_len, table and p then count a request's own keys behind the prefix (its own first key is
- * place 0 of table[i, 0], wherever the prefix ends in its page), and every token sees the whole prefix and its own j <= p. */
+/* trhip_attn for a batch whose requests share their first prefix_len keys (a system prompt, one document, samples
+ * of one prompt): those lie in pages prefix_pages[0 ...] and are read once for all requests, as one product with
+ * every token's rows, instead of once a request. kv_len, table and p then count a request's own keys behind the
+ * prefix (its own first key is place 0 of table[i, 0], wherever the prefix ends in its page), and every token sees
+ * the whole prefix and its own j <= p. */
 int trhip_attn_shared(trhip_ctx *ctx, const trhip_kv *kv, const void *q, int64_t q_stride, void *out, int64_t out_stride,
                       int64_t tokens, int heads, int64_t nreq, const int32_t *q_start, const int32_t *kv_len,
                       const int32_t *table, int64_t max_pages, const int32_t *prefix_pages, int64_t prefix_len,

@@ -58,7 +58,7 @@ struct AttnArgs {
     int part_slots;     // places for the pieces of tiles that are cut (of all tiles behind a prefix), each with an arrival counter
     float *part;        // [place][tile row]: DP sums, then reference (log2 units) and sum of each row
     uint32_t *arrivals;
-    int *parts;         // places in use, then for each place what the joining launch needs (Place); nullptr: the last workgroup of a tile joins it
+    int *parts;         // places in use, then for each what the joining launch needs (Place); nullptr: a tile's last workgroup joins it
 };
 
 namespace {
@@ -529,7 +529,8 @@ __device__ __forceinline__ void values_one_by_one(a16f (&o)[DP / 32], const a16f
 }
 
 // O^T += V^T P^T of 32 keys at LDS address v, P in 16 bits; TWO: in two terms (what the first rounding drops is the
-// second), so that P's rounding does not show beside the output's. EARLY: operands are read before the products, where there are registers for them.
+// second), so that P's rounding does not show beside the output's. EARLY: operands are read before the products, where there
+// are registers for them.
 template <int DP, bool BF, bool TWO, bool EARLY> __device__ __forceinline__ void values(a16f (&o)[DP / 32], const a16f &pr, uint32_t v) {
     const int lane = threadIdx.x & 63, i = lane & 15, h = lane >> 5;
     const int row = 4 * h + (i >> 2), c = 2 * ((lane >> 4) & 1) + ((i >> 1) & 1);
