@@ -242,6 +242,40 @@ def test_keys_that_no_token_sees(backend, dtype, window, sinks):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (4, 1, 64), (6, 1, 256), (33, 1, 96)])
+def test_chunks_of_a_few_tiles(backend, dtype, heads, kv_heads, dim):
+    """Requests of two and three tiles of 32 rows, alone and beside longer ones, whole and in pieces, in a window, behind a prefix."""
+    g = heads // kv_heads
+    most = 96 // g
+    new = [most, 1, max(most // 2, 1), max(most - 1, 1), max(33 // g, 1)]
+    for kv in ([most, 1, 300, 77, 40], [5000, 2600, 9000, 700, 33 + most]):
+        print(dtype, heads, kv_heads, dim, new, kv, flush=True)
+        b = Batch(dtype, heads, kv_heads, dim, 16, new, kv, seed=34)
+        got = check_whole(backend, b)
+        assert np.array_equal(got, b.run(backend))
+        check_whole(backend, b, 50, 3)
+        check_whole(backend, Batch(dtype, heads, kv_heads, dim, 16, new + [most + 1, 200], kv + [900, 200], seed=35))
+        check_whole(backend, Batch(dtype, heads, kv_heads, dim, 16, [max(most // 3, 1)] * 3, [9, 200, 70], prefix=1003, seed=36))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_a_bad_key_in_a_chunk_of_a_few_tiles(backend, dtype, value):
+    for window, sinks in ((0, 0), (40, 4)):
+        b = Batch(dtype, 4, 1, 128, 16, [24, 10], [600, 300], seed=37)
+        clean = b.run(backend, window, sinks)
+        for j in (575, 576, 583, 590, 599):
+            b.v[b.table[0, j // 16], 0, j % 16, 7] = value
+            got = b.run(backend, window, sinks)
+            for t in range(24):
+                if any(R.visible(576 + t, k, window, sinks) for k in (575, 576, 583, 590, 599) if k <= j):
+                    assert not np.isfinite(got[t, :, 7]).any() and np.isfinite(got[t, :, 8]).all()
+                else:
+                    assert np.abs(got[t] - clean[t]).max() <= 2.0 ** -7 * np.abs(clean[t]).max()
+            assert np.array_equal(got[24:], clean[24:])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("value", [float("nan"), float("inf")])
 def test_a_late_key_reaches_only_the_tokens_that_see_it(backend, dtype, value):
     """As above for keys far into long prompts: at a block's edge, in its middle, the last, and one that a window passes."""
