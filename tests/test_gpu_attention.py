@@ -468,6 +468,45 @@ def test_replayed_graph_follows_the_lengths(backend):
     assert L.trhip_graph_destroy(graph) == 0
 
 
+@pytest.mark.parametrize("new,kv,prefix", [([40, 1, 90, 1], [1500, 3000, 400, 7], 0), ([50], [6000], 0), ([1, 1, 2], [40, 300, 9], 2000),
+                                           ([9, 30, 1, 60], [40, 300, 9, 61], 777)])
+def test_replayed_graph_of_every_launch(backend, new, kv, prefix):
+    """Prompts beside tokens, a chunk in joined pieces, few and many rows behind a prefix: captured, then replayed with other
+    lengths and rows between eager calls."""
+    L, ctx, dev = _lib.lib(), backend.ctx, "cuda:0"
+    b = Batch("f16", 8, 2, 128, 16, new, kv, prefix=prefix, seed=38, poison=False)
+    k, v, q = b.k.to(dev), b.v.to(dev), b.q.to(dev)
+    out, eager = (torch.zeros((b.tokens, 8, 128), dtype=torch.float16, device=dev) for _ in range(2))
+    start, lens, table = torch.from_numpy(b.start).to(dev), torch.tensor(b.kv, dtype=torch.int32, device=dev), torch.from_numpy(b.table).to(dev)
+    lead = torch.from_numpy(b.prefix_table).to(dev)
+    cache = tcb_amd.KVCache(tcb_amd.F16, k.shape[0], 16, 2, 128, k.data_ptr(), v.data_ptr())
+
+    def call(to):
+        args = (cache, q.data_ptr(), 1024, to.data_ptr(), 1024, b.tokens, 8, len(new), start.data_ptr(), lens.data_ptr(), table.data_ptr(), b.most)
+        if prefix:
+            backend.AttentionShared(*args, lead.data_ptr(), prefix, max_new=max(new))
+        else:
+            backend.Attention(*args, max_new=max(new))
+
+    torch.cuda.synchronize()
+    call(eager)
+    ctx.sync()
+    assert L.trhip_graph_begin(ctx.h) == 0
+    call(out)
+    graph = ctypes.c_void_p()
+    assert L.trhip_graph_end(ctx.h, ctypes.byref(graph)) == 0
+    for step in range(4):
+        lens.copy_(torch.tensor([max(n, m - 317 * step) for n, m in zip(new, kv)], dtype=torch.int32))
+        q.mul_(-0.9)
+        out.fill_(5.0)
+        torch.cuda.synchronize()
+        call(eager)
+        assert L.trhip_graph_launch(ctx.h, graph) == 0
+        ctx.sync()
+        assert torch.equal(out, eager)
+    assert L.trhip_graph_destroy(graph) == 0
+
+
 def test_refusals(backend):
     x = torch.zeros(4096, dtype=torch.int32, device="cuda:0")
     a = x.data_ptr()
