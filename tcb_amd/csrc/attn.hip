@@ -14,13 +14,13 @@ template <int DP, bool BF, bool PREFIX> __global__ __launch_bounds__(64 * kTokWa
     tokens_of<DP, BF, PREFIX>(p, blockIdx.x, gridDim.x);
 }
 
-// Joins the pieces of a tile's rows, and the shared prefix's: a workgroup for sixteen rows of a place (workgroups of
-// places that hold no tile's first piece end at once).
-template <int DP, bool BF> __global__ __launch_bounds__(256) void attn_join(const AttnArgs p, int tr) {
+// Joins the pieces of a tile's rows, and the shared prefix's: a workgroup for `each` rows of a place (workgroups of places that
+// hold no tile's first piece end at once). All it does is read the pieces, eight in flight a thread.
+template <int DP, bool BF> __global__ __launch_bounds__(256) void attn_join(const AttnArgs p, int tr, int each) {
     constexpr int ST = DP + 2, AT = 8;
     if ((int)blockIdx.x >= p.parts[0]) return;
     const Place t = reinterpret_cast<const Place *>(p.parts + 8)[blockIdx.x];
-    const int g = 16 * blockIdx.y, rows = t.n - g < 16 ? t.n - g : 16;
+    const int g = each * blockIdx.y, rows = t.n - g < each ? t.n - g : each;
     if (t.pieces == 0 || rows <= 0) return;
     const int64_t step = (int64_t)p.kv_heads * tr * ST, pstep = (int64_t)p.tokens * p.heads * ST;
     for (int idx = threadIdx.x; idx < rows * (DP / 4); idx += 256) {
@@ -49,14 +49,17 @@ template <int DP, bool BF> __global__ __launch_bounds__(256) void attn_join(cons
     }
 }
 
-template <int DP, bool BF> int launch_join(trhip_ctx *ctx, const AttnArgs &p, int tr) {
-    hipLaunchKernelGGL((attn_join<DP, BF>), dim3((unsigned)p.part_slots, (unsigned)(tr / 16)), dim3(256), 0, ctx->stream, p, tr);
+template <int DP, bool BF> int launch_join(trhip_ctx *ctx, const AttnArgs &p, int tr, int each) {
+    hipLaunchKernelGGL((attn_join<DP, BF>), dim3((unsigned)p.part_slots, (unsigned)(tr / each)), dim3(256), 0, ctx->stream, p, tr, each);
     return launch_check(ctx, "attention");
 }
-int launch_join(trhip_ctx *ctx, const AttnArgs &p, int dp, bool bf, int tr) {
-    if (dp == 64) return bf ? launch_join<64, true>(ctx, p, tr) : launch_join<64, false>(ctx, p, tr);
-    if (dp == 128) return bf ? launch_join<128, true>(ctx, p, tr) : launch_join<128, false>(ctx, p, tr);
-    return bf ? launch_join<256, true>(ctx, p, tr) : launch_join<256, false>(ctx, p, tr);
+// Sixteen rows a workgroup, four where that would leave CUs without one (a chunk of 64 tokens over 16000 keys: 57.0 us, 48.2 with
+// four; a prompt of 512: 22.5, 25.0, for its idle workgroups).
+int launch_join(trhip_ctx *ctx, const AttnArgs &p, int dp, bool bf, int tr, int64_t tiles, int cus) {
+    const int each = tiles * (tr / 16) < cus ? 4 : 16;
+    if (dp == 64) return bf ? launch_join<64, true>(ctx, p, tr, each) : launch_join<64, false>(ctx, p, tr, each);
+    if (dp == 128) return bf ? launch_join<128, true>(ctx, p, tr, each) : launch_join<128, false>(ctx, p, tr, each);
+    return bf ? launch_join<256, true>(ctx, p, tr, each) : launch_join<256, false>(ctx, p, tr, each);
 }
 
 template <int DP, bool BF, bool PREFIX> int launch_tokens(trhip_ctx *ctx, const AttnArgs &p, int64_t grid) {
@@ -194,12 +197,12 @@ int launch_attn(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c) {
     bool rows_left = !tokens_alone, tokens_left = !rows_alone;
     if (two && prefix) {
         st = launch_attn_two(ctx, tall ? pr : pt, (int)grid_p, tall ? TwoKind::PrefixRows : TwoKind::PrefixTokens, pt, (int)grid_t, dp, bf, (int)grid_p);
-        if (st == TRHIP_OK) st = launch_join(ctx, pt, dp, bf, kTokRows);
+        if (st == TRHIP_OK) st = launch_join(ctx, pt, dp, bf, kTokRows, tiles_of(pt, c, kTokRows), cus);
         tokens_left = false;
     } else if (two) {
         const bool rows_first = c.tokens * p.group / tr >= 3 * c.nreq;
         st = launch_attn_two(ctx, pr, (int)grid_r, TwoKind::Rows, pt, (int)grid_t, dp, bf, rows_first ? (int)grid_r : cus);
-        if (st == TRHIP_OK && cut) st = launch_join(ctx, pr, dp, bf, tr);
+        if (st == TRHIP_OK && cut) st = launch_join(ctx, pr, dp, bf, tr, tiles_r, cus);
         return st;
     } else if (prefix) {
         st = tall ? launch_attn_rows(ctx, pr, dp, bf, true, grid_p) : launch_tokens<true>(ctx, pt, dp, bf, grid_p);
@@ -207,12 +210,12 @@ int launch_attn(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c) {
     if (st != TRHIP_OK) return st;
     if (tokens_left) {
         st = launch_tokens<false>(ctx, pt, dp, bf, grid_t);
-        if (st == TRHIP_OK && prefix) st = launch_join(ctx, pt, dp, bf, kTokRows);
+        if (st == TRHIP_OK && prefix) st = launch_join(ctx, pt, dp, bf, kTokRows, tiles_of(pt, c, kTokRows), cus);
         if (st != TRHIP_OK) return st;
     }
     if (rows_left) {
         st = launch_attn_rows(ctx, pr, dp, bf, false, grid_r);
-        if (st == TRHIP_OK && cut) st = launch_join(ctx, pr, dp, bf, tr);
+        if (st == TRHIP_OK && cut) st = launch_join(ctx, pr, dp, bf, tr, tiles_r, cus);
     }
     return st;
 }

@@ -220,10 +220,10 @@ template <int TR, int BK> __device__ __forceinline__ ReqShape shape_of(const Att
 // Never more than rounds * target pieces, and none of under `least` blocks.
 // Measured, in us, at these constants and at others: kMostRounds 6 (64 tokens of up to 8192 keys 203; 2: 219); kTokLeast 8, two
 // blocks a wave (one token x 4096 keys 13.7; 4: 14.8, 16: 15.2); kTokOver 6 (64 requests of up to 12 tokens 72.6; 3: 78.0;
-// 12: the same); kRowsOver 20 (6 prompts of up to 300 tokens 30.1; 10: 34.4); kRowsLeast 4 (2 and
-// 8 the same).
+// 12: the same); kRowsOver 20 (6 prompts of up to 300 tokens 30.1; 10: 34.4); kRowsLeast 6
+// (32 tokens behind 4096 shared keys 21.8; 4: 22.7, 2: 27.0).
 constexpr int kMostRounds = 6;
-constexpr int kRowsLeast = 4, kRowsOver = 20;  // attn_rows: blocks of a piece at least, and what one costs beside them
+constexpr int kRowsLeast = 6, kRowsOver = 20;  // attn_rows: blocks of a piece at least, and what one costs beside them
 __host__ __device__ inline int piece_blocks(float sum, int n, int most, int target, int rounds, int least, int over) {
     constexpr int kWhole = 0x40000000;
     // (in floats, made a little larger than they can have been rounded down)
