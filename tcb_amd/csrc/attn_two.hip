@@ -1,6 +1,6 @@
 // attn_two.hip -- two kinds of attention work in one launch, two workgroups a CU: few rows, which wait for the cache's bytes,
 // beside many rows (a batch of prompts and tokens) or a shared prefix under its requests' own keys. One after the other, each
-// leaves half the device idle (32 tokens behind 4096 shared keys: 32 us in two launches, 23 in this). The kinds take turns in
+// leaves half the device idle (32 tokens behind 4096 shared keys: 32 us in two launches, 24 in this when it came in). The kinds take turns in
 // runs of `turn` workgroups, so that with as many as there are CUs each CU starts with one of either.
 #include "attn_rows.hpp"
 #include "attn_tokens.hpp"
