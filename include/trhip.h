@@ -236,7 +236,8 @@ typedef struct trhip_kv {
  * ceil((old + add) / page) pages; the fresh ones are taken from free_pages in order, request after request:
  *   table[i, j] = free_pages[base_i + j - have_i], have_i <= j < need_i (other entries are left as they are)
  *   q_start[i] = sum of add_len before i (nreq + 1 values), kv_len[i] = old_len[i] + add_len[i]
- *   slots[t] = the slot of the step's token t (tokens in request order), -1 from the last one up to nslots
+ *   slots[t] = the slot of the step's token t (tokens in request order), -1 from the last one up to nslots and where the page's
+ *              number is negative or its slot past 2^31 - 1
  *   used[0] = pages taken
  * A request that does not fit its table (max_pages) or the free pages left is refused alone: none of its pages are
  * taken, its slots are -1, kv_len[i] = old_len[i], and its tokens keep their places in q_start. (Pages it could

@@ -109,7 +109,8 @@ __global__ __launch_bounds__(THREADS) void page_tables_kernel(int nreq, int page
                 int64_t pg = 0;
                 if (pi < h) pg = table[(c + lo) * max_pages + pi];
                 else pg = free_list[s_base[lo] + (pi - h)];
-                out[u] = (int)((pg << page_log2) + (pos & (page - 1)));
+                const int64_t slot = (pg << page_log2) + (pos & (page - 1));
+                if (slot >= 0 && slot <= 0x7FFFFFFF) out[u] = (int)slot;  // a page number out of range gives no slot
             }
         }
         tok0 = tt;

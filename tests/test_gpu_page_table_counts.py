@@ -60,3 +60,23 @@ def test_pages_taken(backend, old, add, nfree, most):
     assert got[1].tolist() == [0] + np.cumsum(add).tolist()
     assert got[4][0] == want[3] == (got[0] != table).sum() <= nfree
     assert set(got[0][got[0] != table].tolist()) == set(free[:got[4][0]].tolist())
+
+
+@pytest.mark.parametrize("page", [16, 4096])
+def test_page_numbers_out_of_range(backend, page):
+    """A page number whose slots do not fit 32 bits, or a negative one, gives no slot: never another page's (from the free list, from a table)."""
+    last = (2 ** 31 - 1) // page  # of the highest page whose slots fit
+    numbers = [2 ** 32 // page if page > 16 else 2 ** 28, last, last + 1, -1, -2 ** 31, 2 ** 31 - 1, 3]
+    for free in (True, False):
+        print(page, free, flush=True)
+        n = len(numbers)
+        old, table = [0 if free else 1] * n, np.full((n, 2), 5, np.int32)
+        if not free:
+            table[:, 0] = numbers
+        got = run(backend, page, old, [2] * n, numbers if free else [], table, 2 * n)
+        want = []
+        for x in numbers:
+            first = x * page + (0 if free else 1)
+            want += [first + i if 0 <= first + i < 2 ** 31 else -1 for i in range(2)]
+        assert got[3].tolist() == want
+        assert got[4][0] == (n if free else 0)
