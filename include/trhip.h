@@ -239,10 +239,13 @@ typedef struct trhip_kv {
  *   slots[t] = the slot of the step's token t (tokens in request order), -1 from the last one up to nslots and where the page's
  *              number is negative or its slot past 2^31 - 1
  *   used[0] = pages taken
- * A request that does not fit its table (max_pages) or the free pages left is refused alone: none of its pages are
- * taken, its slots are -1, kv_len[i] = old_len[i], and its tokens keep their places in q_start. (Pages it could
- * not have still count against the requests after it.) Tokens past nslots get no slot. kv_len and q_start must not
- * be old_len or add_len. */
+ * A request that does not fit its table (max_pages) or the free pages left is refused whole: none of its pages are
+ * taken, its slots are -1, kv_len[i] = old_len[i], and its tokens keep their places in q_start. Free pages are given
+ * out in order: one refused for want of them keeps its place, so the requests behind it that need a fresh page are
+ * refused too, and none overtakes it (one refused by its table's width holds up nobody). A request was refused
+ * where kv_len[i] != old_len[i] + add_len[i]: its rows of a trhip_attn on these arrays mean nothing (they are taken for
+ * the last tokens of the old keys), and the program brings its tokens again in a later step. Tokens past nslots get
+ * no slot. kv_len and q_start must not be old_len or add_len. */
 int trhip_page_tables(trhip_ctx *ctx, int64_t nreq, int page, const int32_t *old_len, const int32_t *add_len,
                       const int32_t *free_pages, int64_t nfree, int32_t *table, int64_t max_pages, int32_t *q_start,
                       int32_t *kv_len, int32_t *slots, int64_t nslots, int32_t *used);

@@ -80,3 +80,14 @@ def test_page_numbers_out_of_range(backend, page):
             want += [first + i if 0 <= first + i < 2 ** 31 else -1 for i in range(2)]
         assert got[3].tolist() == want
         assert got[4][0] == (n if free else 0)
+
+
+def test_a_refused_request_holds_up_those_that_need_pages(backend):
+    """For want of pages: the requests behind it that need one are refused too. By its table's width: nobody else is."""
+    table = np.full((4, 4), -1, np.int32)
+    table[3, 0] = 9
+    kv_len, slots = run(backend, 16, [0, 0, 0, 3], [10, 60, 5, 2], [1, 2, 3], table, 77)[2:4]
+    assert kv_len.tolist() == [10, 0, 0, 5] and slots.tolist() == list(range(16, 26)) + [-1] * 65 + [9 * 16 + 3, 9 * 16 + 4]
+    kv_len, slots = run(backend, 16, [0, 0, 0, 3], [10, 65, 5, 2], [1, 2, 3], table, 82)[2:4]
+    assert kv_len.tolist() == [10, 0, 5, 5]
+    assert slots.tolist() == list(range(16, 26)) + [-1] * 65 + list(range(32, 37)) + [9 * 16 + 3, 9 * 16 + 4]
