@@ -583,8 +583,8 @@ template <int DP, int NB> __device__ __forceinline__ void softmax_step(Acc<DP> &
 #pragma unroll
         for (int i = 0; i < 16; i++) x = fmaxf(x, s[b][i]);
     x = half_max(x);
-    if (__any(x > A.m + slack)) {
-        const float m = x > A.m + slack ? x : A.m;
+    if (__any(x - A.m > slack)) {  // (a difference: the sum rounds to the next score where they are far from 0)
+        const float m = x - A.m > slack ? x : A.m;
         const float a = m > A.m ? exp2_hw((A.m - m) * scale) : 1.0f;  // A.m = -Inf: 0
         A.l *= a;
 #pragma unroll

@@ -138,13 +138,15 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_
         return make_uint4(x[t][e], x[t][e + 1], x[t][e + 2], x[t][e + 3]);
     };
     // The reference: raised to a block's maximum where that exceeds it by more than 2^8. neg: minus the reference, for the
-    // exponentials' fused step; 0 where scores are too large for that (far) and are made relative first.
+    // exponentials' fused step; 0 where scores are too large for that (far) and are made relative first. Far scores can lie more
+    // than 2^8 apart and next to each other, so their difference is looked at, not a sum that rounds to the next one.
     float neg = 0.0f;
     bool far = false;
+    auto exceeds = [&] { return (top - mf) * p.scale > 8.0f; };
     auto raise = [&](uint32_t (&pk)[NT][8], bool weights) {
         const float y = top * p.scale, r = fabsf(y) > 1048576.0f ? y : ceilf(y);
-        const bool up = r > ms + 8.0f;
-        const float a = up ? exp2_hw(ms - r) : 1.0f;  // from -Inf: 0
+        const bool up = exceeds();
+        const float a = up ? exp2_hw(far && r == y ? (mf - top) * p.scale : ms - r) : 1.0f;  // from -Inf: 0
         ms = up ? r : ms;
         mf = up ? top : mf;
         l *= a;
@@ -242,7 +244,7 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_
             for (int t = 0; t < NT; t++) mask(s[t], rw, t0 + 32 * t);
         }
         top = half_max(maximum(s));
-        if (__any(top * p.scale > ms + 8.0f)) raise(pk, false);
+        if (__any(exceeds())) raise(pk, false);
         relative(s);
         bool odd_here = false;
 #pragma unroll
@@ -273,7 +275,7 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_
         copy_k(c1, 1);
         qk(s, 0);
         top = half_max(maximum(s));
-        bool higher = top * p.scale > ms + 8.0f;
+        bool higher = exceeds();
         a16f s1[NT];
         uint32_t p1[NT][8];
         // Step j, P = j % 2: scores x, weights y of block j - 1; leaves the next scores in xn, this block's weights in yn.
@@ -287,7 +289,7 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_
 #pragma unroll
                 for (int t = 0; t < NT; t++) mask(x[t], rw, t0 + 32 * t);
                 top = half_max(maximum(x));
-                higher = top * p.scale > ms + 8.0f;
+                higher = exceeds();
             }
             if (__any(higher)) raise(y, true);
             relative(x);
@@ -328,7 +330,7 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_
                 }
                 if (i == M - 2) {
                     top = half_max(best);
-                    higher = top * p.scale > ms + 8.0f;
+                    higher = exceeds();
                 }
             }
             l += sum;
