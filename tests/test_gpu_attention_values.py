@@ -86,3 +86,16 @@ def test_far_scores_one_step_apart(backend, dtype, dim, heads, new):
         want = c.v[then].double().numpy()
         assert np.isfinite(got).all()
         assert (np.abs(got - want) <= 2.0 ** -9 * np.abs(want) + 2.0 ** -15 * np.abs(c.v.double().numpy()).max()).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("reqs", [1, 40])
+@pytest.mark.parametrize("scale", [1e-38, 1e-45])
+def test_smallest_scales(backend, dtype, reqs, scale):
+    """All weights are equal: the mean over a shared prefix and the own keys behind it, whichever kernels have the two."""
+    c = Case(dtype, 4, 128, 1, 400, prefix=300, reqs=reqs)
+    g = torch.Generator().manual_seed(reqs)
+    c.q[:], c.k[:] = (torch.randn(x.shape, generator=g).to(x.dtype) for x in (c.q, c.k))
+    c.v[:300], c.v[300:] = 1.0, 5.0
+    got = c.run(backend, scale)
+    assert (np.abs(got - 2.0) <= 2.0 ** -8).all()  # (the mean is 2 and representable: half a unit of bf16 below it)
