@@ -268,7 +268,8 @@ int trhip_kv_append(trhip_ctx *ctx, const trhip_kv *kv, int64_t tokens, const vo
  * anything. What the cache holds where a token's mask hides it never reaches that token, NaN and Inf included; a
  * token that sees no key gets zeros. Products and sums are in fp32 (matrix cores); where a request brings more
  * than 96 rows (tokens times heads / kv->heads) and its tokens see 256 keys and more, the weights e_j are rounded
- * to the cache's type for the product with v; out is rounded once. Results do not depend on the order in which
+ * to the cache's type for the product with v (f16: to 2^-31 of the row's largest where they are smaller than 2^-20 of
+ * it); out is rounded once. Results do not depend on the order in which
  * workgroups run. Entries out of range read as keys and values of 0; kv_len is cut to max_pages * page. max_new:
  * the largest q_start[i + 1] - q_start[i], a hint: a smaller value costs speed, not correctness. Tokens outside
  * every request keep their rows of out. */

@@ -134,7 +134,6 @@ int launch_attn(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c) {
     p.window = (int)c.window;
     p.sinks = (int)c.sinks;
     p.scale = c.scale * 1.44269504088896341f;
-    p.slack = 8.0f / p.scale < 3e38f ? 8.0f / p.scale : 3e38f;  // (finite: less than a first score's excess over -Inf)
     p.by_group.of(p.group);
     p.by_heads.of(p.kv_heads);
     p.out_aligned = (reinterpret_cast<uintptr_t>(c.out) % 8 == 0) && c.out_stride % 4 == 0;

@@ -50,7 +50,7 @@ struct AttnArgs {
     float *prefix_part;  // [split][token][head] partial results of the prefix: DP sums, reference, sum
     int nreq, tokens, heads, kv_heads, group, dim;
     int window, sinks;  // window 0: none
-    float scale, slack; // softmax scale times log2 e; what is 2^8 in units of scores
+    float scale;        // softmax scale times log2 e
     int out_aligned;    // 8-byte aligned rows
     Div by_group, by_heads;  // by group, kv_heads
     int target, rounds; // workgroups at a time, and how often at most
@@ -446,16 +446,24 @@ template <int DP> __device__ __forceinline__ void load_q(const AttnArgs &p, uint
 
 // ---- one block of keys -------------------------------------------------------------------------------------------------
 
+// Weights stand in 16 bits relative to a reference m (log2 units): the row's largest weight is 2^kLift to 2^(kLift + 8). f16 has
+// normal numbers down to 2^-14 and nothing below 2^-24, so its weights stand as high as they can; bf16 reaches as far as fp32.
+template <bool BF> constexpr int kLift = BF ? 0 : 7;
+constexpr float kFar = 1048576.0f;  // scores past 2^20 (log2 units) are made relative to another score first
+
 template <int DP> struct Acc {
     a16f o[DP / 32];
-    float m, l;  // running maximum of the scores; this lane's share of the sum (its half of the keys)
+    float m, f, l;  // reference; the score it came from; this lane's share of the sum (its half of the keys)
+    float most;     // the highest reference so far
+    bool far;
     __device__ __forceinline__ void init() {
 #pragma unroll
         for (int i = 0; i < DP / 32; i++)
 #pragma unroll
             for (int r = 0; r < 16; r++) o[i][r] = 0.0f;
-        m = -__builtin_inff();
+        m = f = most = -__builtin_inff();
         l = 0.0f;
+        far = false;
     }
 };
 
@@ -572,50 +580,53 @@ template <int DP, bool BF, bool TWO, bool EARLY> __device__ __forceinline__ void
     }
 }
 
-// The running softmax's step over NB blocks of 32 scores: scores replaced by exp2(scale (s - m)), m the row's reference.
-// It is raised to the largest score so far, and O^T and the sum are rescaled to it, only where that exceeds it by more than
-// 2^8: weights of up to 2^8 cost no precision, rescaling every time a maximum grows cost a quarter of a token step's
-// instructions. A row that has seen nothing keeps m = -Inf and adds nothing.
-template <int DP, int NB> __device__ __forceinline__ void softmax_step(Acc<DP> &A, a16f (&s)[NB], float scale, float slack) {
-    float x = s[0][0];
+// The running softmax's step over 32 scores: scores replaced by exp2(scale s - m), m the row's reference, a whole power of two
+// (the score itself where that is far from 0). It is raised to the largest score only where that exceeds the one it came from
+// by more than 2^8, and O^T and the sum are then rescaled, exactly: weights of up to 2^8 cost no precision, rescaling every
+// time a maximum grows cost a quarter of a token step's instructions. A row that has seen nothing keeps m = -Inf and adds nothing.
+// f16: where a block's largest weight is below 2^-7 (one early key outweighs the rest), the smaller ones would lose their last bits
+// or vanish. The reference is then lowered to that block, by 2^64 in all at most, and O^T and the sum, which are fp32, are scaled up.
+template <int DP, bool BF> __device__ __forceinline__ void softmax_step(Acc<DP> &A, a16f &s, float scale) {
+    float x = s[0];
 #pragma unroll
-    for (int b = 0; b < NB; b++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) x = fmaxf(x, s[b][i]);
+    for (int i = 0; i < 16; i++) x = fmaxf(x, s[i]);
     x = half_max(x);
-    if (__any(x - A.m > slack)) {  // (a difference: the sum rounds to the next score where they are far from 0)
-        const float m = x - A.m > slack ? x : A.m;
-        const float a = m > A.m ? exp2_hw((A.m - m) * scale) : 1.0f;  // A.m = -Inf: 0
+    const float d = (x - A.f) * scale;  // (a difference: a sum rounds to the next score where they are far from 0)
+    const bool low = !BF && d < -14.0f && x > -__builtin_inff() && !A.far && A.m > A.most - 64.0f;
+    if (__any(d > 8.0f || low)) {
+        const bool move = d > 8.0f || low;
+        float y = x * scale;
+        if (!BF) {
+            const float least = A.most - 64.0f + kLift<BF>;
+            const bool cut = low && y < least;
+            y = cut ? least : y;
+            x = cut ? least * __builtin_amdgcn_rcpf(scale) : x;
+        }
+        const bool far = fabsf(y) > kFar;
+        const float r = far ? y : ceilf(y) - kLift<BF>;
+        const float a = move ? exp2_hw(far && A.far ? (A.f - x) * scale : A.m - r) : 1.0f;  // from -Inf: 0
         A.l *= a;
 #pragma unroll
         for (int d = 0; d < DP / 32; d++)
 #pragma unroll
             for (int i = 0; i < 16; i++) A.o[d][i] *= a;
-        A.m = m;
+        A.m = move ? r : A.m;
+        A.f = move ? x : A.f;
+        A.far = move ? far : A.far;
+        A.most = fmaxf(A.most, A.m);
     }
-    const float mu = A.m == -__builtin_inff() ? 0.0f : A.m, ms = mu * scale;
-    // One fused step an element. The rounding of ms is the same factor in every weight and cancels, as long as it is
-    // small: where scores are past 2^20 the difference is taken first.
-    const bool far = __any(fabsf(ms) > 1048576.0f);
+    // One fused step an element. Where scores are far the difference is taken first.
+    const float neg = A.far || A.m == -__builtin_inff() ? 0.0f : -A.m;
+    if (__any(A.far)) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[i] -= A.far ? A.f : 0.0f;
+    }
     float l = 0.0f;
-    if (far) {
 #pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) s[b][i] = (s[b][i] - mu) * scale;
-    } else {
-#pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) s[b][i] = fmaf(s[b][i], scale, -ms);
+    for (int i = 0; i < 16; i++) {
+        s[i] = exp2_hw(fmaf(s[i], scale, neg));
+        l += s[i];
     }
-#pragma unroll
-    for (int b = 0; b < NB; b++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            s[b][i] = exp2_hw(s[b][i]);
-            l += s[b][i];
-        }
     A.l += l;
 }
 

@@ -11,8 +11,9 @@
 // it made the compiler copy O^T between registers at every join, a third of the instructions (616 us, 597 without).
 //
 // The softmax's reference (what is subtracted from a row's scores) is a whole power of two, raised only when a block's
-// maximum exceeds it by more than 2^8: then the sums, O^T and the pending weights are multiplied by a power of two, exactly.
-// The weights stay below 2^9, inside f16 and bf16, and lose no precision to a reference that is a little low. The row's sum is
+// maximum exceeds it by more than 2^8: then the sums, O^T and the pending weights are multiplied by a power of two, exactly (f16
+// weights below its normal numbers lose bits). The weights stay below 2^9 in bf16 and 2^16 in f16, where they stand 2^7 higher: below 2^-14 f16
+// loses bits, below 2^-25 everything, so a weight is held to 2^-11 of itself or 2^-31 of the row's largest. The row's sum is
 // taken of the weights in fp32; for the product with V the skewed loop rounds them to 16 bits, to nearest, so that many
 // keys' roundings average out. Rows that see fewer than kFewKeys keys go through the plain step, which multiplies a second
 // term of each weight (what the rounding dropped): as near as with weights in fp32, for half again as many products (the
@@ -144,9 +145,10 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_
     bool far = false;
     auto exceeds = [&] { return (top - mf) * p.scale > 8.0f; };
     auto raise = [&](uint32_t (&pk)[NT][8], bool weights) {
-        const float y = top * p.scale, r = fabsf(y) > 1048576.0f ? y : ceilf(y);
-        const bool up = exceeds();
-        const float a = up ? exp2_hw(far && r == y ? (mf - top) * p.scale : ms - r) : 1.0f;  // from -Inf: 0
+        const float y = top * p.scale;
+        const bool up = exceeds(), to_far = fabsf(y) > kFar;
+        const float r = to_far ? y : ceilf(y) - kLift<BF>;
+        const float a = up ? exp2_hw(far && to_far ? (mf - top) * p.scale : ms - r) : 1.0f;  // from -Inf: 0
         ms = up ? r : ms;
         mf = up ? top : mf;
         l *= a;
@@ -160,7 +162,7 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_
 #pragma unroll
                 for (int i = 0; i < 8; i++) pk[t][i] = pack2<BF>(wide_lo<BF>(pk[t][i]) * a, wide_hi<BF>(pk[t][i]) * a);
         }
-        far = fabsf(ms) > 1048576.0f && ms != -__builtin_inff();
+        far = up ? to_far : far;
         neg = far || ms == -__builtin_inff() ? 0.0f : -ms;
     };
     auto relative = [&](a16f (&x)[NT]) {

@@ -108,17 +108,16 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void tokens_o
         pieces(b + D * kTokWaves, pg, s);
         pg = pages_of(b + (D + 1) * kTokWaves);
         wait_vmcnt(AHEAD);
-        a16f x[1];
-        x[0] = scores<DP, BF>(ring + slot * L::SLOT, q);
+        a16f x = scores<DP, BF>(ring + slot * L::SLOT, q);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot has been read
         copy_k(s, slot);
         const bool all = all_see(rw, t, 32);
-        if (!all) mask(x[0], rw, t);
-        softmax_step<DP, 1>(A, x, p.scale, p.slack);
+        if (!all) mask(x, rw, t);
+        softmax_step<DP, BF>(A, x, p.scale);
         wait_vmcnt(AHEAD);
         const uint32_t v = ring + (slot + 1) * L::SLOT;
-        if (!all && mixed && odd_values<DP, BF>(v)) values_one_by_one<DP, BF>(A.o, x[0], v, rw.hi, rw.lo, rw.sinks, t);
-        else values<DP, BF, true, true>(A.o, x[0], v);
+        if (!all && mixed && odd_values<DP, BF>(v)) values_one_by_one<DP, BF>(A.o, x, v, rw.hi, rw.lo, rw.sinks, t);
+        else values<DP, BF, true, true>(A.o, x, v);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         copy_v(s, slot + 1);
         slot = slot + 2 == L::SLOTS ? 0 : slot + 2;
@@ -136,7 +135,7 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void tokens_o
             for (int g = 0; g < 4; g++)
                 *reinterpret_cast<float4 *>(mine + r * L::OSTRIDE + 32 * d + 8 * g + 4 * h) =
                     make_float4(A.o[d][4 * g], A.o[d][4 * g + 1], A.o[d][4 * g + 2], A.o[d][4 * g + 3]);
-        if (h == 0) ml[w * 32 + r] = make_float2(A.m * p.scale, l);
+        if (h == 0) ml[w * 32 + r] = make_float2(A.m, l);
     }
     __syncthreads();
     const bool direct = !PREFIX && it.nsplit == 1 && p.prefix_splits == 0;

@@ -99,3 +99,95 @@ def test_smallest_scales(backend, dtype, reqs, scale):
     c.v[:300], c.v[300:] = 1.0, 5.0
     got = c.run(backend, scale)
     assert (np.abs(got - 2.0) <= 2.0 ** -8).all()  # (the mean is 2 and representable: half a unit of bf16 below it)
+
+
+def dominated(heads, dim, new, kv, prefix, reqs, gap, at, seed):
+    """f16: one key `gap` nats above all others, with values of 0; the others' scores are equal up to 0.5, their values about 1."""
+    c = Case("f16", heads, dim, new, kv, prefix=prefix, reqs=reqs)
+    g = torch.Generator().manual_seed(seed)
+    c.q[:, :, 0] = 1.0
+    c.k[:, 0] = 0.5 * torch.rand(kv, generator=g)
+    c.v[:] = (1.0 + 0.5 * torch.randn((kv, dim), generator=g)).half()
+    c.k[at, 0], c.v[at] = gap, 0.0
+    return c
+
+
+def formula(c):
+    """(out, spread) of the formula in float64 on the device, scale 1: spread = sum_j e_j |v_j| / sum_j e_j."""
+    k, v = c.k.to(DEV).double(), c.v.to(DEV).double()
+    s = c.q.to(DEV).double().view(c.new * c.heads, c.dim) @ k.t().contiguous()
+    see = torch.arange(c.kv, device=DEV) <= (torch.arange(c.new, device=DEV) + c.kv - c.new).repeat_interleave(c.heads).unsqueeze(1)
+    e = torch.softmax(s.masked_fill(~see, -math.inf), 1)
+    return [(e @ x).view(c.new, c.heads, c.dim).cpu().numpy() for x in (v, v.abs())]
+
+
+@pytest.mark.parametrize("gap", [10.0, 17.4, 22.0, 30.0])
+@pytest.mark.parametrize("heads,dim,new,kv,prefix,reqs,at", [
+    (4, 128, 1, 131071, 0, 1, 0), (8, 64, 1, 30001, 0, 1, 17000), (4, 256, 1, 20000, 0, 3, 19999), (1, 96, 20, 9000, 0, 1, 5),
+    (4, 128, 1, 20300, 20000, 1, 3), (4, 128, 1, 6000, 0, 500, 0), (4, 64, 1, 3000, 0, 700, 100), (2, 256, 1, 3000, 0, 300, 7)])
+def test_small_weights_of_tokens(backend, gap, heads, dim, new, kv, prefix, reqs, at):
+    """The output is what the small weights leave. Two 16-bit terms lose 2^-18 of a weight (they are on a grid of 2^-24 where a block's
+    largest is 2^-7 at least), sums in fp32 2^-24 a term in numerator and denominator, exp2 and the divide 2^-20, the output's rounding
+    2^-11; 31 keys beside the large one are held to 2^-31 of it."""
+    print(gap, heads, dim, new, kv, prefix, flush=True)
+    c = dominated(heads, dim, new, kv, prefix, reqs, gap, at, 1)
+    got, (want, spread) = c.run(backend, 1.0), formula(c)
+    tol = 2.0 ** -11 * np.abs(want) + spread * (2.0 ** -18 + 2 * kv * 2.0 ** -24 + 2.0 ** -20) + 32 * 2.0 ** -31 * np.abs(c.v.double().numpy()).max() + 2.0 ** -25
+    off = np.abs(got - want)
+    assert (off <= tol).all(), (off.max(), np.abs(want).max(), (off / tol).max())
+
+
+@pytest.mark.parametrize("gap", [10.0, 17.4, 19.0])
+@pytest.mark.parametrize("heads,dim,new,kv,prefix,reqs,at", [
+    (4, 128, 60, 131071, 0, 1, 0), (4, 64, 60, 30001, 0, 1, 17000), (4, 256, 30, 20000, 0, 1, 5), (8, 128, 30, 250, 0, 1, 5), (4, 128, 1, 20300, 20000, 40, 3),
+    (4, 128, 60, 6000, 0, 300, 0), (4, 64, 60, 3000, 0, 300, 300), (2, 256, 60, 3000, 0, 300, 300),
+    (4, 256, 1, 9300, 9000, 40, 8000)])
+def test_small_weights_of_many_rows(backend, gap, heads, dim, new, kv, prefix, reqs, at):
+    """As above with weights rounded once: 2^-11 of a weight, or 2^-31 of the row's largest where that is more."""
+    print(gap, heads, dim, new, kv, prefix, flush=True)
+    c = dominated(heads, dim, new, kv, prefix, reqs, gap, at, 2)
+    got, (want, spread) = c.run(backend, 1.0), formula(c)
+    most = np.abs(c.v.double().numpy()).max()
+    tol = 2.0 ** -11 * np.abs(want) + spread * (2.0 ** -11 + 2 * kv * 2.0 ** -24 + 2.0 ** -20) + kv * 2.0 ** -31 * most + 2.0 ** -25
+    off = np.abs(got - want)
+    assert (off <= tol).all(), (off.max(), np.abs(want).max(), (off / tol).max())
+
+
+def test_small_and_large_blocks_in_turn(backend):
+    """f16: every other block of a wave's keys 20 to 40 bits below the ones between them, of both kinds first: references go up and down."""
+    for heads, new, step in ((4, 1, 128), (4, 1, 32), (4, 60, 64)):
+        c = Case("f16", heads, 128, new, 6000)
+        g = torch.Generator().manual_seed(step)
+        c.q[:, :, 0] = 1.0
+        j = torch.arange(c.kv)
+        for first in (0, 1):
+            print(heads, new, step, first, flush=True)
+            low = (j // step) % 2 == first
+            c.k[:, 0] = torch.where(low, -14.0 - 14.0 * torch.rand(c.kv, generator=g), torch.rand(c.kv, generator=g)).half()
+            c.v[:] = torch.where(low.unsqueeze(1), 60000.0, 0.5).half() * (1 + torch.rand((c.kv, 128), generator=g)).half().clamp(max=1.0)
+            got, (want, spread) = c.run(backend, 1.0), formula(c)
+            one = 2.0 ** -11 if new > 1 else 2.0 ** -18
+            tol = 2.0 ** -11 * np.abs(want) + spread * (one + 2 * c.kv * 2.0 ** -24 + 2.0 ** -20) + 2.0 ** -25
+            tol += 60000 * 2.0 ** -31 * (1.0 if new > 1 else 2.0 ** -8)  # (a few large weights among each block's, and what 2^-31 of them is)
+            assert (np.abs(got - want) <= tol).all(), (np.abs(got - want) / tol).max()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("steps", [(0, -200, -190, -178, -160, -300, -15, -280), (-3000, -2900, 0, -2900, -2950, -60, -80, -2000),
+                                   (0, -3e6, -2e6, -70, -3e6, -90, -3e6, -10), (-3e6, -2.5e6, -3e6, 5, -3e6, -60, -2e6, 0)])
+def test_references_that_fall_and_rise(backend, dtype, steps):
+    """Blocks of one score each (powers of two), far below the largest and rising again, in the order one wave takes them: whole tiles and
+    pieces, few rows and many. The sums stay finite and hold the largest blocks."""
+    t = TORCH[dtype]
+    for heads, new, reqs in ((4, 1, 500), (4, 1, 1), (4, 60, 300), (4, 60, 1)):
+        print(dtype, steps, heads, new, reqs, flush=True)
+        c = Case(dtype, heads, 64, new, 128 * len(steps) + 70, reqs=reqs)
+        far = max(abs(x) for x in steps) > 6e4
+        c.q[:, :, 0] = 1024.0 if far else 1.0
+        score = torch.tensor(steps, dtype=torch.float64).repeat_interleave(128).repeat(2)[:c.kv]
+        c.k[:, 0] = (score / c.q[0, 0, 0].double()).to(t)
+        c.v[:] = torch.randn((c.kv, 64), generator=torch.Generator().manual_seed(3)).to(t)
+        got, want = c.run(backend, math.log(2.0)), c.want(math.log(2.0))
+        # equal weights within a block: 2^-9 (a weight, the output), fp32 sums, 2^-4 of a far score's unit between blocks more than 5 apart
+        tol = 2.0 ** -8 * np.abs(c.v.double().numpy()).max()
+        assert np.isfinite(got).all() and (np.abs(got - want) <= tol).all(), np.abs(got - want).max()
