@@ -144,8 +144,8 @@ int launch_attn(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c) {
     // 64 requests of up to 12 tokens over 2000 keys, 4 heads a kv head, took 72.6 us there, 63.9 here; of up to 24 tokens (96 rows)
     // 79.6 and 80.4. Which there are is known only from the hint, so both are launched unless it (or the sizes) rules one
     // out. Each takes the requests of its own length, or all of them when it is alone.
-    const int64_t most_rows = (c.max_new < c.tokens ? c.max_new : c.tokens) * p.group;
-    const bool tokens_alone = most_rows <= kTokMost, rows_alone = !tokens_alone && c.tokens == c.nreq * c.max_new;
+    const int64_t most_new = c.max_new < c.tokens ? c.max_new : c.tokens;
+    const bool tokens_alone = most_new * p.group <= kTokMost, rows_alone = !tokens_alone && c.tokens == c.nreq * most_new;
     AttnArgs pt = p, pr = p;
     pt.target = cus * (dp <= 128 ? 2 : 1);
     pt.row_lo = 0;

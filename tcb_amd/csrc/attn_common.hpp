@@ -176,6 +176,8 @@ struct Item {
     int parts;       // places in use by the launch
 };
 
+constexpr int kTokMost = 96;  // rows of a request that goes to attn_tokens (attn.hip)
+
 struct ReqShape {
     int q0, nq, kv, tiles, nb;
 };

@@ -209,8 +209,9 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_
         lds_barrier();
         odd = *flag != 0;
     }
-    // Blocks go through the skewed loop in pairs (an odd one last through a plain step), except where rows see few keys.
-    const bool few = all.hi_min + 1 < kFewKeys || (p.window > 0 && p.window < kFewKeys);
+    // Blocks go through the skewed loop in pairs (an odd one last through a plain step), except where rows see few keys and in a
+    // short request (one that a wrong hint of the sizes brought here), whose weights have two terms in attn_tokens too.
+    const bool few = all.hi_min + 1 < kFewKeys || (p.window > 0 && p.window < kFewKeys) || (!PREFIX && it.nq * p.group <= kTokMost);
     const int pairs = !L::SKEW || few || odd ? 0 : nb & ~1;
     auto qk = [&](a16f (&x)[NT], int place) {
         if constexpr (L::SKEW) {

@@ -15,7 +15,6 @@
 namespace trhip {
 namespace {
 
-constexpr int kTokMost = 96;  // rows of a request at most (attn.hip)
 constexpr int kTokRows = 32, kTokBlock = 32, kTokWaves = 4, kTokLeast = 8, kTokOver = 6;
 
 template <int DP> struct TokLds {

@@ -191,3 +191,24 @@ def test_references_that_fall_and_rise(backend, dtype, steps):
         # equal weights within a block: 2^-9 (a weight, the output), fp32 sums, 2^-4 of a far score's unit between blocks more than 5 apart
         tol = 2.0 ** -8 * np.abs(c.v.double().numpy()).max()
         assert np.isfinite(got).all() and (np.abs(got - want) <= tol).all(), np.abs(got - want).max()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("new,max_new", [([1, 199], 100), ([20, 60, 40], 40), ([1] + [0] * 29 + [119], 4000)])
+def test_a_wrong_hint_keeps_a_short_requests_weights(backend, dtype, new, max_new):
+    """Weights midway between two 16-bit numbers, all rounded the same way: with two terms the output is the rounded formula's, with one it is
+    off by more. A request of up to 96 rows gets two, also where max_new says that all requests are longer ones."""
+    from test_gpu_attention import Batch
+    b = Batch(dtype, 4, 1, 128, 16, new, [2000] + [max(n, 1) for n in new[1:]], seed=41, poison=False)
+    b.q[:], b.k[:], b.v[:] = 0, 0, 1
+    b.q[:, :, 0] = 1.0
+    s = -0.99609375 if dtype == "bf16" else -0.99951171875  # 2^s is 0.00136 above 0.5 (bf16 steps 0.0039), 0.000169 (f16 0.00049)
+    for j in range(2000):
+        b.k[b.table[0, j // 16], 0, j % 16, 0] = s
+    b.k[b.table[0, 3], 0, 5, 0] = 0.0
+    b.v[b.table[0, 3], 0, 5] = 0.0  # (its weight is 1)
+    got = b.run(backend, scale=math.log(2.0), max_new=max_new)[0]
+    u, w = (2.0 ** -9, 2000 - new[0]) if dtype == "bf16" else (2.0 ** -12, 2000 - new[0])
+    want = w * 2.0 ** s / (1 + w * 2.0 ** s)
+    print(dtype, new, got[0, 0], want, flush=True)
+    assert (np.abs(got - want) <= u * want + 2.0 ** -15).all()
