@@ -271,8 +271,9 @@ int trhip_kv_append(trhip_ctx *ctx, const trhip_kv *kv, int64_t tokens, const vo
  * to the cache's type for the product with v (f16: to 2^-31 of the row's largest where they are smaller than 2^-20 of
  * it); out is rounded once. Results do not depend on the order in which
  * workgroups run. Entries out of range read as keys and values of 0; kv_len is cut to max_pages * page. max_new:
- * the largest q_start[i + 1] - q_start[i], a hint: a smaller value costs speed, not correctness. Tokens outside
- * every request keep their rows of out. */
+ * the largest q_start[i + 1] - q_start[i], a hint, not a limit. One that is too large (tokens, if nothing is known) costs
+ * token steps up to a quarter of their time; one that is too small sends prompts to the kernel of few rows, which takes up
+ * to twice as long and does not round weights. Tokens outside every request keep their rows of out. */
 int trhip_attn(trhip_ctx *ctx, const trhip_kv *kv, const void *q, int64_t q_stride, void *out, int64_t out_stride,
                int64_t tokens, int heads, int64_t nreq, const int32_t *q_start, const int32_t *kv_len,
                const int32_t *table, int64_t max_pages, int64_t max_new, int64_t window, int64_t sinks, float scale);
