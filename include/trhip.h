@@ -270,7 +270,8 @@ int trhip_kv_append(trhip_ctx *ctx, const trhip_kv *kv, int64_t tokens, const vo
  * than 96 rows (tokens times heads / kv->heads) and its tokens see 256 keys and more, the weights e_j are rounded
  * to the cache's type for the product with v (f16: to 2^-31 of the row's largest where they are smaller than 2^-20 of
  * it); out is rounded once. Results do not depend on the order in which
- * workgroups run. Entries out of range read as keys and values of 0; kv_len is cut to max_pages * page. max_new:
+ * workgroups run. Entries out of range read as keys and values of 0; kv_len is cut to max_pages * page, which must be
+ * below 2^31 - 4096 (and so must prefix_len). max_new:
  * the largest q_start[i + 1] - q_start[i], a hint, not a limit. One that is too large (tokens, if nothing is known) costs
  * token steps up to a quarter of their time; one that is too small sends prompts to the kernel of few rows, which takes up
  * to twice as long and does not round weights. Tokens outside every request keep their rows of out. */

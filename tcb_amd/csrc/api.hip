@@ -294,7 +294,8 @@ int attention(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c, const char 
     if (c.heads < 1 || c.heads % kv->heads != 0) return bad("the heads must be a multiple of the cache's");
     if (!(c.scale > 0.0f) || c.scale > 1e30f) return bad("the scale must be positive and finite");
     if (c.tokens == 0 || c.nreq == 0) return TRHIP_OK;
-    if (c.nreq > kMaxInt || c.max_pages > kMaxInt || c.max_pages * kv->page > kMaxInt || c.window > kMaxInt || c.sinks > kMaxInt ||
+    // (the kernels round key counts up to blocks and pages in 32 bits)
+    if (c.nreq > kMaxInt || c.max_pages > kMaxInt || c.max_pages * kv->page > kMaxInt - 4096 || c.window > kMaxInt || c.sinks > kMaxInt ||
         c.prefix_len > kMaxInt - 4096 || c.tokens > kMaxInt / c.heads)
         return bad("size past 2^31 - 1");
     if (!c.q || !c.out || !c.q_start || !c.kv_len || (c.max_pages > 0 && !c.table) || (c.prefix_len > 0 && !c.prefix_table))
