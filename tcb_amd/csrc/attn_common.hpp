@@ -45,7 +45,6 @@ struct AttnArgs {
     int64_t max_pages;
     const int *q_start, *kv_len;
     const int *prefix_table;  // shared prefix: pages of its prefix_len keys (0: none)
-    int64_t prefix_pages;
     int prefix_len, prefix_splits;
     float *prefix_part;  // [split][token][head] partial results of the prefix: DP sums, reference, sum
     int nreq, tokens, heads, kv_heads, group, dim;
