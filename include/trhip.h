@@ -219,7 +219,8 @@ int trhip_gemm_q_swiglu(trhip_ctx *ctx, const trhip_wstore *w, const float *x, f
                         int64_t K, int mode);
 
 /* ---- The paged key/value cache and the attention over it -------------------------------------------------------------
- * What a program needs between the merged q/k/v product and the output projection. The cache is the caller's memory:
+ * Between the merged q/k/v product and the output projection (positions, if the model turns q and k by them, are applied by
+ * the program in between). The cache is the caller's memory:
  * two planes k and v of [pages][heads][page][dim] elements (f16 or bf16, 16-byte aligned), its pages dealt to
  * requests by page tables. page: keys a page, a power of two from 16 to 4096; dim: a multiple of 8 up to 256. Lengths, page
  * numbers and slots are int32 on the device, so a step can be captured into a graph and replayed while they change.
@@ -285,7 +286,13 @@ int trhip_attn(trhip_ctx *ctx, const trhip_kv *kv, const void *q, int64_t q_stri
  * of one prompt): those lie in pages prefix_pages[0 ...] and are read once for all requests, as one product with
  * every token's rows, instead of once a request. kv_len, table and p then count a request's own keys behind the
  * prefix (its own first key is place 0 of table[i, 0], wherever the prefix ends in its page), and every token sees
- * the whole prefix and its own j <= p. */
+ * the whole prefix and its own j <= p.
+ * Over the prefix all tokens' rows are one product, so the rule of rounded weights goes by the whole batch there: where it
+ * brings more than 96 rows and the prefix has 256 keys and more, each token's weights over the prefix are rounded to
+ * the cache's type, a single token's too (bf16 outputs are then off by 1.4 times the rounding of an fp32 result); over its
+ * own keys trhip_attn's rule holds. trhip_attn on tables that name the prefix's pages first does not round them, where
+ * the prefix ends with a page. Partial results lie in the context's workspace in fp32, as rows of dim (rounded up to 64,
+ * 128 or 256) + 2: at most 3 * tokens * heads + 160 * nreq * kv->heads + 900000 of them. */
 int trhip_attn_shared(trhip_ctx *ctx, const trhip_kv *kv, const void *q, int64_t q_stride, void *out, int64_t out_stride,
                       int64_t tokens, int heads, int64_t nreq, const int32_t *q_start, const int32_t *kv_len,
                       const int32_t *table, int64_t max_pages, const int32_t *prefix_pages, int64_t prefix_len,

@@ -25,7 +25,8 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-ffp-contract=o
          "-Wall", "-Wno-unused-function", "-Wno-unused-variable"]
 # attn.hip, attn_rows256.hip: matrix instructions take their accumulators in architectural registers where they fit. The
 # compiler's default for waves of over 256 registers keeps every accumulator in the other file, a move away from the softmax
-# (one token x 300 keys 11.6 -> 10.6 us, 39 requests of heads of 256 130 -> 71).
+# (us with and without: one token x 300 keys 10.8, 12.3; 64 tokens x 8192 204, 210; 39 tokens with heads of 256 70, 135; a prompt of 4096
+# with 16 such heads 249, 633).
 VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
 FILE_FLAGS = {"attn.hip": VGPR_FORM, "attn_rows256.hip": VGPR_FORM}
 

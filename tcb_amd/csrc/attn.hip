@@ -173,7 +173,9 @@ int launch_attn(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c) {
     const int64_t part = (part_t + part_r) * (dp + 2);
     const int64_t places = 8 + 8 * (int64_t)(pt.part_slots > pr.part_slots ? pt.part_slots : pr.part_slots);
     // the prefix: all tokens' rows are one tall product, its keys cut to fill the device
-    const bool tall = rows > kTokMost;  // (24 tokens of 4 heads behind 20000 keys: 40.8 us as rows, 35.5)
+    // (24 tokens of 4 heads behind 20000 keys: 40.8 us as rows, 35.5). Rows of short requests get weights of one term there; with two, 192 x 2
+    // tokens behind 30001 keys would take 330 us, not 246, and 32 behind 4096 23.7, not 21.9.
+    const bool tall = rows > kTokMost;
     const int ptr = tall ? tr : kTokRows, pbk = tall ? br : kTokBlock;
     const int64_t ptiles = (rows + ptr - 1) / ptr;
     int splits = 0;

@@ -220,7 +220,8 @@ template <int TR, int BK> __device__ __forceinline__ ReqShape shape_of(const Att
 //   dealt out         (sum + over (sum / c + n)) / target + c + over, least at c = sqrt(over sum / target)
 // Never more than rounds * target pieces, and none of under `least` blocks.
 // Measured, in us, at these constants and at others: kMostRounds 6 (64 tokens of up to 8192 keys 203; 2: 219); kTokLeast 8, two
-// blocks a wave (one token x 4096 keys 13.7; 4: 14.8, 16: 15.2); kTokOver 6 (64 requests of up to 12 tokens 72.6; 3: 78.0;
+// blocks a wave (one token x 300 keys 10.6; 4: 10.9, 2: 12.0; x 4096 keys 13.9; 4: 15.1, 16: 15.7; 16 tokens in a window of 256
+// 12.3; 4: 14.5; 8 tokens behind 1000 shared keys 13.6; 4: 14.3, 16: 15.2); kTokOver 6 (64 requests of up to 12 tokens 72.6; 3: 78.0;
 // 12: the same); kRowsOver 20 (6 prompts of up to 300 tokens 30.1; 10: 34.4); kRowsLeast 6
 // (32 tokens behind 4096 shared keys 21.8; 4: 22.7, 2: 27.0).
 constexpr int kMostRounds = 6;

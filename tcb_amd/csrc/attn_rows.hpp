@@ -2,8 +2,8 @@
 //
 // A workgroup takes a tile of 128 rows, 32 a wave (attn_common.hpp), and goes through its keys in blocks of 64 that its waves
 // copy into LDS together. What bounds it are the matrix instructions, the softmax's instructions beside them and the
-// power that both draw: a causal prompt of 8192 tokens, 32 heads of 128, takes 502 us, 1.1 PFLOP/s, at a clock of 1.67 GHz
-// (2.4 without load), where a large library product reaches 1.63 PFLOP/s. Blocks are taken in a skewed loop: step j
+// power that both draw: a causal prompt of 8192 tokens, 32 heads of 128, takes 502 to 543 us (it differs by the card), 1.0 to 1.1 PFLOP/s,
+// at a clock of 1.67 GHz (2.4 without load), where a large library product reaches 1.63 PFLOP/s. Blocks are taken in a skewed loop: step j
 // multiplies K of block j + 1 and V of block j - 1 while it takes the exponentials of block j, three independent pieces of work
 // in one run of instructions, and two waves share a SIMD. Masks only touch the scores there. Every instruction in it
 // counts: choosing each copied row by the mask took 32 of 165 vector instructions and 3.5% of the time. Rows that see few
@@ -34,9 +34,9 @@ template <int V> struct Const {
 template <int DP> struct RowsShape {
     static constexpr int WAVES = 4, BK = 64, NT = BK / 32;
     // Heads of over 128: their accumulators leave no registers for a second block's scores and weights, so a plain step, one
-    // workgroup a CU, operands eight products ahead (prompt of 4096, 16 heads of 256: 250 us; 652 without those).
+    // workgroup a CU, operands eight products ahead (prompt of 4096, 16 heads of 256: 248 us).
     static constexpr bool SKEW = DP != 256;
-    static constexpr int PER_CU = DP == 256 ? 1 : 2;  // workgroups a CU: by registers
+    static constexpr int PER_CU = DP == 256 ? 1 : 2;  // workgroups a CU: by registers, for heads of 256 by LDS as well (128 KB)
     static constexpr int THREADS = 64 * WAVES, TR = 32 * WAVES;
     static constexpr int TILE = BK * DP * 2;       // bytes of a block's keys or values
     static constexpr int PI = DP / 32;             // copies a wave makes of a block: a sixteen-row piece
