@@ -11,12 +11,7 @@ namespace trhip {
 namespace {
 
 template <int DP, bool BF, bool PREFIX> __global__ __launch_bounds__(64 * kTokWaves) void attn_tokens(const AttnArgs p) {
-    tokens_of<DP, BF, PREFIX>(p, 0, blockIdx.x, gridDim.x);
-}
-
-// (inlined in the short joining kernel it costs 1 us of 48 in a chunk of 64 tokens over 16000 keys, not called)
-template <bool BF> __device__ __attribute__((noinline)) void put_odd_apart(const AttnArgs *args, int req, int q0, int row, int head, int d, int hi) {
-    put_odd4<BF>(args, req, q0, row, head, d, hi);
+    tokens_of<DP, BF, PREFIX>(p, blockIdx.x, gridDim.x);
 }
 
 // Joins the pieces of a tile's rows, and the shared prefix's: a workgroup for `each` rows of a place (workgroups of places that
@@ -50,9 +45,7 @@ template <int DP, bool BF> __global__ __launch_bounds__(256) void attn_join(cons
             for (int u = 0; u < AT; u++)
                 if (s0 + u < all) j.add(ml[u].x, ml[u].y, a[u].x, a[u].y, b[u].x, b[u].y);
         }
-        const int hi = t.kv - t.nq + tok;
-        if (__builtin_expect(put4<BF>(p, t.q0, row, t.head, d, j.o, j.l, p.prefix_splits > 0 || hi >= 0), 0))
-            put_odd_apart<BF>(args_again(0), t.req, t.q0, row, t.head, d, hi);
+        put4<BF>(p, t.q0, row, t.head, d, j.o, j.l, p.prefix_splits > 0 || t.kv - t.nq + tok >= 0);
     }
 }
 

@@ -164,7 +164,7 @@ template <int BK> __device__ __forceinline__ Span span_of(int hi, int lo, int si
 
 // A place's tile, for the launch that joins its pieces: pieces 0: another place has it.
 struct Place {
-    int pieces, q0, nq, kv, r0, n, head, req;
+    int pieces, q0, nq, kv, r0, n, head, unused;
 };
 
 struct Item {
@@ -498,21 +498,16 @@ __device__ __forceinline__ bool all_see(const Rows &w, int t, int n) {
     return t + n - 1 <= w.hi_min && (t >= w.lo_max || t + n <= w.sinks);
 }
 
-// Values (or packed outputs) that are infinities or NaN set a half's top bit in odd16(x) & kOdd.
-constexpr uint32_t kOdd = 0x80008000u;
-template <bool BF> __device__ __forceinline__ uint32_t odd16(uint32_t x) {  // (two of them: an exponent of all ones carries)
-    return BF ? (x & 0x7F807F80u) + 0x00800080u : (x & 0x7C007C00u) + 0x04000400u;
-}
-
 // Whether 32 rows of values at LDS address v hold an infinity or a NaN (exponent all ones).
 template <int DP, bool BF> __device__ __forceinline__ bool odd_values(uint32_t v) {
+    constexpr uint32_t E = BF ? 0x7F807F80u : 0x7C007C00u, U = BF ? 0x00800080u : 0x04000400u;
     uint32_t any = 0;
 #pragma unroll
     for (int i = 0; i < DP / 16; i++) {
         const u32x4 x = lds16(v + i * 1024 + (threadIdx.x & 63) * 16);
-        any |= odd16<BF>(x.x) | odd16<BF>(x.y) | odd16<BF>(x.z) | odd16<BF>(x.w);
+        any |= ((x.x & E) + U) | ((x.y & E) + U) | ((x.z & E) + U) | ((x.w & E) + U);
     }
-    return __any((any & kOdd) != 0);
+    return __any((any & 0x80008000u) != 0);
 }
 
 // O^T += V^T P^T key by key in fp32, a key's values reaching only the rows that see it: for blocks where some rows see
@@ -649,10 +644,9 @@ __device__ __forceinline__ float2 agent_load(const float *p) {
 }
 
 // Four finished outputs of row `row` (of the request's kv head) from dimension d; l: the row's sum. A row whose mask
-// leaves nothing (hi < 0) is 0; a sum of 0 over visible keys is the formula's 0 / 0. True: one is not finite although the sum is
-// positive and finite, so put_odd4 has to say what it is.
-template <bool BF> __device__ __forceinline__ bool put4(const AttnArgs &p, int q0, int row, int head, int d, const float (&o)[4], float l, bool sees) {
-    if (d >= p.dim) return false;
+// leaves nothing (hi < 0) is 0; a sum of 0 over visible keys is the formula's 0 / 0.
+template <bool BF> __device__ __forceinline__ void put4(const AttnArgs &p, int q0, int row, int head, int d, const float (&o)[4], float l, bool sees) {
+    if (d >= p.dim) return;
     const int t = p.by_group(row), g = row - t * p.group;
     uint16_t *dst = p.out + (int64_t)(q0 + t) * p.out_stride + (int64_t)(head * p.group + g) * p.dim + d;
     const float inv = 1.0f / l;  // one division, an fp32 rounding more
@@ -667,66 +661,6 @@ template <bool BF> __device__ __forceinline__ bool put4(const AttnArgs &p, int q
         dst[1] = (uint16_t)(w.x >> 16);
         dst[2] = (uint16_t)w.y;
         dst[3] = (uint16_t)(w.y >> 16);
-    }
-    return __builtin_expect(((odd16<BF>(w.x) | odd16<BF>(w.y)) & kOdd) != 0, 0) && l > 0.0f && l < __builtin_inff();
-}
-
-// Which of four elements from d are +Inf (bits 0-3), -Inf (4-7) or NaN (8-11) in the values of keys [from, to).
-template <bool BF> __device__ __forceinline__ uint32_t odd_in(const AttnArgs &p, const int *table, int head, int d, int from, int to) {
-    uint32_t seen = 0;
-    for (int j = from, end; j < to; j = end) {
-        const int page = table[j >> p.page_log2], next = ((j >> p.page_log2) + 1) << p.page_log2;
-        end = next < to ? next : to;
-        if ((uint32_t)page >= (uint32_t)p.npages) continue;
-        const uint8_t *at = p.v + (int64_t)page * p.page_bytes + (int64_t)head * p.head_bytes + d * 2;
-        for (int i = j; i < end; i += 4) {
-            uint2 x[4];
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const int k = i + u < end ? i + u : end - 1;
-                x[u] = *reinterpret_cast<const uint2 *>(at + (k & ((1 << p.page_log2) - 1)) * p.dim * 2);
-            }
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                if (((odd16<BF>(x[u].x) | odd16<BF>(x[u].y)) & kOdd) == 0) continue;
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const uint32_t h = ((r < 2 ? x[u].x : x[u].y) >> (16 * (r & 1))) & 0xFFFFu, e = BF ? 0x7F80u : 0x7C00u;
-                    if ((h & e) == e) seen |= 1u << (r + ((h & 0x7FFFu) != e ? 8 : h >> 15 ? 4 : 0));
-                }
-            }
-        }
-    }
-    return seen;
-}
-
-// put4's outputs where a visible value is not finite. The matrix products make NaN of an infinity in most places (a weight's second
-// term may be 0 or negative, a weight may be 0 in 16 bits), but every weight of the formula is positive, so its sums are: the
-// infinity where all that the row sees are of one sign, else NaN. The row's keys are read again for it, in this rare case only
-// (req: the request; hi: the row's last key). Outputs that no such value explains (sums past the largest number) stay.
-// at: where the kernel's AttnArgs lie among its arguments. They are read anew here, so that none has to be kept for it (kept, they
-// cost a prompt with heads of 256 4% of its time).
-__device__ __forceinline__ const AttnArgs *args_again(int at) {
-    uint64_t block = reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr());
-    asm volatile("" : "+s"(block));
-    return reinterpret_cast<const AttnArgs *>(block + at);
-}
-template <bool BF> __device__ __forceinline__ void put_odd4(const AttnArgs *args, int req, int q0, int row, int head, int d, int hi) {
-    const AttnArgs &p = *args;
-    if (d >= p.dim) return;
-    const int *table = p.table + (int64_t)req * p.max_pages;
-    const int t = p.by_group(row), g = row - t * p.group;
-    uint16_t *dst = p.out + (int64_t)(q0 + t) * p.out_stride + (int64_t)(head * p.group + g) * p.dim + d;
-    constexpr uint32_t E = BF ? 0x7F80u : 0x7C00u, NAN16 = BF ? 0x7FC0u : 0x7E00u;
-    if ((dst[0] & E) != E && (dst[1] & E) != E && (dst[2] & E) != E && (dst[3] & E) != E) return;
-    const int lo = p.window > 0 && hi >= p.window ? hi - p.window + 1 : 0;
-    uint32_t seen = odd_in<BF>(p, table, head, d, lo, hi + 1);
-    seen |= odd_in<BF>(p, table, head, d, 0, p.sinks < lo ? p.sinks : lo);
-    seen |= odd_in<BF>(p, p.prefix_table, head, d, 0, p.prefix_len);
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-        const uint32_t is = seen >> r;
-        if ((dst[r] & E) == E && (is & 0x111u)) dst[r] = (uint16_t)((is & 0x100u) || (is & 0x11u) == 0x11u ? NAN16 : is & 1u ? E : E | 0x8000u);
     }
 }
 
@@ -752,7 +686,7 @@ struct Join {
 // The last workgroup of a tile joins its pieces (agent-coherent loads: other workgroups of this launch wrote them). The
 // WAVES waves take every WAVES-th piece, eight loads of each in flight, and join their sums in LDS (`room` bytes at `lds`).
 template <int DP, int TR, bool BF, int WAVES>
-__device__ __forceinline__ void join_tile(const AttnArgs &p, int args, const Item &it, int r0, int n, float *lds, int room) {
+__device__ __forceinline__ void join_tile(const AttnArgs &p, const Item &it, int r0, int n, float *lds, int room) {
     constexpr int ST = DP + 2, AT = 8;
     const int lane = threadIdx.x & 63, w = uni(threadIdx.x >> 6), items = n * (DP / 4);
     const int chunk = room / (WAVES * 6 * 4) / 64 * 64;
@@ -793,8 +727,7 @@ __device__ __forceinline__ void join_tile(const AttnArgs &p, int args, const Ite
                 const float *x = lds + (u * chunk + i) * 6;
                 j.add(x[0], x[1], x[2], x[3], x[4], x[5]);
             }
-            const int hi = it.kv - it.nq + p.by_group(row);
-            if (__builtin_expect(put4<BF>(p, it.q0, row, it.head, d, j.o, j.l, hi >= 0), 0)) put_odd4<BF>(args_again(args), it.req, it.q0, row, it.head, d, hi);
+            put4<BF>(p, it.q0, row, it.head, d, j.o, j.l, it.kv - it.nq + p.by_group(row) >= 0);
         }
         __syncthreads();
     }
@@ -803,7 +736,7 @@ __device__ __forceinline__ void join_tile(const AttnArgs &p, int args, const Ite
 // For the joining launch: this item's place, and (by workgroup 0) how many there are.
 __device__ __forceinline__ void leave_place(const AttnArgs &p, const Item &it, int r0, int n) {
     if (threadIdx.x == 0)
-        reinterpret_cast<Place *>(p.parts + 8)[it.slot] = Place{it.split == 0 ? it.nsplit : 0, it.q0, it.nq, it.kv, r0, n, it.head, it.req};
+        reinterpret_cast<Place *>(p.parts + 8)[it.slot] = Place{it.split == 0 ? it.nsplit : 0, it.q0, it.nq, it.kv, r0, n, it.head, 0};
 }
 __device__ __forceinline__ void leave_count(const AttnArgs &p, const Item &it, int wg) {
     if (p.parts && wg == 0 && threadIdx.x == 0) p.parts[0] = it.parts;

@@ -43,8 +43,8 @@ template <int DP> struct RowsShape {
     static constexpr int BYTES = 4 * TILE + 16;  // two blocks of each are in LDS
 };
 
-// PREFIX: rows are all tokens' and keys the shared prefix's; results go to prefix_part. args: args_again.
-template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_tile(const AttnArgs &p, int args, int wg, int grid) {
+// PREFIX: rows are all tokens' and keys the shared prefix's; results go to prefix_part.
+template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_tile(const AttnArgs &p, int wg, int grid) {
     using L = RowsShape<DP>;
     constexpr int BK = L::BK, NT = L::NT;
     extern __shared__ __attribute__((aligned(1024))) uint4 smem[];
@@ -187,6 +187,7 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_
     bool odd = false;
     const bool gap = all.lo_min > all.sinks;
     if (!PREFIX && (mixed || gap)) {
+        constexpr uint32_t E = BF ? 0x7F807F80u : 0x7C007C00u, U = BF ? 0x00800080u : 0x04000400u;
         const int l0 = gap ? (all.lo_min & ~15) < all.sinks ? all.sinks : all.lo_min & ~15 : all.lo_min;
         const uint32_t e0 = ((uint32_t)all.sinks + 15) & ~15u;
         const int e1 = e0 < (uint32_t)l0 ? (int)e0 : l0;
@@ -199,12 +200,12 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_
             if ((uint32_t)page >= (uint32_t)p.npages) continue;
             const uint4 x = *reinterpret_cast<const uint4 *>(p.v + (int64_t)page * p.page_bytes + (int64_t)it.head * p.head_bytes +
                                                              (int64_t)((t & ((1 << p.page_log2) - 1)) * p.dim * 2 + c * 16));
-            any |= odd16<BF>(x.x) | odd16<BF>(x.y) | odd16<BF>(x.z) | odd16<BF>(x.w);
+            any |= ((x.x & E) + U) | ((x.y & E) + U) | ((x.z & E) + U) | ((x.w & E) + U);
         }
         int *flag = reinterpret_cast<int *>(smem) + 4 * L::TILE / 4;
         if (tid == 0) *flag = 0;
         lds_barrier();
-        if (any & kOdd) *flag = 1;
+        if (any & 0x80008000u) *flag = 1;
         lds_barrier();
         odd = *flag != 0;
     }
@@ -354,14 +355,6 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_
 
     const bool direct = !PREFIX && it.nsplit == 1 && p.prefix_splits == 0;
     const float sum = half_sum(l);
-    float zero = 0.0f;  // NaN where a sum of values is not finite
-    if (direct) {
-#pragma unroll
-        for (int d = 0; d < DP / 32; d++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) zero = fmaf(o[d][i], 0.0f, zero);
-    }
-    const bool odd_sums = !(zero == 0.0f) && sum > 0.0f && sum < __builtin_inff();
     if ((lane & 31) < wn) {
         const int r = wr + (lane & 31), row = r0 + r, t = p.by_group(row);
         float *part = PREFIX ? p.prefix_part + ((int64_t)it.split * p.tokens * p.heads + (int64_t)t * p.heads + it.head * p.group +
@@ -382,17 +375,13 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void rows_of_
                 }
             }
         if (!direct && h == 0) *reinterpret_cast<float2 *>(part + DP) = make_float2(ms, sum);
-        if (odd_sums) {
-#pragma unroll 1
-            for (int at = 4 * h; at < DP; at += 8) put_odd4<BF>(args_again(args), it.req, it.q0, row, it.head, at, keys - it.nq + t);
-        }
     }
     if (!direct && !PREFIX) leave_place(p, it, r0, n);
 }
 
 template <int DP, bool BF, bool PREFIX>
 __global__ __launch_bounds__(RowsShape<DP>::THREADS, RowsShape<DP>::PER_CU) void attn_rows(const AttnArgs p) {
-    rows_of_tile<DP, BF, PREFIX>(p, 0, blockIdx.x, gridDim.x);
+    rows_of_tile<DP, BF, PREFIX>(p, blockIdx.x, gridDim.x);
 }
 
 template <int DP, bool BF, bool PREFIX> int launch_rows(trhip_ctx *ctx, const AttnArgs &p, int64_t grid) {

@@ -26,8 +26,8 @@ template <int DP> struct TokLds {
     static constexpr int BYTES = kTokWaves * (WAVE + 32 * 8) + 16;
 };
 
-// PREFIX: rows are all tokens' and keys the shared prefix's; results go to prefix_part. args: args_again.
-template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void tokens_of(const AttnArgs &p, int args, int wg, int grid) {
+// PREFIX: rows are all tokens' and keys the shared prefix's; results go to prefix_part.
+template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void tokens_of(const AttnArgs &p, int wg, int grid) {
     using L = TokLds<DP>;
     extern __shared__ __attribute__((aligned(1024))) uint4 smem[];  // nothing else is shared: the rows' swizzle needs them aligned
     const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6);
@@ -150,7 +150,7 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void tokens_o
             j.add(ml[u * 32 + r].x, ml[u * 32 + r].y, o.x, o.y, o.z, o.w);
         }
         if (direct) {
-            if (__builtin_expect(put4<BF>(p, it.q0, row, it.head, d, j.o, j.l, keys - it.nq + t >= 0), 0)) put_odd4<BF>(args_again(args), it.req, it.q0, row, it.head, d, keys - it.nq + t);
+            put4<BF>(p, it.q0, row, it.head, d, j.o, j.l, keys - it.nq + t >= 0);
         } else if (PREFIX) {
             float *dst = p.prefix_part + ((int64_t)it.split * p.tokens * p.heads + (int64_t)t * p.heads + it.head * p.group +
                                           (row - t * p.group)) * (DP + 2);
@@ -170,7 +170,7 @@ template <int DP, bool BF, bool PREFIX> __device__ __forceinline__ void tokens_o
         return;
     }
     if (last_piece(p, it, reinterpret_cast<int *>(ml + kTokWaves * 32)))
-        join_tile<DP, kTokRows, BF, kTokWaves>(p, args, it, r0, n, reinterpret_cast<float *>(smem), kTokWaves * L::WAVE);
+        join_tile<DP, kTokRows, BF, kTokWaves>(p, it, r0, n, reinterpret_cast<float *>(smem), kTokWaves * L::WAVE);
 }
 
 }  // namespace

@@ -10,9 +10,6 @@ namespace {
 
 static_assert(RowsShape<128>::THREADS == 64 * kTokWaves && RowsShape<64>::PER_CU == 2 && RowsShape<128>::PER_CU == 2, "one launch shape");
 
-// Where b lies behind a and na (args_again).
-constexpr int kArgsB = (sizeof(AttnArgs) + sizeof(int) + alignof(AttnArgs) - 1) / alignof(AttnArgs) * alignof(AttnArgs);
-
 template <int DP, bool BF, TwoKind KIND>
 __global__ __launch_bounds__(64 * kTokWaves, 2) void attn_two(const AttnArgs a, int na, const AttnArgs b, int nb, int turn) {
     const int runs = (na + turn - 1) / turn, other = (nb + turn - 1) / turn, both = runs < other ? runs : other;  // runs of either
@@ -21,11 +18,11 @@ __global__ __launch_bounds__(64 * kTokWaves, 2) void attn_two(const AttnArgs a, 
     const int at = (run < 2 * both ? run / 2 : run - both) * turn + in;
     if (first) {
         if (at >= na) return;
-        if constexpr (KIND == TwoKind::PrefixTokens) tokens_of<DP, BF, true>(a, 0, at, na);
-        else rows_of_tile<DP, BF, KIND == TwoKind::PrefixRows>(a, 0, at, na);
+        if constexpr (KIND == TwoKind::PrefixTokens) tokens_of<DP, BF, true>(a, at, na);
+        else rows_of_tile<DP, BF, KIND == TwoKind::PrefixRows>(a, at, na);
     } else {
         if (at >= nb) return;
-        tokens_of<DP, BF, false>(b, kArgsB, at, nb);
+        tokens_of<DP, BF, false>(b, at, nb);
     }
 }
 
