@@ -266,8 +266,9 @@ int trhip_kv_append(trhip_ctx *ctx, const trhip_kv *kv, int64_t tokens, const vo
  *   out[t, a] = sum_j e_j v_j / sum_j e_j, e_j = exp(scale * q.k_j - max), over j <= p with
  *               p - window < j or j < sinks (window 0: no window, every j <= p)
  * Key j lies in page table[i, j / page]; pages that no token sees are not read, so their entries may hold
- * anything. What the cache holds where a token's mask hides it never reaches that token, NaN and Inf included; a
- * token that sees no key gets zeros. Products and sums are in fp32 (matrix cores); where a request brings more
+ * anything. What the cache holds where a token's mask hides it never reaches that token, NaN and Inf included. A
+ * value that a token sees and that is not finite makes that element of its row NaN (not the formula's infinity), whatever
+ * the key's weight, and no other element. A token that sees no key gets zeros. Products and sums are in fp32 (matrix cores); where a request brings more
  * than 96 rows (tokens times heads / kv->heads) and its tokens see 256 keys and more, the weights e_j are rounded
  * to the cache's type for the product with v (f16: to 2^-31 of the row's largest where they are smaller than 2^-20 of
  * it); out is rounded once. Results do not depend on the order in which

@@ -644,7 +644,9 @@ __device__ __forceinline__ float2 agent_load(const float *p) {
 }
 
 // Four finished outputs of row `row` (of the request's kv head) from dimension d; l: the row's sum. A row whose mask
-// leaves nothing (hi < 0) is 0; a sum of 0 over visible keys is the formula's 0 / 0.
+// leaves nothing (hi < 0) is 0; a sum of 0 over visible keys is the formula's 0 / 0. A sum of values that is not finite is NaN: of
+// an infinity the products leave either (a weight's second term, or the weight in 16 bits, may be 0 or negative), and which must
+// not hang on the batch or the block.
 template <bool BF> __device__ __forceinline__ void put4(const AttnArgs &p, int q0, int row, int head, int d, const float (&o)[4], float l, bool sees) {
     if (d >= p.dim) return;
     const int t = p.by_group(row), g = row - t * p.group;
@@ -652,7 +654,7 @@ template <bool BF> __device__ __forceinline__ void put4(const AttnArgs &p, int q
     const float inv = 1.0f / l;  // one division, an fp32 rounding more
     float y[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) y[i] = sees ? o[i] * inv : 0.0f;
+    for (int i = 0; i < 4; i++) y[i] = sees ? fmaf(o[i], 0.0f, o[i] * inv) : 0.0f;
     const uint2 w = make_uint2(pack2<BF>(y[0], y[1]), pack2<BF>(y[2], y[3]));
     if (p.out_aligned) {
         *reinterpret_cast<uint2 *>(dst) = w;

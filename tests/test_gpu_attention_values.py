@@ -212,3 +212,72 @@ def test_a_wrong_hint_keeps_a_short_requests_weights(backend, dtype, new, max_ne
     want = w * 2.0 ** s / (1 + w * 2.0 ** s)
     print(dtype, new, got[0, 0], want, flush=True)
     assert (np.abs(got - want) <= u * want + 2.0 ** -15).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("heads,dim,new,kv,prefix,reqs", [
+    (4, 128, 1, 300, 0, 1), (8, 64, 3, 5000, 0, 1), (4, 256, 1, 900, 0, 300), (4, 72, 20, 2000, 0, 3), (4, 128, 60, 200, 0, 1), (4, 128, 200, 1500, 0, 1),
+    (4, 128, 30, 9000, 0, 1), (2, 256, 100, 700, 0, 1), (4, 128, 1, 1100, 1000, 1), (4, 128, 2, 1100, 1000, 40), (4, 64, 40, 640, 600, 2)])
+def test_values_that_are_not_finite_and_seen(backend, dtype, heads, dim, new, kv, prefix, reqs):
+    """A visible value that is not finite makes its element NaN, that one alone, in every row that sees it and in no other: in blocks that all
+    rows see and in others, in pieces, behind a prefix, with weights that are far below a 16-bit number."""
+    t, inf = TORCH[dtype], float("inf")
+    c = Case(dtype, heads, dim, new, kv, prefix=prefix, reqs=reqs)
+    g = torch.Generator().manual_seed(kv)
+    c.q[:], c.k[:], c.v[:] = (torch.randn(x.shape, generator=g).to(t) for x in (c.q, c.k, c.v))
+    spots = [(3, 0, inf), (kv // 2, 1, -inf), (5, 2, float("nan")), (0, 3, inf), (kv - new - 1, 3, -inf), (kv // 3, dim - 1, -inf), (kv - 1, 5, inf),
+             (kv - new, 6, -inf), (kv - 1 - new // 2, 7, float("nan"))]
+    for low in (False, True):
+        print(dtype, heads, dim, new, kv, prefix, reqs, low, flush=True)
+        if low:  # the weights of those keys that all rows see are 2^-60 of the others' and less
+            c.q[:, :, 4], c.k[:, 4] = 8.0, 0.0
+            for j, _, _ in spots:
+                c.k[j, 4] = -64.0 if j < kv - new else 0.0
+        scale = 0.25 if low else dim ** -0.5
+        clean, v = c.run(backend, scale), c.v.clone()
+        odd = np.zeros(clean.shape, bool)
+        for j, d, x in spots:
+            c.v[j, d] = x
+            odd[[i for i in range(new) if j <= kv - new + i], :, d] = True
+        got = c.run(backend, scale)
+        c.v = v
+        assert np.isfinite(clean).all() and np.array_equal(np.isnan(got), odd) and np.isfinite(got[~odd]).all()
+        assert np.abs(got[~odd] - clean[~odd]).max() <= 2.0 ** -7 * np.abs(clean).max()
+
+
+def test_values_that_are_not_finite_in_a_window(backend):
+    """As above where a window and first tokens decide who sees them."""
+    inf = float("inf")
+    for dtype, heads, dim, new, kv in (("bf16", 4, 128, 1, 700), ("f16", 4, 128, 60, 700), ("bf16", 2, 256, 80, 900), ("f16", 4, 64, 20, 500)):
+        print(dtype, dim, new, kv, flush=True)
+        c = Case(dtype, heads, dim, new, kv)
+        g = torch.Generator().manual_seed(kv)
+        c.q[:], c.k[:], c.v[:] = (torch.randn(x.shape, generator=g).to(c.k.dtype) for x in (c.q, c.k, c.v))
+        window, sinks = 100, 5
+        clean = c.run(backend, dim ** -0.5, window=window, sinks=sinks)
+        odd = np.zeros(clean.shape, bool)
+        for j, d, x in ((2, 0, inf), (5, 1, inf), (kv - new - 70, 2, -inf), (kv - new - 99, 3, inf), (kv - new - 100, 4, inf), (4, 2, -inf), (kv - new, 6, inf)):
+            c.v[j, d] = x
+            odd[[i for i in range(new) if j <= kv - new + i and (kv - new + i - window < j or j < sinks)], :, d] = True
+        got = c.run(backend, dim ** -0.5, window=window, sinks=sinks)
+        assert np.array_equal(np.isnan(got), odd) and np.isfinite(got[~odd]).all()
+        assert np.abs(got[~odd] - clean[~odd]).max() <= 2.0 ** -7 * np.abs(clean).max()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_values_that_are_not_finite_in_mixed_batches(backend, dtype, dim):
+    """Prompts beside tokens, whose kernels share a launch: each row has its own request's, of its own kv head."""
+    from test_gpu_attention import Batch
+    for new, kv in (([1, 200, 1, 40], [300, 260, 5000, 700]), ([200, 1], [200, 37]), ([150, 0, 12], [9000, 3, 12])):
+        print(dtype, dim, new, kv, flush=True)
+        b = Batch(dtype, 8, 2, dim, 16, new, kv, seed=44)
+        clean = b.run(backend)
+        odd = np.zeros(clean.shape, bool)
+        for i, n in enumerate(kv):
+            for j, d, x in ((0, 8 * i + 1, float("inf")), (n // 2, 8 * i + 2, float("-inf")), (n - 1, 8 * i + 3, float("inf")), (n // 3, 8 * i + 4, float("nan"))):
+                b.v[b.table[i, j // 16], 1, j % 16, d] = x
+                odd[[b.start[i] + t for t in range(new[i]) if j <= n - new[i] + t], 4:, d] = True
+        got = b.run(backend)
+        assert np.array_equal(np.isnan(got), odd) and np.isfinite(got[~odd]).all()
+        assert np.abs(got[~odd] - clean[~odd]).max() <= 2.0 ** -7 * np.abs(clean[~odd]).max()
