@@ -34,7 +34,7 @@ template <int V> struct Const {
 template <int DP> struct RowsShape {
     static constexpr int WAVES = 4, BK = 64, NT = BK / 32;
     // Heads of over 128: their accumulators leave no registers for a second block's scores and weights, so a plain step, one
-    // workgroup a CU, operands eight products ahead (prompt of 4096, 16 heads of 256: 248 us).
+    // workgroup a CU, operands eight products ahead (prompt of 4096, 16 heads of 256: 250 us).
     static constexpr bool SKEW = DP != 256;
     static constexpr int PER_CU = DP == 256 ? 1 : 2;  // workgroups a CU: by registers, for heads of 256 by LDS as well (128 KB)
     static constexpr int THREADS = 64 * WAVES, TR = 32 * WAVES;
