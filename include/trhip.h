@@ -297,6 +297,84 @@ int trhip_attn_shared(trhip_ctx *ctx, const trhip_kv *kv, const void *q, int64_t
                       const int32_t *table, int64_t max_pages, const int32_t *prefix_pages, int64_t prefix_len,
                       int64_t max_new, float scale);
 
+/* ---- Positions ---------------------------------------------------------------------------------------------------------
+ * Rotary positions: pair i of a head's first 2P elements, P the pairs of all axes, is turned by an angle,
+ *   (x, y) -> (x cos a - y sin a, x sin a + y cos a),  a = pos[axis(i)][t] * factors[i] * base^(-s(i)),
+ * and elements behind them stay as they are. Text has one axis; images and video have a position in time, height and width.
+ * pairs[a]: pairs that axis a turns. They are dealt out in runs (axis 0 turns the first pairs[0] pairs, and so on), or with
+ * TRHIP_ROPE_DEALT one by one to the axes in turn, as long as an axis has some left. s(i) = i / P, or with TRHIP_ROPE_LADDERS
+ * j / pairs[a] for the j-th pair of axis a. The two elements of pair i are i and P + i, or with TRHIP_ROPE_NEIGHBOURS 2i and 2i + 1.
+ * factors: P fp32 multipliers in device memory, or null (all 1). */
+enum { TRHIP_ROPE_NEIGHBOURS = 1, TRHIP_ROPE_DEALT = 2, TRHIP_ROPE_LADDERS = 4 };
+typedef struct trhip_rope_spec {
+    int axes;     /* 1 to 4 */
+    int pairs[4]; /* of the axes there are; none negative, 1 to 256 together */
+    int flags;
+    double base; /* positive and finite */
+    const float *factors;
+} trhip_rope_spec;
+
+/* Turns `heads` heads of dim elements, one behind the other in each token's row, x + t * x_stride to out + t * out_stride
+ * (type: TRHIP_F32, TRHIP_F16 or TRHIP_BF16; strides in elements). q and k heads that lie next to each other in a merged
+ * product's rows are one call. out may be x, with the same stride; else the rows must not overlap. pos: int32 [axes][tokens]
+ * on the device, pos_stride elements between axes; any value. Angles are reduced in 64 bits, so that they are as good far from 0
+ * as near; sines, cosines and products are in fp32, out is rounded once. dim: an even number up to 1024. */
+int trhip_rope(trhip_ctx *ctx, const trhip_rope_spec *spec, const void *x, int64_t x_stride, void *out, int64_t out_stride,
+               int type, int64_t tokens, int heads, int dim, const int32_t *pos, int64_t pos_stride);
+
+/* ---- The paged key/value cache in 4 bits ---------------------------------------------------------------------------------
+ * 4.5 bits an element instead of 16: 32 consecutive elements of a head's row are a block of 4-bit codes c with one f16 scale d,
+ * and element i stands for (c_i - 8) * d. Page tables, slots and lengths are those of the 16-bit cache (trhip_page_tables).
+ * page: a power of two from 16 to 4096; dim: a multiple of 32 up to 256. A plane (k, v: 16-byte aligned) is
+ * pages * heads * page * dim * 9 / 16 bytes: [pages][heads][page / 16] pieces of sixteen places, each 8 * dim bytes of codes and then
+ * 16 * dim / 32 scales, in the order in which the attention multiplies them. In a piece, with B = dim / 32 and the place r:
+ *   element e of a key:    nibble (0, 4, 1, 5, 2, 6, 3, 7)[e % 8] of dword ((e % 32 / 8) * 16 + r) * B + e / 32
+ *   element e of a value:  nibble (0, 4, 2, 6)[r % 4] + e % 2 of dword ((r / 4) * 16 + e % 32 / 2) * B + e / 32
+ *   block b's scale:       scale ((r / 4) * B + b) * 4 + r % 4
+ * (nibble n of a dword: bits 4n to 4n + 3; dwords are little endian). */
+typedef struct trhip_kv4 {
+    int page, heads, dim;
+    int64_t pages;
+    void *k, *v;
+} trhip_kv4;
+
+/* Key and value rows into the cache, as trhip_kv_append: rows k + t * stride and v + t * stride to slot slots[t], a slot below 0 or
+ * past the cache skipped. A block's scale is its element of largest magnitude (the first of equal ones) times -1/8, rounded to
+ * five significant bits (nearest, even), then to f16, at most 7936: so that every value (c - 8) * d is exact in f16 and in bf16.
+ * Its codes are x / d rounded to the nearest whole number (even) within -8 .. 7, plus 8, without any error before that rounding. Blocks whose
+ * scale is 0 hold zeros (code 8), so magnitudes below 2^-22 vanish; beyond 63488 they are cut to it. A block with an
+ * infinity or a NaN has scale NaN: all of its elements read as NaN. Two tokens with the same slot leave a mix of both rows. */
+int trhip_kv4_append(trhip_ctx *ctx, const trhip_kv4 *kv, int64_t tokens, const void *k, const void *v, int type,
+                     int64_t stride, const int32_t *slots);
+
+/* The other way round: the values that slot slots[t] stands for, to rows k + t * stride and v + t * stride of type (exact in all three
+ * where trhip_kv4_append wrote them; otherwise rounded once). Rows of a slot below 0 or past the cache stay as they are. */
+int trhip_kv4_read(trhip_ctx *ctx, const trhip_kv4 *kv, int64_t tokens, void *k, void *v, int type, int64_t stride,
+                   const int32_t *slots);
+
+/* trhip_attn over the 4-bit cache: same masks, tables, lengths, hints and limits. q and out are of `type` (TRHIP_F16 or TRHIP_BF16).
+ * A block whose scale is not finite reads as NaN where a token sees it: in its elements of the result as a value, in the whole row
+ * of the head as a key. What a token's mask hides never reaches it. */
+int trhip_kv4_attn(trhip_ctx *ctx, const trhip_kv4 *kv, const void *q, int type, int64_t q_stride, void *out, int64_t out_stride,
+                   int64_t tokens, int heads, int64_t nreq, const int32_t *q_start, const int32_t *kv_len,
+                   const int32_t *table, int64_t max_pages, int64_t max_new, int64_t window, int64_t sinks, float scale);
+
+/* ---- The next token ------------------------------------------------------------------------------------------------------
+ * A token for each row of logits (rows logits + r * stride of vocab elements, type TRHIP_F32, TRHIP_F16 or TRHIP_BF16), from a given
+ * random number u[r] in [0, 1). Settings are read on the device, one a row; a null array switches that setting off.
+ * Weights w_i = exp((l_i - max) / temperature) (null: 1). In descending order (of equal logits the lowest index first) are kept
+ *   the first top_k (0 and below: all),
+ *   of those the shortest run whose weights reach top_p of their sum (1 and above, NaN: all; 0 and below: the first),
+ *   of those the ones of at least min_p times the largest weight (0 and below, NaN: all; 1 and above: the largest),
+ * so the first is always kept. token[r] is the first kept index at which the running sum of kept weights, by index, exceeds u
+ * times their sum (u of 1 and above: the last kept one whose weight is not 0; below 0 and NaN: as 0); logprob[r] (may be null) the logarithm of its weight in
+ * their sum. A temperature of 0, below, or NaN takes the largest logit (logprob 0). -Inf and NaN are never taken; where there is
+ * +Inf, only entries of +Inf have weight (each the same). A row with nothing else has token -1 and logprob NaN. Weights and sums are in 64 bits, so
+ * the token is the definition's unless u lies within some 1e-13 of a border. vocab: up to 2^24. */
+int trhip_sample(trhip_ctx *ctx, const void *logits, int type, int64_t stride, int64_t rows, int64_t vocab,
+                 const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p, const float *u,
+                 int32_t *token, float *logprob);
+
 /* Quantize fp32 rows to Q8 activation blocks on the device (tensor/cpu_quant_q8.go:39-68):
  * q [M, K] int8, d [M, K/blk] fp32, bs [M, K/16] int16; blk is 32 or 256. Exposed for
  * parity tests and for callers that reuse one quantized activation across weights. */

@@ -64,6 +64,11 @@ SIGNATURES = [
     ("trhip_kv_append", INT, [P, P, I64, P, P, INT, I64, P]),
     ("trhip_attn", INT, [P, P, P, I64, P, I64, I64, INT, I64, P, P, P, I64, I64, I64, I64, F32_T]),
     ("trhip_attn_shared", INT, [P, P, P, I64, P, I64, I64, INT, I64, P, P, P, I64, P, I64, I64, F32_T]),
+    ("trhip_rope", INT, [P, P, P, I64, P, I64, INT, I64, INT, INT, P, I64]),
+    ("trhip_kv4_append", INT, [P, P, I64, P, P, INT, I64, P]),
+    ("trhip_kv4_read", INT, [P, P, I64, P, P, INT, I64, P]),
+    ("trhip_kv4_attn", INT, [P, P, P, INT, I64, P, I64, I64, INT, I64, P, P, P, I64, I64, I64, I64, F32_T]),
+    ("trhip_sample", INT, [P, P, INT, I64, I64, I64, P, P, P, P, P, P, P]),
     ("trhip_rows_plan", INT, [INT, I64, I64, I64, INT, ctypes.POINTER(I64)]),
     ("trhip_set_launch_shape", INT, [P, INT, INT, INT, INT, INT]),
 ]
@@ -74,11 +79,22 @@ class KV(ctypes.Structure):
     _fields_ = [("dtype", INT), ("page", INT), ("heads", INT), ("dim", INT), ("pages", I64), ("k", P), ("v", P)]
 
 
+class KV4(ctypes.Structure):
+    """trhip_kv4"""
+    _fields_ = [("page", INT), ("heads", INT), ("dim", INT), ("pages", I64), ("k", P), ("v", P)]
+
+
+class RopeSpec(ctypes.Structure):
+    """trhip_rope_spec"""
+    _fields_ = [("axes", INT), ("pairs", INT * 4), ("flags", INT), ("base", ctypes.c_double), ("factors", P)]
+
+
 # Status codes and enums (include/trhip.h)
 OK, ERR_INVALID, ERR_OOM, ERR_HIP, ERR_LAUNCH, ERR_UNSUPPORTED, ERR_NO_DEVICE, ERR_BAD_SCALE = range(8)
 Q8, Q4, Q4K, Q6K = 1, 2, 3, 4
 MODE_EXACT, MODE_FAST = 0, 1
 F32, F16, BF16 = 0, 1, 2
+ROPE_NEIGHBOURS, ROPE_DEALT, ROPE_LADDERS = 1, 2, 4
 KNOB_KL, KNOB_FAST_Q4K, KNOB_EXACT_ROWS, KNOB_EXACT_LANES, KNOB_ACTQ_TM, KNOB_ROWS16, KNOB_KL_GRID, KNOB_ROWS, KNOB_FAST_GEMM = range(1, 10)
 
 

@@ -229,6 +229,39 @@ class KVCache:
                 b.free()
 
 
+class KV4Cache:
+    """A paged key/value cache in 4 bits (trhip_kv4): planes k and v in the caller's memory, plane_bytes() each, or allocated
+    here (NewKV4Cache) and then freed with release()."""
+
+    def __init__(self, pages, page, heads, dim, k, v):
+        self.pages, self.page, self.heads, self.dim = int(pages), int(page), int(heads), int(dim)
+        self.k, self.v = k, v
+        self.c = _lib.KV4(self.page, self.heads, self.dim, self.pages, _ptr(k), _ptr(v))
+        self.ref = ctypes.byref(self.c)
+
+    @staticmethod
+    def plane_bytes(pages, page, heads, dim):
+        return int(pages) * page * heads * dim * 9 // 16
+
+    def release(self):
+        for b in (self.k, self.v):
+            if isinstance(b, DeviceBuffer):
+                b.free()
+
+
+class RopeSpec:
+    """How rotary positions turn a head's pairs (trhip_rope_spec). pairs: pairs that each axis turns, one to four axes; factors: device
+    memory of as many fp32 multipliers as there are pairs (kept by the caller), or None."""
+
+    def __init__(self, pairs, base=10000.0, neighbours=False, dealt=False, ladders=False, factors=None):
+        if not 1 <= len(pairs) <= 4:
+            raise ValueError("one to four axes")
+        self.pairs, self.factors = tuple(int(n) for n in pairs), factors
+        flags = (_lib.ROPE_NEIGHBOURS if neighbours else 0) | (_lib.ROPE_DEALT if dealt else 0) | (_lib.ROPE_LADDERS if ladders else 0)
+        self.c = _lib.RopeSpec(len(pairs), (ctypes.c_int * 4)(*self.pairs), flags, base, None if factors is None else _ptr(factors))
+        self.ref = ctypes.byref(self.c)
+
+
 class QuantBackend:
     """The quantized-matmul slice of the reference's Backend, on one MI355X context."""
 
@@ -319,6 +352,41 @@ class QuantBackend:
         _check(_lib.lib().trhip_attn_shared(self.ctx.h, kv.ref, _ptr(q), q_stride, _ptr(out), out_stride, tokens, heads, nreq,
                                             _ptr(q_start), _ptr(kv_len), _ptr(table), max_pages, _ptr(prefix_pages), prefix_len,
                                             max_new, scale), self.ctx.h)
+
+    def Rope(self, spec, x, x_stride, out, out_stride, xtype, tokens, heads, dim, pos, pos_stride):
+        """Rotary positions on `heads` heads of each row, out may be x (trhip_rope). pos: int32 [axes][tokens], pos_stride apart."""
+        _check(_lib.lib().trhip_rope(self.ctx.h, spec.ref, _ptr(x), x_stride, _ptr(out), out_stride, xtype, tokens, heads, dim,
+                                     _ptr(pos), pos_stride), self.ctx.h)
+
+    def NewKV4Cache(self, pages, page, heads, dim):
+        """A 4-bit cache of `pages` pages of `page` keys in device memory of this context; what it holds is unset."""
+        nbytes = max(KV4Cache.plane_bytes(pages, page, heads, dim), 1)
+        k = self.ctx.alloc(nbytes)
+        try:
+            return KV4Cache(pages, page, heads, dim, k, self.ctx.alloc(nbytes))
+        except Exception:
+            k.free()
+            raise
+
+    def KV4Append(self, kv, tokens, k, v, ktype, stride, slots):
+        """KVAppend to a 4-bit cache (trhip_kv4_append)."""
+        _check(_lib.lib().trhip_kv4_append(self.ctx.h, kv.ref, tokens, _ptr(k), _ptr(v), ktype, stride, _ptr(slots)), self.ctx.h)
+
+    def KV4Read(self, kv, tokens, k, v, ktype, stride, slots):
+        """The values in a 4-bit cache's slots, to key and value rows (trhip_kv4_read)."""
+        _check(_lib.lib().trhip_kv4_read(self.ctx.h, kv.ref, tokens, _ptr(k), _ptr(v), ktype, stride, _ptr(slots)), self.ctx.h)
+
+    def KV4Attention(self, kv, q, qtype, q_stride, out, out_stride, tokens, heads, nreq, q_start, kv_len, table, max_pages, max_new=None,
+                     window=0, sinks=0, scale=None):
+        """Attention over a 4-bit cache, q and out of qtype (F16 or BF16; trhip_kv4_attn). max_new, scale: as above."""
+        scale, max_new = kv.dim ** -0.5 if scale is None else scale, _max_new(max_new, tokens, nreq)
+        _check(_lib.lib().trhip_kv4_attn(self.ctx.h, kv.ref, _ptr(q), qtype, q_stride, _ptr(out), out_stride, tokens, heads, nreq,
+                                         _ptr(q_start), _ptr(kv_len), _ptr(table), max_pages, max_new, window, sinks, scale), self.ctx.h)
+
+    def Sample(self, logits, ltype, stride, rows, vocab, u, token, logprob=None, temperature=None, top_k=None, top_p=None, min_p=None):
+        """A token for each row of logits from the random numbers u (trhip_sample). Settings are device arrays, one value a row."""
+        opt = [None if x is None else _ptr(x) for x in (temperature, top_k, top_p, min_p, logprob)]
+        _check(_lib.lib().trhip_sample(self.ctx.h, _ptr(logits), ltype, stride, rows, vocab, *opt[:4], _ptr(u), _ptr(token), opt[4]), self.ctx.h)
 
     def close(self):
         self.ctx.close()

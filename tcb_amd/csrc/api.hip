@@ -284,26 +284,70 @@ int check_kv(trhip_ctx *ctx, const trhip_kv *kv, const char *what) {
     return TRHIP_OK;
 }
 
-// trhip_attn and trhip_attn_shared: checks, then the launch.
-int attention(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c, const char *what) {
-    const int st = check_kv(ctx, kv, what);
-    if (st != TRHIP_OK) return st;
+int check_kv4(trhip_ctx *ctx, const trhip_kv4 *kv, const char *what) {
+    auto bad = [&](int code, const char *why) { return fail(ctx, code, std::string(what) + ": " + why); };
+    if (!kv) return bad(TRHIP_ERR_INVALID, "null cache");
+    if (bad_page(kv->page)) return bad(TRHIP_ERR_INVALID, "the page must be a power of two, 16 to 4096");
+    if (kv->dim < 32 || kv->dim > 256 || kv->dim % 32 != 0) return bad(TRHIP_ERR_UNSUPPORTED, "the head size must be a multiple of 32 up to 256");
+    if (kv->heads < 1 || kv->heads > 65536 || kv->pages < 0 || kv->pages > kMaxInt || (int64_t)kv->pages * kv->page > kMaxInt)
+        return bad(TRHIP_ERR_INVALID, "bad head or page count");
+    if (kv->pages > 0 && (!kv->k || !kv->v)) return bad(TRHIP_ERR_INVALID, "null cache planes");
+    if (reinterpret_cast<uintptr_t>(kv->k) % 16 || reinterpret_cast<uintptr_t>(kv->v) % 16)
+        return bad(TRHIP_ERR_INVALID, "the cache planes must be 16-byte aligned");
+    return TRHIP_OK;
+}
+
+bool bad_type(int type) { return type != TRHIP_F32 && type != TRHIP_F16 && type != TRHIP_BF16; }
+
+// What the entry points of attention check beside the cache; *some: whether there is anything to do.
+int check_attention(trhip_ctx *ctx, const AttnCall &c, int kv_heads, int page, int dim, const char *what, bool *some) {
+    *some = false;
     auto bad = [&](const char *why) { return fail(ctx, TRHIP_ERR_INVALID, std::string(what) + ": " + why); };
     if (c.tokens < 0 || c.nreq < 0 || c.max_pages < 0 || c.max_new < 0 || c.window < 0 || c.sinks < 0 || c.prefix_len < 0)
         return bad("negative size");
-    if (c.heads < 1 || c.heads % kv->heads != 0) return bad("the heads must be a multiple of the cache's");
+    if (c.heads < 1 || c.heads % kv_heads != 0) return bad("the heads must be a multiple of the cache's");
     if (!(c.scale > 0.0f) || c.scale > 1e30f) return bad("the scale must be positive and finite");
     if (c.tokens == 0 || c.nreq == 0) return TRHIP_OK;
     // (the kernels round key counts up to blocks and pages in 32 bits)
-    if (c.nreq > kMaxInt || c.max_pages > kMaxInt || c.max_pages * kv->page > kMaxInt - 4096 || c.window > kMaxInt || c.sinks > kMaxInt ||
+    if (c.nreq > kMaxInt || c.max_pages > kMaxInt || c.max_pages * page > kMaxInt - 4096 || c.window > kMaxInt || c.sinks > kMaxInt ||
         c.prefix_len > kMaxInt - 4096 || c.tokens > kMaxInt / c.heads)
         return bad("size past 2^31 - 1");
     if (!c.q || !c.out || !c.q_start || !c.kv_len || (c.max_pages > 0 && !c.table) || (c.prefix_len > 0 && !c.prefix_table))
         return bad("null pointer");
     if (reinterpret_cast<uintptr_t>(c.q) % 2 || reinterpret_cast<uintptr_t>(c.out) % 2) return bad("q or out is not aligned to its type");
-    if (c.q_stride < (int64_t)c.heads * kv->dim || c.out_stride < (int64_t)c.heads * kv->dim) return bad("rows overlap");
+    if (c.q_stride < (int64_t)c.heads * dim || c.out_stride < (int64_t)c.heads * dim) return bad("rows overlap");
+    *some = true;
+    return TRHIP_OK;
+}
+
+// trhip_attn and trhip_attn_shared: checks, then the launch.
+int attention(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c, const char *what) {
+    int st = check_kv(ctx, kv, what);
+    if (st != TRHIP_OK) return st;
+    bool some = false;
+    st = check_attention(ctx, c, kv->heads, kv->page, kv->dim, what, &some);
+    if (st != TRHIP_OK || !some) return st;
     DevGuard g(ctx);
     return launch_attn(ctx, kv, c);
+}
+
+// trhip_kv4_append and trhip_kv4_read: checks; *some: whether there is anything to do.
+int check_kv4_rows(trhip_ctx *ctx, const trhip_kv4 *kv, int64_t tokens, const void *k, const void *v, int type, int64_t stride,
+                   const int32_t *slots, const char *what, bool *some) {
+    *some = false;
+    const int st = check_kv4(ctx, kv, what);
+    if (st != TRHIP_OK) return st;
+    auto bad = [&](const char *why) { return fail(ctx, TRHIP_ERR_INVALID, std::string(what) + ": " + why); };
+    if (tokens < 0) return bad("negative size");
+    if (bad_type(type)) return bad("bad element type");
+    if (tokens == 0) return TRHIP_OK;
+    if (tokens > kMaxInt) return bad("size past 2^31 - 1");
+    if (!k || !v || !slots) return bad("null pointer");
+    if (stride < (int64_t)kv->heads * kv->dim) return bad("rows overlap");
+    const uintptr_t e = type == TRHIP_F32 ? 4 : 2;
+    if (reinterpret_cast<uintptr_t>(k) % e || reinterpret_cast<uintptr_t>(v) % e) return bad("k or v is not aligned to its type");
+    *some = true;
+    return TRHIP_OK;
 }
 
 // Threads for host passes over `bytes` bytes: one below 4 MiB, where starting threads costs more than it saves.
@@ -1131,6 +1175,87 @@ int trhip_attn_shared(trhip_ctx *ctx, const trhip_kv *kv, const void *q, int64_t
     AttnCall c = {q, out, q_stride, out_stride, tokens, heads, nreq, q_start, kv_len, table, max_pages, max_new, prefix_pages,
                   prefix_len, 0, 0, scale};
     return attention(ctx, kv, c, "attn_shared");
+}
+
+int trhip_rope(trhip_ctx *ctx, const trhip_rope_spec *spec, const void *x, int64_t x_stride, void *out, int64_t out_stride,
+               int type, int64_t tokens, int heads, int dim, const int32_t *pos, int64_t pos_stride) {
+    if (!ctx) return TRHIP_ERR_INVALID;
+    auto bad = [&](const char *why) { return fail(ctx, TRHIP_ERR_INVALID, std::string("rope: ") + why); };
+    if (!spec) return bad("null spec");
+    if (spec->axes < 1 || spec->axes > 4) return bad("one to four axes");
+    int64_t pairs = 0;
+    for (int a = 0; a < spec->axes; a++) {
+        if (spec->pairs[a] < 0) return bad("negative size");
+        pairs += spec->pairs[a];
+    }
+    if (spec->flags & ~(TRHIP_ROPE_NEIGHBOURS | TRHIP_ROPE_DEALT | TRHIP_ROPE_LADDERS)) return bad("unknown flags");
+    if (!(spec->base > 0.0) || spec->base > 1e300) return bad("the base must be positive and finite");
+    if (reinterpret_cast<uintptr_t>(spec->factors) % 4) return bad("factors are not aligned to their type");
+    if (tokens < 0) return bad("negative size");
+    if (bad_type(type)) return bad("bad element type");
+    if (heads < 1 || heads > 65536) return bad("bad head count");
+    if (dim < 2 || dim > 1024 || dim % 2) return fail(ctx, TRHIP_ERR_UNSUPPORTED, "rope: the head size must be even, up to 1024");
+    if (pairs < 1 || pairs > 256 || 2 * pairs > dim) return bad("1 to 256 pairs, no more than half a head");
+    if (tokens == 0) return TRHIP_OK;
+    if (tokens > kMaxInt) return bad("size past 2^31 - 1");
+    if (!x || !out || !pos) return bad("null pointer");
+    const uintptr_t e = type == TRHIP_F32 ? 4 : 2, xa = reinterpret_cast<uintptr_t>(x), oa = reinterpret_cast<uintptr_t>(out);
+    if (xa % e || oa % e || reinterpret_cast<uintptr_t>(pos) % 4) return bad("x, out or pos is not aligned to its type");
+    const int64_t row = (int64_t)heads * dim;
+    if ((tokens > 1 && (x_stride < row || out_stride < row)) || (spec->axes > 1 && pos_stride < tokens)) return bad("rows overlap");
+    if (x == out && tokens > 1 && x_stride != out_stride) return bad("in place, both strides must be the same");
+    DevGuard g(ctx);
+    return launch_rope(ctx, *spec, x, x_stride, out, out_stride, type, tokens, heads, dim, pos, pos_stride);
+}
+
+int trhip_kv4_append(trhip_ctx *ctx, const trhip_kv4 *kv, int64_t tokens, const void *k, const void *v, int type, int64_t stride,
+                     const int32_t *slots) {
+    if (!ctx) return TRHIP_ERR_INVALID;
+    bool some = false;
+    const int st = check_kv4_rows(ctx, kv, tokens, k, v, type, stride, slots, "kv4_append", &some);
+    if (st != TRHIP_OK || !some) return st;
+    DevGuard g(ctx);
+    return launch_kv4_append(ctx, kv, tokens, k, v, type, stride, slots);
+}
+
+int trhip_kv4_read(trhip_ctx *ctx, const trhip_kv4 *kv, int64_t tokens, void *k, void *v, int type, int64_t stride, const int32_t *slots) {
+    if (!ctx) return TRHIP_ERR_INVALID;
+    bool some = false;
+    const int st = check_kv4_rows(ctx, kv, tokens, k, v, type, stride, slots, "kv4_read", &some);
+    if (st != TRHIP_OK || !some) return st;
+    DevGuard g(ctx);
+    return launch_kv4_read(ctx, kv, tokens, k, v, type, stride, slots);
+}
+
+int trhip_kv4_attn(trhip_ctx *ctx, const trhip_kv4 *kv, const void *q, int type, int64_t q_stride, void *out, int64_t out_stride,
+                   int64_t tokens, int heads, int64_t nreq, const int32_t *q_start, const int32_t *kv_len, const int32_t *table,
+                   int64_t max_pages, int64_t max_new, int64_t window, int64_t sinks, float scale) {
+    if (!ctx) return TRHIP_ERR_INVALID;
+    int st = check_kv4(ctx, kv, "kv4_attn");
+    if (st != TRHIP_OK) return st;
+    if (type != TRHIP_F16 && type != TRHIP_BF16) return fail(ctx, TRHIP_ERR_UNSUPPORTED, "kv4_attn: q and out must be f16 or bf16");
+    AttnCall c = {q, out, q_stride, out_stride, tokens, heads, nreq, q_start, kv_len, table, max_pages, max_new, nullptr, 0, window,
+                  sinks, scale};
+    bool some = false;
+    st = check_attention(ctx, c, kv->heads, kv->page, kv->dim, "kv4_attn", &some);
+    if (st != TRHIP_OK || !some) return st;
+    DevGuard g(ctx);
+    return launch_kv4_attn(ctx, kv, c, type);
+}
+
+int trhip_sample(trhip_ctx *ctx, const void *logits, int type, int64_t stride, int64_t rows, int64_t vocab, const float *temperature,
+                 const int32_t *top_k, const float *top_p, const float *min_p, const float *u, int32_t *token, float *logprob) {
+    if (!ctx) return TRHIP_ERR_INVALID;
+    auto bad = [&](const char *why) { return fail(ctx, TRHIP_ERR_INVALID, std::string("sample: ") + why); };
+    if (rows < 0 || vocab < 0) return bad("negative size");
+    if (bad_type(type)) return bad("bad element type");
+    if (rows == 0) return TRHIP_OK;
+    if (vocab < 1 || vocab > (1 << 24) || rows > (1 << 20)) return bad("1 to 2^24 entries and up to 2^20 rows");
+    if (!logits || !u || !token) return bad("null pointer");
+    if (rows > 1 && stride < vocab) return bad("rows overlap");
+    if (reinterpret_cast<uintptr_t>(logits) % (type == TRHIP_F32 ? 4 : 2)) return bad("logits are not aligned to their type");
+    DevGuard g(ctx);
+    return launch_sample(ctx, logits, type, stride, rows, vocab, temperature, top_k, top_p, min_p, u, token, logprob);
 }
 
 int trhip_quantize_q8(trhip_ctx *ctx, const float *x, int64_t M, int64_t K, int blk, int8_t *q, float *d,

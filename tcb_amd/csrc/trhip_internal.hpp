@@ -499,4 +499,14 @@ struct AttnCall {
     float scale;
 };
 int launch_attn(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c);
+// Rotary positions (rope.hip), the 4-bit cache (kv4.hip), attention over it (attn4.hip; io: type of q and out), sampling
+// (sample.hip); arguments as the entry points check them.
+int launch_rope(trhip_ctx *ctx, const trhip_rope_spec &spec, const void *x, int64_t x_stride, void *out, int64_t out_stride, int io,
+                int64_t tokens, int heads, int dim, const int *pos, int64_t pos_stride);
+int launch_kv4_append(trhip_ctx *ctx, const trhip_kv4 *kv, int64_t tokens, const void *k, const void *v, int io, int64_t stride,
+                      const int *slots);
+int launch_kv4_read(trhip_ctx *ctx, const trhip_kv4 *kv, int64_t tokens, void *k, void *v, int io, int64_t stride, const int *slots);
+int launch_kv4_attn(trhip_ctx *ctx, const trhip_kv4 *kv, const AttnCall &c, int io);
+int launch_sample(trhip_ctx *ctx, const void *logits, int io, int64_t stride, int64_t rows, int64_t vocab, const float *temperature,
+                  const int *top_k, const float *top_p, const float *min_p, const float *u, int *token, float *logprob);
 }  // namespace trhip
