@@ -5,6 +5,7 @@
 //
 // Here: the kernel of few rows (attn_tokens.hpp), the joining launch, and the call's plan. Many rows: attn_rows.hpp. Both in one
 // launch, for batches that have both and for a shared prefix beside its requests' own keys: attn_two.hip.
+#include "attn_plan.hpp"
 #include "attn_tokens.hpp"
 
 namespace trhip {
@@ -77,32 +78,6 @@ template <bool PREFIX> int launch_tokens(trhip_ctx *ctx, const AttnArgs &p, int 
     return bf ? launch_tokens<256, true, PREFIX>(ctx, p, grid) : launch_tokens<256, false, PREFIX>(ctx, p, grid);
 }
 
-constexpr int kAnyRows = 0x7FFFFFFF;
-
-// Tiles of a batch of these sizes, at most.
-int64_t tiles_of(const AttnArgs &p, const AttnCall &c, int tile_rows) {
-    int64_t tiles = c.tokens * p.group / tile_rows + c.nreq;
-    if (p.row_hi != kAnyRows) {
-        const int64_t few = (p.row_hi + tile_rows - 1) / tile_rows * c.nreq;
-        tiles = tiles < few ? tiles : few;
-    }
-    return tiles * p.kv_heads;
-}
-
-// The launch's workgroups: as many items as a batch of these sizes can have (find_item), whatever its lengths are. The rounds
-// that pieces may take go by the tiles there will be: a tile a request beside longer ones.
-int64_t plan_items(AttnArgs &p, const AttnCall &c, int tile_rows, int block, int least) {
-    const int64_t tiles = tiles_of(p, c, tile_rows), one = c.nreq * p.kv_heads, usual = p.row_hi != kAnyRows && one < tiles ? one : tiles;
-    const int64_t blocks = ((c.max_pages << p.page_log2) + block - 1) / block, most = tiles * ((blocks + least - 1) / least + 1);
-    const int64_t k = (2 * usual + p.target - 1) / p.target;
-    p.rounds = (int)(k < kMostRounds ? k : kMostRounds);
-    p.part_slots = p.rounds * p.target;
-    int64_t items = p.part_slots < most ? p.part_slots : most;
-    if (tiles > items) items = tiles;
-    if (c.prefix_len > 0) p.part_slots = (int)items;
-    return items;
-}
-
 }  // namespace
 
 int launch_attn(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c) {
@@ -145,13 +120,13 @@ int launch_attn(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c) {
     // 79.6 and 80.4. Which there are is known only from the hint, so both are launched unless it (or the sizes) rules one
     // out. Each takes the requests of its own length, or all of them when it is alone.
     const int64_t most_new = c.max_new < c.tokens ? c.max_new : c.tokens;
-    const bool tokens_alone = most_new * p.group <= kTokMost, rows_alone = !tokens_alone && c.tokens == c.nreq * most_new;
+    const bool tokens_alone = most_new * p.group <= kTokMost, rows_alone = !tokens_alone && (c.long_only || c.tokens == c.nreq * most_new);
     AttnArgs pt = p, pr = p;
     pt.target = cus * (dp <= 128 ? 2 : 1);
     pt.row_lo = 0;
     pt.row_hi = tokens_alone ? kAnyRows : kTokMost;
     pr.target = cus * attn_rows_per_cu(dp);
-    pr.row_lo = rows_alone ? 0 : kTokMost;
+    pr.row_lo = rows_alone && !c.long_only ? 0 : kTokMost;
     pr.row_hi = kAnyRows;
     const int tr = attn_rows_tile(), br = attn_rows_block();
     const bool prefix = c.prefix_len > 0;

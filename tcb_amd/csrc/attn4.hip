@@ -1,84 +1,483 @@
-// attn4.hip -- attention over the 4-bit paged cache.
-#include "attn_common.hpp"
+// attn4.hip -- attention over the 4-bit paged cache (kv4.hpp) for few rows, and the call's plan.
+//
+// Rows, work items, pieces and joins are those of the 16-bit cache's kernel of few rows (attn_common.hpp): a workgroup takes a tile of
+// 16 or 32 rows (the heads of a few tokens that read one kv head) and a piece of the keys; its four waves take every fourth block of
+// 32 keys and join through LDS. What differs is the block.
+//
+// Nothing of a block goes through LDS: the codes lie in memory as the matrix instructions' operands want them, so a lane loads
+// its part of a piece of sixteen places as it stands. Two nibbles c masked out of a dword become 1024 + c (or 64 + c) in f16 by
+// setting the exponent, and c - 8, exactly, by one packed subtraction: nine instructions open eight codes. (Left as c 2^-24, below f16's
+// normal range, five would do, but the matrix units sum such products to 2^-18 only.)
+//   S^T of a block of 32 elements: q.(c - 8), then times the key's scale, in fp32, summed over the blocks. q is scaled by a power of two
+//   to f16's upper end.
+//   O^T += V^T P^T: the value's scale goes to the weight, w = p s (there is one product a block of 32 elements).
+// The weights p s stand in f16, in one term for bf16 results (their rounding of 2^-12 is a sixteenth of the result's) and in two
+// for f16 ones. So that they neither overflow nor vanish, the softmax's reference includes the largest scale the wave has met.
+#include "attn_plan.hpp"
 #include "kv4.hpp"
 
 namespace trhip {
 namespace {
 
-struct Attn4Args {
-    const uint16_t *q;
-    uint16_t *out;
-    const uint8_t *k, *v;
-    int64_t q_stride, out_stride, max_pages, pages;
-    const int *q_start, *kv_len, *table;
-    int tokens, nreq, heads, kv_heads, dim, page_log2, window, sinks, io;
-    float scale;
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x3 __attribute__((ext_vector_type(3)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+
+constexpr int kTwoSets = 4;  // blocks of elements up to which a workgroup's registers hold two sets of rows
+constexpr int kWaves = 4, kBlock = 32, kLeast = 8, kOver = 6;
+
+template <int NG, int NC> struct Shape4 {
+    static constexpr int DIM = 32 * NG, ROWS = 16 * NC;
+    static constexpr int OSTRIDE = DIM + 4;  // floats between rows of a wave's results
+    static constexpr int WAVE = ROWS * OSTRIDE * 4;
+    static constexpr int BYTES = kWaves * (WAVE + ROWS * 8) + 16;
 };
 
-__device__ __forceinline__ float wave_sum(float x) {
-    for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
-    return x;
+__device__ __forceinline__ f4 mma16(u32x4 a, u32x4 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(a8h, a), __builtin_bit_cast(a8h, b), c, 0, 0, 0);
+}
+// Maximum and sum over the four lanes that hold one row.
+__device__ __forceinline__ float row_max(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const auto s = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return half_max(fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1])));
+}
+__device__ __forceinline__ float row_sum(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const auto s = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return half_sum(__uint_as_float(s[0]) + __uint_as_float(s[1]));
 }
 
-// One wave a token and head, a key at a time, up to four elements a lane.
-__global__ __launch_bounds__(64) void attn4_simple(const Attn4Args p) {
-    const int t = blockIdx.x, head = blockIdx.y, lane = threadIdx.x, kvh = head / (p.heads / p.kv_heads);
-    int req = -1, start = 0, end = 0;
-    for (int i = 0; i < p.nreq; i++) {
-        int a = p.q_start[i], b = p.q_start[i + 1];
-        a = a < 0 ? 0 : a > p.tokens ? p.tokens : a;
-        b = b < a ? a : b > p.tokens ? p.tokens : b;
-        if (t >= a && t < b) req = i, start = a, end = b;
-    }
-    if (req < 0) return;
-    const int64_t cap = p.max_pages << p.page_log2;
-    int kv = p.kv_len[req];
-    kv = kv < 0 ? 0 : (int64_t)kv > cap ? (int)cap : kv;
-    const int pos = kv - (end - start) + (t - start);
-    constexpr int nib[8] = {0, 4, 1, 5, 2, 6, 3, 7};
-    float q[4] = {}, o[4] = {}, m = -__builtin_inff(), l = 0.0f;
-    for (int u = 0; u < 4; u++)
-        if (lane + 64 * u < p.dim) q[u] = h16_to_f32(p.q[(int64_t)t * p.q_stride + head * p.dim + lane + 64 * u], p.io);
-    for (int j = 0; j <= pos; j++) {
-        if (p.window > 0 && j <= pos - p.window && j >= p.sinks) {
-            j = pos - p.window;
-            continue;
+// The f16 operand c - 8 of a dword's eight codes: nibbles 0 and 4, 1 and 5, 2 and 6, 3 and 7.
+__device__ __forceinline__ u32x4 open8(uint32_t y) {
+    const uint32_t z = y >> 8;
+    const h2 a = {(_Float16)-1032.0f, (_Float16)-1032.0f}, b = {(_Float16)-72.0f, (_Float16)-72.0f};
+    auto even = [&](uint32_t x) { return __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, (x & 0x000F000Fu) | 0x64006400u) + a); };
+    auto odd = [&](uint32_t x) { return __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, (x & 0x00F000F0u) | 0x54005400u) + b); };
+    return (u32x4){even(y), odd(y), even(z), odd(z)};
+}
+
+// N dwords at a lane's offset of a piece; past its end zeros.
+template <int N> struct Dwords {
+    uint32_t v[N];
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t d, int at) {
+#pragma unroll
+        for (int i = 0; i + 4 <= N; i += 4) {
+            const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(d, at + 4 * i, 0, 0);
+            v[i] = x.x, v[i + 1] = x.y, v[i + 2] = x.z, v[i + 3] = x.w;
         }
-        const int page = p.table[(int64_t)req * p.max_pages + (j >> p.page_log2)];
-        float s = 0.0f, v[4] = {};
-        if ((uint32_t)page < (uint32_t)p.pages) {
-            const Kv4Place at = kv4_place(((int64_t)page << p.page_log2) + (j & ((1 << p.page_log2) - 1)), p.page_log2, p.kv_heads, kvh, p.dim);
-            for (int u = 0; u < 4; u++) {
-                const int e = lane + 64 * u;
-                if (e >= p.dim) continue;
-                const uint32_t kd = *reinterpret_cast<const uint16_t *>(p.k + at.piece + kv4_scale_at(at.r, e / 32, p.dim));
-                const uint32_t vd = *reinterpret_cast<const uint16_t *>(p.v + at.piece + kv4_scale_at(at.r, e / 32, p.dim));
-                const int kc = *reinterpret_cast<const uint32_t *>(p.k + at.piece + kv4_key_at(at.r, e & ~7, p.dim)) >> (4 * nib[e & 7]) & 15;
-                const int vc = p.v[at.piece + kv4_value_at(at.r, e, p.dim)] >> (4 * (e & 1)) & 15;
-                const float nan = __builtin_nanf("");
-                s = fmaf(q[u], (kd >> 10 & 31) == 31 ? nan : kv4_value(kc, kd), s);
-                v[u] = (vd >> 10 & 31) == 31 ? nan : kv4_value(vc, vd);
+        constexpr int i = N & ~3;
+        if constexpr (N % 4 == 3) {
+            const u32x3 x = __builtin_amdgcn_raw_buffer_load_b96(d, at + 4 * i, 0, 0);
+            v[i] = x.x, v[i + 1] = x.y, v[i + 2] = x.z;
+        } else if constexpr (N % 4 == 2) {
+            const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(d, at + 4 * i, 0, 0);
+            v[i] = x.x, v[i + 1] = x.y;
+        } else if constexpr (N % 4 == 1) {
+            v[i] = __builtin_amdgcn_raw_buffer_load_b32(d, at + 4 * i, 0, 0);
+        }
+    }
+};
+__device__ __forceinline__ float half_lo(uint32_t v) { return (float)__builtin_bit_cast(h2, v)[0]; }
+__device__ __forceinline__ float half_hi(uint32_t v) { return (float)__builtin_bit_cast(h2, v)[1]; }
+
+// A piece of sixteen places of one plane in a lane: its codes and the scales of its four places, [block][place].
+template <int NG> struct Piece4 {
+    Dwords<NG> codes;
+    Dwords<2 * NG> scales;
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t d) {
+        const int lane = threadIdx.x & 63;
+        codes.load(d, 4 * NG * lane);
+        scales.load(d, 256 * NG + 8 * NG * (lane >> 4));
+    }
+    __device__ __forceinline__ float scale(int b, int i) const {
+        const uint32_t v = scales.v[2 * b + (i >> 1)];
+        return i & 1 ? half_hi(v) : half_lo(v);
+    }
+};
+
+// What the rows of one set of sixteen see: this lane's row, and the extremes over the set's rows.
+struct Rows4 {
+    int hi, lo;
+};
+
+template <int NG> struct Acc4 {
+    f4 o[NG][2];
+    float m, f, l;  // reference (log2 units, with the lift and the scales'); the score it came from; this lane's share of the sum
+    float most;     // the highest reference so far
+    bool far;
+};
+
+template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves) void attn4_few(const AttnArgs p) {
+    using S = Shape4<NG, NC>;
+    constexpr bool TWO = !BF;
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6), c = lane & 15, quarter = lane >> 4;
+    Item it;
+    if (!find_item<S::ROWS, kBlock, kLeast, kOver>(p, blockIdx.x, gridDim.x, it)) return;
+    const int *table = p.table + (int64_t)it.req * p.max_pages;
+    const int keys = it.kv;
+    const int r0 = it.tile * S::ROWS, left = it.nq * p.group - r0, n = left < S::ROWS ? left : S::ROWS;
+    // masks: this lane's rows, then the extremes over the tile
+    const int first = keys - it.nq;
+    auto low = [&](int hi) { return p.window > 0 && hi >= p.window ? hi - p.window + 1 : 0; };
+    Rows4 rows[NC];
+#pragma unroll
+    for (int s = 0; s < NC; s++) {
+        const int r = 16 * s + c, row = r0 + (r < n ? r : n - 1);
+        rows[s].hi = first + p.by_group(row);
+        rows[s].lo = low(rows[s].hi);
+    }
+    const int hi_min = uni(first + p.by_group(r0)), hi_max = uni(first + p.by_group(r0 + n - 1)), lo_min = uni(low(hi_min)), lo_max = uni(low(hi_max));
+    const Span sp = span_of<kBlock>(hi_max, lo_min, p.sinks);
+    const int nb = sp.count(), piece = it.nsplit == 1 ? nb : (nb + it.nsplit - 1) / it.nsplit;
+    const int b0 = it.split * piece, b1 = b0 + piece < nb ? b0 + piece : nb;
+
+    // q in f16 operands, scaled by a power of two to at most 2^15
+    u32x4 q[NC][NG];
+    float sc[NC];
+#pragma unroll
+    for (int s = 0; s < NC; s++) {
+        const int r = 16 * s + c, row = r0 + (r < n ? r : 0), t = p.by_group(row), g0 = row - t * p.group;
+        const uint16_t *src = p.q + (int64_t)(it.q0 + t) * p.q_stride + (int64_t)(it.head * p.group + g0) * p.dim + 8 * quarter;
+        uint4 raw[NG];
+#pragma unroll
+        for (int g = 0; g < NG; g++) __builtin_memcpy(&raw[g], src + 32 * g, 16);  // (rows need be aligned to their type only)
+        float top = 0.0f;
+        auto each = [&](int g, auto use) {
+            const uint32_t x[4] = {raw[g].x, raw[g].y, raw[g].z, raw[g].w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) use(i, wide_lo<BF>(x[i]), wide_hi<BF>(x[i]));
+        };
+#pragma unroll
+        for (int g = 0; g < NG; g++) each(g, [&](int, float a, float b) { top = fmaxf(top, fmaxf(fabsf(a), fabsf(b))); });
+        top = row_max(top);
+        int e = 141 - (int)(__float_as_uint(top) >> 23);
+        e = e > 126 ? 126 : e;
+        const float up = __uint_as_float((uint32_t)(e + 127) << 23);
+        sc[s] = ldexpf(p.scale, -e);
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            each(g, [&](int i, float a, float b) { q[s][g][i] = __builtin_bit_cast(uint32_t, (h2){(_Float16)(a * up), (_Float16)(b * up)}); });
+        }
+    }
+
+    // Block b's two pages, fetched a step before they are used, and its two pieces' bytes; past the last block nothing but zeros.
+    auto key_of = [&](int b) { return kBlock * sp.block(b); };
+    auto pages_of = [&](int b) {
+        const int t = b < b1 ? key_of(b) : 0, hi = b < b1 ? hi_max : -1;
+        return make_int2(page16(p, table, t, hi), page16(p, table, t + 16, hi));
+    };
+    struct Where {
+        int64_t off;
+        int bytes;
+    };
+    auto where_of = [&](int b, int half, int page) {
+        const int t = (b < b1 ? key_of(b) : 0) + 16 * half;
+        bool some = b < b1 && t <= hi_max && !(p.sinks <= t && lo_min >= t + 16);
+        if ((uint32_t)page >= (uint32_t)p.npages) page = 0, some = false;
+        const int64_t off = uni64((int64_t)page * p.page_bytes + (int64_t)it.head * p.head_bytes +
+                                  (int64_t)((t & ((1 << p.page_log2) - 1)) >> 4) * (9 * S::DIM));
+        return Where{off, uni(some ? 9 * S::DIM : 0)};
+    };
+    auto load = [&](Piece4<NG> &x, const uint8_t *plane, const Where &at) {
+        x.load(__builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(plane + at.off), 0, at.bytes, 0x00020000));
+    };
+    int2 pages = pages_of(b0 + w);
+    Where at[2] = {where_of(b0 + w, 0, pages.x), where_of(b0 + w, 1, pages.y)};
+    Piece4<NG> k[2], v[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) load(k[h], p.k, at[h]);
+#pragma unroll
+    for (int h = 0; h < 2; h++) load(v[h], p.v, at[h]);
+    pages = pages_of(b0 + w + kWaves);
+
+    Acc4<NG> A[NC];
+#pragma unroll
+    for (int s = 0; s < NC; s++) {
+        A[s].m = A[s].f = A[s].most = -__builtin_inff();
+        A[s].l = 0.0f;
+        A[s].far = false;
+#pragma unroll
+        for (int g = 0; g < NG; g++) A[s].o[g][0] = A[s].o[g][1] = (f4){0, 0, 0, 0};
+    }
+    int tl = -24;                // the values' scales met so far are at most 2^tl,
+    uint32_t limit = 0x0001u;    // in f16
+
+    for (int b = b0 + w; b < b1; b += kWaves) {
+        const int t = key_of(b);
+        const Where next[2] = {where_of(b + kWaves, 0, pages.x), where_of(b + kWaves, 1, pages.y)};
+        pages = pages_of(b + 2 * kWaves);
+        float x[NC][8];
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                const u32x4 a = open8(k[h].codes.v[g]);
+#pragma unroll
+                for (int s = 0; s < NC; s++) {
+                    const f4 d = mma16(a, q[s][g], (f4){0, 0, 0, 0});
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[s][4 * h + i] = g == 0 ? k[h].scale(g, i) * d[i] : fmaf(k[h].scale(g, i), d[i], x[s][4 * h + i]);
+                }
+            }
+#pragma unroll
+        for (int h = 0; h < 2; h++) load(k[h], p.k, next[h]);
+        // the scales of the values: larger ones than so far, and ones that are not finite
+        uint32_t big = 0;
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int i = 0; i < 2 * NG; i++) {
+                const uint32_t a = v[h].scales.v[i] & 0x7FFF7FFFu;
+                big = big > (a & 0xFFFFu) ? big : a & 0xFFFFu;
+                big = big > (a >> 16) ? big : a >> 16;
+            }
+        const bool all = t + kBlock - 1 <= hi_min && (t >= lo_max || t + kBlock <= p.sinks);
+        if (__any(big > limit)) {
+            uint32_t finite = 0;
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                bool bad[NC] = {};
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        uint32_t &d = v[h].scales.v[2 * g + (i >> 1)];
+                        const int sh = 16 * (i & 1);
+                        const uint32_t u = d >> sh & 0x7FFFu;
+                        if (u < 0x7C00u) {
+                            finite = finite > u ? finite : u;
+                        } else {  // it reaches the rows that see it, and no other
+                            const int key = t + 16 * h + 4 * quarter + i;
+#pragma unroll
+                            for (int s = 0; s < NC; s++) bad[s] = bad[s] || (key <= rows[s].hi && (key >= rows[s].lo || key < p.sinks));
+                            d &= ~(0xFFFFu << sh);
+                        }
+                    }
+#pragma unroll
+                for (int s = 0; s < NC; s++) {
+                    const float nan = row_max(bad[s] ? 1.0f : 0.0f) > 0.0f ? __builtin_nanf("") : 0.0f;
+                    A[s].o[g][0] += nan;
+                    A[s].o[g][1] += nan;
+                }
+            }
+            float top = row_max(__uint_as_float(finite << 13) * 0x1p112f);  // f16's bits as fp32's: exact, subnormal ones too
+            top = fmaxf(top, __shfl_xor(top, 1));
+            if (uni(__float_as_uint(top)) > __float_as_uint(ldexpf(1.0f, tl))) {
+                const uint32_t u = uni(__float_as_uint(top));
+                const int to = (int)(u >> 23) - 127 + ((u & 0x7FFFFFu) != 0), by = to - tl;
+                tl = to;
+                limit = __builtin_bit_cast(uint16_t, (_Float16)ldexpf(1.0f, tl));
+                const float less = ldexpf(1.0f, -by);
+#pragma unroll
+                for (int s = 0; s < NC; s++) {
+                    A[s].m += (float)by;
+                    A[s].most += (float)by;
+                    A[s].l *= less;
+#pragma unroll
+                    for (int g = 0; g < NG; g++) A[s].o[g][0] *= less, A[s].o[g][1] *= less;
+                }
             }
         }
-        s = wave_sum(s) * p.scale;
-        const float n = fmaxf(m, s), a = m == n ? 1.0f : __builtin_amdgcn_exp2f((m - n) * 1.44269504f), e = __builtin_amdgcn_exp2f((s - n) * 1.44269504f);
-        m = n;
-        l = l * a + e;
-        for (int u = 0; u < 4; u++) o[u] = o[u] * a + e * v[u];
+#pragma unroll
+        for (int s = 0; s < NC; s++) {
+            Acc4<NG> &B = A[s];
+            float least = x[s][0], top = x[s][0];
+#pragma unroll
+            for (int i = 1; i < 8; i++) top = fmaxf(top, x[s][i]), least = fminf(least, x[s][i]);
+            if (__any(top == __builtin_inff() || least == -__builtin_inff())) {  // a key's scale is infinite: its score is NaN
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[s][i] = fmaf(x[s][i], 0.0f, x[s][i]);
+                top = x[s][0];
+#pragma unroll
+                for (int i = 1; i < 8; i++) top = fmaxf(top, x[s][i]);
+            }
+            if (!all) {
+                const int from = t + 4 * quarter, dh = rows[s].hi - from, dl = rows[s].lo - from, ds = p.sinks - from;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int e = 16 * (i >> 2) + (i & 3);
+                    x[s][i] = e <= dh && (e >= dl || e < ds) ? x[s][i] : -__builtin_inff();
+                }
+                top = x[s][0];
+#pragma unroll
+                for (int i = 1; i < 8; i++) top = fmaxf(top, x[s][i]);
+            }
+            top = row_max(top);
+            // The reference, as in softmax_step: raised to the largest score where that exceeds it by more than 2^8, lowered (by 2^64 in
+            // all at most) to a block whose largest weight is below 2^-14. Weights stand 2^7 above it, in units of the largest scale.
+            const float d = (top - B.f) * sc[s], lift = 7.0f - (float)tl;
+            const bool fall = d < -14.0f && top > -__builtin_inff() && !B.far && B.m > B.most - 64.0f;
+            if (__any(d > (B.far ? 0.0f : 8.0f) || fall)) {
+                const bool move = d > (B.far ? 0.0f : 8.0f) || fall;
+                float y = top * sc[s];
+                const float bottom = B.most - 64.0f + lift;
+                const bool cut = fall && y < bottom;
+                y = cut ? bottom : y;
+                const float from = cut ? bottom * __builtin_amdgcn_rcpf(sc[s]) : top;
+                const bool far = fabsf(y) > kFar;
+                const float r = (far ? y : ceilf(y)) - lift;
+                const float a = move ? exp2_hw(far && B.far ? (B.f - from) * sc[s] : B.m - r) : 1.0f;  // from -Inf: 0
+                B.l *= a;
+#pragma unroll
+                for (int g = 0; g < NG; g++) B.o[g][0] *= a, B.o[g][1] *= a;
+                B.m = move ? r : B.m;
+                B.f = move ? from : B.f;
+                B.far = move ? far : B.far;
+                B.most = fmaxf(B.most, B.m);
+            }
+            const float neg = B.far ? lift : B.m == -__builtin_inff() ? 0.0f : -B.m;
+            if (__any(B.far)) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[s][i] -= B.far ? B.f : 0.0f;
+            }
+            float l = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                x[s][i] = exp2_hw(fmaf(x[s][i], sc[s], neg));
+                l += x[s][i];
+            }
+            B.l += l;
+        }
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            const u32x4 y = open8(v[0].codes.v[g]), z = open8(v[1].codes.v[g]), a0 = {y.x, y.z, z.x, z.z}, a1 = {y.y, y.w, z.y, z.w};
+#pragma unroll
+            for (int s = 0; s < NC; s++) {
+                u32x4 hi, lo;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int h = i >> 1, j = 2 * (i & 1);
+                    const float e0 = x[s][4 * h + j], e1 = x[s][4 * h + j + 1], d0 = v[h].scale(g, j), d1 = v[h].scale(g, j + 1);
+                    hi[i] = __builtin_bit_cast(uint32_t, (h2){(_Float16)(e0 * d0), (_Float16)(e1 * d1)});
+                    // (hidden: the compiler would round the products anew for the second term, in another way)
+                    if (TWO) hi[i] = hide(hi[i]);
+                    const h2 f = __builtin_bit_cast(h2, (uint32_t)hi[i]);
+                    if (TWO) lo[i] = __builtin_bit_cast(uint32_t, (h2){(_Float16)fmaf(e0, d0, -(float)f[0]), (_Float16)fmaf(e1, d1, -(float)f[1])});
+                }
+                A[s].o[g][0] = mma16(a0, hi, A[s].o[g][0]);
+                A[s].o[g][1] = mma16(a1, hi, A[s].o[g][1]);
+                if (TWO) {
+                    A[s].o[g][0] = mma16(a0, lo, A[s].o[g][0]);
+                    A[s].o[g][1] = mma16(a1, lo, A[s].o[g][1]);
+                }
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++) load(v[h], p.v, next[h]);
     }
-    for (int u = 0; u < 4; u++)
-        if (lane + 64 * u < p.dim)
-            p.out[(int64_t)t * p.out_stride + head * p.dim + lane + 64 * u] = (uint16_t)f32_to_h16(pos >= 0 ? o[u] / l : 0.0f, p.io);
+    // the four waves' results, through LDS
+    float *mine = lds + w * (S::WAVE / 4);
+    float2 *ml = reinterpret_cast<float2 *>(lds + kWaves * (S::WAVE / 4));
+#pragma unroll
+    for (int s = 0; s < NC; s++) {
+        const float l = row_sum(A[s].l);
+        const int r = 16 * s + c;
+        if (r >= n) continue;
+#pragma unroll
+        for (int g = 0; g < NG; g++) {
+            const f4 a = A[s].o[g][0], b = A[s].o[g][1];
+            float *dst = mine + r * S::OSTRIDE + 32 * g + 8 * quarter;
+            *reinterpret_cast<float4 *>(dst) = make_float4(a[0], b[0], a[1], b[1]);
+            *reinterpret_cast<float4 *>(dst + 4) = make_float4(a[2], b[2], a[3], b[3]);
+        }
+        if (quarter == 0) ml[w * S::ROWS + r] = make_float2(A[s].m, l);
+    }
+    __syncthreads();
+    const bool direct = it.nsplit == 1;
+    for (int idx = tid; idx < n * (S::DIM / 4); idx += 64 * kWaves) {
+        const int r = idx / (S::DIM / 4), d = (idx - r * (S::DIM / 4)) * 4, row = r0 + r, tok = p.by_group(row);
+        Join j;
+        j.init();
+#pragma unroll
+        for (int u = 0; u < kWaves; u++) {
+            const float4 o = *reinterpret_cast<const float4 *>(lds + u * (S::WAVE / 4) + r * S::OSTRIDE + d);
+            j.add(ml[u * S::ROWS + r].x, ml[u * S::ROWS + r].y, o.x, o.y, o.z, o.w);
+        }
+        if (direct) {
+            put4<BF>(p, it.q0, row, it.head, d, j.o, j.l, keys - it.nq + tok >= 0);
+        } else {
+            float *dst = p.part + ((int64_t)it.slot * S::ROWS + r) * (S::DIM + 2);
+            agent_store(dst + d, j.o[0], j.o[1]);
+            agent_store(dst + d + 2, j.o[2], j.o[3]);
+            if (d == 0) agent_store(dst + S::DIM, j.m, j.l);
+        }
+    }
+    if (direct) return;
+    if (last_piece(p, it, reinterpret_cast<int *>(ml + kWaves * S::ROWS)))
+        join_tile<S::DIM, S::ROWS, BF, kWaves>(p, it, r0, n, lds, kWaves * S::WAVE);
+}
+
+template <int NG, int NC, bool BF> int launch_few(trhip_ctx *ctx, const AttnArgs &p, int64_t grid) {
+    const void *fn = reinterpret_cast<const void *>(attn4_few<NG, NC, BF>);
+    const int st = allow_dyn_lds(ctx, fn, Shape4<NG, NC>::BYTES, "kv4_attn");
+    if (st != TRHIP_OK) return st;
+    hipLaunchKernelGGL((attn4_few<NG, NC, BF>), dim3((unsigned)grid), dim3(64 * kWaves), (Shape4<NG, NC>::BYTES), ctx->stream, p);
+    return launch_check(ctx, "kv4_attn");
+}
+template <int NG> int launch_few(trhip_ctx *ctx, const AttnArgs &p, int sets, bool bf, int64_t grid) {
+    if (NG > kTwoSets || sets == 1) return bf ? launch_few<NG, 1, true>(ctx, p, grid) : launch_few<NG, 1, false>(ctx, p, grid);
+    else return bf ? launch_few<NG, NG <= kTwoSets ? 2 : 1, true>(ctx, p, grid) : launch_few<NG, NG <= kTwoSets ? 2 : 1, false>(ctx, p, grid);
+}
+int launch_few(trhip_ctx *ctx, const AttnArgs &p, int sets, bool bf, int64_t grid) {
+    switch (p.dim / 32) {
+    case 1: return launch_few<1>(ctx, p, sets, bf, grid);
+    case 2: return launch_few<2>(ctx, p, sets, bf, grid);
+    case 3: return launch_few<3>(ctx, p, sets, bf, grid);
+    case 4: return launch_few<4>(ctx, p, sets, bf, grid);
+    case 5: return launch_few<5>(ctx, p, sets, bf, grid);
+    case 6: return launch_few<6>(ctx, p, sets, bf, grid);
+    case 7: return launch_few<7>(ctx, p, sets, bf, grid);
+    default: return launch_few<8>(ctx, p, sets, bf, grid);
+    }
 }
 
 }  // namespace
 
 int launch_kv4_attn(trhip_ctx *ctx, const trhip_kv4 *kv, const AttnCall &c, int io) {
-    const Attn4Args p = {static_cast<const uint16_t *>(c.q), static_cast<uint16_t *>(c.out), static_cast<const uint8_t *>(kv->k),
-                         static_cast<const uint8_t *>(kv->v), c.q_stride, c.out_stride, c.max_pages, kv->pages, c.q_start, c.kv_len, c.table,
-                         (int)c.tokens, (int)c.nreq, c.heads, kv->heads, kv->dim, __builtin_ctz((unsigned)kv->page), (int)c.window, (int)c.sinks, io, c.scale};
-    hipLaunchKernelGGL(attn4_simple, dim3((unsigned)c.tokens, (unsigned)c.heads), dim3(64), 0, ctx->stream, p);
-    return launch_check(ctx, "kv4_attn");
+    AttnArgs p = {};
+    p.q = static_cast<const uint16_t *>(c.q);
+    p.out = static_cast<uint16_t *>(c.out);
+    p.q_stride = c.q_stride;
+    p.out_stride = c.out_stride;
+    p.k = static_cast<const uint8_t *>(kv->k);
+    p.v = static_cast<const uint8_t *>(kv->v);
+    p.head_bytes = kv->page * kv->dim / 16 * 9;
+    p.page_bytes = (int64_t)p.head_bytes * kv->heads;
+    p.npages = kv->pages;
+    p.page_log2 = __builtin_ctz((unsigned)kv->page);
+    p.table = c.table;
+    p.max_pages = c.max_pages;
+    p.q_start = c.q_start;
+    p.kv_len = c.kv_len;
+    p.nreq = (int)c.nreq;
+    p.tokens = (int)c.tokens;
+    p.heads = c.heads;
+    p.kv_heads = kv->heads;
+    p.group = c.heads / kv->heads;
+    p.dim = kv->dim;
+    p.window = (int)c.window;
+    p.sinks = (int)c.sinks;
+    p.scale = c.scale * 1.44269504088896341f;
+    p.by_group.of(p.group);
+    p.by_heads.of(p.kv_heads);
+    p.out_aligned = (reinterpret_cast<uintptr_t>(c.out) % 8 == 0) && c.out_stride % 4 == 0;
+    p.arrivals = ctx->arrivals;
+    const int cus = ctx->sm_count > 0 ? ctx->sm_count : 256;
+    const int64_t most_new = c.max_new < c.tokens ? c.max_new : c.tokens;
+    p.target = cus * 2;
+    p.row_lo = 0;
+    p.row_hi = kAnyRows;
+    const int sets = most_new * p.group <= 16 || kv->dim > 32 * kTwoSets ? 1 : 2, rows = 16 * sets;
+    const int64_t grid = plan_items(p, c, rows, kBlock, kLeast);
+    if (grid >= ((int64_t)1 << 31)) return fail(ctx, TRHIP_ERR_INVALID, "kv4_attn: too many rows");
+    int st = TRHIP_OK;
+    float *ws = static_cast<float *>(workspace(ctx, (size_t)p.part_slots * rows * (kv->dim + 2) * sizeof(float), &st));
+    if (!ws) return st;
+    p.part = ws;
+    return launch_few(ctx, p, sets, io == TRHIP_BF16, grid);
 }
 
 }  // namespace trhip

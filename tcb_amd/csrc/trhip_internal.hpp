@@ -497,6 +497,7 @@ struct AttnCall {
     const int *prefix_table;  // prefix_len 0: none
     int64_t prefix_len, window, sinks;
     float scale;
+    bool long_only = false;  // only the requests of more than kTokMost rows (the hint must not rule them out)
 };
 int launch_attn(trhip_ctx *ctx, const trhip_kv *kv, const AttnCall &c);
 // Rotary positions (rope.hip), the 4-bit cache (kv4.hip), attention over it (attn4.hip; io: type of q and out), sampling

@@ -46,3 +46,20 @@ def pack(codes, d, value):
             at = 8 * dim + 2 * (((r // 4) * blocks + b) * 4 + r % 4)
             plane[..., at:at + 2] = np.ascontiguousarray(d[:, :, r::16, b].astype(np.float16)).view(np.uint8).reshape(pages, heads, page // 16, 2)
     return plane
+
+
+HALF = {"bf16": 2.0 ** -8, "f16": 2.0 ** -11}  # half a step, relative
+
+
+def bound(dtype, dim, n, long, out, spread, reach, largest):
+    """How far an fp32 computation over the cache's values may be from the float64 one (out, spread and reach as in paged_ref.attend;
+    largest: the largest value there is). The output's rounding (half a step); the weights' rounding: to the output's type in a long request that sees
+    many keys, else to f16 (half a step of it is 2^-11) for bf16 and to two f16 terms (2^-21) for f16; fp32 sums of dim products in each
+    score (dim 2^-24 of their absolute sum, entering numerator and denominator through e) and of n weights (n 2^-24), 2^-20 for exp2
+    and the divide. Small weights: a weight times its value's scale stands in f16 numbers of 2^-24 at least, the row's largest weight being 2^6 at
+    least above the largest scale's next power of two, so it is off by up to 2^-25 of 2^6 / 2, times codes of up to 8: 2^-30 of the largest
+    value a key, 2^-25 of a weight in a long request. (fp32 exponentials end at 2^-126, far below.)"""
+    half = HALF[dtype]
+    weights = (half if long else 2.0 ** -11 if dtype == "bf16" else 2.0 ** -21) + 2 * dim * 2.0 ** -24 * reach + 2 * n * 2.0 ** -24 + 2.0 ** -20
+    floor = n * 2.0 ** -30 * largest + (n * 2.0 ** -25 * spread if long and dtype == "f16" else 0.0)
+    return half * np.abs(out) + (1 + half) * (weights * spread + floor) + (2.0 ** -25 if dtype == "f16" else 1e-38)

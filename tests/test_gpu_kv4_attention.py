@@ -85,11 +85,8 @@ class Batch:
             kk, vv = (R.rows_of(c, self.table[i], m, self.page) for c in (k, v))
             o, spread, reach = R.attend(q, kk, vv, m - n, scale, window, sinks)
             outs.append(o)
-            # A weight times its value's scale goes through the matrix units as f16 numbers of 2^-24 at least, the row's largest weight being
-            # 2^6 at least above the largest scale's next power of two: so the smallest ones are off by up to 2^-25 of 2^6 / 2, times codes
-            # of up to 8, 2^-30 of the largest value a key. (fp32 exponentials end at 2^-126, far below.)
-            floor = m * 2.0 ** -30 * np.abs(np.nan_to_num(vv)).max(initial=0.0)
-            tols.append(R.bound(self.dtype, self.dim, m, o, spread, reach) + floor)
+            largest = np.abs(np.nan_to_num(vv)).max(initial=0.0)
+            tols.append(K4.bound(self.dtype, self.dim, m, n * (self.heads // self.kv_heads) > 96, o, spread, reach, largest))
         return np.concatenate(outs), np.concatenate(tols)
 
     def check(self, tb, window=0, sinks=0, scale=None, **how):
