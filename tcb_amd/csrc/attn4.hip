@@ -13,6 +13,7 @@
 //   O^T += V^T P^T: the value's scale goes to the weight, w = p s (there is one product a block of 32 elements).
 // The weights p s stand in f16, in one term for bf16 results (their rounding of 2^-12 is a sixteenth of the result's) and in two
 // for f16 ones. So that they neither overflow nor vanish, the softmax's reference includes the largest scale the wave has met.
+#include "attn4_image.hpp"
 #include "attn_plan.hpp"
 #include "kv4.hpp"
 
@@ -25,6 +26,7 @@ typedef uint32_t u32x3 __attribute__((ext_vector_type(3)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 
 constexpr int kTwoSets = 4;  // blocks of elements up to which a workgroup's registers hold two sets of rows
+constexpr int64_t kMostImage = (int64_t)2 << 30;  // bytes of a plane of opened keys at most: a hundredth of the memory
 constexpr int kWaves = 4, kBlock = 32, kLeast = 8, kOver = 6;
 
 template <int NG, int NC> struct Shape4 {
@@ -467,10 +469,33 @@ int launch_kv4_attn(trhip_ctx *ctx, const trhip_kv4 *kv, const AttnCall &c, int 
     p.arrivals = ctx->arrivals;
     const int cus = ctx->sm_count > 0 ? ctx->sm_count : 256;
     const int64_t most_new = c.max_new < c.tokens ? c.max_new : c.tokens;
+    // Requests of more than kTokMost rows: their keys go to the workspace in 16 bits and the 16-bit cache's kernel of many rows takes
+    // them, where the workspace may hold the longest ones that the sizes allow. Which there are is known only from the hint.
+    const int64_t most_long = c.tokens * p.group / (kTokMost + 1), longs = most_long < c.nreq ? most_long : c.nreq;
+    const double image_bytes = (double)longs * (double)c.max_pages * (double)p.page_bytes * (32.0 / 9.0);
+    const bool image = most_new * p.group > kTokMost && longs > 0 && longs < 65536 && c.max_pages > 0 && image_bytes <= (double)kMostImage &&
+                       (double)c.nreq * (double)c.max_pages <= (double)(kMostImage / 4);
+    if (image) {
+        const int64_t plane = (longs * c.max_pages * (p.page_bytes / 9 * 32) + 255) & ~(int64_t)255, tables = c.nreq * c.max_pages * 4;
+        int st = TRHIP_OK;
+        uint8_t *room = static_cast<uint8_t *>(workspace2(ctx, (size_t)(2 * plane + tables), &st));
+        if (!room) return st;
+        const Image4 im = {p.k, p.v, reinterpret_cast<uint16_t *>(room), reinterpret_cast<uint16_t *>(room + plane), reinterpret_cast<int *>(room + 2 * plane),
+                           p.q_start, p.kv_len, p.table, p.max_pages, p.npages, p.nreq, p.tokens, p.group, p.kv_heads, p.dim, p.page_log2, kTokMost,
+                           p.window, p.sinks, io == TRHIP_BF16};
+        st = launch_attn4_image(ctx, im, (int)longs);
+        if (st != TRHIP_OK) return st;
+        const trhip_kv open = {io, kv->page, kv->heads, kv->dim, longs * c.max_pages, room, room + plane};
+        AttnCall lc = c;
+        lc.table = im.out_table;
+        lc.long_only = true;
+        st = launch_attn(ctx, &open, lc);
+        if (st != TRHIP_OK) return st;
+    }
     p.target = cus * 2;
     p.row_lo = 0;
-    p.row_hi = kAnyRows;
-    const int sets = most_new * p.group <= 16 || kv->dim > 32 * kTwoSets ? 1 : 2, rows = 16 * sets;
+    p.row_hi = image ? kTokMost : kAnyRows;
+    const int sets = (p.row_hi != kAnyRows || most_new * p.group > 16) && kv->dim <= 32 * kTwoSets ? 2 : 1, rows = 16 * sets;
     const int64_t grid = plan_items(p, c, rows, kBlock, kLeast);
     if (grid >= ((int64_t)1 << 31)) return fail(ctx, TRHIP_ERR_INVALID, "kv4_attn: too many rows");
     int st = TRHIP_OK;

@@ -179,16 +179,13 @@ def test_tokens_that_see_nothing(backend):
 
 def test_rows_outside_every_request(backend):
     """Rows before, behind and between the requests stay as they are."""
-    b = Batch("bf16", 4, 1, 64, 16, [2, 3, 2], [20, 30, 7])
-    want, tol = b.want()
     for n in (1, 200):
         c = Batch("bf16", 4, 1, 64, 16, [2, n, 2], [20, n + 30, 7])
-        full = c.run(backend)
-        c.new, c.kv, c.tokens = c.new, c.kv, c.tokens
+        want, tol = c.want()
         c.table, c.kv = c.table[[0, 2]], [c.kv[0], c.kv[2]]
         c.start = np.array([0, 2, 2 + n + 2], np.int32)  # the second request takes the tokens in between as its own first ones
-        got = c.run(backend)
-        assert np.array_equal(got[:2], full[:2]) and np.array_equal(got[-2:], full[-2:])
+        off = np.abs(c.run(backend) - want) - tol  # (its last two tokens see what they saw, by another kernel where there are many)
+        assert off[:2].max() <= 0 and off[-2:].max() <= 0
         c.table, c.kv, c.start = c.table[:1], c.kv[:1], np.array([0, 2], np.int32)
         assert (c.run(backend)[2:] == 7).all()
 
