@@ -1,22 +1,41 @@
 // sample.hip -- the next token of each row of logits: temperature, top-k, top-p and min-p, from a given random number.
+//
+// One launch that reads every logit once. A row is cut into stripes of 256 entries, dealt in turn to the waves of its workgroups,
+// which hold them in registers. A workgroup leaves, as the row's settings need it,
+//   the weight of each of its stripes, relative to its own largest logit (rows without a filter, and the sum that top_p is a part of),
+//   its largest entries, by a threshold that at least as many of its threads' maxima reach (rows with a filter).
+// The row's last workgroup finishes it: without a filter it finds the stripe in which the random number falls, and there the entry;
+// with one it sorts the entries that the workgroups left (some hundreds), cuts the run that is kept, and walks it by index. The
+// workgroups' shares are what a row whose large entries lie anywhere needs with room to spare; whether they are complete is checked, and a row
+// where they are not (a flat one, of which thousands are kept, or one whose largest entries lie in few stripes) goes on to whole(),
+// which reads the row again several times.
+//
+// Weights and their sums are in 64 bits, since one border among a hundred thousand has to be met: e^x by a table of 64 powers and a
+// polynomial of degree 5, ten operations.
 #include "trhip_internal.hpp"
 
 namespace trhip {
 namespace {
 
+constexpr int kThreads = 512, kWaves = kThreads / 64, kStripe = 256, kMost = 1024;  // kMost: entries that are sorted at most
+constexpr int kBins = 2048;
+
 struct SampleArgs {
     const void *logits;
     int io;
     int64_t stride;
-    int vocab;
+    int vocab, stripes, groups, room;  // room: entries that a workgroup may leave
+    int wide;                          // four entries at a time
     const float *temperature;
     const int *top_k;
     const float *top_p, *min_p, *u;
     int *token;
     float *logprob;
+    double *mass;           // [row][stripe]
+    unsigned long long *list;  // [row][workgroup][room]: key, ~index
+    uint32_t *left;         // [row][workgroup][4]: largest key, threshold (0: all entries left), entries left, unused
+    uint32_t *arrivals;     // [row]
 };
-
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
 
 // A logit as an unsigned number in the same order; NaN and -Inf are 0.
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -29,187 +48,549 @@ __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k &
 
 struct Row {
     const void *x;
-    int io, vocab;
+    int io, vocab, wide;
     __device__ __forceinline__ uint32_t key(int i) const {
         return key_of(io == TRHIP_F32 ? static_cast<const float *>(x)[i] : h16_to_f32(static_cast<const uint16_t *>(x)[i], io));
     }
+    // entries i .. i + 3 (i a multiple of 4); 0 past the last
+    __device__ __forceinline__ void keys4(int i, uint32_t (&k)[4]) const {
+        if (wide && i + 4 <= vocab) {
+            float f[4];
+            if (io == TRHIP_F32) {
+                *reinterpret_cast<float4 *>(f) = *reinterpret_cast<const float4 *>(static_cast<const float *>(x) + i);
+            } else {
+                const uint2 y = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(x) + i);
+                f[0] = h16_to_f32(y.x & 0xFFFFu, io), f[1] = h16_to_f32(y.x >> 16, io);
+                f[2] = h16_to_f32(y.y & 0xFFFFu, io), f[3] = h16_to_f32(y.y >> 16, io);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++) k[u] = key_of(f[u]);
+        } else {
+#pragma unroll
+            for (int u = 0; u < 4; u++) k[u] = i + u < vocab ? key(i + u) : 0;
+        }
+    }
 };
+
+// e^((l - max) / T) of a key. e^t = 2^(n / 64) e^r, n = rint(64 t / ln 2), |r| <= ln 2 / 128: what r^6 / 720 leaves out is 2^-54.
 struct Weight {
     uint32_t top;
     double max, inv;
+    const double *table;  // 2^(j / 64)
     __device__ __forceinline__ double operator()(uint32_t k) const {
-        return k == top ? 1.0 : k == 0 ? 0.0 : exp(((double)of_key(k) - max) * inv);
+        const double t = ((double)of_key(k) - max) * inv;
+        if (k == top) return 1.0;
+        if (k == 0) return 0.0;
+        if (!(t > -700.0)) return exp(t);
+        const double n = rint(t * 92.33248261689366);
+        const double r = fma(-n, 3.623510646634843e-19, fma(-n, 0.010830424696249145, t));  // (ln 2 / 64 in two parts)
+        double y = fma(r, 8.3333333333333332e-3, 4.1666666666666664e-2);
+        y = fma(r, y, 1.6666666666666666e-1);
+        y = fma(r, y, 0.5);
+        y = fma(r, y, 1.0);
+        const int i = (int)n;
+        const double p = table[i & 63];
+        const double s = fma(p, r * y, p);
+        return __longlong_as_double(__double_as_longlong(s) + ((long long)(i >> 6) << 52));
     }
 };
 
-template <class T> __device__ T sum_all(T v, T *lds) {
-    const int tid = threadIdx.x;
-    lds[tid] = v;
-    __syncthreads();
-    for (int o = kThreads / 2; o; o >>= 1) {
-        if (tid < o) lds[tid] += lds[tid + o];
-        __syncthreads();
-    }
-    v = lds[0];
-    __syncthreads();
-    return v;
+struct Setting {
+    float t, tp, low;
+    int k;  // 0: all
+    bool greedy;
+    double u;
+};
+__device__ __forceinline__ Setting setting_of(const SampleArgs &p, int r) {
+    Setting s;
+    s.t = p.temperature ? p.temperature[r] : 1.0f;
+    s.greedy = !(s.t > 0.0f);
+    s.k = s.greedy ? 1 : p.top_k ? p.top_k[r] : 0;
+    if (s.k < 0 || s.k >= p.vocab) s.k = 0;
+    if (s.greedy) s.k = 1;
+    s.tp = s.greedy ? 1.0f : p.top_p ? p.top_p[r] : 1.0f;
+    if (!(s.tp < 1.0f)) s.tp = 1.0f;
+    s.low = s.greedy || !p.min_p ? 0.0f : p.min_p[r];
+    if (!(s.low > 0.0f)) s.low = 0.0f;
+    if (s.low > 1.0f) s.low = 1.0f;
+    const float u = p.u[r];
+    s.u = u >= 0.0f ? (double)u : 0.0;
+    return s;
 }
-template <class T> __device__ T before_me(T v, T *lds, T &total) {  // sum over the threads before this one
-    const int tid = threadIdx.x;
-    lds[tid] = v;
-    __syncthreads();
-    for (int o = 1; o < kThreads; o <<= 1) {
-        const T y = tid >= o ? lds[tid - o] : T(0);
-        __syncthreads();
-        lds[tid] += y;
-        __syncthreads();
-    }
-    total = lds[kThreads - 1];
-    v = tid ? lds[tid - 1] : T(0);
-    __syncthreads();
-    return v;
+// How many entries of the whole row its workgroups should cover, and a workgroup's share of them: the mean, four standard deviations of
+// entries that lie anywhere, and six.
+constexpr int kCover = 256;
+__device__ __forceinline__ int share_of(int n, int groups) {
+    const float m = (float)n * __builtin_amdgcn_rcpf((float)groups);
+    const int s = (int)(m + 4.0f * __builtin_amdgcn_sqrtf(m) + 6.0f);
+    return s < n ? s : n;
 }
 
-// A workgroup a row. What is kept is a run of the descending order: its last key, and how many entries of that key, by index.
-__global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
-    __shared__ double s_d[kThreads];
-    __shared__ uint32_t s_u[kThreads];
-    __shared__ uint32_t s_count[256];
-    __shared__ unsigned long long s_mass[256];
-    __shared__ uint32_t s_pick[3];
-    __shared__ unsigned long long s_above;
-    const int tid = threadIdx.x, r = blockIdx.x;
-    const Row x = {static_cast<const char *>(p.logits) + r * p.stride * (p.io == TRHIP_F32 ? 4 : 2), p.io, p.vocab};
-    uint32_t top = 0;
-    for (int i = tid; i < p.vocab; i += kThreads) {
-        const uint32_t k = x.key(i);
-        top = k > top ? k : top;
+struct Lds {
+    double table[64];
+    double sum[kThreads];
+    unsigned long long sorted[kMost];
+    double weight[kMost];
+    unsigned long long bins[kBins];
+    uint32_t u[kThreads];
+    uint32_t small[16];
+    double wave[kWaves];
+};
+
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+        const uint32_t w = __shfl_xor(v, o);
+        v = v > w ? v : w;
     }
-    s_u[tid] = top;
+    return v;
+}
+// Over the workgroup; every thread gets the result. (A barrier before the first use of s.u / s.wave is the caller's.)
+__device__ uint32_t all_max(uint32_t v, Lds &s) {
+    v = wave_max(v);
     __syncthreads();
-    for (int o = kThreads / 2; o; o >>= 1) {
-        if (tid < o) s_u[tid] = s_u[tid] > s_u[tid + o] ? s_u[tid] : s_u[tid + o];
+    if ((threadIdx.x & 63) == 0) s.u[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = s.u[0];
+    for (int w = 1; w < kWaves; w++) v = v > s.u[w] ? v : s.u[w];
+    return v;
+}
+__device__ double all_sum(double v, Lds &s) {
+    v = wave_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s.wave[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = s.wave[0];
+    for (int w = 1; w < kWaves; w++) v += s.wave[w];
+    return v;
+}
+// Sum over the threads before this one, and over all.
+template <class T> __device__ T before_me(T v, T *lds, T &total) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    T x = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const T y = __shfl_up(x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 63) lds[w] = x;
+    __syncthreads();
+    T base = T(0);
+    total = T(0);
+    for (int i = 0; i < kWaves; i++) {
+        if (i == w) base = total;
+        total += lds[i];
+    }
+    const T up = __shfl_up(x, 1);
+    return base + (lane ? up : T(0));
+}
+
+// Sorts s.sorted[0 .. n2), n2 a power of two, n2 <= kMost: largest first, or smallest.
+__device__ void sort(Lds &s, int n2, bool falling) {
+    for (int k = 2; k <= n2; k <<= 1)
+        for (int j = k >> 1; j; j >>= 1) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < n2 / 2; i += kThreads) {
+                const int a = 2 * i - (i & (j - 1)), b = a + j;
+                const unsigned long long x = s.sorted[a], y = s.sorted[b];
+                const bool down = ((a & k) == 0) == falling;
+                if (down ? x < y : x > y) s.sorted[a] = y, s.sorted[b] = x;
+            }
+        }
+    __syncthreads();
+}
+
+__device__ __forceinline__ void result(const SampleArgs &p, int r, int token, double w, double total) {
+    p.token[r] = token;
+    if (p.logprob) p.logprob[r] = (float)log(w / total);
+}
+
+// A row that is kept from `cut` up (of its key the first `ties` by index; weights of at least low): the entry in which u falls.
+__device__ void pick(const SampleArgs &p, int r, const Row &x, const Weight &w, uint32_t cut, uint32_t ties, double low, double u, Lds &s) {
+    const int tid = threadIdx.x;
+    // a thread's share: whole fours, in a row
+    const int each = ((p.vocab + kThreads - 1) / kThreads + 3) & ~3, i0 = tid * each < p.vocab ? tid * each : p.vocab, i1 = i0 + each < p.vocab ? i0 + each : p.vocab;
+    uint32_t eq = 0, total_eq, eq0 = 0;
+    if (ties != 0xFFFFFFFFu) {
+        for (int i = i0; i < i1; i += 4) {
+            uint32_t k[4];
+            x.keys4(i, k);
+            for (int v = 0; v < 4; v++) eq += k[v] == cut;
+        }
+        eq0 = before_me(eq, s.u, total_eq);
+    }
+    auto walk = [&](auto use) {
+        uint32_t n = eq0;
+        for (int i = i0; i < i1; i += 4) {
+            uint32_t k[4];
+            x.keys4(i, k);
+            for (int v = 0; v < 4; v++) {
+                const bool keep = k[v] != 0 && (k[v] > cut || (k[v] == cut && n < ties));
+                n += k[v] == cut;
+                if (!keep) continue;
+                const double y = w(k[v]);
+                if (y >= low) use(i + v, y);
+            }
+        }
+    };
+    double sum = 0, total;
+    walk([&](int, double y) { sum += y; });
+    const double start = before_me(sum, s.wave, total), goal = u * total;
+    __syncthreads();
+    if (tid == 0) s.small[0] = 0x7FFFFFFF, s.small[1] = 0;
+    __syncthreads();
+    uint32_t found = 0x7FFFFFFF, last = 0;
+    double run = start;
+    if (sum > 0)
+        walk([&](int i, double y) {
+            run += y;
+            if (y > 0) last = (uint32_t)i;
+            if (run > goal && found == 0x7FFFFFFF) found = (uint32_t)i;
+        });
+    if (found != 0x7FFFFFFF) atomicMin(&s.small[0], found);
+    if (last) atomicMax(&s.small[1], last);
+    __syncthreads();
+    if (tid == 0) {
+        const int token = (int)(s.small[0] != 0x7FFFFFFF ? s.small[0] : s.small[1]);
+        result(p, r, token, w(x.key(token)), total);
+    }
+}
+
+// A row by itself: the cut by top-k, then by top-p, each by counting (or weighing) entries in bins of the key, eight bits at a time
+// from the top.
+__device__ __noinline__ void whole(const SampleArgs &p, int r, const Row &x, const Weight &w, const Setting &st, Lds &s) {
+    const int tid = threadIdx.x;
+    uint32_t cut = 1, ties = 0xFFFFFFFFu;  // kept: keys above cut, and the first `ties` of cut
+    int bits = 62;
+    while ((p.vocab - 1) >> (62 - bits)) bits--;
+    const double unit = __longlong_as_double((long long)(1023 + bits) << 52);
+    const int fours = (p.vocab + 3) / 4;
+    auto each = [&](auto use) {
+        for (int i = tid; i < fours; i += kThreads) {
+            uint32_t k[4];
+            x.keys4(4 * i, k);
+            for (int v = 0; v < 4; v++) use(k[v]);
+        }
+    };
+    for (int phase = 0; phase < 2; phase++) {
+        double goal;  // entries, or weight, to reach
+        if (phase == 0) {
+            if (st.k == 0) continue;
+            goal = st.k;
+        } else {
+            if (!(st.tp < 1.0f)) continue;
+            double sum = 0;
+            each([&](uint32_t k) {
+                if (k > cut || (k == cut && ties == 0xFFFFFFFFu)) sum += w(k);
+            });
+            sum = all_sum(sum, s);
+            if (ties != 0xFFFFFFFFu) sum += (double)ties * w(cut);
+            goal = (double)st.tp * sum * unit;
+        }
+        uint32_t prefix = 0, mask = 0;
+        unsigned long long above = 0;
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            __syncthreads();
+            if (tid < 256) s.bins[tid] = 0;
+            __syncthreads();
+            each([&](uint32_t k) {
+                if ((k & mask) != prefix || k < cut) return;
+                if (phase == 0) atomicAdd(&s.bins[k >> shift & 255], 1ull);
+                else if (k > cut || ties == 0xFFFFFFFFu) atomicAdd(&s.bins[k >> shift & 255], (unsigned long long)rint(w(k) * unit));
+            });
+            __syncthreads();
+            if (tid == 0) {
+                if (phase == 1 && ties != 0xFFFFFFFFu && (cut & mask) == prefix) s.bins[cut >> shift & 255] += (unsigned long long)(rint(w(cut) * unit) * ties);
+                unsigned long long run = above;
+                int at = -1;
+                for (int b = 255; b >= 0; b--) {
+                    const unsigned long long n = s.bins[b];
+                    if (n == 0) continue;
+                    at = b;
+                    above = run;
+                    run += n;
+                    if ((double)run >= goal) break;
+                }
+                s.small[0] = at < 0 ? 0 : at;
+                s.bins[256] = above;
+            }
+            __syncthreads();
+            above = s.bins[256];
+            prefix |= s.small[0] << shift;
+            mask |= 255u << shift;
+        }
+        // of key `prefix` as many as it takes
+        if (phase == 0) {
+            ties = (uint32_t)(st.k - (int)above);
+        } else {
+            double n = ceil((goal - (double)above) / rint(w(prefix) * unit));
+            n = n < 1 ? 1 : n;
+            const uint32_t most = prefix == cut ? ties : 0xFFFFFFFFu;
+            ties = n < (double)most ? (uint32_t)n : most;
+        }
+        cut = prefix;
         __syncthreads();
     }
-    top = s_u[0];
+    pick(p, r, x, w, cut, ties, (double)st.low, st.u, s);
+}
+
+__device__ __forceinline__ uint32_t agent_get(const uint32_t *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ unsigned long long agent_get(const unsigned long long *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ double agent_get(const double *p) {
+    return __longlong_as_double((long long)agent_get(reinterpret_cast<const unsigned long long *>(p)));
+}
+template <class T> __device__ __forceinline__ void agent_put(T *p, T v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+template <int J> __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
+    __shared__ Lds s;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, r = blockIdx.y, g = blockIdx.x;
+    const Row x = {static_cast<const char *>(p.logits) + r * p.stride * (p.io == TRHIP_F32 ? 4 : 2), p.io, p.vocab, p.wide};
+    const Setting st = setting_of(p, r);
+    const bool filtered = st.k > 0 || st.tp < 1.0f || st.low > 0.0f, weigh = !filtered || (st.k == 0 && st.tp < 1.0f);
+    uint32_t key[J][4], top = 0;
+    auto stripe = [&](int j) { return g + p.groups * (w + kWaves * j); };
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+        if (stripe(j) < p.stripes) x.keys4(stripe(j) * kStripe + 4 * lane, key[j]);
+        else key[j][0] = key[j][1] = key[j][2] = key[j][3] = 0;
+    }
+    if (tid < 64) s.table[tid] = exp2((double)tid / 64.0);
+#pragma unroll
+    for (int j = 0; j < J; j++)
+#pragma unroll
+        for (int v = 0; v < 4; v++) top = top > key[j][v] ? top : key[j][v];
+    s.u[tid] = top;
+    if (tid == 0) s.small[0] = 0;
     __syncthreads();
-    if (top == 0) {
+    uint32_t mine[kWaves];  // every wave has all threads' maxima
+    top = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; i++) {
+        mine[i] = s.u[64 * i + lane];
+        top = top > mine[i] ? top : mine[i];
+    }
+    top = wave_max(top);
+    if (weigh && top != 0) {
+        const Weight wt = {top, (double)of_key(top), st.greedy ? 1.0 : 1.0 / (double)st.t, s.table};
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            if (stripe(j) >= p.stripes) break;
+            const double sum = wave_sum((wt(key[j][0]) + wt(key[j][1])) + (wt(key[j][2]) + wt(key[j][3])));
+            if (lane == 0) agent_put(p.mass + (int64_t)r * p.stripes + stripe(j), sum);
+        }
+    }
+    uint32_t bound = 0, left = 0;
+    if (filtered && top != 0) {
+        const int cover = st.k > 0 ? st.k : kCover;
+        const int share = share_of(cover, p.groups);
+        const bool many = share * 11 / 10 * p.groups > kMost || share * 5 / 4 + 8 > p.room;  // (too many to sort)
+        if (many) {
+            left = 0xFFFFFFFFu;
+        } else {
+            // a threshold that `share` to share * 9 / 8 threads' maxima reach: halving between the smallest and the largest
+            uint32_t lo = 0, hi = top;  // count(>= lo) >= share (or lo is 0)
+            bound = 0;
+            for (int step = 0; step < 32 && lo < hi; step++) {
+                const uint32_t mid = step == 0 ? top : lo + (hi - lo + 1) / 2;
+                int n = 0;
+#pragma unroll
+                for (int i = 0; i < kWaves; i++) n += __popcll(__ballot(mine[i] >= mid));
+                if (n >= share) {
+                    lo = mid;
+                    if (n <= share + share / 8) break;
+                } else {
+                    hi = mid - 1;
+                }
+            }
+            bound = lo;
+            unsigned long long *to = p.list + ((int64_t)r * p.groups + g) * p.room;
+#pragma unroll
+            for (int j = 0; j < J; j++)
+#pragma unroll
+                for (int v = 0; v < 4; v++) {
+                    const bool is = key[j][v] != 0 && key[j][v] >= bound;
+                    const uint64_t m = __ballot(is);
+                    if (m == 0) continue;
+                    uint32_t at = 0;
+                    if (lane == 0) at = atomicAdd(&s.small[0], (uint32_t)__popcll(m));
+                    at = __builtin_amdgcn_readfirstlane(at) + __popcll(m & (((uint64_t)1 << lane) - 1));
+                    if (is && at < (uint32_t)p.room)
+                        agent_put(to + at, ((unsigned long long)key[j][v] << 32) | (uint32_t)~(stripe(j) * kStripe + 4 * lane + v));
+                }
+            __syncthreads();
+            left = s.small[0];
+        }
+    }
+    if (tid == 0) {
+        uint32_t *mine_left = p.left + ((int64_t)r * p.groups + g) * 4;
+        agent_put(mine_left, top);
+        agent_put(mine_left + 1, bound);
+        agent_put(mine_left + 2, left);
+    }
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0);  // this thread's stores have completed
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __syncthreads();
+    if (tid == 0) {
+        const bool last = __hip_atomic_fetch_add(&p.arrivals[r], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)p.groups - 1;
+        if (last) agent_put(&p.arrivals[r], 0u);
+        s.small[1] = last;
+    }
+    __syncthreads();
+    if (!s.small[1]) return;
+
+    // ---- the row's last workgroup ----
+    const uint32_t *lefts = p.left + (int64_t)r * p.groups * 4;
+    uint32_t row_top = 0, complete = 0, total_left = 0;
+    for (int i = tid; i < p.groups; i += kThreads) {
+        const uint32_t a = agent_get(lefts + 4 * i), b = agent_get(lefts + 4 * i + 1), n = agent_get(lefts + 4 * i + 2);
+        row_top = row_top > a ? row_top : a;
+        complete = complete > b ? complete : b;  // every entry from here up has been left by its workgroup
+        total_left = n > (uint32_t)p.room || total_left > kMost ? 0x7FFFFFFFu : total_left + n;
+    }
+    row_top = all_max(row_top, s);
+    if (row_top == 0) {
         if (tid == 0) {
             p.token[r] = -1;
             if (p.logprob) p.logprob[r] = __builtin_nanf("");
         }
         return;
     }
-    const float t = p.temperature ? p.temperature[r] : 1.0f, tp = p.top_p ? p.top_p[r] : 1.0f, mp = p.min_p ? p.min_p[r] : 0.0f;
-    const float u0 = p.u[r], u = u0 >= 0.0f ? u0 : 0.0f;
-    const bool greedy = !(t > 0.0f);
-    const int tk = greedy ? 1 : p.top_k ? p.top_k[r] : 0;
-    const Weight w = {top, (double)of_key(top), greedy ? 1.0 : 1.0 / (double)t};
-    uint32_t cut = 1, ties = 0xFFFFFFFFu;  // kept: keys above cut, and the first `ties` of cut
-    int bits = 62;
-    while ((p.vocab - 1) >> (62 - bits)) bits--;
-    const double unit = ldexp(1.0, bits);
-    for (int phase = 0; phase < 2; phase++) {
-        double goal;  // entries, or weight, to reach
-        if (phase == 0) {
-            if (tk <= 0 || tk >= p.vocab) continue;
-            goal = tk;
-        } else {
-            if (!(tp < 1.0f) || greedy) continue;
-            double sum = 0;
-            for (int i = tid; i < p.vocab; i += kThreads) {
-                const uint32_t k = x.key(i);
-                if (k > cut || (k == cut && ties == 0xFFFFFFFFu)) sum += w(k);
+    const Weight wt = {row_top, (double)of_key(row_top), st.greedy ? 1.0 : 1.0 / (double)st.t, s.table};
+    // the stripes' weights, relative to the row's largest logit: a thread's share of the stripes in a row
+    double total = 0, before = 0;
+    const int each = (p.stripes + kThreads - 1) / kThreads, s0 = tid * each < p.stripes ? tid * each : p.stripes, s1 = s0 + each < p.stripes ? s0 + each : p.stripes;
+    auto stripe_mass = [&](int i) {
+        const uint32_t a = agent_get(lefts + 4 * (i % p.groups));
+        return a == 0 ? 0.0 : agent_get(p.mass + (int64_t)r * p.stripes + i) * wt(a);
+    };
+    if (weigh) {
+        double sum = 0;
+        for (int i = s0; i < s1; i++) sum += stripe_mass(i);
+        before = before_me(sum, s.wave, total);
+    }
+    if (!filtered) {
+        const double goal = st.u * total;
+        __syncthreads();
+        if (tid == 0) s.small[2] = 0x7FFFFFFF, s.small[3] = 0;
+        __syncthreads();
+        double run = before;
+        for (int i = s0; i < s1; i++) {
+            const double y = stripe_mass(i);
+            if (y > 0) atomicMax(&s.small[3], (uint32_t)i);
+            if (run + y > goal && y > 0) {
+                atomicMin(&s.small[2], (uint32_t)i);
+                break;
             }
-            sum = sum_all(sum, s_d);
-            if (ties != 0xFFFFFFFFu) sum += (double)ties * w(cut);
-            goal = (double)tp * sum * unit;
+            run += y;
         }
-        uint32_t prefix = 0, mask = 0;
-        unsigned long long above = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) s_count[tid] = 0, s_mass[tid] = 0;
-            __syncthreads();
-            for (int i = tid; i < p.vocab; i += kThreads) {
-                const uint32_t k = x.key(i);
-                if ((k & mask) != prefix || k < cut) continue;
-                const uint32_t b = k >> shift & 255;
-                if (phase == 0) atomicAdd(&s_count[b], 1u);
-                else if (k > cut || ties == 0xFFFFFFFFu) atomicAdd(&s_mass[b], (unsigned long long)rint(w(k) * unit));
-            }
-            __syncthreads();
-            if (tid == 0) {
-                if (phase == 1 && ties != 0xFFFFFFFFu && (cut & mask) == prefix) s_mass[cut >> shift & 255] += (unsigned long long)(rint(w(cut) * unit) * ties);
-                unsigned long long run = above;
-                int b = 255, pick = -1;
-                unsigned long long pick_above = above;
-                for (; b >= 0; b--) {
-                    const unsigned long long n = phase == 0 ? s_count[b] : s_mass[b];
-                    const bool some = phase == 0 ? n > 0 : n > 0;
-                    if (some) pick = b, pick_above = run;
-                    run += n;
-                    if (some && (double)run >= goal) break;
-                }
-                s_pick[0] = pick < 0 ? 0 : pick;
-                s_above = pick_above;
-            }
-            __syncthreads();
-            above = s_above;
-            prefix |= s_pick[0] << shift;
-            mask |= 255u << shift;
-            __syncthreads();
+        __syncthreads();
+        const int at = (int)(s.small[2] != 0x7FFFFFFF ? s.small[2] : s.small[3]);  // (none: u of 1 and above)
+        if (at >= s0 && at < s1) {
+            run = before;
+            for (int i = s0; i < at; i++) run += stripe_mass(i);
+            s.wave[0] = run;
         }
-        // of key `prefix` as many as it takes
-        if (phase == 0) {
-            cut = prefix;
-            ties = (uint32_t)(tk - (int)above);
-        } else {
-            const double each = rint(w(prefix) * unit);
-            double n = ceil((goal - (double)above) / each);
-            n = n < 1 ? 1 : n;
-            const uint32_t most = prefix == cut ? ties : 0xFFFFFFFFu;
-            ties = n < (double)most ? (uint32_t)n : most;
-            cut = prefix;
+        __syncthreads();
+        if (w != 0) return;
+        uint32_t k[4];
+        x.keys4(at * kStripe + 4 * lane, k);
+        double y[4], sum = 0;
+#pragma unroll
+        for (int v = 0; v < 4; v++) y[v] = wt(k[v]), sum += y[v];
+        double incl = sum;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const double z = __shfl_up(incl, o);
+            if (lane >= o) incl += z;
+        }
+        run = s.wave[0] + (incl - sum);
+        int found = 0x7FFFFFFF, last = -1;
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            run += y[v];
+            if (y[v] > 0) last = 4 * lane + v;
+            if (y[v] > 0 && run > goal && found == 0x7FFFFFFF) found = 4 * lane + v;
+        }
+        for (int o = 32; o; o >>= 1) {
+            const int a = __shfl_xor(found, o), b = __shfl_xor(last, o);
+            found = found < a ? found : a;
+            last = last > b ? last : b;
+        }
+        if (lane == 0) {
+            const int token = at * kStripe + (found != 0x7FFFFFFF ? found : last);
+            result(p, r, token, wt(x.key(token)), total);
+        }
+        return;
+    }
+    complete = all_max(complete, s);
+    uint32_t n_all;
+    const uint32_t n_before = before_me(total_left, s.u, n_all);
+    const uint32_t worst = all_max(total_left, s);
+    if (worst > kMost || n_all > kMost) return whole(p, r, x, wt, st, s);
+    {
+        uint32_t at = n_before;
+        for (int i = tid; i < p.groups; i += kThreads) {
+            const uint32_t n = agent_get(lefts + 4 * i + 2);
+            const unsigned long long *from = p.list + ((int64_t)r * p.groups + i) * p.room;
+            for (uint32_t j = 0; j < n; j++) s.sorted[at++] = agent_get(from + j);
         }
     }
-    const double low = mp >= 1.0f ? 1.0 : mp > 0.0f ? (double)mp : 0.0;
-    if (greedy) ties = 1;
-    // each thread's run of entries: how many of the cut's key, the kept weight, then the thread in which u falls
-    const int each = (p.vocab + kThreads - 1) / kThreads, i0 = tid * each, i1 = i0 + each < p.vocab ? i0 + each : p.vocab;
-    uint32_t eq = 0, total_eq;
-    for (int i = i0; i < i1; i++) eq += x.key(i) == cut;
-    const uint32_t eq0 = before_me(eq, s_u, total_eq);
-    auto walk = [&](auto use) {
-        uint32_t n = eq0;
-        for (int i = i0; i < i1; i++) {
-            const uint32_t k = x.key(i);
-            const bool keep = k > cut || (k == cut && n < ties);
-            n += k == cut;
-            if (!keep || k == 0) continue;
-            const double y = w(k);
-            if (y >= low) use(i, y);
-        }
-    };
-    double sum = 0, total;
-    walk([&](int, double y) { sum += y; });
-    const double start = before_me(sum, s_d, total);
-    const double goal = (double)u * total;
-    if (tid == 0) s_pick[0] = 0x7FFFFFFF, s_pick[1] = 0;
+    int n = (int)n_all, n2 = 2;
+    while (n2 < n) n2 <<= 1;
+    for (int i = n + tid; i < n2; i += kThreads) s.sorted[i] = 0;
+    sort(s, n2, true);
+    // weights and their running sum, two entries a thread
+    static_assert(kMost == 2 * kThreads, "two entries a thread");
+    const uint32_t k0 = (uint32_t)(s.sorted[2 * tid < n2 ? 2 * tid : 0] >> 32), k1 = (uint32_t)(s.sorted[2 * tid + 1 < n2 ? 2 * tid + 1 : 0] >> 32);
+    const bool in0 = 2 * tid < n && (st.k == 0 || 2 * tid < st.k), in1 = 2 * tid + 1 < n && (st.k == 0 || 2 * tid + 1 < st.k);
+    const double w0 = in0 ? wt(k0) : 0.0, w1 = in1 ? wt(k1) : 0.0;
+    double sum;
+    const double run0 = before_me(w0 + w1, s.wave, sum), run1 = run0 + w0;
+    // entries that are certain: all of those from `complete` up are here
+    const bool sure0 = 2 * tid < n && k0 >= complete, sure1 = 2 * tid + 1 < n && k1 >= complete;
+    const double goal = (double)st.tp * (st.k > 0 ? sum : total);
+    const bool keep0 = in0 && (tid == 0 || ((st.tp >= 1.0f || run0 < goal) && w0 >= (double)st.low));
+    const bool keep1 = in1 && (st.tp >= 1.0f || run1 < goal) && w1 >= (double)st.low;
+    const int kept = __syncthreads_count(keep0) + __syncthreads_count(keep1);
+    const bool doubt = (keep0 && !sure0) || (keep1 && !sure1);
+    // (the run ends inside what is certain, or with top_k, or with the last entry there is)
+    const bool end = complete == 0 || (st.k > 0 && kept == st.k);
+    const int sure = __syncthreads_count(sure0) + __syncthreads_count(sure1);
+    if (__syncthreads_or(doubt) || (!end && kept >= sure) || (st.k > 0 && st.tp < 1.0f && sure < (st.k < n ? st.k : n) && complete != 0) || (st.k > n && complete != 0))
+        return whole(p, r, x, wt, st, s);
+    // what is kept, by index
+    unsigned long long e0 = 0, e1 = 0;
+    if (2 * tid < n2) e0 = s.sorted[2 * tid], e1 = s.sorted[2 * tid + 1];
+    s.weight[2 * tid] = w0, s.weight[2 * tid + 1] = w1;
+    n2 = 2;
+    while (n2 < kept) n2 <<= 1;
     __syncthreads();
-    int found = 0x7FFFFFFF, last = -1;
-    double run = start;
-    walk([&](int i, double y) {
-        run += y;
-        if (y > 0) last = i;
-        if (run > goal && found == 0x7FFFFFFF) found = i;
-    });
-    if (found != 0x7FFFFFFF) atomicMin(&s_pick[0], (uint32_t)found);
-    if (last >= 0) atomicMax(&s_pick[1], (uint32_t)last);
+    const unsigned long long none = ~0ull;
+    if (2 * tid < n2) s.sorted[2 * tid] = keep0 ? ((unsigned long long)(uint32_t)~(uint32_t)e0 << 32) | (uint32_t)(2 * tid) : none;
+    if (2 * tid + 1 < n2) s.sorted[2 * tid + 1] = keep1 ? ((unsigned long long)(uint32_t)~(uint32_t)e1 << 32) | (uint32_t)(2 * tid + 1) : none;
+    sort(s, n2, false);
+    const bool a0 = 2 * tid < kept, a1 = 2 * tid + 1 < kept;
+    const double v0 = a0 ? s.weight[(uint32_t)s.sorted[2 * tid]] : 0.0, v1 = a1 ? s.weight[(uint32_t)s.sorted[2 * tid + 1]] : 0.0;
+    double kept_sum;
+    const double q0 = before_me(v0 + v1, s.wave, kept_sum) + v0, q1 = q0 + v1, at = st.u * kept_sum;
+    __syncthreads();
+    if (tid == 0) s.small[2] = 0x7FFFFFFF, s.small[3] = 0;
+    __syncthreads();
+    if (a0 && q0 > at) atomicMin(&s.small[2], (uint32_t)(2 * tid));
+    if (a1 && q1 > at) atomicMin(&s.small[2], (uint32_t)(2 * tid + 1));
+    if (a0 && v0 > 0) atomicMax(&s.small[3], (uint32_t)(2 * tid));
+    if (a1 && v1 > 0) atomicMax(&s.small[3], (uint32_t)(2 * tid + 1));
     __syncthreads();
     if (tid == 0) {
-        const int token = s_pick[0] != 0x7FFFFFFF ? (int)s_pick[0] : (int)s_pick[1];
-        p.token[r] = token;
-        if (p.logprob) p.logprob[r] = (float)log(w(x.key(token)) / total);
+        const unsigned long long e = s.sorted[s.small[2] != 0x7FFFFFFF ? s.small[2] : s.small[3]];
+        result(p, r, (int)(e >> 32), s.weight[(uint32_t)e], kept_sum);
     }
 }
 
@@ -217,9 +598,41 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
 
 int launch_sample(trhip_ctx *ctx, const void *logits, int io, int64_t stride, int64_t rows, int64_t vocab, const float *temperature,
                   const int *top_k, const float *top_p, const float *min_p, const float *u, int *token, float *logprob) {
-    const SampleArgs p = {logits, io, stride, (int)vocab, temperature, top_k, top_p, min_p, u, token, logprob};
-    hipLaunchKernelGGL(sample_kernel, dim3((unsigned)rows), dim3(kThreads), 0, ctx->stream, p);
-    return launch_check(ctx, "sample");
+    const int64_t cus = ctx->sm_count > 0 ? ctx->sm_count : 256, stripes = (vocab + kStripe - 1) / kStripe, esize = io == TRHIP_F32 ? 4 : 2;
+    // stripes a wave: few for few rows, so that they lie on many CUs
+    int64_t each = 1;
+    auto groups_of = [&](int64_t j) { return (stripes + kWaves * j - 1) / (kWaves * j); };
+    while (each < 8 && rows * groups_of(each) > 2 * cus) each *= 2;
+    while (each < 8 && groups_of(each) > kThreads / 8) each *= 2;
+    const int64_t groups = groups_of(each);
+    const double mean = (double)kMost / 2 / (double)groups;
+    int64_t room = (int64_t)(mean + 4.0 * __builtin_sqrt(mean) + 6.0) * 3 / 2 + 16;
+    if (room > kMost) room = kMost;
+    // rows of a launch: an arrival counter each, and at most 2^28 bytes of workspace where more than one row
+    const int64_t row_bytes = stripes * 8 + groups * room * 8 + groups * 16;
+    int64_t most = (int64_t)1 << 28;
+    most = most / row_bytes < 1 ? 1 : most / row_bytes;
+    if (most > 32768) most = 32768;
+    if (most > rows) most = rows;
+    int st = TRHIP_OK;
+    uint8_t *ws = static_cast<uint8_t *>(workspace(ctx, (size_t)(most * row_bytes), &st));
+    if (!ws) return st;
+    const int wide = reinterpret_cast<uintptr_t>(logits) % (4 * esize) == 0 && stride % 4 == 0;
+    for (int64_t r0 = 0; r0 < rows; r0 += most) {
+        const int64_t n = rows - r0 < most ? rows - r0 : most;
+        SampleArgs p = {static_cast<const char *>(logits) + r0 * stride * esize, io, stride, (int)vocab, (int)stripes, (int)groups, (int)room, wide,
+                        temperature ? temperature + r0 : nullptr, top_k ? top_k + r0 : nullptr, top_p ? top_p + r0 : nullptr, min_p ? min_p + r0 : nullptr, u + r0,
+                        token + r0, logprob ? logprob + r0 : nullptr, reinterpret_cast<double *>(ws),
+                        reinterpret_cast<unsigned long long *>(ws + most * stripes * 8), reinterpret_cast<uint32_t *>(ws + most * (stripes + groups * room) * 8), ctx->arrivals};
+        const dim3 grid((unsigned)groups, (unsigned)n);
+        if (each == 1) hipLaunchKernelGGL(sample_kernel<1>, grid, dim3(kThreads), 0, ctx->stream, p);
+        else if (each == 2) hipLaunchKernelGGL(sample_kernel<2>, grid, dim3(kThreads), 0, ctx->stream, p);
+        else if (each == 4) hipLaunchKernelGGL(sample_kernel<4>, grid, dim3(kThreads), 0, ctx->stream, p);
+        else hipLaunchKernelGGL(sample_kernel<8>, grid, dim3(kThreads), 0, ctx->stream, p);
+        st = launch_check(ctx, "sample");
+        if (st != TRHIP_OK) return st;
+    }
+    return TRHIP_OK;
 }
 
 }  // namespace trhip
