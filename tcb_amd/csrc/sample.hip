@@ -33,6 +33,7 @@ struct SampleArgs {
     float *logprob;
     double *mass;           // [row][stripe]
     unsigned long long *list;  // [row][workgroup][room]: key, ~index
+    unsigned long long *hist;  // [row][workgroup][kBins]: weight in bins of its logits, from the largest down, in units of 2^-48
     uint32_t *left;         // [row][workgroup][4]: largest key, threshold (0: all entries left), entries left, unused
     uint32_t *arrivals;     // [row]
 };
@@ -128,27 +129,62 @@ __device__ __forceinline__ int share_of(int n, int groups) {
 
 struct Lds {
     double table[64];
-    double sum[kThreads];
     unsigned long long sorted[kMost];
     double weight[kMost];
-    unsigned long long bins[kBins];
+    union {
+        unsigned long long bins[kBins];
+        struct {
+            uint32_t from[kMost], count[kMost];  // a workgroup's entries
+        };
+        unsigned long long stripe[kMost];
+    };
     uint32_t u[kThreads];
     uint32_t small[16];
     double wave[kWaves];
 };
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+// Bins of a thirty-second of a nat, of logits over the temperature: the number of a key's bin, which rises with it.
+__device__ __forceinline__ int bin_of(uint32_t k, float per) {
+    return (int)floorf(fminf(fmaxf(of_key(k) * per, -536870912.0f), 536870912.0f));
 }
+
+// Inclusive sums over the wave's lanes, in six lane moves (row_shr 1, 2, 4, 8, then row_bcast 15 and 31).
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t moved(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS> __device__ __forceinline__ double moved(double v) {
+    const long long x = __double_as_longlong(v);
+    const uint32_t lo = moved<CTRL, ROWS>((uint32_t)x), hi = moved<CTRL, ROWS>((uint32_t)(x >> 32));
+    return __longlong_as_double((long long)(((unsigned long long)hi << 32) | lo));
+}
+template <class T> __device__ __forceinline__ T running(T v) {
+    v += moved<0x111, 0xF>(v);
+    v += moved<0x112, 0xF>(v);
+    v += moved<0x114, 0xF>(v);
+    v += moved<0x118, 0xF>(v);
+    v += moved<0x142, 0xA>(v);
+    return v + moved<0x143, 0xC>(v);
+}
+// The lane before's value; 0 in the first.
+template <class T> __device__ __forceinline__ T before_lane(T v) {
+    const T up = __shfl_up(v, 1);
+    return (threadIdx.x & 63) ? up : T(0);
+}
+__device__ __forceinline__ double of_lane(double v, int lane) {
+    const long long x = __double_as_longlong(v);
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)x, lane), hi = __builtin_amdgcn_readlane((uint32_t)(x >> 32), lane);
+    return __longlong_as_double((long long)(((unsigned long long)hi << 32) | lo));
+}
+__device__ __forceinline__ uint32_t of_lane(uint32_t v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ double wave_sum(double v) { return of_lane(running(v), 63); }
 __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) {
-        const uint32_t w = __shfl_xor(v, o);
-        v = v > w ? v : w;
-    }
-    return v;
+    auto up = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+    v = up(v, moved<0x111, 0xF>(v));
+    v = up(v, moved<0x112, 0xF>(v));
+    v = up(v, moved<0x114, 0xF>(v));
+    v = up(v, moved<0x118, 0xF>(v));
+    v = up(v, moved<0x142, 0xA>(v));
+    return of_lane(up(v, moved<0x143, 0xC>(v)), 63);
 }
 // Over the workgroup; every thread gets the result. (A barrier before the first use of s.u / s.wave is the caller's.)
 __device__ uint32_t all_max(uint32_t v, Lds &s) {
@@ -172,23 +208,18 @@ __device__ double all_sum(double v, Lds &s) {
 // Sum over the threads before this one, and over all.
 template <class T> __device__ T before_me(T v, T *lds, T &total) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    T x = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const T y = __shfl_up(x, o);
-        if (lane >= o) x += y;
-    }
+    const T x = running(v);
     __syncthreads();
     if (lane == 63) lds[w] = x;
     __syncthreads();
     T base = T(0);
     total = T(0);
+#pragma unroll
     for (int i = 0; i < kWaves; i++) {
         if (i == w) base = total;
         total += lds[i];
     }
-    const T up = __shfl_up(x, 1);
-    return base + (lane ? up : T(0));
+    return base + before_lane(x);
 }
 
 // Sorts s.sorted[0 .. n2), n2 a power of two, n2 <= kMost: largest first, or smallest.
@@ -259,6 +290,237 @@ __device__ void pick(const SampleArgs &p, int r, const Row &x, const Weight &w, 
     if (tid == 0) {
         const int token = (int)(s.small[0] != 0x7FFFFFFF ? s.small[0] : s.small[1]);
         result(p, r, token, w(x.key(token)), total);
+    }
+}
+
+__device__ __forceinline__ uint32_t agent_get(const uint32_t *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ unsigned long long agent_get(const unsigned long long *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ double agent_get(const double *p) {
+    return __longlong_as_double((long long)agent_get(reinterpret_cast<const unsigned long long *>(p)));
+}
+template <class T> __device__ __forceinline__ void agent_put(T *p, T v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// The entry of stripe `at` (keys k, four a lane) in which the goal falls, the weights before the stripe being `before`; by one wave.
+template <class F>
+__device__ __forceinline__ void last_stripe(const SampleArgs &p, int r, int at, double before, double goal, double total, const uint32_t (&k)[4], F weight) {
+    const int lane = threadIdx.x & 63;
+    double y[4], sum = 0;
+#pragma unroll
+    for (int v = 0; v < 4; v++) y[v] = weight(k[v], (uint32_t)(at * kStripe + 4 * lane + v)), sum += y[v];
+    double run = before + before_lane(running(sum)), chosen = 0, final = 0;
+    int found = -1, last = -1;
+#pragma unroll
+    for (int v = 0; v < 4; v++) {
+        run += y[v];
+        if (y[v] > 0) last = v, final = y[v];
+        if (y[v] > 0 && run > goal && found < 0) found = v, chosen = y[v];
+    }
+    const uint64_t over = __ballot(found >= 0), some = __ballot(last >= 0);
+    const int src = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : 0;
+    if (lane == src) result(p, r, at * kStripe + 4 * lane + (over ? found : last), over ? chosen : final, total);
+}
+
+// Sorts one element a lane: largest first, or smallest.
+__device__ __forceinline__ unsigned long long sort64(unsigned long long e, bool falling) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int k = 2; k <= 64; k <<= 1)
+#pragma unroll
+        for (int j = k >> 1; j; j >>= 1) {
+            const unsigned long long o = __shfl_xor(e, j);
+            const bool first = (lane & j) == 0, down = ((lane & k) == 0) == falling;  // this lane keeps the larger one
+            e = (first == down) == (e > o) ? e : o;
+        }
+    return e;
+}
+
+// A filtered row whose kept run is among its largest 64 entries, by one wave: those that a threshold leaves of the n in s.sorted.
+// False: it is not, or that is not certain.
+__device__ bool top64(const SampleArgs &p, int r, const Weight &wt, const Setting &st, double total, uint32_t complete, int n, Lds &s) {
+    const int lane = threadIdx.x & 63;
+    constexpr int PER = kMost / 64;
+    uint32_t k[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++) k[i] = 64 * i + lane < n ? (uint32_t)(s.sorted[64 * i + lane] >> 32) : 0;
+    uint32_t lo = 1, hi = wt.top;  // at least `want` entries reach lo
+    int count = n;
+    const int want = st.k > 0 ? st.k : 48;
+    for (int step = 0; step < 40 && count > 64 && lo < hi; step++) {
+        const uint32_t mid = lo + (hi - lo + 1) / 2;
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < PER; i++) c += __popcll(__ballot(k[i] >= mid));
+        if (c >= want) lo = mid, count = c;
+        else hi = mid - 1;
+    }
+    if (count > 64) return false;
+    int at = 0;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const uint64_t m = __ballot(k[i] >= lo);
+        if (k[i] >= lo) s.weight[at + __popcll(m & (((uint64_t)1 << lane) - 1))] = __longlong_as_double((long long)s.sorted[64 * i + lane]);
+        at += __popcll(m);
+    }
+    __builtin_amdgcn_wave_barrier();
+    unsigned long long e = lane < count ? (unsigned long long)__double_as_longlong(s.weight[lane]) : 0;
+    e = sort64(e, true);
+    const uint32_t key = (uint32_t)(e >> 32);
+    const bool in = lane < count && (st.k == 0 || lane < st.k);
+    const double w = in ? wt(key) : 0.0, incl = running(w), before = before_lane(incl), sum = of_lane(incl, 63);
+    // every entry from here up is in these lanes
+    const uint32_t from = count < n && lo > complete ? lo : complete;
+    const bool sure = lane < count && key >= from, all = from == 0 || (from <= 1 && complete == 0);
+    const double goal = (double)st.tp * (st.k > 0 ? sum : total);
+    const bool keep = in && (lane == 0 || ((st.tp >= 1.0f || before < goal) && w >= (double)st.low));
+    const int kept = __popcll(__ballot(keep)), certain = __popcll(__ballot(sure));
+    if (!all) {
+        if (kept > certain || (kept == certain && kept != st.k)) return false;  // (the run may go on past what is here)
+        if (st.k > 0 && st.tp < 1.0f && certain < st.k) return false;           // (nor is the sum certain)
+    }
+    unsigned long long by = keep ? ((unsigned long long)(uint32_t)~(uint32_t)e << 32) | (uint32_t)lane : ~0ull;
+    by = sort64(by, false);
+    const double v = __shfl(w, (int)((uint32_t)by & 63)), mine = lane < kept ? v : 0.0, run = running(mine), kept_sum = of_lane(run, 63), goal_u = st.u * kept_sum;
+    const uint64_t over = __ballot(lane < kept && run > goal_u), some = __ballot(lane < kept && v > 0);
+    const int pos = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
+    const uint32_t token = of_lane((uint32_t)(by >> 32), pos);
+    const double chosen = of_lane(mine, pos);
+    if (lane == 0) result(p, r, (int)token, chosen, kept_sum);
+    return true;
+}
+
+// A row without top_k whose kept run is long: the bin in which it ends, from the workgroups' bins; then one pass over the row, which weighs the
+// stripes' entries above that bin and takes the bin's own entries out to sort them; then the stripe in which u falls.
+__device__ __noinline__ void sweep(const SampleArgs &p, int r, const Row &x, const Weight &wt, const Setting &st, double total, Lds &s);
+__device__ __noinline__ void whole(const SampleArgs &p, int r, const Row &x, const Weight &w, const Setting &st, Lds &s);
+
+__device__ __noinline__ void sweep(const SampleArgs &p, int r, const Row &x, const Weight &wt, const Setting &st, double total, Lds &s) {
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const float per = 32.0f / st.t;
+    const int first = bin_of(wt.top, per);
+    const double low = (double)st.low, goal = (double)st.tp * total;
+    int end = 0x7FFFFFFF;  // the bin in which the run ends, counted from the largest logit's down
+    double above = 0;      // the weight of those before it
+    if (st.tp < 1.0f) {
+        static_assert(kBins == 4 * kThreads, "four bins a thread");
+        double mine[4] = {};
+        const uint32_t *lefts = p.left + (int64_t)r * p.groups * 4;
+        for (int g = 0; g < p.groups; g++) {
+            const uint32_t a = agent_get(lefts + 4 * g);
+            if (a == 0) continue;
+            const int shift = first - bin_of(a, per);
+            const double unit = wt(a) * 0x1p-48;
+            const unsigned long long *from = p.hist + ((int64_t)r * p.groups + g) * kBins;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int at = 4 * tid + i - shift;
+                if (at >= 0) mine[i] += (double)agent_get(from + at) * unit;
+            }
+        }
+        double all;
+        double run = before_me((mine[0] + mine[1]) + (mine[2] + mine[3]), s.wave, all);
+        __syncthreads();
+        if (tid == 0) s.small[5] = kBins - 1;
+        __syncthreads();
+        const double start = run;
+        for (int i = 0; i < 4; i++) {
+            run += mine[i];
+            if (mine[i] > 0 && run >= goal) {
+                atomicMin(&s.small[5], (uint32_t)(4 * tid + i));
+                break;
+            }
+        }
+        __syncthreads();
+        end = (int)s.small[5];
+        if (end >> 2 == tid) {
+            run = start;
+            for (int i = 0; i < (end & 3); i++) run += mine[i];
+            s.wave[0] = run;
+        }
+        __syncthreads();
+        above = s.wave[0];
+        __syncthreads();
+    }
+    // the stripes' weights, in units of 2^-44, and the entries of the last bin
+    if (tid == 0) s.small[6] = 0;
+    for (int i = tid; i < kMost; i += kThreads) s.stripe[i] = 0;
+    __syncthreads();
+    constexpr int AT = 4;
+    for (int b0 = w; b0 < p.stripes; b0 += AT * kWaves) {
+        uint32_t k[AT][4];
+#pragma unroll
+        for (int a = 0; a < AT; a++) {
+            if (b0 + a * kWaves < p.stripes) x.keys4((b0 + a * kWaves) * kStripe + 4 * lane, k[a]);
+            else k[a][0] = k[a][1] = k[a][2] = k[a][3] = 0;
+        }
+#pragma unroll
+        for (int a = 0; a < AT; a++) {
+            double sum = 0;
+#pragma unroll
+            for (int v = 0; v < 4; v++) {
+                const int b = k[a][v] ? first - bin_of(k[a][v], per) : 0x7FFFFFFF;
+                const bool in = k[a][v] != 0 && b < end, is = k[a][v] != 0 && b == end;
+                if (__any(in)) {
+                    const double y = in ? wt(k[a][v]) : 0.0;
+                    sum += y >= low ? y : 0.0;
+                }
+                const uint64_t m = __ballot(is);
+                if (m) {
+                    uint32_t at = 0;
+                    if (lane == 0) at = atomicAdd(&s.small[6], (uint32_t)__popcll(m));
+                    at = __builtin_amdgcn_readfirstlane(at) + __popcll(m & (((uint64_t)1 << lane) - 1));
+                    if (is && at < kMost) s.sorted[at] = ((unsigned long long)k[a][v] << 32) | (uint32_t)~((b0 + a * kWaves) * kStripe + 4 * lane + v);
+                }
+            }
+            const double all = wave_sum(sum);
+            if (lane == 0 && b0 + a * kWaves < p.stripes) s.stripe[b0 + a * kWaves] = (unsigned long long)rint(all * 0x1p44);
+        }
+    }
+    __syncthreads();
+    const int n = (int)s.small[6];
+    if (n > kMost) return whole(p, r, x, wt, st, s);
+    unsigned long long least = ~0ull;  // the last entry that is kept of that bin
+    if (n > 0) {
+        int n2 = 2;
+        while (n2 < n) n2 <<= 1;
+        for (int i = n + tid; i < n2; i += kThreads) s.sorted[i] = 0;
+        sort(s, n2, true);
+        const unsigned long long e0 = 2 * tid < n ? s.sorted[2 * tid] : 0, e1 = 2 * tid + 1 < n ? s.sorted[2 * tid + 1] : 0;
+        const double w0 = e0 ? wt((uint32_t)(e0 >> 32)) : 0.0, w1 = e1 ? wt((uint32_t)(e1 >> 32)) : 0.0;
+        double sum;
+        const double run0 = above + before_me(w0 + w1, s.wave, sum), run1 = run0 + w0;
+        const bool keep0 = e0 && ((end == 0 && tid == 0) || (run0 < goal && w0 >= low)), keep1 = e1 && run1 < goal && w1 >= low;
+        if (keep0) atomicAdd(&s.stripe[(uint32_t)~(uint32_t)e0 / kStripe], (unsigned long long)rint(w0 * 0x1p44));
+        if (keep1) atomicAdd(&s.stripe[(uint32_t)~(uint32_t)e1 / kStripe], (unsigned long long)rint(w1 * 0x1p44));
+        const int kept = __syncthreads_count(keep0) + __syncthreads_count(keep1);
+        if (kept > 0) least = s.sorted[kept - 1];
+    }
+    __syncthreads();
+    static_assert(kMost == 2 * kThreads, "two stripes a thread");
+    const double m0 = (double)s.stripe[2 * tid] * 0x1p-44, m1 = (double)s.stripe[2 * tid + 1] * 0x1p-44;
+    double kept_sum;
+    const double before = before_me(m0 + m1, s.wave, kept_sum), goal_u = st.u * kept_sum;
+    __syncthreads();
+    if (tid == 0) s.small[2] = 0x7FFFFFFF, s.small[3] = 0;
+    __syncthreads();
+    if (m0 > 0 && before + m0 > goal_u) atomicMin(&s.small[2], (uint32_t)(2 * tid));
+    if (m1 > 0 && before + m0 + m1 > goal_u) atomicMin(&s.small[2], (uint32_t)(2 * tid + 1));
+    if (m0 > 0) atomicMax(&s.small[3], (uint32_t)(2 * tid));
+    if (m1 > 0) atomicMax(&s.small[3], (uint32_t)(2 * tid + 1));
+    __syncthreads();
+    const int at = (int)(s.small[2] != 0x7FFFFFFF ? s.small[2] : s.small[3]);
+    if (at >> 1 == tid) s.wave[0] = at & 1 ? before + m0 : before;
+    __syncthreads();
+    if (w == 0) {
+        uint32_t k[4];
+        x.keys4(at * kStripe + 4 * lane, k);
+        auto weight = [&](uint32_t key, uint32_t i) {
+            if (key == 0) return 0.0;
+            const int b = first - bin_of(key, per);
+            if (b > end || (b == end && ((((unsigned long long)key << 32) | (uint32_t)~i) < least || least == ~0ull))) return 0.0;
+            const double y = wt(key);
+            return y >= low || key == wt.top ? y : 0.0;
+        };
+        last_stripe(p, r, at, s.wave[0], goal_u, kept_sum, k, weight);
     }
 }
 
@@ -340,13 +602,6 @@ __device__ __noinline__ void whole(const SampleArgs &p, int r, const Row &x, con
     pick(p, r, x, w, cut, ties, (double)st.low, st.u, s);
 }
 
-__device__ __forceinline__ uint32_t agent_get(const uint32_t *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ unsigned long long agent_get(const unsigned long long *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ double agent_get(const double *p) {
-    return __longlong_as_double((long long)agent_get(reinterpret_cast<const unsigned long long *>(p)));
-}
-template <class T> __device__ __forceinline__ void agent_put(T *p, T v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-
 template <int J> __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs p) {
     __shared__ Lds s;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, r = blockIdx.y, g = blockIdx.x;
@@ -384,6 +639,23 @@ template <int J> __global__ __launch_bounds__(kThreads) void sample_kernel(const
             const double sum = wave_sum((wt(key[j][0]) + wt(key[j][1])) + (wt(key[j][2]) + wt(key[j][3])));
             if (lane == 0) agent_put(p.mass + (int64_t)r * p.stripes + stripe(j), sum);
         }
+    }
+    if (st.k == 0 && st.tp < 1.0f && top != 0) {
+        for (int i = tid; i < kBins; i += kThreads) s.bins[i] = 0;
+        __syncthreads();
+        const Weight wt = {top, (double)of_key(top), 1.0 / (double)st.t, s.table};
+        const float per = 32.0f / st.t;
+        const int first = bin_of(top, per);
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int v = 0; v < 4; v++) {
+                if (key[j][v] == 0) continue;
+                const int b = first - bin_of(key[j][v], per);
+                atomicAdd(&s.bins[b < kBins ? b : kBins - 1], (unsigned long long)rint(wt(key[j][v]) * 0x1p48));
+            }
+        __syncthreads();
+        for (int i = tid; i < kBins; i += kThreads) agent_put(p.hist + ((int64_t)r * p.groups + g) * kBins + i, s.bins[i]);
     }
     uint32_t bound = 0, left = 0;
     if (filtered && top != 0) {
@@ -501,46 +773,52 @@ template <int J> __global__ __launch_bounds__(kThreads) void sample_kernel(const
         if (w != 0) return;
         uint32_t k[4];
         x.keys4(at * kStripe + 4 * lane, k);
-        double y[4], sum = 0;
-#pragma unroll
-        for (int v = 0; v < 4; v++) y[v] = wt(k[v]), sum += y[v];
-        double incl = sum;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const double z = __shfl_up(incl, o);
-            if (lane >= o) incl += z;
-        }
-        run = s.wave[0] + (incl - sum);
-        int found = 0x7FFFFFFF, last = -1;
-#pragma unroll
-        for (int v = 0; v < 4; v++) {
-            run += y[v];
-            if (y[v] > 0) last = 4 * lane + v;
-            if (y[v] > 0 && run > goal && found == 0x7FFFFFFF) found = 4 * lane + v;
-        }
-        for (int o = 32; o; o >>= 1) {
-            const int a = __shfl_xor(found, o), b = __shfl_xor(last, o);
-            found = found < a ? found : a;
-            last = last > b ? last : b;
-        }
-        if (lane == 0) {
-            const int token = at * kStripe + (found != 0x7FFFFFFF ? found : last);
-            result(p, r, token, wt(x.key(token)), total);
-        }
+        last_stripe(p, r, at, s.wave[0], goal, total, k, [&](uint32_t key, uint32_t) { return wt(key); });
         return;
     }
     complete = all_max(complete, s);
     uint32_t n_all;
     const uint32_t n_before = before_me(total_left, s.u, n_all);
     const uint32_t worst = all_max(total_left, s);
-    if (worst > kMost || n_all > kMost) return whole(p, r, x, wt, st, s);
+    const double goal_all = (double)st.tp * total;
+    auto otherwise = [&] {
+        // (sweep's sums end at 2^-45 of the largest weight: smaller ones are kept by the smallest min_p alone)
+        if (st.k == 0 && p.stripes <= kMost && (st.tp < 1.0f || st.low > 0x1p-40f)) sweep(p, r, x, wt, st, total, s);
+        else whole(p, r, x, wt, st, s);
+    };
+    if (worst > kMost || n_all > kMost) return otherwise();
     {
-        uint32_t at = n_before;
+        uint32_t from = n_before;
         for (int i = tid; i < p.groups; i += kThreads) {
             const uint32_t n = agent_get(lefts + 4 * i + 2);
-            const unsigned long long *from = p.list + ((int64_t)r * p.groups + i) * p.room;
-            for (uint32_t j = 0; j < n; j++) s.sorted[at++] = agent_get(from + j);
+            s.from[i] = from, s.count[i] = n;
+            from += n;
         }
+        __syncthreads();
+        constexpr int AT = 4;
+        for (int i0 = tid; i0 < p.groups * p.room; i0 += AT * kThreads) {
+            unsigned long long e[AT];
+            uint32_t to[AT];
+#pragma unroll
+            for (int v = 0; v < AT; v++) {
+                const int i = i0 + v * kThreads, gi = i < p.groups * p.room ? i / p.room : 0, slot = i - gi * p.room;
+                const bool is = i < p.groups * p.room && (uint32_t)slot < s.count[gi];
+                to[v] = is ? s.from[gi] + slot : 0xFFFFFFFFu;
+                e[v] = is ? agent_get(p.list + ((int64_t)r * p.groups + gi) * p.room + slot) : 0;
+            }
+#pragma unroll
+            for (int v = 0; v < AT; v++)
+                if (to[v] != 0xFFFFFFFFu) s.sorted[to[v]] = e[v];
+        }
+        __syncthreads();
+    }
+    if (st.k <= 64) {
+        if (w == 0) {
+            const bool done = top64(p, r, wt, st, total, complete, (int)n_all, s);
+            if (lane == 0) s.small[4] = done;
+        }
+        __syncthreads();
+        if (s.small[4]) return;
     }
     int n = (int)n_all, n2 = 2;
     while (n2 < n) n2 <<= 1;
@@ -555,7 +833,7 @@ template <int J> __global__ __launch_bounds__(kThreads) void sample_kernel(const
     const double run0 = before_me(w0 + w1, s.wave, sum), run1 = run0 + w0;
     // entries that are certain: all of those from `complete` up are here
     const bool sure0 = 2 * tid < n && k0 >= complete, sure1 = 2 * tid + 1 < n && k1 >= complete;
-    const double goal = (double)st.tp * (st.k > 0 ? sum : total);
+    const double goal = st.k > 0 ? (double)st.tp * sum : goal_all;
     const bool keep0 = in0 && (tid == 0 || ((st.tp >= 1.0f || run0 < goal) && w0 >= (double)st.low));
     const bool keep1 = in1 && (st.tp >= 1.0f || run1 < goal) && w1 >= (double)st.low;
     const int kept = __syncthreads_count(keep0) + __syncthreads_count(keep1);
@@ -564,7 +842,7 @@ template <int J> __global__ __launch_bounds__(kThreads) void sample_kernel(const
     const bool end = complete == 0 || (st.k > 0 && kept == st.k);
     const int sure = __syncthreads_count(sure0) + __syncthreads_count(sure1);
     if (__syncthreads_or(doubt) || (!end && kept >= sure) || (st.k > 0 && st.tp < 1.0f && sure < (st.k < n ? st.k : n) && complete != 0) || (st.k > n && complete != 0))
-        return whole(p, r, x, wt, st, s);
+        return otherwise();
     // what is kept, by index
     unsigned long long e0 = 0, e1 = 0;
     if (2 * tid < n2) e0 = s.sorted[2 * tid], e1 = s.sorted[2 * tid + 1];
@@ -609,7 +887,7 @@ int launch_sample(trhip_ctx *ctx, const void *logits, int io, int64_t stride, in
     int64_t room = (int64_t)(mean + 4.0 * __builtin_sqrt(mean) + 6.0) * 3 / 2 + 16;
     if (room > kMost) room = kMost;
     // rows of a launch: an arrival counter each, and at most 2^28 bytes of workspace where more than one row
-    const int64_t row_bytes = stripes * 8 + groups * room * 8 + groups * 16;
+    const int64_t row_bytes = (stripes + groups * (room + kBins + 2)) * 8;
     int64_t most = (int64_t)1 << 28;
     most = most / row_bytes < 1 ? 1 : most / row_bytes;
     if (most > 32768) most = 32768;
@@ -623,7 +901,8 @@ int launch_sample(trhip_ctx *ctx, const void *logits, int io, int64_t stride, in
         SampleArgs p = {static_cast<const char *>(logits) + r0 * stride * esize, io, stride, (int)vocab, (int)stripes, (int)groups, (int)room, wide,
                         temperature ? temperature + r0 : nullptr, top_k ? top_k + r0 : nullptr, top_p ? top_p + r0 : nullptr, min_p ? min_p + r0 : nullptr, u + r0,
                         token + r0, logprob ? logprob + r0 : nullptr, reinterpret_cast<double *>(ws),
-                        reinterpret_cast<unsigned long long *>(ws + most * stripes * 8), reinterpret_cast<uint32_t *>(ws + most * (stripes + groups * room) * 8), ctx->arrivals};
+                        reinterpret_cast<unsigned long long *>(ws + most * stripes * 8), reinterpret_cast<unsigned long long *>(ws + most * (stripes + groups * room) * 8),
+                        reinterpret_cast<uint32_t *>(ws + most * (stripes + groups * (room + kBins)) * 8), ctx->arrivals};
         const dim3 grid((unsigned)groups, (unsigned)n);
         if (each == 1) hipLaunchKernelGGL(sample_kernel<1>, grid, dim3(kThreads), 0, ctx->stream, p);
         else if (each == 2) hipLaunchKernelGGL(sample_kernel<2>, grid, dim3(kThreads), 0, ctx->stream, p);
