@@ -12,7 +12,7 @@ struct Kv4Args {
     uint8_t *kc, *vc;
     int page_log2, heads, dim;
     int64_t places, stride;
-    int tokens, wide;  // wide: rows are aligned to 16 bytes
+    int tokens, wide, run;  // wide: rows are aligned to 16 bytes; run: tokens of a workgroup
     const int *slots;
 };
 
@@ -27,6 +27,10 @@ __device__ __forceinline__ int together(const Kv4Args &p, int t, int64_t &slot) 
 #pragma unroll
     for (int i = 0; i < 4; i++) row = row && (int64_t)p.slots[first + i] == slot - at + i;
     return !row ? 1 : at == 0 ? 4 : 0;
+}
+
+template <int CTRL> __device__ __forceinline__ uint32_t quad(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
 }
 
 template <int IO> __device__ __forceinline__ void get8(const void *src, int64_t at, bool wide, float (&f)[8]) {
@@ -55,9 +59,20 @@ template <int IO> __device__ __forceinline__ void get8(const void *src, int64_t 
 template <int IO> __device__ __forceinline__ void put8(void *dst, int64_t at, bool wide, const float (&f)[8]) {
     if constexpr (IO == TRHIP_F32) {
         float *d = static_cast<float *>(dst) + at;
-        if (wide) {
-            *reinterpret_cast<float4 *>(d) = make_float4(f[0], f[1], f[2], f[3]);
-            *reinterpret_cast<float4 *>(d + 4) = make_float4(f[4], f[5], f[6], f[7]);
+        if (wide) {  // four lanes' 128 bytes in two runs of 64: first the first two lanes' eights
+            const int lane = threadIdx.x & 3;
+            d -= 8 * lane;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                float y[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t lo = i == 0 ? quad<0x50>(__float_as_uint(f[j])) : quad<0xFA>(__float_as_uint(f[j]));  // lanes 0 0 1 1, 2 2 3 3
+                    const uint32_t hi = i == 0 ? quad<0x50>(__float_as_uint(f[4 + j])) : quad<0xFA>(__float_as_uint(f[4 + j]));
+                    y[j] = __uint_as_float(lane & 1 ? hi : lo);
+                }
+                *reinterpret_cast<float4 *>(d + 16 * i + 4 * lane) = make_float4(y[0], y[1], y[2], y[3]);
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < 8; i++) d[i] = f[i];
@@ -78,9 +93,6 @@ template <int IO> __device__ __forceinline__ void put8(void *dst, int64_t at, bo
 
 // The block's element of largest magnitude, the first of equal ones, from each of its four lanes' eight. (As whole numbers magnitudes
 // are in the same order, infinities and NaN above all others.)
-template <int CTRL> __device__ __forceinline__ uint32_t quad(uint32_t v) {
-    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
-}
 __device__ __forceinline__ float largest(const float (&f)[8]) {
     uint32_t m = __float_as_uint(f[0]);
 #pragma unroll
@@ -183,7 +195,9 @@ template <int IO, bool APPEND> __global__ __launch_bounds__(256) void kv4_rows_k
     const int x = blockIdx.x * blockDim.x + threadIdx.x;
     const bool value = x >= row;
     const int y = value ? x - row : x, head = y / (4 * blocks), e = y - head * (4 * blocks), b = e >> 2, q = e & 3;
-    for (int t = blockIdx.y; t < p.tokens; t += gridDim.y) {
+    // (a workgroup a token would leave all work to every fourth, and workgroups are dealt to the XCDs in turn: two of eight would do it)
+    for (int t0 = blockIdx.y * p.run; t0 < p.tokens; t0 += gridDim.y * p.run)
+    for (int t = t0; t < t0 + p.run && t < p.tokens; t++) {
         int64_t slot;
         const int n = together(p, t, slot);
         if (n == 0 || x >= 2 * row) continue;
@@ -205,10 +219,12 @@ template <bool APPEND>
 int launch(trhip_ctx *ctx, const trhip_kv4 *kv, int64_t tokens, void *k, void *v, int io, int64_t stride, const int *slots) {
     const int64_t size = io == TRHIP_F32 ? 4 : 2;
     const bool wide = reinterpret_cast<uintptr_t>(k) % 16 == 0 && reinterpret_cast<uintptr_t>(v) % 16 == 0 && stride * size % 16 == 0;
+    const int run = tokens >= 256 ? 4 : 1;
     const Kv4Args p = {static_cast<uint8_t *>(kv->k), static_cast<uint8_t *>(kv->v), __builtin_ctz((unsigned)kv->page), kv->heads, kv->dim,
-                       kv->pages * kv->page, stride, (int)tokens, wide, slots};
+                       kv->pages * kv->page, stride, (int)tokens, wide, run, slots};
     const int eights = kv->heads * kv->dim / 4, threads = eights >= 256 ? 256 : (eights + 63) / 64 * 64;
-    const dim3 grid((unsigned)((eights + threads - 1) / threads), (unsigned)(tokens < 65535 ? tokens : 65535));
+    const int64_t y = (tokens + run - 1) / run;
+    const dim3 grid((unsigned)((eights + threads - 1) / threads), (unsigned)(y < 65535 ? y : 65535));
     if (io == TRHIP_F32) hipLaunchKernelGGL((kv4_rows_kernel<TRHIP_F32, APPEND>), grid, dim3(threads), 0, ctx->stream, p, k, v);
     else if (io == TRHIP_F16) hipLaunchKernelGGL((kv4_rows_kernel<TRHIP_F16, APPEND>), grid, dim3(threads), 0, ctx->stream, p, k, v);
     else hipLaunchKernelGGL((kv4_rows_kernel<TRHIP_BF16, APPEND>), grid, dim3(threads), 0, ctx->stream, p, k, v);
