@@ -28,12 +28,28 @@ typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 constexpr int kTwoSets = 4;  // blocks of elements up to which a workgroup's registers hold two sets of rows
 constexpr int64_t kMostImage = (int64_t)2 << 30;  // bytes of a plane of opened keys at most: a hundredth of the memory
 constexpr int kWaves = 4, kBlock = 32, kLeast = 8, kOver = 6;
+#ifndef SLOTS_
+#define SLOTS_ 2
+#endif
+#ifndef MINW_
+#define MINW_ 3
+#endif
+#ifndef PERCU_
+#define PERCU_ 3
+#endif
+constexpr int kSlots = SLOTS_;
 
 template <int NG, int NC> struct Shape4 {
     static constexpr int DIM = 32 * NG, ROWS = 16 * NC;
+    // a piece of sixteen places in LDS: copies of 1024 bytes, the last of 256 where that is enough
+    static constexpr int BYTES_IN = 288 * NG, WHOLE = BYTES_IN / 1024, TAIL = BYTES_IN % 1024, COPIES = WHOLE + (TAIL > 0);
+    static constexpr int PIECE = WHOLE * 1024 + (TAIL == 0 ? 0 : TAIL <= 256 ? 256 : 1024);
+    static constexpr int SLOT = 4 * PIECE;  // a block's two pieces of keys and two of values
+    static constexpr int SLOTS = NG == 8 ? 2 : NG >= 5 ? 2 : kSlots;
     static constexpr int OSTRIDE = DIM + 4;  // floats between rows of a wave's results
-    static constexpr int WAVE = ROWS * OSTRIDE * 4;
-    static constexpr int BYTES = kWaves * (WAVE + ROWS * 8) + 16;
+    static constexpr int RING = SLOTS * SLOT, OUT = ROWS * (OSTRIDE * 4 + 8);
+    static constexpr int WAVE = RING > OUT ? RING : OUT;
+    static constexpr int BYTES = kWaves * WAVE;
 };
 
 __device__ __forceinline__ f4 mma16(u32x4 a, u32x4 b, f4 c) {
@@ -53,48 +69,42 @@ __device__ __forceinline__ float row_sum(float x) {
 
 // The f16 operand c - 8 of a dword's eight codes: nibbles 0 and 4, 1 and 5, 2 and 6, 3 and 7.
 __device__ __forceinline__ u32x4 open8(uint32_t y) {
-    const uint32_t z = y >> 8;
+    const uint32_t z = y >> 8, m0 = 0x000F000Fu, e0 = 0x64006400u, m1 = 0x00F000F0u, e1 = 0x54005400u;
     const h2 a = {(_Float16)-1032.0f, (_Float16)-1032.0f}, b = {(_Float16)-72.0f, (_Float16)-72.0f};
     auto even = [&](uint32_t x) { return __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, (x & 0x000F000Fu) | 0x64006400u) + a); };
     auto odd = [&](uint32_t x) { return __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, (x & 0x00F000F0u) | 0x54005400u) + b); };
     return (u32x4){even(y), odd(y), even(z), odd(z)};
 }
 
-// N dwords at a lane's offset of a piece; past its end zeros.
-template <int N> struct Dwords {
-    uint32_t v[N];
-    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t d, int at) {
+// N dwords of LDS, W at a time.
+template <int N, int W> __device__ __forceinline__ void read_lds(uint32_t (&v)[N], uint32_t at) {
+    typedef uint32_t vec __attribute__((ext_vector_type(W)));
+    typedef const __attribute__((address_space(3))) vec *lp;
 #pragma unroll
-        for (int i = 0; i + 4 <= N; i += 4) {
-            const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(d, at + 4 * i, 0, 0);
-            v[i] = x.x, v[i + 1] = x.y, v[i + 2] = x.z, v[i + 3] = x.w;
-        }
-        constexpr int i = N & ~3;
-        if constexpr (N % 4 == 3) {
-            const u32x3 x = __builtin_amdgcn_raw_buffer_load_b96(d, at + 4 * i, 0, 0);
-            v[i] = x.x, v[i + 1] = x.y, v[i + 2] = x.z;
-        } else if constexpr (N % 4 == 2) {
-            const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(d, at + 4 * i, 0, 0);
-            v[i] = x.x, v[i + 1] = x.y;
-        } else if constexpr (N % 4 == 1) {
-            v[i] = __builtin_amdgcn_raw_buffer_load_b32(d, at + 4 * i, 0, 0);
+    for (int i = 0; i < N; i += W) {
+        if constexpr (W == 1) {
+            typedef const __attribute__((address_space(3))) uint32_t *up;
+            v[i] = *(up)(at + 4 * i);
+        } else {
+            const vec x = *(lp)(at + 4 * i);
+#pragma unroll
+            for (int j = 0; j < W; j++) v[i + j] = x[j];
         }
     }
-};
+}
 __device__ __forceinline__ float half_lo(uint32_t v) { return (float)__builtin_bit_cast(h2, v)[0]; }
 __device__ __forceinline__ float half_hi(uint32_t v) { return (float)__builtin_bit_cast(h2, v)[1]; }
 
 // A piece of sixteen places of one plane in a lane: its codes and the scales of its four places, [block][place].
 template <int NG> struct Piece4 {
-    Dwords<NG> codes;
-    Dwords<2 * NG> scales;
-    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t d) {
+    uint32_t codes[NG], scales[2 * NG];
+    __device__ __forceinline__ void read(uint32_t at) {
         const int lane = threadIdx.x & 63;
-        codes.load(d, 4 * NG * lane);
-        scales.load(d, 256 * NG + 8 * NG * (lane >> 4));
+        read_lds<NG, NG % 4 == 0 ? 4 : NG % 2 == 0 ? 2 : 1>(codes, at + 4 * NG * lane);
+        read_lds<2 * NG, NG % 2 == 0 ? 4 : 2>(scales, at + 256 * NG + 8 * NG * (lane >> 4));
     }
     __device__ __forceinline__ float scale(int b, int i) const {
-        const uint32_t v = scales.v[2 * b + (i >> 1)];
+        const uint32_t v = scales[2 * b + (i >> 1)];
         return i & 1 ? half_hi(v) : half_lo(v);
     }
 };
@@ -111,7 +121,7 @@ template <int NG> struct Acc4 {
     bool far;
 };
 
-template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves) void attn4_few(const AttnArgs p) {
+template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves, NG * NC <= 4 ? MINW_ : 1) void attn4_few(const AttnArgs p) {
     using S = Shape4<NG, NC>;
     constexpr bool TWO = !BF;
     extern __shared__ __attribute__((aligned(16))) float lds[];
@@ -183,17 +193,32 @@ template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves) voi
                                   (int64_t)((t & ((1 << p.page_log2) - 1)) >> 4) * (9 * S::DIM));
         return Where{off, uni(some ? 9 * S::DIM : 0)};
     };
-    auto load = [&](Piece4<NG> &x, const uint8_t *plane, const Where &at) {
-        x.load(__builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(plane + at.off), 0, at.bytes, 0x00020000));
+    const uint32_t ring = lds_addr(lds) + w * S::WAVE, voff = 16 * lane, voff4 = 4 * lane;
+    auto copy = [&](const uint8_t *plane, const Where &at, uint32_t to) {
+        const dma_rsrc d = dma_desc(plane + at.off, at.bytes);
+#pragma unroll
+        for (int i = 0; i < S::COPIES; i++) {
+            if (i < S::WHOLE || S::TAIL > 256) dma16(d, to + 1024 * i, voff, 1024 * i);
+            else dma4(d, to + 1024 * i, voff4, 1024 * i);
+        }
     };
-    int2 pages = pages_of(b0 + w);
-    Where at[2] = {where_of(b0 + w, 0, pages.x), where_of(b0 + w, 1, pages.y)};
-    Piece4<NG> k[2], v[2];
+    // Copies in flight behind the ones of a block's keys (or values): those of its values, and of SLOTS - 1 blocks.
+    constexpr int AHEAD = 4 * S::COPIES * S::SLOTS - 2 * S::COPIES;
+    Where at[2];
+    int2 pages[S::SLOTS + 1];
 #pragma unroll
-    for (int h = 0; h < 2; h++) load(k[h], p.k, at[h]);
+    for (int i = 0; i <= S::SLOTS; i++) pages[i] = pages_of(b0 + w + i * kWaves);
 #pragma unroll
-    for (int h = 0; h < 2; h++) load(v[h], p.v, at[h]);
-    pages = pages_of(b0 + w + kWaves);
+    for (int i = 0; i < S::SLOTS; i++) {
+        const int b = b0 + w + i * kWaves;
+        at[0] = where_of(b, 0, pages[i].x), at[1] = where_of(b, 1, pages[i].y);
+#pragma unroll
+        for (int h = 0; h < 2; h++) copy(p.k, at[h], ring + i * S::SLOT + h * S::PIECE);
+#pragma unroll
+        for (int h = 0; h < 2; h++) copy(p.v, at[h], ring + i * S::SLOT + (2 + h) * S::PIECE);
+    }
+    int2 page = pages[S::SLOTS];
+    uint32_t slot = ring;
 
     Acc4<NG> A[NC];
 #pragma unroll
@@ -209,14 +234,21 @@ template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves) voi
 
     for (int b = b0 + w; b < b1; b += kWaves) {
         const int t = key_of(b);
-        const Where next[2] = {where_of(b + kWaves, 0, pages.x), where_of(b + kWaves, 1, pages.y)};
-        pages = pages_of(b + 2 * kWaves);
+        const Where next[2] = {where_of(b + S::SLOTS * kWaves, 0, page.x), where_of(b + S::SLOTS * kWaves, 1, page.y)};
+        page = pages_of(b + (S::SLOTS + 1) * kWaves);
+        Piece4<NG> k[2], v[2];
+        wait_vmcnt(AHEAD);
+#pragma unroll
+        for (int h = 0; h < 2; h++) k[h].read(slot + h * S::PIECE);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the keys' part of the slot has been read
+#pragma unroll
+        for (int h = 0; h < 2; h++) copy(p.k, next[h], slot + h * S::PIECE);
         float x[NC][8];
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
             for (int g = 0; g < NG; g++) {
-                const u32x4 a = open8(k[h].codes.v[g]);
+                const u32x4 a = open8(k[h].codes[g]);
 #pragma unroll
                 for (int s = 0; s < NC; s++) {
                     const f4 d = mma16(a, q[s][g], (f4){0, 0, 0, 0});
@@ -224,18 +256,23 @@ template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves) voi
                     for (int i = 0; i < 4; i++) x[s][4 * h + i] = g == 0 ? k[h].scale(g, i) * d[i] : fmaf(k[h].scale(g, i), d[i], x[s][4 * h + i]);
                 }
             }
+        wait_vmcnt(AHEAD);
 #pragma unroll
-        for (int h = 0; h < 2; h++) load(k[h], p.k, next[h]);
-        // the scales of the values: larger ones than so far, and ones that are not finite
+        for (int h = 0; h < 2; h++) v[h].read(slot + (2 + h) * S::PIECE);
+        // the scales of the values, a few a lane: larger ones than so far, and ones that are not finite
         uint32_t big = 0;
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+        for (int i = lane; i < 16 * NG; i += 64) {
+            typedef const __attribute__((address_space(3))) uint32_t *up;
+            const int h = i >= 8 * NG, j = i - h * 8 * NG;
+            const uint32_t a = *(up)(slot + (2 + h) * S::PIECE + 256 * NG + 4 * j) & 0x7FFF7FFFu;
+            big = big > (a & 0xFFFFu) ? big : a & 0xFFFFu;
+            big = big > (a >> 16) ? big : a >> 16;
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the values' part has been read
 #pragma unroll
-            for (int i = 0; i < 2 * NG; i++) {
-                const uint32_t a = v[h].scales.v[i] & 0x7FFF7FFFu;
-                big = big > (a & 0xFFFFu) ? big : a & 0xFFFFu;
-                big = big > (a >> 16) ? big : a >> 16;
-            }
+        for (int h = 0; h < 2; h++) copy(p.v, next[h], slot + (2 + h) * S::PIECE);
+        slot = slot + S::SLOT == ring + S::RING ? ring : slot + S::SLOT;
         const bool all = t + kBlock - 1 <= hi_min && (t >= lo_max || t + kBlock <= p.sinks);
         if (__any(big > limit)) {
             uint32_t finite = 0;
@@ -246,7 +283,7 @@ template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves) voi
                 for (int h = 0; h < 2; h++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        uint32_t &d = v[h].scales.v[2 * g + (i >> 1)];
+                        uint32_t &d = v[h].scales[2 * g + (i >> 1)];
                         const int sh = 16 * (i & 1);
                         const uint32_t u = d >> sh & 0x7FFFu;
                         if (u < 0x7C00u) {
@@ -345,7 +382,7 @@ template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves) voi
         }
 #pragma unroll
         for (int g = 0; g < NG; g++) {
-            const u32x4 y = open8(v[0].codes.v[g]), z = open8(v[1].codes.v[g]), a0 = {y.x, y.z, z.x, z.z}, a1 = {y.y, y.w, z.y, z.w};
+            const u32x4 y = open8(v[0].codes[g]), z = open8(v[1].codes[g]), a0 = {y.x, y.z, z.x, z.z}, a1 = {y.y, y.w, z.y, z.w};
 #pragma unroll
             for (int s = 0; s < NC; s++) {
                 u32x4 hi, lo;
@@ -367,12 +404,11 @@ template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves) voi
                 }
             }
         }
-#pragma unroll
-        for (int h = 0; h < 2; h++) load(v[h], p.v, next[h]);
     }
-    // the four waves' results, through LDS
+    wait_vmcnt(0);
+    // the four waves' results, through LDS: rows, then references and sums
     float *mine = lds + w * (S::WAVE / 4);
-    float2 *ml = reinterpret_cast<float2 *>(lds + kWaves * (S::WAVE / 4));
+    auto ml = [&](int u) { return reinterpret_cast<float2 *>(lds + u * (S::WAVE / 4) + S::ROWS * S::OSTRIDE); };
 #pragma unroll
     for (int s = 0; s < NC; s++) {
         const float l = row_sum(A[s].l);
@@ -385,7 +421,7 @@ template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves) voi
             *reinterpret_cast<float4 *>(dst) = make_float4(a[0], b[0], a[1], b[1]);
             *reinterpret_cast<float4 *>(dst + 4) = make_float4(a[2], b[2], a[3], b[3]);
         }
-        if (quarter == 0) ml[w * S::ROWS + r] = make_float2(A[s].m, l);
+        if (quarter == 0) ml(w)[r] = make_float2(A[s].m, l);
     }
     __syncthreads();
     const bool direct = it.nsplit == 1;
@@ -396,7 +432,8 @@ template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves) voi
 #pragma unroll
         for (int u = 0; u < kWaves; u++) {
             const float4 o = *reinterpret_cast<const float4 *>(lds + u * (S::WAVE / 4) + r * S::OSTRIDE + d);
-            j.add(ml[u * S::ROWS + r].x, ml[u * S::ROWS + r].y, o.x, o.y, o.z, o.w);
+            const float2 y = ml(u)[r];
+            j.add(y.x, y.y, o.x, o.y, o.z, o.w);
         }
         if (direct) {
             put4<BF>(p, it.q0, row, it.head, d, j.o, j.l, keys - it.nq + tok >= 0);
@@ -408,8 +445,8 @@ template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves) voi
         }
     }
     if (direct) return;
-    if (last_piece(p, it, reinterpret_cast<int *>(ml + kWaves * S::ROWS)))
-        join_tile<S::DIM, S::ROWS, BF, kWaves>(p, it, r0, n, lds, kWaves * S::WAVE);
+    if (last_piece(p, it, reinterpret_cast<int *>(lds)))
+        join_tile<S::DIM, S::ROWS, BF, kWaves>(p, it, r0, n, lds + 4, S::BYTES - 16);
 }
 
 template <int NG, int NC, bool BF> int launch_few(trhip_ctx *ctx, const AttnArgs &p, int64_t grid) {
@@ -492,7 +529,7 @@ int launch_kv4_attn(trhip_ctx *ctx, const trhip_kv4 *kv, const AttnCall &c, int 
         st = launch_attn(ctx, &open, lc);
         if (st != TRHIP_OK) return st;
     }
-    p.target = cus * 2;
+    p.target = cus * PERCU_;
     p.row_lo = 0;
     p.row_hi = image ? kTokMost : kAnyRows;
     const int sets = (p.row_hi != kAnyRows || most_new * p.group > 16) && kv->dim <= 32 * kTwoSets ? 2 : 1, rows = 16 * sets;
