@@ -67,14 +67,23 @@ __device__ __forceinline__ float row_sum(float x) {
     return half_sum(__uint_as_float(s[0]) + __uint_as_float(s[1]));
 }
 
-// The f16 operand c - 8 of a dword's eight codes: nibbles 0 and 4, 1 and 5, 2 and 6, 3 and 7.
-__device__ __forceinline__ u32x4 open8(uint32_t y) {
-    const uint32_t z = y >> 8, m0 = 0x000F000Fu, e0 = 0x64006400u, m1 = 0x00F000F0u, e1 = 0x54005400u;
-    const h2 a = {(_Float16)-1032.0f, (_Float16)-1032.0f}, b = {(_Float16)-72.0f, (_Float16)-72.0f};
-    auto even = [&](uint32_t x) { return __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, (x & 0x000F000Fu) | 0x64006400u) + a); };
-    auto odd = [&](uint32_t x) { return __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, (x & 0x00F000F0u) | 0x54005400u) + b); };
-    return (u32x4){even(y), odd(y), even(z), odd(z)};
-}
+// The f16 operand c - 8 of a dword's eight codes: nibbles 0 and 4, 1 and 5, 2 and 6, 3 and 7. (The constants are hidden, so that they stay
+// in registers: an instruction that masks and sets takes no constants of its own.)
+struct Open8 {
+    uint32_t even_bits, even_one, odd_bits, odd_one;
+    __device__ __forceinline__ void init() {
+        even_bits = 0x000F000Fu, odd_bits = 0x00F000F0u, even_one = 0x64006400u, odd_one = 0x54005400u;
+        asm("" : "+s"(even_bits), "+s"(odd_bits));
+        asm("" : "+v"(even_one), "+v"(odd_one));
+    }
+    __device__ __forceinline__ u32x4 operator()(uint32_t y) const {
+        const uint32_t z = y >> 8;
+        const h2 a = {(_Float16)-1032.0f, (_Float16)-1032.0f}, b = {(_Float16)-72.0f, (_Float16)-72.0f};
+        auto even = [&](uint32_t x) { return __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, (x & even_bits) | even_one) + a); };
+        auto odd = [&](uint32_t x) { return __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, (x & odd_bits) | odd_one) + b); };
+        return (u32x4){even(y), odd(y), even(z), odd(z)};
+    }
+};
 
 // N dwords of LDS, W at a time.
 template <int N, int W> __device__ __forceinline__ void read_lds(uint32_t (&v)[N], uint32_t at) {
@@ -220,6 +229,8 @@ template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves, NG 
     int2 page = pages[S::SLOTS];
     uint32_t slot = ring;
 
+    Open8 open8;
+    open8.init();
     Acc4<NG> A[NC];
 #pragma unroll
     for (int s = 0; s < NC; s++) {
@@ -253,7 +264,7 @@ template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves, NG 
                 for (int s = 0; s < NC; s++) {
                     const f4 d = mma16(a, q[s][g], (f4){0, 0, 0, 0});
 #pragma unroll
-                    for (int i = 0; i < 4; i++) x[s][4 * h + i] = g == 0 ? k[h].scale(g, i) * d[i] : fmaf(k[h].scale(g, i), d[i], x[s][4 * h + i]);
+                    for (int i = 0; i < 4; i++) x[s][4 * h + i] = fmaf(k[h].scale(g, i), d[i], g == 0 ? 0.0f : x[s][4 * h + i]);
                 }
             }
         wait_vmcnt(AHEAD);
@@ -275,35 +286,38 @@ template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves, NG 
         slot = slot + S::SLOT == ring + S::RING ? ring : slot + S::SLOT;
         const bool all = t + kBlock - 1 <= hi_min && (t >= lo_max || t + kBlock <= p.sinks);
         if (__any(big > limit)) {
-            uint32_t finite = 0;
+            uint32_t finite = big;
+            if (__any(big >= 0x7C00u)) {
+                finite = 0;
 #pragma unroll
-            for (int g = 0; g < NG; g++) {
-                bool bad[NC] = {};
+                for (int g = 0; g < NG; g++) {
+                    bool bad[NC] = {};
 #pragma unroll
-                for (int h = 0; h < 2; h++)
+                    for (int h = 0; h < 2; h++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        uint32_t &d = v[h].scales[2 * g + (i >> 1)];
-                        const int sh = 16 * (i & 1);
-                        const uint32_t u = d >> sh & 0x7FFFu;
-                        if (u < 0x7C00u) {
-                            finite = finite > u ? finite : u;
-                        } else {  // it reaches the rows that see it, and no other
-                            const int key = t + 16 * h + 4 * quarter + i;
+                        for (int i = 0; i < 4; i++) {
+                            uint32_t &d = v[h].scales[2 * g + (i >> 1)];
+                            const int sh = 16 * (i & 1);
+                            const uint32_t u = d >> sh & 0x7FFFu;
+                            if (u < 0x7C00u) {
+                                finite = finite > u ? finite : u;
+                            } else {  // it reaches the rows that see it, and no other
+                                const int key = t + 16 * h + 4 * quarter + i;
 #pragma unroll
-                            for (int s = 0; s < NC; s++) bad[s] = bad[s] || (key <= rows[s].hi && (key >= rows[s].lo || key < p.sinks));
-                            d &= ~(0xFFFFu << sh);
+                                for (int s = 0; s < NC; s++) bad[s] = bad[s] || (key <= rows[s].hi && (key >= rows[s].lo || key < p.sinks));
+                                d &= ~(0xFFFFu << sh);
+                            }
                         }
-                    }
 #pragma unroll
-                for (int s = 0; s < NC; s++) {
-                    const float nan = row_max(bad[s] ? 1.0f : 0.0f) > 0.0f ? __builtin_nanf("") : 0.0f;
-                    A[s].o[g][0] += nan;
-                    A[s].o[g][1] += nan;
+                    for (int s = 0; s < NC; s++) {
+                        const float nan = row_max(bad[s] ? 1.0f : 0.0f) > 0.0f ? __builtin_nanf("") : 0.0f;
+                        A[s].o[g][0] += nan;
+                        A[s].o[g][1] += nan;
+                    }
                 }
             }
-            float top = row_max(__uint_as_float(finite << 13) * 0x1p112f);  // f16's bits as fp32's: exact, subnormal ones too
-            top = fmaxf(top, __shfl_xor(top, 1));
+            // (f16's bits as fp32's: exact, subnormal ones too)
+            const float top = __uint_as_float(__builtin_amdgcn_readlane(scan64((int)(finite << 13), 0, [](int a, int b) { return a > b ? a : b; }), 63)) * 0x1p112f;
             if (uni(__float_as_uint(top)) > __float_as_uint(ldexpf(1.0f, tl))) {
                 const uint32_t u = uni(__float_as_uint(top));
                 const int to = (int)(u >> 23) - 127 + ((u & 0x7FFFFFu) != 0), by = to - tl;
@@ -390,7 +404,7 @@ template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves, NG 
                 for (int i = 0; i < 4; i++) {
                     const int h = i >> 1, j = 2 * (i & 1);
                     const float e0 = x[s][4 * h + j], e1 = x[s][4 * h + j + 1], d0 = v[h].scale(g, j), d1 = v[h].scale(g, j + 1);
-                    hi[i] = __builtin_bit_cast(uint32_t, (h2){(_Float16)(e0 * d0), (_Float16)(e1 * d1)});
+                    hi[i] = __builtin_bit_cast(uint32_t, (h2){(_Float16)fmaf(e0, d0, 0.0f), (_Float16)fmaf(e1, d1, 0.0f)});  // (fused: with the rounding in one instruction)
                     // (hidden: the compiler would round the products anew for the second term, in another way)
                     if (TWO) hi[i] = hide(hi[i]);
                     const h2 f = __builtin_bit_cast(h2, (uint32_t)hi[i]);
