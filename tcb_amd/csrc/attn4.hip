@@ -28,16 +28,9 @@ typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 constexpr int kTwoSets = 4;  // blocks of elements up to which a workgroup's registers hold two sets of rows
 constexpr int64_t kMostImage = (int64_t)2 << 30;  // bytes of a plane of opened keys at most: a hundredth of the memory
 constexpr int kWaves = 4, kBlock = 32, kLeast = 8, kOver = 6;
-#ifndef SLOTS_
-#define SLOTS_ 2
-#endif
-#ifndef MINW_
-#define MINW_ 3
-#endif
-#ifndef PERCU_
-#define PERCU_ 3
-#endif
-constexpr int kSlots = SLOTS_;
+
+// Workgroups a CU, by registers (blocks: 32-element blocks of a row times sets of rows).
+constexpr int per_cu(int blocks) { return blocks <= 4 ? 3 : blocks <= 8 ? 2 : 1; }
 
 template <int NG, int NC> struct Shape4 {
     static constexpr int DIM = 32 * NG, ROWS = 16 * NC;
@@ -45,7 +38,7 @@ template <int NG, int NC> struct Shape4 {
     static constexpr int BYTES_IN = 288 * NG, WHOLE = BYTES_IN / 1024, TAIL = BYTES_IN % 1024, COPIES = WHOLE + (TAIL > 0);
     static constexpr int PIECE = WHOLE * 1024 + (TAIL == 0 ? 0 : TAIL <= 256 ? 256 : 1024);
     static constexpr int SLOT = 4 * PIECE;  // a block's two pieces of keys and two of values
-    static constexpr int SLOTS = NG == 8 ? 2 : NG >= 5 ? 2 : kSlots;
+    static constexpr int SLOTS = 2;
     static constexpr int OSTRIDE = DIM + 4;  // floats between rows of a wave's results
     static constexpr int RING = SLOTS * SLOT, OUT = ROWS * (OSTRIDE * 4 + 8);
     static constexpr int WAVE = RING > OUT ? RING : OUT;
@@ -130,7 +123,7 @@ template <int NG> struct Acc4 {
     bool far;
 };
 
-template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves, NG * NC <= 4 ? MINW_ : 1) void attn4_few(const AttnArgs p) {
+template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves, per_cu(NG * NC)) void attn4_few(const AttnArgs p) {
     using S = Shape4<NG, NC>;
     constexpr bool TWO = !BF;
     extern __shared__ __attribute__((aligned(16))) float lds[];
@@ -543,10 +536,10 @@ int launch_kv4_attn(trhip_ctx *ctx, const trhip_kv4 *kv, const AttnCall &c, int 
         st = launch_attn(ctx, &open, lc);
         if (st != TRHIP_OK) return st;
     }
-    p.target = cus * PERCU_;
     p.row_lo = 0;
     p.row_hi = image ? kTokMost : kAnyRows;
-    const int sets = (p.row_hi != kAnyRows || most_new * p.group > 16) && kv->dim <= 32 * kTwoSets ? 2 : 1, rows = 16 * sets;
+    const int sets = (p.row_hi != kAnyRows || most_new * p.group > 16) && kv->dim <= 32 * kTwoSets ? 2 : 1, rows = 16 * sets, blocks = kv->dim / 32 * sets;
+    p.target = cus * per_cu(blocks);
     const int64_t grid = plan_items(p, c, rows, kBlock, kLeast);
     if (grid >= ((int64_t)1 << 31)) return fail(ctx, TRHIP_ERR_INVALID, "kv4_attn: too many rows");
     int st = TRHIP_OK;
