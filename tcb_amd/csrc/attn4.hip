@@ -100,10 +100,9 @@ __device__ __forceinline__ float half_hi(uint32_t v) { return (float)__builtin_b
 // A piece of sixteen places of one plane in a lane: its codes and the scales of its four places, [block][place].
 template <int NG> struct Piece4 {
     uint32_t codes[NG], scales[2 * NG];
-    __device__ __forceinline__ void read(uint32_t at) {
-        const int lane = threadIdx.x & 63;
-        read_lds<NG, NG % 4 == 0 ? 4 : NG % 2 == 0 ? 2 : 1>(codes, at + 4 * NG * lane);
-        read_lds<2 * NG, NG % 2 == 0 ? 4 : 2>(scales, at + 256 * NG + 8 * NG * (lane >> 4));
+    __device__ __forceinline__ void read(uint32_t at, uint32_t scales_at) {  // this lane's part of the codes, its quarter's of the scales
+        read_lds<NG, NG % 4 == 0 ? 4 : NG % 2 == 0 ? 2 : 1>(codes, at);
+        read_lds<2 * NG, NG % 2 == 0 ? 4 : 2>(scales, scales_at + 256 * NG);
     }
     __device__ __forceinline__ float scale(int b, int i) const {
         const uint32_t v = scales[2 * b + (i >> 1)];
@@ -177,27 +176,31 @@ template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves, per
         }
     }
 
-    // Block b's two pages, fetched a step before they are used, and its two pieces' bytes; past the last block nothing but zeros.
+    // Where the pieces lie: a lane has the byte offset of one of the next 64 pieces that this wave takes (two a block), negative for one that
+    // no row sees or whose page is out of range, and past the last block. (As scalars, piece by piece, they took half as many instructions
+    // as all the rest of a block.)
     auto key_of = [&](int b) { return kBlock * sp.block(b); };
-    auto pages_of = [&](int b) {
-        const int t = b < b1 ? key_of(b) : 0, hi = b < b1 ? hi_max : -1;
-        return make_int2(page16(p, table, t, hi), page16(p, table, t + 16, hi));
+    uint32_t off_lo = 0, off_hi = 0;
+    auto place = [&](int i) {  // from the wave's i-th block on
+        const int b = b0 + w + (i + (lane >> 1)) * kWaves, t = key_of(b < b1 ? b : b0) + 16 * (lane & 1);
+        const bool some = b < b1 && t <= hi_max && !(p.sinks <= t && lo_min >= t + 16);
+        const int page = some ? table[t >> p.page_log2] : -1;
+        int64_t off = (int64_t)page * p.page_bytes + (int64_t)it.head * p.head_bytes + (int64_t)((t & ((1 << p.page_log2) - 1)) >> 4) * (9 * S::DIM);
+        if ((uint32_t)page >= (uint32_t)p.npages) off = -1;
+        off_lo = (uint32_t)off, off_hi = (uint32_t)(off >> 32);
     };
     struct Where {
-        int64_t off;
-        int bytes;
+        uint32_t lo, hi, bytes;
     };
-    auto where_of = [&](int b, int half, int page) {
-        const int t = (b < b1 ? key_of(b) : 0) + 16 * half;
-        bool some = b < b1 && t <= hi_max && !(p.sinks <= t && lo_min >= t + 16);
-        if ((uint32_t)page >= (uint32_t)p.npages) page = 0, some = false;
-        const int64_t off = uni64((int64_t)page * p.page_bytes + (int64_t)it.head * p.head_bytes +
-                                  (int64_t)((t & ((1 << p.page_log2) - 1)) >> 4) * (9 * S::DIM));
-        return Where{off, uni(some ? 9 * S::DIM : 0)};
+    auto where_of = [&](int i, int half) {
+        const int at = (2 * i + half) & 63;
+        Where x = {(uint32_t)__builtin_amdgcn_readlane((int)off_lo, at), (uint32_t)__builtin_amdgcn_readlane((int)off_hi, at), 0};
+        x.bytes = (uint32_t)(9 * S::DIM) & ~(uint32_t)((int)x.hi >> 31);
+        return x;
     };
     const uint32_t ring = lds_addr(lds) + w * S::WAVE, voff = 16 * lane, voff4 = 4 * lane;
     auto copy = [&](const uint8_t *plane, const Where &at, uint32_t to) {
-        const dma_rsrc d = dma_desc(plane + at.off, at.bytes);
+        const dma_rsrc d = dma_desc(plane + (int64_t)(((uint64_t)at.hi << 32) | at.lo), at.bytes);
 #pragma unroll
         for (int i = 0; i < S::COPIES; i++) {
             if (i < S::WHOLE || S::TAIL > 256) dma16(d, to + 1024 * i, voff, 1024 * i);
@@ -206,20 +209,15 @@ template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves, per
     };
     // Copies in flight behind the ones of a block's keys (or values): those of its values, and of SLOTS - 1 blocks.
     constexpr int AHEAD = 4 * S::COPIES * S::SLOTS - 2 * S::COPIES;
-    Where at[2];
-    int2 pages[S::SLOTS + 1];
-#pragma unroll
-    for (int i = 0; i <= S::SLOTS; i++) pages[i] = pages_of(b0 + w + i * kWaves);
+    place(0);
 #pragma unroll
     for (int i = 0; i < S::SLOTS; i++) {
-        const int b = b0 + w + i * kWaves;
-        at[0] = where_of(b, 0, pages[i].x), at[1] = where_of(b, 1, pages[i].y);
+        const Where at[2] = {where_of(i, 0), where_of(i, 1)};
 #pragma unroll
         for (int h = 0; h < 2; h++) copy(p.k, at[h], ring + i * S::SLOT + h * S::PIECE);
 #pragma unroll
         for (int h = 0; h < 2; h++) copy(p.v, at[h], ring + i * S::SLOT + (2 + h) * S::PIECE);
     }
-    int2 page = pages[S::SLOTS];
     uint32_t slot = ring;
 
     Open8 open8;
@@ -236,14 +234,16 @@ template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves, per
     int tl = -24;                // the values' scales met so far are at most 2^tl,
     uint32_t limit = 0x0001u;    // in f16
 
-    for (int b = b0 + w; b < b1; b += kWaves) {
+    int turn = S::SLOTS;  // the wave's block whose copies are next
+    for (int b = b0 + w; b < b1; b += kWaves, turn++) {
         const int t = key_of(b);
-        const Where next[2] = {where_of(b + S::SLOTS * kWaves, 0, page.x), where_of(b + S::SLOTS * kWaves, 1, page.y)};
-        page = pages_of(b + (S::SLOTS + 1) * kWaves);
+        if ((turn & 31) == 0) place(turn);
+        const Where next[2] = {where_of(turn, 0), where_of(turn, 1)};
         Piece4<NG> k[2], v[2];
+        const uint32_t at = slot + 4 * NG * lane, scales_at = slot + 8 * NG * quarter;
         wait_vmcnt(AHEAD);
 #pragma unroll
-        for (int h = 0; h < 2; h++) k[h].read(slot + h * S::PIECE);
+        for (int h = 0; h < 2; h++) k[h].read(at + h * S::PIECE, scales_at + h * S::PIECE);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the keys' part of the slot has been read
 #pragma unroll
         for (int h = 0; h < 2; h++) copy(p.k, next[h], slot + h * S::PIECE);
@@ -262,7 +262,7 @@ template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves, per
             }
         wait_vmcnt(AHEAD);
 #pragma unroll
-        for (int h = 0; h < 2; h++) v[h].read(slot + (2 + h) * S::PIECE);
+        for (int h = 0; h < 2; h++) v[h].read(at + (2 + h) * S::PIECE, scales_at + (2 + h) * S::PIECE);
         // the scales of the values, a few a lane: larger ones than so far, and ones that are not finite
         uint32_t big = 0;
 #pragma unroll
