@@ -52,13 +52,13 @@ __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k &
 struct Row {
     const void *x;
     int io, vocab, wide;
-    __device__ __forceinline__ uint32_t key(int i) const {
-        return key_of(io == TRHIP_F32 ? static_cast<const float *>(x)[i] : h16_to_f32(static_cast<const uint16_t *>(x)[i], io));
+    __device__ __forceinline__ float value(int i) const {
+        return io == TRHIP_F32 ? static_cast<const float *>(x)[i] : h16_to_f32(static_cast<const uint16_t *>(x)[i], io);
     }
-    // entries i .. i + 3 (i a multiple of 4); 0 past the last
-    __device__ __forceinline__ void keys4(int i, uint32_t (&k)[4]) const {
+    __device__ __forceinline__ uint32_t key(int i) const { return key_of(value(i)); }
+    // entries i .. i + 3 (i a multiple of 4); NaN past the last
+    __device__ __forceinline__ void values4(int i, float (&f)[4]) const {
         if (wide && i + 4 <= vocab) {
-            float f[4];
             if (io == TRHIP_F32) {
                 *reinterpret_cast<float4 *>(f) = *reinterpret_cast<const float4 *>(static_cast<const float *>(x) + i);
             } else {
@@ -66,12 +66,17 @@ struct Row {
                 f[0] = h16_to_f32(y.x & 0xFFFFu, io), f[1] = h16_to_f32(y.x >> 16, io);
                 f[2] = h16_to_f32(y.y & 0xFFFFu, io), f[3] = h16_to_f32(y.y >> 16, io);
             }
-#pragma unroll
-            for (int u = 0; u < 4; u++) k[u] = key_of(f[u]);
         } else {
 #pragma unroll
-            for (int u = 0; u < 4; u++) k[u] = i + u < vocab ? key(i + u) : 0;
+            for (int u = 0; u < 4; u++) f[u] = i + u < vocab ? value(i + u) : __builtin_nanf("");
         }
+    }
+    // and their keys, 0 past the last
+    __device__ __forceinline__ void keys4(int i, uint32_t (&k)[4]) const {
+        float f[4];
+        values4(i, f);
+#pragma unroll
+        for (int u = 0; u < 4; u++) k[u] = key_of(f[u]);
     }
 };
 
@@ -122,7 +127,7 @@ __device__ __forceinline__ Setting setting_of(const SampleArgs &p, int r) {
 }
 // How many entries of the whole row its workgroups should cover, and a workgroup's share of them: the mean, four standard deviations of
 // entries that lie anywhere, and six.
-constexpr int kCover = 160;
+constexpr int kCover = 128;
 __device__ __forceinline__ int share_of(int n, int groups) {
     const float m = (float)n * __builtin_amdgcn_rcpf((float)groups);
     const int s = (int)(m + 4.0f * __builtin_amdgcn_sqrtf(m) + 6.0f);
@@ -226,7 +231,7 @@ template <int J> __global__ __launch_bounds__(kRead) void sample_read(const Samp
 #pragma unroll
                 for (int v = 0; v < 4; v++) {
                     const int b = first - bin_of(key[j][v], per);
-                    if (key[j][v] != 0) atomicAdd(&s_bins[b < kBins ? b : kBins - 1], (unsigned long long)rint(y[v] * 0x1p48));
+                    if (key[j][v] != 0 && b < kBins) atomicAdd(&s_bins[b], (unsigned long long)rint(y[v] * 0x1p48));
                 }
             }
             const double sum = wave_sum((y[0] + y[1]) + (y[2] + y[3]));
@@ -235,10 +240,10 @@ template <int J> __global__ __launch_bounds__(kRead) void sample_read(const Samp
     }
     if (filtered && top != 0) {
         const int share = share_of(st.k > 0 ? st.k : kCover, p.groups);
-        if (share * 11 / 10 * p.groups > kMost || share * 5 / 4 + 8 > p.room) {  // (too many to sort)
+        if ((share + share / 6 + 3) * p.groups > kMost || share * 5 / 4 + 8 > p.room) {  // (too many to sort)
             left = 0xFFFFFFFFu;
         } else {
-            // a threshold that `share` to share * 9 / 8 threads' maxima reach: halving between the smallest and the largest
+            // a threshold that `share` to share * 9 / 8 + 2 threads' maxima reach: halving between the smallest and the largest
             auto count = [&](uint32_t k) {
                 int n = 0;
 #pragma unroll
@@ -254,7 +259,7 @@ template <int J> __global__ __launch_bounds__(kRead) void sample_read(const Samp
                     const int n = count(mid);
                     if (n >= share) {
                         lo = mid;
-                        if (n <= share + share / 8) break;
+                        if (n <= share + share / 8 + 2) break;
                     } else {
                         hi = mid - 1;
                     }
@@ -262,18 +267,25 @@ template <int J> __global__ __launch_bounds__(kRead) void sample_read(const Samp
             }
             bound = lo;
             unsigned long long *to = p.list + ((int64_t)r * p.groups + g) * p.room;
+            uint32_t n = 0;
 #pragma unroll
             for (int j = 0; j < J; j++)
 #pragma unroll
-                for (int v = 0; v < 4; v++) {
-                    const bool is = key[j][v] != 0 && key[j][v] >= bound;
-                    const uint64_t m = __ballot(is);
-                    if (m == 0) continue;
-                    uint32_t at = 0;
-                    if (lane == 0) at = atomicAdd(&s_left, (uint32_t)__popcll(m));
-                    at = __builtin_amdgcn_readfirstlane(at) + __popcll(m & (((uint64_t)1 << lane) - 1));
-                    if (is && at < (uint32_t)p.room) to[at] = ((unsigned long long)key[j][v] << 32) | (uint32_t)~(stripe(j) * kStripe + 4 * lane + v);
-                }
+                for (int v = 0; v < 4; v++) n += key[j][v] != 0 && key[j][v] >= bound;
+            const uint32_t incl = running(n);
+            uint32_t base = 0;
+            if (lane == 63 && incl != 0) base = atomicAdd(&s_left, incl);
+            uint32_t at = of_lane(base, 63) + (incl - n);
+            if (n != 0) {
+#pragma unroll
+                for (int j = 0; j < J; j++)
+#pragma unroll
+                    for (int v = 0; v < 4; v++)
+                        if (key[j][v] != 0 && key[j][v] >= bound) {
+                            if (at < (uint32_t)p.room) to[at] = ((unsigned long long)key[j][v] << 32) | (uint32_t)~(stripe(j) * kStripe + 4 * lane + v);
+                            at++;
+                        }
+            }
         }
     }
     __syncthreads();
@@ -445,7 +457,7 @@ __device__ __forceinline__ bool top64(const SampleArgs &p, int r, const Weight &
         else hi = mid - 1;
     }
     if (count > 64) return false;
-    unsigned long long *some = reinterpret_cast<unsigned long long *>(s.weight);
+    unsigned long long *some = s.bins;
     int at = 0;
 #pragma unroll
     for (int i = 0; i < PER; i++) {
@@ -500,12 +512,23 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
     const Row x = {static_cast<const char *>(p.logits) + r * p.stride * (p.io == TRHIP_F32 ? 4 : 2), p.io, p.vocab, p.wide};
     const uint4 *lefts = p.left + (int64_t)r * p.groups;
     static_assert(kEnd == kMost, "an entry, a workgroup or a stripe a thread");
-    uint4 left = {0, 0, 0, 0};
-    if (tid < p.groups) left = lefts[tid];
+    // every wave goes through all workgroups' records: the row's largest key, the key from which up every entry has been left by
+    // its workgroup, how many a workgroup left at most and all together, and how many those before each one
+    uint32_t top = 0, complete = 0, worst = 0, n_all = 0;
+    for (int g0 = 0; g0 < p.groups; g0 += 64) {
+        uint4 left = {0, 0, 0, 0};
+        if (g0 + lane < p.groups) left = lefts[g0 + lane];
+        const uint32_t a = wave_max(left.x), b = wave_max(left.y), c = wave_max(left.z), n = left.z < kMost ? left.z : kMost, sum = running(n);
+        top = top > a ? top : a;
+        complete = complete > b ? complete : b;
+        worst = worst > c ? worst : c;
+        if (w == 0 && g0 + lane < p.groups) s.from[g0 + lane] = n_all + (sum - n), s.count[g0 + lane] = n;
+        n_all += of_lane(sum, 63);
+    }
     const Setting st = setting_of(p, r);
     const bool filtered = st.k > 0 || st.tp < 1.0f || st.low > 0.0f;
     if (tid < 64) s.table[tid] = exp2((double)tid / 64.0);
-    const uint32_t top = all_max(left.x, s);
+    __syncthreads();
     if (top == 0) {
         if (tid == 0) {
             p.token[r] = -1;
@@ -514,45 +537,48 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
         return;
     }
     const Weight wt = {top, (double)of_key(top), st.greedy ? 1.0 : 1.0 / (double)st.t, s.table};
+    const bool weighed = !filtered || (st.k == 0 && st.tp < 1.0f);
     // the workgroups' largest logits' weights, by which theirs are multiplied
-    s.weight[tid] = left.x ? wt(left.x) : 0.0;
-    __syncthreads();
+    if (weighed) {
+        if (tid < p.groups) {
+            const uint32_t k = lefts[tid].x;
+            s.weight[tid] = k ? wt(k) : 0.0;
+        }
+        __syncthreads();
+    }
     auto mass = [&](int i) {
         const double unit = s.weight[i % p.groups];
         return unit > 0 ? p.mass[(int64_t)r * p.stripes + i] * unit : 0.0;
     };
     if (!filtered) return by_stripes(p, r, x, st.u, s, mass, [&](uint32_t key, uint32_t) { return wt(key); });
     double total = 0;
-    if (st.k == 0 && st.tp < 1.0f) {
+    if (weighed) {
         double sum = 0;
         for (int i = tid; i < p.stripes; i += kEnd) sum += mass(i);
         before_me(sum, s.wave, total);
     }
-    const uint32_t complete = all_max(left.y, s);  // every entry from here up has been left by its workgroup
-    const uint32_t worst = all_max(left.z > (uint32_t)p.room ? 0x7FFFFFFFu : left.z, s);
-    uint32_t n_all;
-    const uint32_t n_before = before_me(worst > kMost ? 0u : left.z, s.u, n_all);
     bool done = false;
-    if (worst <= kMost && n_all <= kMost) {
+    if (worst <= (uint32_t)p.room && n_all <= kMost) {
         const int n = (int)n_all;
-        s.from[tid] = n_before, s.count[tid] = tid < p.groups ? left.z : 0;
-        __syncthreads();
-        for (int i = tid; i < p.groups * p.room; i += kEnd) {
-            const int g = i / p.room, slot = i - g * p.room;
-            if ((uint32_t)slot < s.count[g]) s.sorted[s.from[g] + slot] = p.list[((int64_t)r * p.groups + g) * p.room + slot];
+        // (a wave a workgroup's entries; two at a time, so that their loads are in flight together)
+        for (int g = w; g < p.groups; g += 2 * kWaves) {
+            const int g1 = g + kWaves < p.groups ? g + kWaves : g;
+            const uint32_t n0 = s.count[g], n1 = g1 != g ? s.count[g1] : 0, f0 = s.from[g], f1 = s.from[g1];
+            const unsigned long long *l0 = p.list + ((int64_t)r * p.groups + g) * p.room, *l1 = p.list + ((int64_t)r * p.groups + g1) * p.room;
+            for (uint32_t i = lane; i < (n0 > n1 ? n0 : n1); i += 64) {
+                const unsigned long long e0 = i < n0 ? l0[i] : 0, e1 = i < n1 ? l1[i] : 0;
+                if (i < n0) s.sorted[f0 + i] = e0;
+                if (i < n1) s.sorted[f1 + i] = e1;
+            }
         }
         __syncthreads();
         if (st.k <= 64) {
-            const double keep_weight = s.weight[tid];
-            __syncthreads();
             if (w == 0) {
                 const bool is = top64(p, r, wt, st, total, complete, n, s);
                 if (lane == 0) s.small[1] = is;
             }
             __syncthreads();
             if (s.small[1]) return;
-            s.weight[tid] = keep_weight;
-            __syncthreads();
         }
         {
             sort(s, n, true);
@@ -569,12 +595,13 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
             done = complete == 0 || !(kept > certain || (kept == certain && kept != st.k) || (st.k > 0 && st.tp < 1.0f && certain < st.k));
             if (done) {
                 // what is kept, by index
-                s.weight[tid] = y;
+                double *weights = reinterpret_cast<double *>(s.bins);
+                weights[tid] = y;
                 __syncthreads();
                 if (tid < kept) s.sorted[tid] = ((unsigned long long)(uint32_t)~(uint32_t)e << 32) | (uint32_t)tid;
                 sort(s, kept, false);
                 const unsigned long long by = tid < kept ? s.sorted[tid] : 0;
-                const double v = tid < kept ? s.weight[(uint32_t)by] : 0.0;
+                const double v = tid < kept ? weights[(uint32_t)by] : 0.0;
                 double kept_sum;
                 const double up = before_me(v, s.wave, kept_sum) + v, goal_u = st.u * kept_sum;
                 int t = first_of(tid < kept && up > goal_u, s);
@@ -584,26 +611,24 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
             }
         }
     }
-    // ---- read again: what is kept are the entries (key, then ~index) from `least` up, of weights from low up ----
-    unsigned long long least = 0;
+    // ---- read again: what is kept are the entries above `cut`, and of that value those up to index `last`; of weights from low up ----
+    float cut = -3.4028234663852886e38f;
+    int last = 0x7FFFFFFF;
     int bits = 62;
     while ((p.vocab - 1) >> (62 - bits)) bits--;
-    const double unit = __longlong_as_double((long long)(1023 + bits) << 52), per_unit = 1.0 / unit;
-    constexpr int AT = 2;
-    auto entry = [&](uint32_t key, int i) { return ((unsigned long long)key << 32) | (uint32_t)~i; };
-    auto each = [&](auto use) {  // use(first of four, keys) for every four entries, a wave's stripe after its other
+    const double unit = __longlong_as_double((long long)(1023 + bits) << 52);
+    constexpr int AT = 4;
+    auto kept_at = [&](float f, int i) { return f > cut || (f == cut && i <= last); };  // (values: NaN is never kept)
+    auto each = [&](auto use) {  // use(first of four, values) for every four entries, a wave's stripes one after the other
         for (int b0 = w; b0 < p.stripes; b0 += AT * kWaves) {
-            uint32_t k[AT][4];
+            float f[AT][4];
 #pragma unroll
-            for (int a = 0; a < AT; a++) {
-                if (b0 + a * kWaves < p.stripes) x.keys4((b0 + a * kWaves) * kStripe + 4 * lane, k[a]);
-                else k[a][0] = k[a][1] = k[a][2] = k[a][3] = 0;
-            }
+            for (int a = 0; a < AT; a++) x.values4(b0 + a * kWaves < p.stripes ? (b0 + a * kWaves) * kStripe + 4 * lane : p.vocab, f[a]);
 #pragma unroll
-            for (int a = 0; a < AT; a++)
-                if (b0 + a * kWaves < p.stripes) use(b0 + a * kWaves, k[a]);
+            for (int a = 0; a < AT; a++) use((b0 + a * kWaves) * kStripe + 4 * lane, f[a]);
         }
     };
+    auto finite = [](uint32_t k) { return k < 0x00800000u ? -3.4028234663852886e38f : of_key(k); };  // the smallest value of key k or above
     for (int phase = 0; phase < 2; phase++) {
         if (phase == 0 ? st.k == 0 : st.tp >= 1.0f) continue;
         const bool weigh = phase == 1;
@@ -615,13 +640,23 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
             const int first = bin_of(top, per);
             double mine[2] = {};
             static_assert(kBins == 2 * kEnd, "two bins a thread");
-            for (int g = 0; g < p.groups; g++) {
-                const double by = s.weight[g] * (unit * 0x1p-48);
-                if (by == 0) continue;
-                const int at = 2 * tid - (first - bin_of(lefts[g].x, per));
-                const unsigned long long *from = p.hist + ((int64_t)r * p.groups + g) * kBins;
-                if (at >= 0) mine[0] += (double)from[at] * by;
-                if (at >= -1) mine[1] += (double)from[at + 1] * by;
+            if (tid < p.groups) s.from[tid] = s.weight[tid] > 0 ? (uint32_t)(first - bin_of(lefts[tid].x, per)) : 0;
+            __syncthreads();
+            constexpr int GA = 8;
+            for (int g0 = 0; g0 < p.groups; g0 += GA) {
+                unsigned long long a[GA][2];
+                double by[GA];
+#pragma unroll
+                for (int v = 0; v < GA; v++) {
+                    const int g = g0 + v < p.groups ? g0 + v : g0;
+                    by[v] = g0 + v < p.groups ? s.weight[g] * (unit * 0x1p-48) : 0.0;
+                    const int at = 2 * tid - (int)s.from[g];
+                    const unsigned long long *from = p.hist + ((int64_t)r * p.groups + g) * kBins;
+                    a[v][0] = by[v] > 0 && at >= 0 && at < kBins ? from[at] : 0;
+                    a[v][1] = by[v] > 0 && at >= -1 && at < kBins - 1 ? from[at + 1] : 0;
+                }
+#pragma unroll
+                for (int v = 0; v < GA; v++) mine[0] += (double)a[v][0] * by[v], mine[1] += (double)a[v][1] * by[v];
             }
             goal = (double)st.tp * total * unit;
             double all;
@@ -629,9 +664,9 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
             const int t = first_of(mine[0] + mine[1] > 0 && run + (mine[0] + mine[1]) >= goal, s);
             __syncthreads();
             if (tid == (t < kEnd ? t : kEnd - 1)) {
-                const bool second = !(mine[0] > 0 && run + mine[0] >= goal);
+                const bool second = t == kEnd || !(mine[0] > 0 && run + mine[0] >= goal);
                 s.small[2] = (uint32_t)(2 * tid + second);
-                s.sum = second ? run + mine[0] : run;
+                s.sum = t == kEnd ? 0.0 : second ? run + mine[0] : run;
             }
             __syncthreads();
             const int bin = first - (int)s.small[2];
@@ -646,43 +681,49 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
                 }
                 return a;
             };
-            lo = (int)s.small[2] == kBins - 1 ? 1 : from_bin(bin);
-            hi = from_bin(bin + 1) - 1;
-            if (hi < lo) hi = lo;
+            if (t < kEnd) {  // (else the run ends below the bins: all keys)
+                lo = from_bin(bin);
+                hi = from_bin(bin + 1) - 1;
+                if (hi < lo) hi = lo;
+            }
         } else if (weigh) {
             double sum = 0, all;
-            each([&](int b, const uint32_t (&k)[4]) {
+            each([&](int i, const float (&f)[4]) {
 #pragma unroll
                 for (int v = 0; v < 4; v++)
-                    if (k[v] != 0 && entry(k[v], b * kStripe + 4 * lane + v) >= least) sum += wt(k[v]);
+                    if (kept_at(f[v], i + v)) sum += wt(key_of(f[v]));
             });
             before_me(sum, s.wave, all);
             goal = (double)st.tp * all * unit;
-            lo = (uint32_t)(least >> 32);
+            lo = key_of(cut);
         }
-        bool counted = false;
         int inside = 0;
         for (;;) {
-            if (!counted) {  // how many they are
-                if (tid == 0) s.small[3] = 0;
-                __syncthreads();
-                uint32_t n = 0;
-                each([&](int b, const uint32_t (&k)[4]) {
+            // how many they are, and the first of them
+            const float from = finite(lo), to = of_key(hi == 0x7FFFFFFFu ? hi - 1 : hi);  // (that key would be -0, which has 0's)
+            if (tid == 0) s.small[3] = 0;
+            __syncthreads();
+            each([&](int i, const float (&f)[4]) {
+                bool is[4], some = false;
 #pragma unroll
-                    for (int v = 0; v < 4; v++) {
-                        const bool is = k[v] >= lo && k[v] <= hi && entry(k[v], b * kStripe + 4 * lane + v) >= least;
-                        const uint64_t m = __ballot(is);
-                        if (m == 0) continue;
-                        uint32_t at = 0;
-                        if (lane == 0) at = atomicAdd(&s.small[3], (uint32_t)__popcll(m));
-                        at = __builtin_amdgcn_readfirstlane(at) + __popcll(m & (((uint64_t)1 << lane) - 1));
-                        if (is && at < kMost) s.sorted[at] = entry(k[v], b * kStripe + 4 * lane + v);
+                for (int v = 0; v < 4; v++) is[v] = f[v] >= from && f[v] <= to, some = some || is[v];
+                if (!__any(some)) return;
+                uint32_t n = 0;
+#pragma unroll
+                for (int v = 0; v < 4; v++) is[v] = is[v] && kept_at(f[v], i + v), n += is[v];
+                const uint32_t incl = running(n);
+                uint32_t base = 0;
+                if (lane == 63 && incl != 0) base = atomicAdd(&s.small[3], incl);
+                uint32_t at = of_lane(base, 63) + (incl - n);
+#pragma unroll
+                for (int v = 0; v < 4; v++)
+                    if (is[v]) {
+                        if (at < kMost) s.sorted[at] = ((unsigned long long)key_of(f[v]) << 32) | (uint32_t)~(i + v);
+                        at++;
                     }
-                });
-                __syncthreads();
-                inside = (int)s.small[3];
-                counted = true;
-            }
+            });
+            __syncthreads();
+            inside = (int)s.small[3];
             if (inside <= kMost || lo == hi) break;
             // too many: in 2048 bins of their keys, from the largest down
             const uint32_t width = (hi - lo) / kBins + 1;
@@ -696,11 +737,13 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
                 else if (rest >= (int64_t)width) q++;
                 return q < kBins ? q : kBins - 1;
             };
-            each([&](int b, const uint32_t (&k)[4]) {
+            each([&](int i, const float (&f)[4]) {
 #pragma unroll
                 for (int v = 0; v < 4; v++)
-                    if (k[v] >= lo && k[v] <= hi && entry(k[v], b * kStripe + 4 * lane + v) >= least)
-                        atomicAdd(&s.bins[sub(k[v])], weigh ? (unsigned long long)rint(wt(k[v]) * unit) : 1ull);
+                    if (f[v] >= from && f[v] <= to && kept_at(f[v], i + v)) {
+                        const uint32_t k = key_of(f[v]);
+                        atomicAdd(&s.bins[sub(k)], weigh ? (unsigned long long)rint(wt(k) * unit) : 1ull);
+                    }
             });
             __syncthreads();
             const double m0 = (double)s.bins[2 * tid], m1 = (double)s.bins[2 * tid + 1];
@@ -720,7 +763,6 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
             const uint32_t new_hi = hi - q * width;
             lo = new_hi - lo >= width ? new_hi - (width - 1) : lo;
             hi = new_hi;
-            counted = false;
             __syncthreads();
         }
         if (inside <= kMost) {
@@ -731,8 +773,9 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
             const double run = above + before_me(y, s.wave, sum);
             // the last entry before which the goal has not been reached
             const int t = last_of(tid < inside && (run < goal || (tid == 0 && above == 0)), s);
-            if (t >= 0) least = s.sorted[t];
-            else least = ((unsigned long long)hi + 1) << 32;  // none of these
+            const unsigned long long e_last = s.sorted[t >= 0 ? t : 0];
+            cut = t >= 0 ? of_key((uint32_t)(e_last >> 32)) : of_key(hi);
+            last = t >= 0 ? (int)~(uint32_t)e_last : -1;  // (none of these: what is above them)
         } else {
             // one key many times: as many as it takes, by index
             double n = weigh ? ceil((goal - above) / (wt(lo) * unit)) : goal - above;
@@ -742,36 +785,45 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
             const int per = ((p.vocab + kEnd - 1) / kEnd + 3) & ~3, i0 = tid * per < p.vocab ? tid * per : p.vocab, i1 = i0 + per < p.vocab ? i0 + per : p.vocab;
             uint32_t mine = 0, all;
             for (int i = i0; i < i1; i += 4) {
-                uint32_t k[4];
-                x.keys4(i, k);
+                float f[4];
+                x.values4(i, f);
 #pragma unroll
-                for (int v = 0; v < 4; v++) mine += k[v] == lo && entry(k[v], i + v) >= least;
+                for (int v = 0; v < 4; v++) mine += f[v] == of_key(lo) && kept_at(f[v], i + v);
             }
-            uint32_t seen = before_me(mine, s.u, all);
+            const uint32_t seen = before_me(mine, s.u, all);
             __syncthreads();
             if (take > seen && take <= seen + mine) {
+                uint32_t n = seen;
                 for (int i = i0; i < i1; i++)
-                    if (x.key(i) == lo && entry(lo, i) >= least && ++seen == take) s.small[2] = (uint32_t)i;
+                    if (x.value(i) == of_key(lo) && kept_at(x.value(i), i) && ++n == take) s.small[2] = (uint32_t)i;
             }
             __syncthreads();
-            least = take ? entry(lo, (int)s.small[2]) : ((unsigned long long)lo + 1) << 32;
+            const int at = (int)s.small[2];
+            __syncthreads();
+            cut = of_key(lo);
+            last = take ? at : -1;
         }
         __syncthreads();
     }
     // the stripes' weights
     const double low = (double)st.low;
     auto weight = [&](uint32_t key, uint32_t i) {
-        if (key == 0 || entry(key, (int)i) < least) return 0.0;
+        if (key == 0 || !kept_at(of_key(key), (int)i)) return 0.0;
         const double y = wt(key);
         return y >= low ? y : 0.0;
     };
     double *to = p.mass + (int64_t)r * p.stripes;
-    each([&](int b, const uint32_t (&k)[4]) {
-        double sum = 0;
+    each([&](int i, const float (&f)[4]) {
+        bool some = false;
 #pragma unroll
-        for (int v = 0; v < 4; v++) sum += weight(k[v], (uint32_t)(b * kStripe + 4 * lane + v));
-        sum = wave_sum(sum);
-        if (lane == 0) __hip_atomic_store(to + b, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        for (int v = 0; v < 4; v++) some = some || f[v] >= cut;
+        double sum = 0;
+        if (__any(some)) {
+#pragma unroll
+            for (int v = 0; v < 4; v++) sum += weight(key_of(f[v]), (uint32_t)(i + v));
+            sum = wave_sum(sum);
+        }
+        if (lane == 0 && i < p.vocab) __hip_atomic_store(to + i / kStripe, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     });
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
@@ -788,7 +840,7 @@ int launch_sample(trhip_ctx *ctx, const void *logits, int io, int64_t stride, in
     int64_t each = 1;
     auto groups_of = [&](int64_t j) { return (stripes + WAVES * j - 1) / (WAVES * j); };
     while (each < 8 && rows * groups_of(each) > 2 * cus) each *= 2;
-    while (each < 8 && groups_of(each) > 64) each *= 2;
+    while (each < 8 && groups_of(each) > 32) each *= 2;  // (a workgroup's share of a row's largest entries has a part that does not shrink)
     const int64_t groups = groups_of(each);  // (at most 1024: one a thread of the second launch)
     const double mean = (double)kMost / 2 / (double)groups;
     int64_t room = (int64_t)(mean + 4.0 * __builtin_sqrt(mean) + 6.0) * 3 / 2 + 16;

@@ -131,6 +131,22 @@ def test_flat_rows(backend, vocab):
         check(backend, x.to(torch.bfloat16), u, k=[3 + 97 * i for i in range(16)], p=[0.99] * 16)
 
 
+def test_around_zero(backend):
+    """Cuts at -0, 0 and the smallest numbers, many of each; and rows of nothing but negative or positive values."""
+    g = torch.Generator().manual_seed(4)
+    some = torch.tensor([-1.0, -1e-38, -1e-45, -0.0, 0.0, 1e-45, 1e-38, 1.0])
+    for vocab in (300, 9000, 130000):
+        x = some[torch.randint(0, 8, (12, vocab), generator=g)]
+        u = [(2 * i + 1) / 24 for i in range(12)]
+        check(backend, x, u, k=[1 + vocab * i // 12 for i in range(12)])
+        check(backend, x, u, p=[0.05 + 0.08 * i for i in range(12)])
+        check(backend, x, u, k=[1 + vocab * (i + 1) // 13 for i in range(12)], p=[0.97 - 0.08 * i for i in range(12)])
+        y = torch.randn((12, vocab), generator=g) * 0.5
+        for z in (y - 40.0, y + 40.0, y * 1e-3, y * 1e-41):
+            check(backend, z, u, p=[0.05 + 0.08 * i for i in range(12)])
+            check(backend, z, u, k=[1 + vocab * i // 12 for i in range(12)], low=[0.1] * 12)
+
+
 def test_order_of_the_rows_values(backend):
     """The largest first, last, in the middle; falling and rising rows; only one entry of weight."""
     for vocab in (100, 5000, 70000):
