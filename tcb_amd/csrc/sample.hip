@@ -580,7 +580,14 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
             __syncthreads();
             if (s.small[1]) return;
         }
-        {
+        // (entries whose weights together do not reach top_p of the row are not sorted)
+        bool enough = true;
+        if (st.k == 0 && st.tp < 1.0f && complete != 0) {
+            double sum;
+            before_me(tid < n ? wt((uint32_t)(s.sorted[tid] >> 32)) : 0.0, s.wave, sum);
+            enough = sum >= (double)st.tp * total;
+        }
+        if (enough) {
             sort(s, n, true);
             const unsigned long long e = tid < n ? s.sorted[tid] : 0;
             const uint32_t key = (uint32_t)(e >> 32);
@@ -646,17 +653,22 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
             for (int g0 = 0; g0 < p.groups; g0 += GA) {
                 unsigned long long a[GA][2];
                 double by[GA];
+                int off[GA];
 #pragma unroll
                 for (int v = 0; v < GA; v++) {
                     const int g = g0 + v < p.groups ? g0 + v : g0;
                     by[v] = g0 + v < p.groups ? s.weight[g] * (unit * 0x1p-48) : 0.0;
                     const int at = 2 * tid - (int)s.from[g];
                     const unsigned long long *from = p.hist + ((int64_t)r * p.groups + g) * kBins;
-                    a[v][0] = by[v] > 0 && at >= 0 && at < kBins ? from[at] : 0;
-                    a[v][1] = by[v] > 0 && at >= -1 && at < kBins - 1 ? from[at + 1] : 0;
+                    off[v] = at;  // (loads without conditions are in flight together)
+                    a[v][0] = from[at < 0 ? 0 : at];
+                    a[v][1] = from[at < -1 ? 0 : at + 1];
                 }
 #pragma unroll
-                for (int v = 0; v < GA; v++) mine[0] += (double)a[v][0] * by[v], mine[1] += (double)a[v][1] * by[v];
+                for (int v = 0; v < GA; v++) {
+                    mine[0] += off[v] >= 0 ? (double)a[v][0] * by[v] : 0.0;
+                    mine[1] += off[v] >= -1 ? (double)a[v][1] * by[v] : 0.0;
+                }
             }
             goal = (double)st.tp * total * unit;
             double all;
