@@ -125,12 +125,13 @@ __device__ __forceinline__ Setting setting_of(const SampleArgs &p, int r) {
     s.u = u >= 0.0f ? (double)u : 0.0;
     return s;
 }
-// How many entries of the whole row its workgroups should cover, and a workgroup's share of them: the mean, four standard deviations of
-// entries that lie anywhere, and six.
+// How many entries of the whole row its workgroups should cover, and a workgroup's share of them: the mean, three standard deviations of
+// entries that lie anywhere, and four. (Four and six left no room for k 293 of 1 x 128256, 32 workgroups, in the 1024 that are sorted:
+// 112 us by reading again, 31 so.)
 constexpr int kCover = 128;
 __device__ __forceinline__ int share_of(int n, int groups) {
     const float m = (float)n * __builtin_amdgcn_rcpf((float)groups);
-    const int s = (int)(m + 4.0f * __builtin_amdgcn_sqrtf(m) + 6.0f);
+    const int s = (int)(m + 3.0f * __builtin_amdgcn_sqrtf(m) + 4.0f);
     return s < n ? s : n;
 }
 
@@ -855,7 +856,7 @@ int launch_sample(trhip_ctx *ctx, const void *logits, int io, int64_t stride, in
     while (each < 8 && groups_of(each) > 32) each *= 2;  // (a workgroup's share of a row's largest entries has a part that does not shrink)
     const int64_t groups = groups_of(each);  // (at most 1024: one a thread of the second launch)
     const double mean = (double)kMost / 2 / (double)groups;
-    int64_t room = (int64_t)(mean + 4.0 * __builtin_sqrt(mean) + 6.0) * 3 / 2 + 16;
+    int64_t room = (int64_t)(mean + 3.0 * __builtin_sqrt(mean) + 4.0) * 3 / 2 + 16;
     if (room > kMost) room = kMost;
     // rows of a launch: at most 2^28 bytes of workspace where more than one
     const int64_t row_bytes = (stripes + groups * (room + kBins + 2)) * 8;
