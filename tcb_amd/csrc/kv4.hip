@@ -3,6 +3,7 @@
 // A workgroup takes a token, or the four tokens of four places in a row (a quarter of a piece), whose value codes share dwords: written
 // together they are dwords, by themselves bytes. A lane has eight elements of each token's row, four lanes a block. Every element moves
 // once, so bytes bound it; of few tokens it is a launch.
+#include "attn_common.hpp"
 #include "kv4.hpp"
 
 namespace trhip {
@@ -49,10 +50,10 @@ template <int IO> __device__ __forceinline__ void get8(const void *src, int64_t 
             const uint4 y = *reinterpret_cast<const uint4 *>(s);
             const uint32_t w[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-            for (int j = 0; j < 4; j++) f[2 * j] = h16_to_f32(w[j] & 0xFFFFu, IO), f[2 * j + 1] = h16_to_f32(w[j] >> 16, IO);
+            for (int j = 0; j < 4; j++) f[2 * j] = wide_lo<IO == TRHIP_BF16>(w[j]), f[2 * j + 1] = wide_hi<IO == TRHIP_BF16>(w[j]);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; i++) f[i] = h16_to_f32(s[i], IO);
+            for (int i = 0; i < 8; i++) f[i] = wide_lo<IO == TRHIP_BF16>(s[i]);
         }
     }
 }
@@ -81,7 +82,7 @@ template <int IO> __device__ __forceinline__ void put8(void *dst, int64_t at, bo
         uint16_t *d = static_cast<uint16_t *>(dst) + at;
         uint32_t w[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) w[j] = f32_to_h16(f[2 * j], IO) | (f32_to_h16(f[2 * j + 1], IO) << 16);
+        for (int j = 0; j < 4; j++) w[j] = pack2<IO == TRHIP_BF16>(f[2 * j], f[2 * j + 1]);
         if (wide) {
             *reinterpret_cast<uint4 *>(d) = make_uint4(w[0], w[1], w[2], w[3]);
         } else {
@@ -91,21 +92,36 @@ template <int IO> __device__ __forceinline__ void put8(void *dst, int64_t at, bo
     }
 }
 
-// The block's element of largest magnitude, the first of equal ones, from each of its four lanes' eight. (As whole numbers magnitudes
-// are in the same order, infinities and NaN above all others.)
+// The block's element of largest magnitude, the first of equal ones, from each of its four lanes' eight. As whole numbers the positive
+// ones are in order, and without a sign the negative ones; infinities and NaN are above all others. Only where the largest of both
+// signs are the same size (in a block of 32 normally distributed bf16 numbers one time in sixty) the elements are looked through.
 __device__ __forceinline__ float largest(const float (&f)[8]) {
-    uint32_t m = __float_as_uint(f[0]);
+    int p = (int)__float_as_uint(f[0]);
+    uint32_t n = __float_as_uint(f[0]);
 #pragma unroll
     for (int i = 1; i < 8; i++) {
         const uint32_t b = __float_as_uint(f[i]);
-        m = (b & 0x7FFFFFFFu) > (m & 0x7FFFFFFFu) ? b : m;
+        p = p > (int)b ? p : (int)b, n = n > b ? n : b;
     }
-    const int lane = threadIdx.x & 3;
-    const uint32_t a = quad<0xB1>(m);  // lanes 1, 0, 3, 2
-    m = (a & 0x7FFFFFFFu) > (m & 0x7FFFFFFFu) || ((a & 0x7FFFFFFFu) == (m & 0x7FFFFFFFu) && (lane & 1)) ? a : m;
-    const uint32_t b = quad<0x4E>(m);  // lanes 2, 3, 0, 1
-    m = (b & 0x7FFFFFFFu) > (m & 0x7FFFFFFFu) || ((b & 0x7FFFFFFFu) == (m & 0x7FFFFFFFu) && (lane & 2)) ? b : m;
-    return __uint_as_float(m);
+    int a = (int)quad<0xB1>((uint32_t)p);  // lanes 1, 0, 3, 2
+    uint32_t c = quad<0xB1>(n);
+    p = p > a ? p : a, n = n > c ? n : c;
+    a = (int)quad<0x4E>((uint32_t)p), c = quad<0x4E>(n);  // lanes 2, 3, 0, 1
+    p = p > a ? p : a, n = n > c ? n : c;
+    const uint32_t size = n & 0x7FFFFFFFu;  // of the most negative where there is one
+    bool neg = (int)n < 0 && (p < 0 || size > (uint32_t)p);
+    if (__any((int)n < 0 && size == (uint32_t)p)) {
+        uint32_t sign = 2;  // of this lane's first of that size
+#pragma unroll
+        for (int i = 7; i >= 0; i--) {
+            const uint32_t b = __float_as_uint(f[i]);
+            sign = (b & 0x7FFFFFFFu) == size ? b >> 31 : sign;
+        }
+        const uint32_t s0 = quad<0x00>(sign), s1 = quad<0x55>(sign), s2 = quad<0xAA>(sign), s3 = quad<0xFF>(sign);
+        const uint32_t first = s0 != 2 ? s0 : s1 != 2 ? s1 : s2 != 2 ? s2 : s3;
+        if ((int)n < 0 && size == (uint32_t)p) neg = first == 1;
+    }
+    return __uint_as_float(neg ? n : (uint32_t)p);
 }
 
 constexpr int kKeyNibble[8] = {0, 4, 1, 5, 2, 6, 3, 7};
@@ -121,9 +137,15 @@ __device__ __forceinline__ void append_rows(const Kv4Args &p, const void *src, u
 #pragma unroll
     for (int i = 0; i < T; i++) {
         h[i] = kv4_scale(largest(f[i]));
-        const float d = f16_to_f32((uint16_t)h[i]), inv = 1.0f / d;
+        const float d = f16_to_f32((uint16_t)h[i]);
+        const bool none = !(fabsf(d) > 0.0f);  // a scale of 0, or a block that is not finite: code 8 throughout
+        const float inv = none ? 0.0f : 1.0f / d;
+        if (__any(h[i] == 0x7E00u)) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) code[i][j] = (uint32_t)kv4_code(f[i][j], d, inv);
+            for (int j = 0; j < 8; j++) f[i][j] = none ? 0.0f : f[i][j];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) code[i][j] = kv4_code(f[i][j], none ? 0.0f : d, inv);
     }
     uint16_t *scale = reinterpret_cast<uint16_t *>(piece + kv4_scale_at(r, b, p.dim));
     if (q == 0) {
@@ -133,9 +155,11 @@ __device__ __forceinline__ void append_rows(const Kv4Args &p, const void *src, u
     if (!value) {
 #pragma unroll
         for (int i = 0; i < T; i++) {
-            uint32_t w = 0;
+            constexpr int element[8] = {0, 2, 4, 6, 1, 3, 5, 7};  // of each nibble
+            uint32_t w = code[i][element[7]];
 #pragma unroll
-            for (int j = 0; j < 8; j++) w |= code[i][j] << (4 * kKeyNibble[j]);
+            for (int j = 6; j >= 0; j--) w = (w << 4) + code[i][element[j]];
+            w -= kCode * 0x11111111u;
             reinterpret_cast<uint32_t *>(piece)[(q * 16 + r + i) * blocks + b] = w;
         }
     } else {
@@ -143,17 +167,19 @@ __device__ __forceinline__ void append_rows(const Kv4Args &p, const void *src, u
         for (int j = 0; j < 4; j++) {  // elements 8 q + 2 j and the next
             uint32_t *dst = reinterpret_cast<uint32_t *>(piece) + ((r >> 2) * 16 + 4 * q + j) * blocks + b;
             if constexpr (T == 4) {
-                constexpr int byte[4] = {0, 2, 1, 3};
+                constexpr int token[4] = {0, 2, 1, 3};  // of each byte
                 uint32_t w = 0;
 #pragma unroll
-                for (int i = 0; i < 4; i++) w |= (code[i][2 * j] | (code[i][2 * j + 1] << 4)) << (8 * byte[i]);
-                *dst = w;
+                for (int i = 3; i >= 0; i--) w = (((w << 4) + code[token[i]][2 * j + 1]) << 4) + code[token[i]][2 * j];
+                *dst = w - kCode * 0x11111111u;
             } else {
-                reinterpret_cast<uint8_t *>(dst)[((r & 1) << 1) | ((r >> 1) & 1)] = (uint8_t)(code[0][2 * j] | (code[0][2 * j + 1] << 4));
+                reinterpret_cast<uint8_t *>(dst)[((r & 1) << 1) | ((r >> 1) & 1)] = (uint8_t)((code[0][2 * j] & 15) | (code[0][2 * j + 1] << 4));
             }
         }
     }
 }
+
+__device__ __forceinline__ float byte_of(uint32_t w, int i) { return (float)((w >> (8 * i)) & 0xFFu); }
 
 template <int IO, int T>
 __device__ __forceinline__ void read_rows(const Kv4Args &p, void *dst, const uint8_t *piece, bool value, int64_t to, int r, int b, int q) {
@@ -167,24 +193,25 @@ __device__ __forceinline__ void read_rows(const Kv4Args &p, void *dst, const uin
     }
 #pragma unroll
     for (int i = 0; i < (value ? 4 : T); i++) {
+        // (the even nibbles and the odd ones, a byte each)
         if (!value) {
-            const uint32_t w = reinterpret_cast<const uint32_t *>(piece)[(q * 16 + r + i) * blocks + b];
+            const uint32_t w = reinterpret_cast<const uint32_t *>(piece)[(q * 16 + r + i) * blocks + b], lo = w & 0x0F0F0F0Fu, hi = (w >> 4) & 0x0F0F0F0Fu;
 #pragma unroll
-            for (int j = 0; j < 8; j++) f[i < T ? i : 0][j] = (float)((int)((w >> (4 * kKeyNibble[j])) & 15) - 8);
+            for (int j = 0; j < 8; j++) f[i < T ? i : 0][j] = byte_of((kKeyNibble[j] & 1) ? hi : lo, kKeyNibble[j] >> 1);
         } else {
-            const uint32_t w = reinterpret_cast<const uint32_t *>(piece)[((r >> 2) * 16 + 4 * q + i) * blocks + b];
+            const uint32_t w = reinterpret_cast<const uint32_t *>(piece)[((r >> 2) * 16 + 4 * q + i) * blocks + b], lo = w & 0x0F0F0F0Fu, hi = (w >> 4) & 0x0F0F0F0Fu;
 #pragma unroll
             for (int t = 0; t < T; t++) {
-                const int at = T == 4 ? t : r & 3, sh = 8 * (((at & 1) << 1) | (at >> 1));
-                f[t][2 * i] = (float)((int)((w >> sh) & 15) - 8);
-                f[t][2 * i + 1] = (float)((int)((w >> (sh + 4)) & 15) - 8);
+                const int at = T == 4 ? t : r & 3, byte = ((at & 1) << 1) | (at >> 1);
+                f[t][2 * i] = byte_of(lo, byte), f[t][2 * i + 1] = byte_of(hi, byte);
             }
         }
     }
 #pragma unroll
     for (int i = 0; i < T; i++) {
+        const float off = -8.0f * d[i];  // c d - 8 d is (c - 8) d: the scale has 11 bits, the code 4
 #pragma unroll
-        for (int j = 0; j < 8; j++) f[i][j] *= d[i];
+        for (int j = 0; j < 8; j++) f[i][j] = fmaf(f[i][j], d[i], off);
         put8<IO>(dst, to + i * p.stride, p.wide, f[i]);
     }
 }

@@ -9,7 +9,7 @@
 
 namespace trhip {
 
-// Where the codes and scales of one place of a page start in its piece, and where an element's nibble lies.
+// Where a place of a page lies, and where its scale of block b is in its piece.
 struct Kv4Place {
     int64_t piece;  // the piece's byte offset in its plane
     int r;          // the place in it
@@ -19,12 +19,6 @@ __device__ __forceinline__ Kv4Place kv4_place(int64_t slot, int page_log2, int h
     return {((((pg * heads + head) << page_log2) + (in & ~15)) >> 4) * (9 * dim), (int)(in & 15)};
 }
 __device__ __forceinline__ int kv4_scale_at(int r, int b, int dim) { return 8 * dim + 2 * ((((r >> 2) * (dim >> 5)) + b) * 4 + (r & 3)); }
-// Byte (from the piece's start) of element e of a value at place r; its nibble is e % 2.
-__device__ __forceinline__ int kv4_value_at(int r, int e, int dim) {
-    return 4 * (((r >> 2) * 16 + ((e & 31) >> 1)) * (dim >> 5) + (e >> 5)) + (((r & 1) << 1) | ((r >> 1) & 1));
-}
-// Byte of dword that holds elements e ... e + 7 of a key at place r (e a multiple of 8).
-__device__ __forceinline__ int kv4_key_at(int r, int e, int dim) { return 4 * ((((e & 31) >> 3) * 16 + r) * (dim >> 5) + (e >> 5)); }
 
 // The scale of a block whose element of largest magnitude is m: m / -8 rounded to five significant bits, then to f16, at most 7936;
 // NaN where m is not finite.
@@ -35,18 +29,15 @@ __device__ __forceinline__ uint32_t kv4_scale(float m) {
     const float r = fminf(__uint_as_float((a + 0x3FFFFu + ((a >> 19) & 1u)) & 0xFFF80000u), 7936.0f);
     return __builtin_bit_cast(uint16_t, (_Float16)r) | (m > 0.0f ? 0x8000u : 0u);
 }
-// clamp(rint(x / d), -8, 7) + 8 without any error before the rounding: r = rint(x * (1 / d)) is one off at most, and x - r d is exact
-// (fused, and x and r d are within a factor of two of each other or r is 0), so comparing it with d / 2 corrects r.
-__device__ __forceinline__ int kv4_code(float x, float d, float inv) {
-    float r = rintf(x * inv);
-    r = fminf(fmaxf(r, -9.0f), 9.0f);
-    const float a = fabsf(d), e = fmaf(-r, d, x), s = d < 0.0f ? -1.0f : 1.0f, over = 2.0f * e * s;  // in units of |d|, twice what is left
-    const bool odd = ((int)r & 1) != 0;
-    if (over > a || (over == a && odd)) r += 1.0f;
-    else if (over < -a || (over == -a && odd)) r -= 1.0f;
-    r = fminf(fmaxf(r, -8.0f), 7.0f);
-    return d == 0.0f || a != a ? 8 : (int)r + 8;
+// clamp(rint(x / d), -8, 7) + 8, plus kCode (a float's bits: the sum with 1.5 * 2^23 + 8 rounds, to even at a half, and its last bits are
+// the code). inv is 1 / d rounded, d has five significant bits. What is rounded, q, is x / d but for 2^-46 of it, rounded once: the
+// remainder x - q0 d has few bits and is exact. Where x / d is half a whole number, q is it. Where it is not, q is not either: x is a
+// neighbour of the half's x or farther, that is 2^-24 (1 + 2^-9) of it at least (such an x has nine bits), and q's rounding is 2^-24 of it
+// at most (less below a power of two, where x's neighbours are as near).
+constexpr uint32_t kCode = 0x4B400000u;
+__device__ __forceinline__ uint32_t kv4_code(float x, float d, float inv) {
+    const float q0 = x * inv, q = fmaf(fmaf(-q0, d, x), inv, q0);
+    return __float_as_uint(__builtin_amdgcn_fmed3f(q, -8.0f, 7.0f) + 12582920.0f);
 }
-__device__ __forceinline__ float kv4_value(int code, uint32_t d) { return (float)(code - 8) * f16_to_f32((uint16_t)d); }
 
 }  // namespace trhip
