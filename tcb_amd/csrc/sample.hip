@@ -80,27 +80,27 @@ struct Row {
     }
 };
 
-// e^((l - max) / T) of a key. e^t = 2^(n / 64) e^r, n = rint(64 t / ln 2), |r| <= ln 2 / 128: what r^6 / 720 leaves out is 2^-54.
+// e^((l - max) / T) of a logit or its key; 0 of NaN and -Inf, 1 of +Inf (max is 1e300 then). e^t = 2^(n / 64) e^r, n = rint(64 t / ln 2),
+// |r| <= ln 2 / 128: what r^6 / 720 leaves out is 2^-54. Twenty operations; t is rounded once more, which is 2^-53 |t|.
 struct Weight {
     uint32_t top;
     double max, inv;
     const double *table;  // 2^(j / 64)
-    __device__ __forceinline__ double operator()(uint32_t k) const {
-        const double t = ((double)of_key(k) - max) * inv;
-        if (k == top) return 1.0;
-        if (k == 0) return 0.0;
-        if (!(t > -700.0)) return exp(t);
-        const double n = rint(t * 92.33248261689366);
+    __device__ __forceinline__ Weight(uint32_t top, double inv, const double *table)
+        : top(top), max(top == 0xFF800000u ? 1e300 : (double)of_key(top)), inv(inv), table(table) {}
+    __device__ __forceinline__ double of(float f) const {
+        const double t = fmin(fmax(((double)f - max) * inv, -1100.0), 0.0);
+        const double z = fma(t, 92.33248261689366, 0x1.8p52), n = z - 0x1.8p52;  // z's low bits are n
         const double r = fma(-n, 3.623510646634843e-19, fma(-n, 0.010830424696249145, t));  // (ln 2 / 64 in two parts)
         double y = fma(r, 8.3333333333333332e-3, 4.1666666666666664e-2);
         y = fma(r, y, 1.6666666666666666e-1);
         y = fma(r, y, 0.5);
         y = fma(r, y, 1.0);
-        const int i = (int)n;
+        const int i = (int)(uint32_t)__double_as_longlong(z);
         const double p = table[i & 63];
-        const double s = fma(p, r * y, p);
-        return __longlong_as_double(__double_as_longlong(s) + ((long long)(i >> 6) << 52));
+        return ldexp(fma(p, r * y, p), i >> 6);
     }
+    __device__ __forceinline__ double operator()(uint32_t k) const { return of(of_key(k)); }
 };
 
 struct Setting {
@@ -219,7 +219,7 @@ template <int J> __global__ __launch_bounds__(kRead) void sample_read(const Samp
     top = wave_max(top);
     uint32_t bound = 0, left = 0;
     if (weigh && top != 0) {
-        const Weight wt = {top, (double)of_key(top), 1.0 / (double)st.t, s_table};
+        const Weight wt(top, 1.0 / (double)st.t, s_table);
         const float per = kPerNat / st.t;
         const int first = bin_of(top, per);
 #pragma unroll
@@ -537,7 +537,7 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
         }
         return;
     }
-    const Weight wt = {top, (double)of_key(top), st.greedy ? 1.0 : 1.0 / (double)st.t, s.table};
+    const Weight wt(top, st.greedy ? 1.0 : 1.0 / (double)st.t, s.table);
     const bool weighed = !filtered || (st.k == 0 && st.tp < 1.0f);
     // the workgroups' largest logits' weights, by which theirs are multiplied
     if (weighed) {
@@ -704,7 +704,7 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
             each([&](int i, const float (&f)[4]) {
 #pragma unroll
                 for (int v = 0; v < 4; v++)
-                    if (kept_at(f[v], i + v)) sum += wt(key_of(f[v]));
+                    sum += wt.of(kept_at(f[v], i + v) ? f[v] : __builtin_nanf(""));
             });
             before_me(sum, s.wave, all);
             goal = (double)st.tp * all * unit;
@@ -820,9 +820,8 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
     }
     // the stripes' weights
     const double low = (double)st.low;
-    auto weight = [&](uint32_t key, uint32_t i) {
-        if (key == 0 || !kept_at(of_key(key), (int)i)) return 0.0;
-        const double y = wt(key);
+    auto weigh_at = [&](float f, int i) {
+        const double y = wt.of(kept_at(f, i) ? f : __builtin_nanf(""));
         return y >= low ? y : 0.0;
     };
     double *to = p.mass + (int64_t)r * p.stripes;
@@ -833,14 +832,15 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
         double sum = 0;
         if (__any(some)) {
 #pragma unroll
-            for (int v = 0; v < 4; v++) sum += weight(key_of(f[v]), (uint32_t)(i + v));
+            for (int v = 0; v < 4; v++) sum += weigh_at(f[v], i + v);
             sum = wave_sum(sum);
         }
         if (lane == 0 && i < p.vocab) __hip_atomic_store(to + i / kStripe, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     });
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    by_stripes(p, r, x, st.u, s, [&](int i) { return __hip_atomic_load(to + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }, weight);
+    by_stripes(p, r, x, st.u, s, [&](int i) { return __hip_atomic_load(to + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); },
+               [&](uint32_t key, uint32_t i) { return weigh_at(of_key(key), (int)i); });
 }
 
 }  // namespace
