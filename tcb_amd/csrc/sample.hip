@@ -625,7 +625,7 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
     int bits = 62;
     while ((p.vocab - 1) >> (62 - bits)) bits--;
     const double unit = __longlong_as_double((long long)(1023 + bits) << 52);
-    constexpr int AT = 4;
+    constexpr int AT = 2;
     auto kept_at = [&](float f, int i) { return f > cut || (f == cut && i <= last); };  // (values: NaN is never kept)
     auto each = [&](auto use) {  // use(first of four, values) for every four entries, a wave's stripes one after the other
         for (int b0 = w; b0 < p.stripes; b0 += AT * kWaves) {
