@@ -80,14 +80,15 @@ struct Row {
     }
 };
 
-// e^((l - max) / T) of a logit or its key; 0 of NaN and -Inf, 1 of +Inf (max is 1e300 then). e^t = 2^(n / 64) e^r, n = rint(64 t / ln 2),
+// e^((l - max) / T) of a logit or its key; 0 of NaN and -Inf, 1 of +Inf (max is 1e300 then, and 1 / T
+// is not quite 0, so that an infinite temperature leaves an infinite logit alone). e^t = 2^(n / 64) e^r, n = rint(64 t / ln 2),
 // |r| <= ln 2 / 128: what r^6 / 720 leaves out is 2^-54. Twenty operations; t is rounded once more, which is 2^-53 |t|.
 struct Weight {
     uint32_t top;
     double max, inv;
     const double *table;  // 2^(j / 64)
     __device__ __forceinline__ Weight(uint32_t top, double inv, const double *table)
-        : top(top), max(top == 0xFF800000u ? 1e300 : (double)of_key(top)), inv(inv), table(table) {}
+        : top(top), max(top == 0xFF800000u ? 1e300 : (double)of_key(top)), inv(fmax(inv, 1e-290)), table(table) {}
     __device__ __forceinline__ double of(float f) const {
         const double t = fmin(fmax(((double)f - max) * inv, -1100.0), 0.0);
         const double z = fma(t, 92.33248261689366, 0x1.8p52), n = z - 0x1.8p52;  // z's low bits are n
@@ -135,9 +136,12 @@ __device__ __forceinline__ int share_of(int n, int groups) {
     return s < n ? s : n;
 }
 
-// Bins of logits over the temperature: the number of a key's bin, which rises with it.
+// Bins of logits over the temperature: the number of a key's bin, which rises with it or stays. (Finite times finite: a temperature may be
+// infinite or so small that its inverse is.)
+__device__ __forceinline__ float bins_a_unit(float t) { return fminf(kPerNat / t, 3.4028234663852886e38f); }
 __device__ __forceinline__ int bin_of(uint32_t k, float per) {
-    return (int)floorf(fminf(fmaxf(of_key(k) * per, -536870912.0f), 536870912.0f));
+    const float f = fminf(fmaxf(of_key(k), -3.4028234663852886e38f), 3.4028234663852886e38f);
+    return (int)floorf(fminf(fmaxf(f * per, -536870912.0f), 536870912.0f));
 }
 
 // Inclusive sums over the wave's lanes, in six lane moves (row_shr 1, 2, 4, 8, then row_bcast 15 and 31).
@@ -220,7 +224,7 @@ template <int J> __global__ __launch_bounds__(kRead) void sample_read(const Samp
     uint32_t bound = 0, left = 0;
     if (weigh && top != 0) {
         const Weight wt(top, 1.0 / (double)st.t, s_table);
-        const float per = kPerNat / st.t;
+        const float per = bins_a_unit(st.t);
         const int first = bin_of(top, per);
 #pragma unroll
         for (int j = 0; j < J; j++) {
@@ -232,7 +236,7 @@ template <int J> __global__ __launch_bounds__(kRead) void sample_read(const Samp
 #pragma unroll
                 for (int v = 0; v < 4; v++) {
                     const int b = first - bin_of(key[j][v], per);
-                    if (key[j][v] != 0 && b < kBins) atomicAdd(&s_bins[b], (unsigned long long)rint(y[v] * 0x1p48));
+                    if (key[j][v] != 0 && (uint32_t)b < (uint32_t)kBins) atomicAdd(&s_bins[b], (unsigned long long)rint(y[v] * 0x1p48));
                 }
             }
             const double sum = wave_sum((y[0] + y[1]) + (y[2] + y[3]));
@@ -644,7 +648,7 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
         uint32_t lo = 1, hi = top;  // the keys among which the run ends
         double above = 0;           // entries, or weight in units, above them
         if (weigh && st.k == 0) {   // from the workgroups' bins
-            const float per = kPerNat / st.t;
+            const float per = bins_a_unit(st.t);
             const int first = bin_of(top, per);
             double mine[2] = {};
             static_assert(kBins == 2 * kEnd, "two bins a thread");

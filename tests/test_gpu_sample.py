@@ -186,6 +186,27 @@ def test_values_that_are_not_finite(backend):
         check(backend, x, [0.7] * 8, **kw)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_temperatures_of_any_size(backend, dtype):
+    """Infinite ones, the largest and the smallest, with logits that are infinite too: entries of +Inf are alone where there are some."""
+    g, ts = torch.Generator().manual_seed(8), [float("inf"), 3e38, 1e38, 1e30, 1e-30, 1e-38, 1e-45]
+    for vocab in (300, 9000, 128256):
+        x = (torch.randn((3 * len(ts), vocab), generator=g) * 3).to(TORCH[dtype])
+        x[1::3, 5] = x[1::3, vocab // 2] = float("inf")
+        x[1::3, 9] = x[2::3, 7] = float("-inf")
+        x[2::3, ::2] = 0.0
+        rows = len(x)
+        u, t = torch.rand(rows, generator=g).tolist(), [a for a in ts for _ in range(3)]
+        alone = x.float()
+        alone[1::3] = torch.where(alone[1::3] == float("inf"), 0.0, float("-inf"))
+        alone = alone.double().numpy()
+        for k, p in (([0] * rows, [1.0] * rows), ([0] * rows, [0.6] * rows), ([50] * rows, [0.6] * rows), ([2000] * rows, [0.9] * rows)):
+            token, lp = sample(backend, x, u, t, k, p)
+            for r in range(rows):
+                want, log, close = choose(alone[r], float(np.float32(t[r])), k[r], float(np.float32(p[r])), 0.0, float(np.float32(u[r])))
+                assert close or (token[r] == want and abs(lp[r] - log) <= 2.0 ** -23 * abs(log) + 1e-11), (vocab, t[r], k[r], p[r], r % 3, token[r], want)
+
+
 def test_no_temperature_is_the_first_largest(backend):
     x = torch.tensor([[1.0, 5.0, 5.0, 2.0], [5.0, 5.0, 5.0, 5.0], [-9.0, -8.0, -8.0, -8.0]])
     token, lp = sample(backend, x, [0.9] * 3, t=[0.0] * 3, k=[3] * 3, p=[0.99] * 3)
