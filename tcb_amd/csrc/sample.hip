@@ -36,7 +36,7 @@ struct SampleArgs {
     float *logprob;
     double *mass;           // [row][stripe]
     unsigned long long *list;  // [row][workgroup][room]: key, ~index
-    unsigned long long *hist;  // [row][workgroup][kBins]: weight in bins of its logits, from the largest's down, in units of 2^-48
+    unsigned long long *hist;  // [row][workgroup][kBins]: weight in bins of its logits, from the largest's down (bin_exponent)
     uint4 *left;               // [row][workgroup]: largest key, threshold (0: all entries left), entries left
 };
 
@@ -144,6 +144,11 @@ __device__ __forceinline__ int bin_of(uint32_t k, float per) {
     return (int)floorf(fminf(fmaxf(f * per, -536870912.0f), 536870912.0f));
 }
 
+// Weights in a bin stand in fixed point, whose sums do not depend on the order; the unit is 2^-(48 + e) of the largest weight, e a little
+// below the bin's distance from it in powers of two, so that a sum's error is that of its largest weight whatever the bin (2^-48 of it). A
+// power of two is 96 ln 2 = 66.54 bins; 984 / 65536 is 1 / 66.6.
+__device__ __forceinline__ int bin_exponent(int b) { return b < 2 ? 0 : ((b - 1) * 984) >> 16; }
+
 // Inclusive sums over the wave's lanes, in six lane moves (row_shr 1, 2, 4, 8, then row_bcast 15 and 31).
 template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t moved(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
@@ -236,7 +241,7 @@ template <int J> __global__ __launch_bounds__(kRead) void sample_read(const Samp
 #pragma unroll
                 for (int v = 0; v < 4; v++) {
                     const int b = first - bin_of(key[j][v], per);
-                    if (key[j][v] != 0 && (uint32_t)b < (uint32_t)kBins) atomicAdd(&s_bins[b], (unsigned long long)rint(y[v] * 0x1p48));
+                    if (key[j][v] != 0 && (uint32_t)b < (uint32_t)kBins) atomicAdd(&s_bins[b], (unsigned long long)rint(ldexp(y[v], 48 + bin_exponent(b))));
                 }
             }
             const double sum = wave_sum((y[0] + y[1]) + (y[2] + y[3]));
@@ -671,8 +676,8 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
                 }
 #pragma unroll
                 for (int v = 0; v < GA; v++) {
-                    mine[0] += off[v] >= 0 ? (double)a[v][0] * by[v] : 0.0;
-                    mine[1] += off[v] >= -1 ? (double)a[v][1] * by[v] : 0.0;
+                    mine[0] += off[v] >= 0 ? ldexp((double)a[v][0], -bin_exponent(off[v])) * by[v] : 0.0;
+                    mine[1] += off[v] >= -1 ? ldexp((double)a[v][1], -bin_exponent(off[v] + 1)) * by[v] : 0.0;
                 }
             }
             goal = (double)st.tp * total * unit;
@@ -744,7 +749,14 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
             if (inside <= kMost || lo == hi) break;
             // too many: in 2048 bins of their keys, from the largest down
             const uint32_t width = (hi - lo) / kBins + 1;
-            for (int i = tid; i < kBins; i += kEnd) s.bins[i] = 0;
+            int *finer = reinterpret_cast<int *>(s.count);  // their units are smaller by the powers of two that their largest weight is below 1
+            for (int i = tid; i < kBins; i += kEnd) {
+                s.bins[i] = 0;
+                if (weigh) {
+                    const uint64_t down = (uint64_t)i * width;
+                    finer[i] = down < hi ? 1022 - (int)((uint64_t)__double_as_longlong(wt((uint32_t)(hi - down))) >> 52) : 0;
+                }
+            }
             __syncthreads();
             const float by_width = 1.0f / (float)width;
             auto sub = [&](uint32_t k) {  // (hi - k) / width
@@ -759,11 +771,12 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
                 for (int v = 0; v < 4; v++)
                     if (f[v] >= from && f[v] <= to && kept_at(f[v], i + v)) {
                         const uint32_t k = key_of(f[v]);
-                        atomicAdd(&s.bins[sub(k)], weigh ? (unsigned long long)rint(wt(k) * unit) : 1ull);
+                        const int q = (int)sub(k);
+                        atomicAdd(&s.bins[q], weigh ? (unsigned long long)rint(ldexp(wt(k), bits + finer[q])) : 1ull);
                     }
             });
             __syncthreads();
-            const double m0 = (double)s.bins[2 * tid], m1 = (double)s.bins[2 * tid + 1];
+            const double m0 = ldexp((double)s.bins[2 * tid], weigh ? -finer[2 * tid] : 0), m1 = ldexp((double)s.bins[2 * tid + 1], weigh ? -finer[2 * tid + 1] : 0);
             double all;
             const double run = above + before_me(m0 + m1, s.wave, all);
             int t = first_of(m0 + m1 > 0 && run + (m0 + m1) >= goal, s);

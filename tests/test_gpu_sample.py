@@ -17,7 +17,8 @@ CLOSE = 1e-12  # of the sum: nearer to a border than this, either side is right
 
 
 def choose(x, t, k, p, low, u):
-    """(token, logprob, whether a border is so close that 64 bits do not decide) of one row."""
+    """(token, logprob, whether a border is so close that 64 bits do not decide) of one row. (Sums in 80 bits: a hundred thousand additions
+    to about 1 would each round by 2^-54, all in one direction where they are equal.)"""
     x = np.where(np.isnan(x), -np.inf, x.astype(np.float64))
     order = np.argsort(-x, kind="stable")
     order = order[x[order] > -np.inf]
@@ -28,7 +29,7 @@ def choose(x, t, k, p, low, u):
     if 0 < k < len(order):
         order = order[:k]
     with np.errstate(invalid="ignore"):
-        w = np.where(x[order] == x[order[0]], 1.0, np.exp((x[order] - x[order[0]]) / t))
+        w = np.where(x[order] == x[order[0]], 1.0, np.exp((x[order] - x[order[0]]) / t)).astype(np.longdouble)
     close, n = False, len(order)
     if p < 1:
         run = np.cumsum(w)
@@ -42,7 +43,7 @@ def choose(x, t, k, p, low, u):
     where = {i: y for i, y in zip(order[:n].tolist(), w[:n].tolist())}
     w = np.array([where[i] for i in keep.tolist()])
     run = np.cumsum(w)
-    goal = max(u, 0.0) * run[-1] if u == u else 0.0
+    goal = max(u, 0.0) * run[-1] if u == u else np.longdouble(0)
     over = np.nonzero(run > goal)[0]
     at = int(over[0]) if len(over) else int(np.nonzero(w > 0)[0][-1])
     if 0 < u < 1:
@@ -205,6 +206,26 @@ def test_temperatures_of_any_size(backend, dtype):
             for r in range(rows):
                 want, log, close = choose(alone[r], float(np.float32(t[r])), k[r], float(np.float32(p[r])), 0.0, float(np.float32(u[r])))
                 assert close or (token[r] == want and abs(lp[r] - log) <= 2.0 ** -23 * abs(log) + 1e-11), (vocab, t[r], k[r], p[r], r % 3, token[r], want)
+
+
+def test_sums_of_many_small_weights(backend):
+    """One large logit, then tens of thousands of equal small ones at several heights: borders of top_p among them, where each weighs some
+    1e-9 of the sum (a rounding of each to a common unit would be off by whole entries)."""
+    g, vocab, rows = torch.Generator().manual_seed(4), 128256, 48
+    x = torch.full((rows, vocab), -40.0)
+    for h, heights in enumerate(([-20.53, -20.61, -20.74, -20.87, -20.95, -21.02], [-24.1, -24.4, -25.3, -26.2, -26.9, -27.7])):
+        for i, y in enumerate(heights):
+            x[h::2, 20000 * i:20000 * (i + 1)] = y
+    x = x[:, torch.randperm(vocab, generator=g)]
+    x[:, 77] = 0.0
+    w = torch.exp(x.double())
+    tail = (w.sum(1) - 1) / w.sum(1)
+    p = (1 - tail * torch.linspace(0.02, 0.98, rows, dtype=torch.float64)).float()
+    u = (1 - tail * torch.rand(rows, generator=g).double()).float()
+    check(backend, x, u.tolist(), p=p.tolist())
+    check(backend, x, u.tolist(), k=[110000 - 300 * r for r in range(rows)], p=p.tolist())
+    check(backend, x + 5, [0.999] * rows, t=[3.0] * rows, p=torch.linspace(0.4, 0.97, rows).tolist())
+    check(backend, x + 5, [0.999] * rows, t=[3.0] * rows, k=[110000 - 300 * r for r in range(rows)], p=torch.linspace(0.4, 0.97, rows).tolist())
 
 
 def test_no_temperature_is_the_first_largest(backend):
