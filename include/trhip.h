@@ -219,8 +219,8 @@ int trhip_gemm_q_swiglu(trhip_ctx *ctx, const trhip_wstore *w, const float *x, f
                         int64_t K, int mode);
 
 /* ---- The paged key/value cache and the attention over it -------------------------------------------------------------
- * Between the merged q/k/v product and the output projection (positions, if the model turns q and k by them, are applied by
- * the program in between). The cache is the caller's memory:
+ * Between the merged q/k/v product and the output projection (and the positions by which a model turns q and k:
+ * trhip_rope). The cache is the caller's memory:
  * two planes k and v of [pages][heads][page][dim] elements (f16 or bf16, 16-byte aligned), its pages dealt to
  * requests by page tables. page: keys a page, a power of two from 16 to 4096; dim: a multiple of 8 up to 256. Lengths, page
  * numbers and slots are int32 on the device, so a step can be captured into a graph and replayed while they change.
@@ -354,7 +354,11 @@ int trhip_kv4_read(trhip_ctx *ctx, const trhip_kv4 *kv, int64_t tokens, void *k,
 
 /* trhip_attn over the 4-bit cache: same masks, tables, lengths, hints and limits. q and out are of `type` (TRHIP_F16 or TRHIP_BF16).
  * A block whose scale is not finite reads as NaN where a token sees it: in its elements of the result as a value, in the whole row
- * of the head as a key. What a token's mask hides never reaches it. */
+ * of the head as a key. What a token's mask hides never reaches it. Weights are rounded: in requests of more than 96 rows, where their
+ * keys may be opened, as trhip_attn's; else to f16 for bf16 results and to two f16 numbers (2^-21) for f16 ones. Where the hint allows requests of more
+ * than 96 rows, their keys are opened into the context's workspace in 16 bits: as many times max_pages pages (2 * page * heads * dim
+ * bytes a plane) as the tokens can make such requests, if that is no more than 2 GiB a plane; beyond it, or with a hint that is too
+ * small, they are read as they are, which takes up to five times as long. */
 int trhip_kv4_attn(trhip_ctx *ctx, const trhip_kv4 *kv, const void *q, int type, int64_t q_stride, void *out, int64_t out_stride,
                    int64_t tokens, int heads, int64_t nreq, const int32_t *q_start, const int32_t *kv_len,
                    const int32_t *table, int64_t max_pages, int64_t max_new, int64_t window, int64_t sinks, float scale);

@@ -517,7 +517,7 @@ int launch_kv4_attn(trhip_ctx *ctx, const trhip_kv4 *kv, const AttnCall &c, int 
     // them, where the workspace may hold the longest ones that the sizes allow. Which there are is known only from the hint.
     const int64_t most_long = c.tokens * p.group / (kTokMost + 1), longs = most_long < c.nreq ? most_long : c.nreq;
     const double image_bytes = (double)longs * (double)c.max_pages * (double)p.page_bytes * (32.0 / 9.0);
-    const bool image = most_new * p.group > kTokMost && longs > 0 && longs < 65536 && c.max_pages > 0 && image_bytes <= (double)kMostImage &&
+    const bool image = most_new * p.group > kTokMost && longs > 0 && longs < 65536 && p.kv_heads < 65536 && c.max_pages > 0 && image_bytes <= (double)kMostImage &&
                        (double)c.nreq * (double)c.max_pages <= (double)(kMostImage / 4);
     if (image) {
         const int64_t plane = (longs * c.max_pages * (p.page_bytes / 9 * 32) + 255) & ~(int64_t)255, tables = c.nreq * c.max_pages * 4;

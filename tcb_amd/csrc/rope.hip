@@ -10,6 +10,7 @@ namespace trhip {
 namespace {
 
 constexpr int kMostPairs = 256, kThreads = 256;
+constexpr int64_t kMostTokens = (int64_t)1 << 24;  // of a launch, which may have 2^32 threads
 
 struct RopeArgs {
     const void *x;
@@ -164,7 +165,7 @@ int launch_rope(trhip_ctx *ctx, const trhip_rope_spec &spec, const void *x, int6
                 int64_t tokens, int heads, int dim, const int *pos, int64_t pos_stride) {
     RopeArgs p = {};
     p.x = x, p.out = out, p.x_stride = x_stride, p.out_stride = out_stride, p.pos_stride = pos_stride;
-    p.tokens = (int)tokens, p.heads = heads, p.dim = dim, p.axes = spec.axes;
+    p.heads = heads, p.dim = dim, p.axes = spec.axes;
     for (int a = 0; a < spec.axes; a++) p.pairs += p.n[a] = spec.pairs[a];
     p.dealt = spec.flags & TRHIP_ROPE_DEALT, p.ladders = spec.flags & TRHIP_ROPE_LADDERS, p.neighbours = spec.flags & TRHIP_ROPE_NEIGHBOURS;
     p.copy = x != out;
@@ -188,10 +189,18 @@ int launch_rope(trhip_ctx *ctx, const trhip_rope_spec &spec, const void *x, int6
     }
     p.each = (int)((heads + splits - 1) / splits);
     const unsigned s = (unsigned)((heads + p.each - 1) / p.each);
-    if (io == TRHIP_F32) wide ? launch<TRHIP_F32, true>(ctx, p, four, s) : launch<TRHIP_F32, false>(ctx, p, four, s);
-    else if (io == TRHIP_F16) wide ? launch<TRHIP_F16, true>(ctx, p, four, s) : launch<TRHIP_F16, false>(ctx, p, four, s);
-    else wide ? launch<TRHIP_BF16, true>(ctx, p, four, s) : launch<TRHIP_BF16, false>(ctx, p, four, s);
-    return launch_check(ctx, "rope");
+    for (int64_t t = 0; t < tokens; t += kMostTokens) {
+        p.tokens = (int)(tokens - t < kMostTokens ? tokens - t : kMostTokens);
+        if (io == TRHIP_F32) wide ? launch<TRHIP_F32, true>(ctx, p, four, s) : launch<TRHIP_F32, false>(ctx, p, four, s);
+        else if (io == TRHIP_F16) wide ? launch<TRHIP_F16, true>(ctx, p, four, s) : launch<TRHIP_F16, false>(ctx, p, four, s);
+        else wide ? launch<TRHIP_BF16, true>(ctx, p, four, s) : launch<TRHIP_BF16, false>(ctx, p, four, s);
+        const int st = launch_check(ctx, "rope");
+        if (st != TRHIP_OK) return st;
+        p.x = static_cast<const char *>(p.x) + kMostTokens * x_stride * size;
+        p.out = static_cast<char *>(p.out) + kMostTokens * out_stride * size;
+        p.pos += kMostTokens;
+    }
+    return TRHIP_OK;
 }
 
 }  // namespace trhip

@@ -124,6 +124,27 @@ def test_many_tokens(backend):
     check(backend, "f32", 2500, 9, 64, [32], far=100000, in_place=True, pad=128)
 
 
+def test_more_tokens_than_a_launch_has(backend):
+    """Small rows of more than 2^26 tokens, in place and to other rows."""
+    n = (1 << 26) + 5
+    pos = (torch.arange(n, dtype=torch.int32, device=DEV) * 7919) % 100003
+    x = torch.ones((n, 2), dtype=torch.float16, device=DEV)
+    x[:, 1] = 0.5
+    out = torch.zeros((n, 4), dtype=torch.float16, device=DEV)
+    torch.cuda.synchronize()
+    spec = tcb_amd.RopeSpec((1,))
+    backend.Rope(spec, x.data_ptr(), 2, out.data_ptr(), 4, tcb_amd.F16, n, 1, 2, pos.data_ptr(), n)
+    backend.Rope(spec, x.data_ptr(), 2, x.data_ptr(), 2, tcb_amd.F16, n, 1, 2, pos.data_ptr(), n)
+    backend.ctx.sync()
+    assert torch.equal(out[:, :2], x) and not out[:, 2:].any()
+    for a in range(0, n, 1 << 23):
+        t = pos[a:a + (1 << 23)].double()
+        c, s = torch.cos(t), torch.sin(t)
+        want = torch.stack([c - 0.5 * s, s + 0.5 * c], 1)
+        # half a step of f16 (of values up to 1.2), and the arithmetic's 2^-20
+        assert ((x[a:a + (1 << 23)].double() - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -20).all(), a
+
+
 def test_values_that_are_not_finite(backend):
     """A NaN or an infinity stays in its pair; elements behind the pairs keep their bits."""
     for dtype in ("f32", "bf16", "f16"):
