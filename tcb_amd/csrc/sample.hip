@@ -462,7 +462,10 @@ __device__ __forceinline__ bool top64(const SampleArgs &p, int r, const Weight &
         const uint32_t mid = lo + (hi - lo + 1) / 2;
         int c = 0;
 #pragma unroll
-        for (int i = 0; i < PER; i++) c += __popcll(__ballot(k[i] >= mid));
+        for (int i = 0; i < PER; i++) {
+            if (i % 4 == 0 && 64 * i >= n) break;
+            c += __popcll(__ballot(k[i] >= mid));
+        }
         if (c >= want) lo = mid, count = c;
         else hi = mid - 1;
     }
@@ -471,6 +474,7 @@ __device__ __forceinline__ bool top64(const SampleArgs &p, int r, const Weight &
     int at = 0;
 #pragma unroll
     for (int i = 0; i < PER; i++) {
+        if (i % 4 == 0 && 64 * i >= n) break;
         const uint64_t m = __ballot(k[i] >= lo);
         if (k[i] >= lo) some[at + __popcll(m & (((uint64_t)1 << lane) - 1))] = s.sorted[64 * i + lane];
         at += __popcll(m);
