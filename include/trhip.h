@@ -356,7 +356,8 @@ int trhip_kv4_read(trhip_ctx *ctx, const trhip_kv4 *kv, int64_t tokens, void *k,
  * A block whose scale is not finite reads as NaN where a token sees it: in its elements of the result as a value, in the whole row
  * of the head as a key. What a token's mask hides never reaches it. Weights are rounded: in requests of more than 96 rows, where their
  * keys may be opened, as trhip_attn's; else to f16 for bf16 results and to two f16 numbers (2^-21) for f16 ones. Where the hint allows requests of more
- * than 96 rows, their keys are opened into the context's workspace in 16 bits: as many times max_pages pages (2 * page * heads * dim
+ * than 96 rows, their keys are opened into the context's workspace in 16 bits
+ * (exactly, where trhip_kv4_append wrote the scales, else rounded once): as many times max_pages pages (2 * page * heads * dim
  * bytes a plane) as the tokens can make such requests, if that is no more than 2 GiB a plane; beyond it, or with a hint that is too
  * small, they are read as they are, which takes up to five times as long. */
 int trhip_kv4_attn(trhip_ctx *ctx, const trhip_kv4 *kv, const void *q, int type, int64_t q_stride, void *out, int64_t out_stride,

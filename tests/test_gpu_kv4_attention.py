@@ -241,6 +241,24 @@ def test_blocks_that_are_not_finite(backend, new, kv):
                 assert (np.abs(got - ref)[clean] <= tol[clean]).all()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_scales_that_append_does_not_write(backend, dtype):
+    """Scales of eleven bits. Values are then (c - 8) d in 15 bits: exact in requests of few rows, rounded once in long ones, by half a step, keys
+    and values alike (a key's rounding moves its score by half a step of its absolute sum)."""
+    b = Batch(dtype, 8, 2, 96, 32, [1, 3, 40, 130], [70, 333, 300, 513], seed=21, size=0.5)
+    rng = np.random.default_rng(2)
+    b.scales = [np.where(np.isnan(d), d, (d.astype(np.float64) * (1 + rng.random(d.shape) / 16)).astype(np.float16)) for d in b.scales]
+    got, (want, tol) = b.run(backend), b.want()
+    k, v = b.values()
+    for i, (n, m) in enumerate(zip(b.new, b.kv)):
+        if n * 4 > 96:
+            kk, vv = (R.rows_of(c, b.table[i], m, b.page) for c in (k, v))
+            _, spread, reach = R.attend(b.q[b.start[i]:b.start[i + 1]].float().numpy(), kk, vv, m - n, b.dim ** -0.5)
+            half = K4.HALF[dtype]
+            tol[b.start[i]:b.start[i + 1]] += (1 + half) * half * spread * (1 + 2 * reach)
+    assert (np.abs(got - want) <= tol).all()
+
+
 def test_sizes_of_values(backend):
     """Values from f16's smallest scales to its largest, growing and falling along the keys: weights times scales must neither
     overflow nor vanish."""
