@@ -78,6 +78,28 @@ struct Row {
 #pragma unroll
         for (int u = 0; u < 4; u++) k[u] = key_of(f[u]);
     }
+    // This lane's entries of stripes first, first + apart, ..., N of them. Where the row has them whole no load is behind a condition, or
+    // the next one would wait for it.
+    template <int N> __device__ __forceinline__ void stripes(int first, int apart, float (&f)[N][4]) const {
+        const int i = first * kStripe + 4 * (int)(threadIdx.x & 63), step = apart * kStripe;
+        const bool in = wide && (first + (N - 1) * apart + 1) * kStripe <= vocab;
+        if (in && io == TRHIP_F32) {
+#pragma unroll
+            for (int a = 0; a < N; a++) *reinterpret_cast<float4 *>(f[a]) = *reinterpret_cast<const float4 *>(static_cast<const float *>(x) + i + a * step);
+        } else if (in) {
+            uint2 y[N];
+#pragma unroll
+            for (int a = 0; a < N; a++) y[a] = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(x) + i + a * step);
+#pragma unroll
+            for (int a = 0; a < N; a++) {
+                f[a][0] = h16_to_f32(y[a].x & 0xFFFFu, io), f[a][1] = h16_to_f32(y[a].x >> 16, io);
+                f[a][2] = h16_to_f32(y[a].y & 0xFFFFu, io), f[a][3] = h16_to_f32(y[a].y >> 16, io);
+            }
+        } else {
+#pragma unroll
+            for (int a = 0; a < N; a++) values4(i + a * step < vocab ? i + a * step : vocab, f[a]);
+        }
+    }
 };
 
 // e^((l - max) / T) of a logit or its key; 0 of NaN and -Inf, 1 of +Inf (max is 1e300 then, and 1 / T
@@ -200,10 +222,13 @@ template <int J> __global__ __launch_bounds__(kRead) void sample_read(const Samp
     const Row x = {static_cast<const char *>(p.logits) + r * p.stride * (p.io == TRHIP_F32 ? 4 : 2), p.io, p.vocab, p.wide};
     uint32_t key[J][4], top = 0;
     auto stripe = [&](int j) { return g + p.groups * (w + WAVES * j); };
+    {
+        float f[J][4];
+        x.stripes(stripe(0), p.groups * WAVES, f);
 #pragma unroll
-    for (int j = 0; j < J; j++) {
-        if (stripe(j) < p.stripes) x.keys4(stripe(j) * kStripe + 4 * lane, key[j]);
-        else key[j][0] = key[j][1] = key[j][2] = key[j][3] = 0;
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int v = 0; v < 4; v++) key[j][v] = key_of(f[j][v]);
     }
     const Setting st = setting_of(p, r);
     const bool filtered = st.k > 0 || st.tp < 1.0f || st.low > 0.0f, weigh = !filtered || (st.k == 0 && st.tp < 1.0f), bins = weigh && filtered;
@@ -643,8 +668,7 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
     auto each = [&](auto use) {  // use(first of four, values) for every four entries, a wave's stripes one after the other
         for (int b0 = w; b0 < p.stripes; b0 += AT * kWaves) {
             float f[AT][4];
-#pragma unroll
-            for (int a = 0; a < AT; a++) x.values4(b0 + a * kWaves < p.stripes ? (b0 + a * kWaves) * kStripe + 4 * lane : p.vocab, f[a]);
+            x.stripes(b0, kWaves, f);
 #pragma unroll
             for (int a = 0; a < AT; a++) use((b0 + a * kWaves) * kStripe + 4 * lane, f[a]);
         }
