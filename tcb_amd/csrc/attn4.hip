@@ -1,8 +1,9 @@
 // attn4.hip -- attention over the 4-bit paged cache (kv4.hpp) for few rows, and the call's plan.
 //
 // Rows, work items, pieces and joins are those of the 16-bit cache's kernel of few rows (attn_common.hpp): a workgroup takes a tile of
-// 16 or 32 rows (the heads of a few tokens that read one kv head) and a piece of the keys; its four waves take every fourth block of
-// 32 keys and join through LDS. What differs is the block.
+// 16 rows (the heads of a few tokens that read one kv head) and a piece of the keys; its four waves take every fourth block of
+// 32 keys and join through LDS. What differs is the block. (Tiles of 32 rows open a block's codes once for two products, but hold half as many
+// waves a CU: 64 requests of up to 12 tokens, 2000 keys, took 57 us against 43, of up to 24 tokens, 8192 keys, 220 against 186.)
 //
 // Nothing of a block goes through LDS: the codes lie in memory as the matrix instructions' operands want them, so a lane loads
 // its part of a piece of sixteen places as it stands. Two nibbles c masked out of a dword become 1024 + c (or 64 + c) in f16 by
@@ -25,15 +26,16 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x3 __attribute__((ext_vector_type(3)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 
-constexpr int kTwoSets = 4;  // blocks of elements up to which a workgroup's registers hold two sets of rows
 constexpr int64_t kMostImage = (int64_t)2 << 30;  // bytes of a plane of opened keys at most: a hundredth of the memory
 constexpr int kWaves = 4, kBlock = 32, kLeast = 8, kOver = 6;
 
-// Workgroups a CU, by registers (blocks: 32-element blocks of a row times sets of rows).
-constexpr int per_cu(int blocks) { return blocks <= 4 ? 3 : blocks <= 8 ? 2 : 1; }
+// Workgroups a CU, by registers (blocks of 32 elements in a row). 64 x 8192 tokens, heads of 128, take 90 us with one and 76 with three; 32 x 4096
+// with heads of 96 take 32 with two and 29 with three; heads of 256 spill with two, 64 x 8192 tokens 223 against 197 with one. Four of up to
+// 64 elements: 46 against 48 there, but 29 against 26 for 64 x 1 tokens of 32 heads on one.
+constexpr int per_cu(int blocks) { return blocks <= 4 ? 3 : blocks <= 7 ? 2 : 1; }
 
-template <int NG, int NC> struct Shape4 {
-    static constexpr int DIM = 32 * NG, ROWS = 16 * NC;
+template <int NG> struct Shape4 {
+    static constexpr int DIM = 32 * NG, ROWS = 16;
     // a piece of sixteen places in LDS: copies of 1024 bytes, the last of 256 where that is enough
     static constexpr int BYTES_IN = 288 * NG, WHOLE = BYTES_IN / 1024, TAIL = BYTES_IN % 1024, COPIES = WHOLE + (TAIL > 0);
     static constexpr int PIECE = WHOLE * 1024 + (TAIL == 0 ? 0 : TAIL <= 256 ? 256 : 1024);
@@ -110,11 +112,6 @@ template <int NG> struct Piece4 {
     }
 };
 
-// What the rows of one set of sixteen see: this lane's row, and the extremes over the set's rows.
-struct Rows4 {
-    int hi, lo;
-};
-
 template <int NG> struct Acc4 {
     f4 o[NG][2];
     float m, f, l;  // reference (log2 units, with the lift and the scales'); the score it came from; this lane's share of the sum
@@ -122,8 +119,8 @@ template <int NG> struct Acc4 {
     bool far;
 };
 
-template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves, per_cu(NG * NC)) void attn4_few(const AttnArgs p) {
-    using S = Shape4<NG, NC>;
+template <int NG, bool BF> __global__ __launch_bounds__(64 * kWaves, per_cu(NG)) void attn4_few(const AttnArgs p) {
+    using S = Shape4<NG>;
     constexpr bool TWO = !BF;
     extern __shared__ __attribute__((aligned(16))) float lds[];
     const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6), c = lane & 15, quarter = lane >> 4;
@@ -135,24 +132,17 @@ template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves, per
     // masks: this lane's rows, then the extremes over the tile
     const int first = keys - it.nq;
     auto low = [&](int hi) { return p.window > 0 && hi >= p.window ? hi - p.window + 1 : 0; };
-    Rows4 rows[NC];
-#pragma unroll
-    for (int s = 0; s < NC; s++) {
-        const int r = 16 * s + c, row = r0 + (r < n ? r : n - 1);
-        rows[s].hi = first + p.by_group(row);
-        rows[s].lo = low(rows[s].hi);
-    }
+    const int my_hi = first + p.by_group(r0 + (c < n ? c : n - 1)), my_lo = low(my_hi);
     const int hi_min = uni(first + p.by_group(r0)), hi_max = uni(first + p.by_group(r0 + n - 1)), lo_min = uni(low(hi_min)), lo_max = uni(low(hi_max));
     const Span sp = span_of<kBlock>(hi_max, lo_min, p.sinks);
     const int nb = sp.count(), piece = it.nsplit == 1 ? nb : (nb + it.nsplit - 1) / it.nsplit;
     const int b0 = it.split * piece, b1 = b0 + piece < nb ? b0 + piece : nb;
 
     // q in f16 operands, scaled by a power of two to at most 2^15
-    u32x4 q[NC][NG];
-    float sc[NC];
-#pragma unroll
-    for (int s = 0; s < NC; s++) {
-        const int r = 16 * s + c, row = r0 + (r < n ? r : 0), t = p.by_group(row), g0 = row - t * p.group;
+    u32x4 q[NG];
+    float sc;
+    {
+        const int row = r0 + (c < n ? c : 0), t = p.by_group(row), g0 = row - t * p.group;
         const uint16_t *src = p.q + (int64_t)(it.q0 + t) * p.q_stride + (int64_t)(it.head * p.group + g0) * p.dim + 8 * quarter;
         uint4 raw[NG];
 #pragma unroll
@@ -169,10 +159,10 @@ template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves, per
         int e = 141 - (int)(__float_as_uint(top) >> 23);
         e = e > 126 ? 126 : e;
         const float up = __uint_as_float((uint32_t)(e + 127) << 23);
-        sc[s] = ldexpf(p.scale, -e);
+        sc = ldexpf(p.scale, -e);
 #pragma unroll
         for (int g = 0; g < NG; g++) {
-            each(g, [&](int i, float a, float b) { q[s][g][i] = __builtin_bit_cast(uint32_t, (h2){(_Float16)(a * up), (_Float16)(b * up)}); });
+            each(g, [&](int i, float a, float b) { q[g][i] = __builtin_bit_cast(uint32_t, (h2){(_Float16)(a * up), (_Float16)(b * up)}); });
         }
     }
 
@@ -222,15 +212,12 @@ template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves, per
 
     Open8 open8;
     open8.init();
-    Acc4<NG> A[NC];
+    Acc4<NG> A;
+    A.m = A.f = A.most = -__builtin_inff();
+    A.l = 0.0f;
+    A.far = false;
 #pragma unroll
-    for (int s = 0; s < NC; s++) {
-        A[s].m = A[s].f = A[s].most = -__builtin_inff();
-        A[s].l = 0.0f;
-        A[s].far = false;
-#pragma unroll
-        for (int g = 0; g < NG; g++) A[s].o[g][0] = A[s].o[g][1] = (f4){0, 0, 0, 0};
-    }
+    for (int g = 0; g < NG; g++) A.o[g][0] = A.o[g][1] = (f4){0, 0, 0, 0};
     int tl = -24;                // the values' scales met so far are at most 2^tl,
     uint32_t limit = 0x0001u;    // in f16
 
@@ -247,18 +234,14 @@ template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves, per
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the keys' part of the slot has been read
 #pragma unroll
         for (int h = 0; h < 2; h++) copy(p.k, next[h], slot + h * S::PIECE);
-        float x[NC][8];
+        float x[8];
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
             for (int g = 0; g < NG; g++) {
-                const u32x4 a = open8(k[h].codes[g]);
+                const f4 d = mma16(open8(k[h].codes[g]), q[g], (f4){0, 0, 0, 0});
 #pragma unroll
-                for (int s = 0; s < NC; s++) {
-                    const f4 d = mma16(a, q[s][g], (f4){0, 0, 0, 0});
-#pragma unroll
-                    for (int i = 0; i < 4; i++) x[s][4 * h + i] = fmaf(k[h].scale(g, i), d[i], g == 0 ? 0.0f : x[s][4 * h + i]);
-                }
+                for (int i = 0; i < 4; i++) x[4 * h + i] = fmaf(k[h].scale(g, i), d[i], g == 0 ? 0.0f : x[4 * h + i]);
             }
         wait_vmcnt(AHEAD);
 #pragma unroll
@@ -284,7 +267,7 @@ template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves, per
                 finite = 0;
 #pragma unroll
                 for (int g = 0; g < NG; g++) {
-                    bool bad[NC] = {};
+                    bool bad = false;
 #pragma unroll
                     for (int h = 0; h < 2; h++)
 #pragma unroll
@@ -296,17 +279,13 @@ template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves, per
                                 finite = finite > u ? finite : u;
                             } else {  // it reaches the rows that see it, and no other
                                 const int key = t + 16 * h + 4 * quarter + i;
-#pragma unroll
-                                for (int s = 0; s < NC; s++) bad[s] = bad[s] || (key <= rows[s].hi && (key >= rows[s].lo || key < p.sinks));
+                                bad = bad || (key <= my_hi && (key >= my_lo || key < p.sinks));
                                 d &= ~(0xFFFFu << sh);
                             }
                         }
-#pragma unroll
-                    for (int s = 0; s < NC; s++) {
-                        const float nan = row_max(bad[s] ? 1.0f : 0.0f) > 0.0f ? __builtin_nanf("") : 0.0f;
-                        A[s].o[g][0] += nan;
-                        A[s].o[g][1] += nan;
-                    }
+                    const float nan = row_max(bad ? 1.0f : 0.0f) > 0.0f ? __builtin_nanf("") : 0.0f;
+                    A.o[g][0] += nan;
+                    A.o[g][1] += nan;
                 }
             }
             // (f16's bits as fp32's: exact, subnormal ones too)
@@ -317,98 +296,88 @@ template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves, per
                 tl = to;
                 limit = __builtin_bit_cast(uint16_t, (_Float16)ldexpf(1.0f, tl));
                 const float less = ldexpf(1.0f, -by);
+                A.m += (float)by;
+                A.most += (float)by;
+                A.l *= less;
 #pragma unroll
-                for (int s = 0; s < NC; s++) {
-                    A[s].m += (float)by;
-                    A[s].most += (float)by;
-                    A[s].l *= less;
-#pragma unroll
-                    for (int g = 0; g < NG; g++) A[s].o[g][0] *= less, A[s].o[g][1] *= less;
-                }
+                for (int g = 0; g < NG; g++) A.o[g][0] *= less, A.o[g][1] *= less;
             }
         }
+        float least = x[0], top = x[0];
 #pragma unroll
-        for (int s = 0; s < NC; s++) {
-            Acc4<NG> &B = A[s];
-            float least = x[s][0], top = x[s][0];
+        for (int i = 1; i < 8; i++) top = fmaxf(top, x[i]), least = fminf(least, x[i]);
+        if (__any(top == __builtin_inff() || least == -__builtin_inff())) {  // a key's scale is infinite: its score is NaN
 #pragma unroll
-            for (int i = 1; i < 8; i++) top = fmaxf(top, x[s][i]), least = fminf(least, x[s][i]);
-            if (__any(top == __builtin_inff() || least == -__builtin_inff())) {  // a key's scale is infinite: its score is NaN
+            for (int i = 0; i < 8; i++) x[i] = fmaf(x[i], 0.0f, x[i]);
+            top = x[0];
 #pragma unroll
-                for (int i = 0; i < 8; i++) x[s][i] = fmaf(x[s][i], 0.0f, x[s][i]);
-                top = x[s][0];
-#pragma unroll
-                for (int i = 1; i < 8; i++) top = fmaxf(top, x[s][i]);
-            }
-            if (!all) {
-                const int from = t + 4 * quarter, dh = rows[s].hi - from, dl = rows[s].lo - from, ds = p.sinks - from;
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int e = 16 * (i >> 2) + (i & 3);
-                    x[s][i] = e <= dh && (e >= dl || e < ds) ? x[s][i] : -__builtin_inff();
-                }
-                top = x[s][0];
-#pragma unroll
-                for (int i = 1; i < 8; i++) top = fmaxf(top, x[s][i]);
-            }
-            top = row_max(top);
-            // The reference, as in softmax_step: raised to the largest score where that exceeds it by more than 2^8, lowered (by 2^64 in
-            // all at most) to a block whose largest weight is below 2^-14. Weights stand 2^7 above it, in units of the largest scale.
-            const float d = (top - B.f) * sc[s], lift = 7.0f - (float)tl;
-            const bool fall = d < -14.0f && top > -__builtin_inff() && !B.far && B.m > B.most - 64.0f;
-            if (__any(d > (B.far ? 0.0f : 8.0f) || fall)) {
-                const bool move = d > (B.far ? 0.0f : 8.0f) || fall;
-                float y = top * sc[s];
-                const float bottom = B.most - 64.0f + lift;
-                const bool cut = fall && y < bottom;
-                y = cut ? bottom : y;
-                const float from = cut ? bottom * __builtin_amdgcn_rcpf(sc[s]) : top;
-                const bool far = fabsf(y) > kFar;
-                const float r = (far ? y : ceilf(y)) - lift;
-                const float a = move ? exp2_hw(far && B.far ? (B.f - from) * sc[s] : B.m - r) : 1.0f;  // from -Inf: 0
-                B.l *= a;
-#pragma unroll
-                for (int g = 0; g < NG; g++) B.o[g][0] *= a, B.o[g][1] *= a;
-                B.m = move ? r : B.m;
-                B.f = move ? from : B.f;
-                B.far = move ? far : B.far;
-                B.most = fmaxf(B.most, B.m);
-            }
-            const float neg = B.far ? lift : B.m == -__builtin_inff() ? 0.0f : -B.m;
-            if (__any(B.far)) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) x[s][i] -= B.far ? B.f : 0.0f;
-            }
-            float l = 0.0f;
+            for (int i = 1; i < 8; i++) top = fmaxf(top, x[i]);
+        }
+        if (!all) {
+            const int from = t + 4 * quarter, dh = my_hi - from, dl = my_lo - from, ds = p.sinks - from;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                x[s][i] = exp2_hw(fmaf(x[s][i], sc[s], neg));
-                l += x[s][i];
+                const int e = 16 * (i >> 2) + (i & 3);
+                x[i] = e <= dh && (e >= dl || e < ds) ? x[i] : -__builtin_inff();
             }
-            B.l += l;
+            top = x[0];
+#pragma unroll
+            for (int i = 1; i < 8; i++) top = fmaxf(top, x[i]);
         }
+        top = row_max(top);
+        // The reference, as in softmax_step: raised to the largest score where that exceeds it by more than 2^8, lowered (by 2^64 in
+        // all at most) to a block whose largest weight is below 2^-14. Weights stand 2^7 above it, in units of the largest scale.
+        const float d = (top - A.f) * sc, lift = 7.0f - (float)tl;
+        const bool fall = d < -14.0f && top > -__builtin_inff() && !A.far && A.m > A.most - 64.0f;
+        if (__any(d > (A.far ? 0.0f : 8.0f) || fall)) {
+            const bool move = d > (A.far ? 0.0f : 8.0f) || fall;
+            float y = top * sc;
+            const float bottom = A.most - 64.0f + lift;
+            const bool cut = fall && y < bottom;
+            y = cut ? bottom : y;
+            const float from = cut ? bottom * __builtin_amdgcn_rcpf(sc) : top;
+            const bool far = fabsf(y) > kFar;
+            const float r = (far ? y : ceilf(y)) - lift;
+            const float a = move ? exp2_hw(far && A.far ? (A.f - from) * sc : A.m - r) : 1.0f;  // from -Inf: 0
+            A.l *= a;
+#pragma unroll
+            for (int g = 0; g < NG; g++) A.o[g][0] *= a, A.o[g][1] *= a;
+            A.m = move ? r : A.m;
+            A.f = move ? from : A.f;
+            A.far = move ? far : A.far;
+            A.most = fmaxf(A.most, A.m);
+        }
+        const float neg = A.far ? lift : A.m == -__builtin_inff() ? 0.0f : -A.m;
+        if (__any(A.far)) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] -= A.far ? A.f : 0.0f;
+        }
+        float l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            x[i] = exp2_hw(fmaf(x[i], sc, neg));
+            l += x[i];
+        }
+        A.l += l;
 #pragma unroll
         for (int g = 0; g < NG; g++) {
             const u32x4 y = open8(v[0].codes[g]), z = open8(v[1].codes[g]), a0 = {y.x, y.z, z.x, z.z}, a1 = {y.y, y.w, z.y, z.w};
+            u32x4 hi, lo;
 #pragma unroll
-            for (int s = 0; s < NC; s++) {
-                u32x4 hi, lo;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int h = i >> 1, j = 2 * (i & 1);
-                    const float e0 = x[s][4 * h + j], e1 = x[s][4 * h + j + 1], d0 = v[h].scale(g, j), d1 = v[h].scale(g, j + 1);
-                    hi[i] = __builtin_bit_cast(uint32_t, (h2){(_Float16)fmaf(e0, d0, 0.0f), (_Float16)fmaf(e1, d1, 0.0f)});  // (fused: with the rounding in one instruction)
-                    // (hidden: the compiler would round the products anew for the second term, in another way)
-                    if (TWO) hi[i] = hide(hi[i]);
-                    const h2 f = __builtin_bit_cast(h2, (uint32_t)hi[i]);
-                    if (TWO) lo[i] = __builtin_bit_cast(uint32_t, (h2){(_Float16)fmaf(e0, d0, -(float)f[0]), (_Float16)fmaf(e1, d1, -(float)f[1])});
-                }
-                A[s].o[g][0] = mma16(a0, hi, A[s].o[g][0]);
-                A[s].o[g][1] = mma16(a1, hi, A[s].o[g][1]);
-                if (TWO) {
-                    A[s].o[g][0] = mma16(a0, lo, A[s].o[g][0]);
-                    A[s].o[g][1] = mma16(a1, lo, A[s].o[g][1]);
-                }
+            for (int i = 0; i < 4; i++) {
+                const int h = i >> 1, j = 2 * (i & 1);
+                const float e0 = x[4 * h + j], e1 = x[4 * h + j + 1], d0 = v[h].scale(g, j), d1 = v[h].scale(g, j + 1);
+                hi[i] = __builtin_bit_cast(uint32_t, (h2){(_Float16)fmaf(e0, d0, 0.0f), (_Float16)fmaf(e1, d1, 0.0f)});  // (fused: with the rounding in one instruction)
+                // (hidden: the compiler would round the products anew for the second term, in another way)
+                if (TWO) hi[i] = hide(hi[i]);
+                const h2 f = __builtin_bit_cast(h2, (uint32_t)hi[i]);
+                if (TWO) lo[i] = __builtin_bit_cast(uint32_t, (h2){(_Float16)fmaf(e0, d0, -(float)f[0]), (_Float16)fmaf(e1, d1, -(float)f[1])});
+            }
+            A.o[g][0] = mma16(a0, hi, A.o[g][0]);
+            A.o[g][1] = mma16(a1, hi, A.o[g][1]);
+            if (TWO) {
+                A.o[g][0] = mma16(a0, lo, A.o[g][0]);
+                A.o[g][1] = mma16(a1, lo, A.o[g][1]);
             }
         }
     }
@@ -416,19 +385,16 @@ template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves, per
     // the four waves' results, through LDS: rows, then references and sums
     float *mine = lds + w * (S::WAVE / 4);
     auto ml = [&](int u) { return reinterpret_cast<float2 *>(lds + u * (S::WAVE / 4) + S::ROWS * S::OSTRIDE); };
-#pragma unroll
-    for (int s = 0; s < NC; s++) {
-        const float l = row_sum(A[s].l);
-        const int r = 16 * s + c;
-        if (r >= n) continue;
+    const float l = row_sum(A.l);
+    if (c < n) {
 #pragma unroll
         for (int g = 0; g < NG; g++) {
-            const f4 a = A[s].o[g][0], b = A[s].o[g][1];
-            float *dst = mine + r * S::OSTRIDE + 32 * g + 8 * quarter;
+            const f4 a = A.o[g][0], b = A.o[g][1];
+            float *dst = mine + c * S::OSTRIDE + 32 * g + 8 * quarter;
             *reinterpret_cast<float4 *>(dst) = make_float4(a[0], b[0], a[1], b[1]);
             *reinterpret_cast<float4 *>(dst + 4) = make_float4(a[2], b[2], a[3], b[3]);
         }
-        if (quarter == 0) ml(w)[r] = make_float2(A[s].m, l);
+        if (quarter == 0) ml(w)[c] = make_float2(A.m, l);
     }
     __syncthreads();
     const bool direct = it.nsplit == 1;
@@ -456,27 +422,23 @@ template <int NG, int NC, bool BF> __global__ __launch_bounds__(64 * kWaves, per
         join_tile<S::DIM, S::ROWS, BF, kWaves>(p, it, r0, n, lds + 4, S::BYTES - 16);
 }
 
-template <int NG, int NC, bool BF> int launch_few(trhip_ctx *ctx, const AttnArgs &p, int64_t grid) {
-    const void *fn = reinterpret_cast<const void *>(attn4_few<NG, NC, BF>);
-    const int st = allow_dyn_lds(ctx, fn, Shape4<NG, NC>::BYTES, "kv4_attn");
+template <int NG, bool BF> int launch_few(trhip_ctx *ctx, const AttnArgs &p, int64_t grid) {
+    const void *fn = reinterpret_cast<const void *>(attn4_few<NG, BF>);
+    const int st = allow_dyn_lds(ctx, fn, Shape4<NG>::BYTES, "kv4_attn");
     if (st != TRHIP_OK) return st;
-    hipLaunchKernelGGL((attn4_few<NG, NC, BF>), dim3((unsigned)grid), dim3(64 * kWaves), (Shape4<NG, NC>::BYTES), ctx->stream, p);
+    hipLaunchKernelGGL((attn4_few<NG, BF>), dim3((unsigned)grid), dim3(64 * kWaves), (Shape4<NG>::BYTES), ctx->stream, p);
     return launch_check(ctx, "kv4_attn");
 }
-template <int NG> int launch_few(trhip_ctx *ctx, const AttnArgs &p, int sets, bool bf, int64_t grid) {
-    if (NG > kTwoSets || sets == 1) return bf ? launch_few<NG, 1, true>(ctx, p, grid) : launch_few<NG, 1, false>(ctx, p, grid);
-    else return bf ? launch_few<NG, NG <= kTwoSets ? 2 : 1, true>(ctx, p, grid) : launch_few<NG, NG <= kTwoSets ? 2 : 1, false>(ctx, p, grid);
-}
-int launch_few(trhip_ctx *ctx, const AttnArgs &p, int sets, bool bf, int64_t grid) {
+int launch_few(trhip_ctx *ctx, const AttnArgs &p, bool bf, int64_t grid) {
     switch (p.dim / 32) {
-    case 1: return launch_few<1>(ctx, p, sets, bf, grid);
-    case 2: return launch_few<2>(ctx, p, sets, bf, grid);
-    case 3: return launch_few<3>(ctx, p, sets, bf, grid);
-    case 4: return launch_few<4>(ctx, p, sets, bf, grid);
-    case 5: return launch_few<5>(ctx, p, sets, bf, grid);
-    case 6: return launch_few<6>(ctx, p, sets, bf, grid);
-    case 7: return launch_few<7>(ctx, p, sets, bf, grid);
-    default: return launch_few<8>(ctx, p, sets, bf, grid);
+    case 1: return bf ? launch_few<1, true>(ctx, p, grid) : launch_few<1, false>(ctx, p, grid);
+    case 2: return bf ? launch_few<2, true>(ctx, p, grid) : launch_few<2, false>(ctx, p, grid);
+    case 3: return bf ? launch_few<3, true>(ctx, p, grid) : launch_few<3, false>(ctx, p, grid);
+    case 4: return bf ? launch_few<4, true>(ctx, p, grid) : launch_few<4, false>(ctx, p, grid);
+    case 5: return bf ? launch_few<5, true>(ctx, p, grid) : launch_few<5, false>(ctx, p, grid);
+    case 6: return bf ? launch_few<6, true>(ctx, p, grid) : launch_few<6, false>(ctx, p, grid);
+    case 7: return bf ? launch_few<7, true>(ctx, p, grid) : launch_few<7, false>(ctx, p, grid);
+    default: return bf ? launch_few<8, true>(ctx, p, grid) : launch_few<8, false>(ctx, p, grid);
     }
 }
 
@@ -538,15 +500,15 @@ int launch_kv4_attn(trhip_ctx *ctx, const trhip_kv4 *kv, const AttnCall &c, int 
     }
     p.row_lo = 0;
     p.row_hi = image ? kTokMost : kAnyRows;
-    const int sets = (p.row_hi != kAnyRows || most_new * p.group > 16) && kv->dim <= 32 * kTwoSets ? 2 : 1, rows = 16 * sets, blocks = kv->dim / 32 * sets;
-    p.target = cus * per_cu(blocks);
+    const int rows = 16;
+    p.target = cus * per_cu(kv->dim / 32);
     const int64_t grid = plan_items(p, c, rows, kBlock, kLeast);
     if (grid >= ((int64_t)1 << 31)) return fail(ctx, TRHIP_ERR_INVALID, "kv4_attn: too many rows");
     int st = TRHIP_OK;
     float *ws = static_cast<float *>(workspace(ctx, (size_t)p.part_slots * rows * (kv->dim + 2) * sizeof(float), &st));
     if (!ws) return st;
     p.part = ws;
-    return launch_few(ctx, p, sets, io == TRHIP_BF16, grid);
+    return launch_few(ctx, p, io == TRHIP_BF16, grid);
 }
 
 }  // namespace trhip

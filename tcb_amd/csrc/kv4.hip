@@ -246,6 +246,7 @@ template <bool APPEND>
 int launch(trhip_ctx *ctx, const trhip_kv4 *kv, int64_t tokens, void *k, void *v, int io, int64_t stride, const int *slots) {
     const int64_t size = io == TRHIP_F32 ? 4 : 2;
     const bool wide = reinterpret_cast<uintptr_t>(k) % 16 == 0 && reinterpret_cast<uintptr_t>(v) % 16 == 0 && stride * size % 16 == 0;
+    // (8192 tokens: in 15.8 us, with one token a workgroup 34; few tokens go faster on a workgroup each, 6.0 us against 6.2)
     const int run = tokens >= 256 ? 4 : 1;
     const Kv4Args p = {static_cast<uint8_t *>(kv->k), static_cast<uint8_t *>(kv->v), __builtin_ctz((unsigned)kv->page), kv->heads, kv->dim,
                        kv->pages * kv->page, stride, (int)tokens, wide, run, slots};
