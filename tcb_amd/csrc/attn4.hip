@@ -14,6 +14,11 @@
 //   O^T += V^T P^T: the value's scale goes to the weight, w = p s (there is one product a block of 32 elements).
 // The weights p s stand in f16, in one term for bf16 results (their rounding of 2^-12 is a sixteenth of the result's) and in two
 // for f16 ones. So that they neither overflow nor vanish, the softmax's reference includes the largest scale the wave has met.
+//
+// A wave copies its next pieces into LDS while it works (two blocks ahead; loads into registers instead: 64 x 8192 tokens 119 us against 97 at
+// that step). What bounds it is its instructions beside the bytes: 64 tokens of 32 heads on 8 of 128, up to 8192 keys, bf16: 77 to 82 us
+// (3.7 to 3.9 TB/s of codes and scales), vector units busy half the time, matrix units a twelfth. A token over 131071 keys, f16: 46 to 48 us;
+// over 300 keys: 8.7, most of it the chain of one block after the other.
 #include "attn4_image.hpp"
 #include "attn_plan.hpp"
 #include "kv4.hpp"
@@ -26,7 +31,10 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x3 __attribute__((ext_vector_type(3)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 
-constexpr int64_t kMostImage = (int64_t)2 << 30;  // bytes of a plane of opened keys at most: a hundredth of the memory
+// Bytes of a plane of opened keys at most: with both a seventieth of the memory. Where the keys of long requests are opened first, a prompt of
+// 8192 tokens takes 525 us, read as they are 1278; 8 prompts of up to 901 beside 32 tokens, window 1000: 87 and 105.
+constexpr int64_t kMostImage = (int64_t)2 << 30;
+// kLeast, kOver: blocks of a piece at least and what a piece costs beside them, in blocks; half and twice of either made no difference.
 constexpr int kWaves = 4, kBlock = 32, kLeast = 8, kOver = 6;
 
 // Workgroups a CU, by registers (blocks of 32 elements in a row). 64 x 8192 tokens, heads of 128, take 90 us with one and 76 with three; 32 x 4096

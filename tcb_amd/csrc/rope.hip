@@ -1,7 +1,8 @@
 // rope.hip -- rotary positions with up to four axes: pair i of a head's elements is turned by pos[axis(i)][t] * frequency(i).
 //
 // A workgroup takes one or four tokens and some of their heads: first the sines and cosines of the tokens' pairs, once for all heads, into
-// LDS, then the heads, 16 bytes a load. Every element moves once in and once out, which is what bounds it.
+// LDS, then the heads, 16 bytes a load. Every element moves once in and once out, which is what bounds it: 8192 tokens of 40 heads of 128 in bf16
+// take 38 us (4.4 TB/s), 16 tokens 4.6, a launch. (Angles by every head anew, 64-bit arithmetic each: 72 us.)
 #include "trhip_internal.hpp"
 
 #include <cmath>

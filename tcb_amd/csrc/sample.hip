@@ -12,7 +12,11 @@
 // times: the bin in which the run ends is opened until its entries can be sorted, then all stripes are weighed.
 //
 // Weights and their sums are in 64 bits, since one border among a hundred thousand has to be met: e^x by a table of 64 powers and a
-// polynomial of degree 5, ten operations.
+// polynomial of degree 5.
+//
+// 1 x 128256, fp32: 10 us without a filter, 16 with top_k 50, 18 with top_p .85 (two launches, the second one's chain of steps by one workgroup);
+// a flat row of which thousands are kept 104, by one CU that reads the row twice more. 256 x 128256: 33 us for the largest (4 TB/s), 54 without a
+// filter, 45 with top_k 50, 87 with top_p .85, where the bins' atomics in LDS bound the first launch.
 #include "trhip_internal.hpp"
 
 namespace trhip {
@@ -151,6 +155,8 @@ __device__ __forceinline__ Setting setting_of(const SampleArgs &p, int r) {
 // How many entries of the whole row its workgroups should cover, and a workgroup's share of them: the mean, three standard deviations of
 // entries that lie anywhere, and four. (Four and six left no room for k 293 of 1 x 128256, 32 workgroups, in the 1024 that are sorted:
 // 112 us by reading again, 31 so.)
+// Without top_k the run of top_p is unknown: 128 entries (with 64, 256 x 128256 of top_p .95 take 144 us against 105, with 256, 1 x 128256 takes
+// 35 against 32).
 constexpr int kCover = 128;
 __device__ __forceinline__ int share_of(int n, int groups) {
     const float m = (float)n * __builtin_amdgcn_rcpf((float)groups);
@@ -663,7 +669,7 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
     int bits = 62;
     while ((p.vocab - 1) >> (62 - bits)) bits--;
     const double unit = __longlong_as_double((long long)(1023 + bits) << 52);
-    constexpr int AT = 2;
+    constexpr int AT = 2;  // (four: registers spill, 256 x 128256 with flat rows among them 187 us against 180)
     auto kept_at = [&](float f, int i) { return f > cut || (f == cut && i <= last); };  // (values: NaN is never kept)
     auto each = [&](auto use) {  // use(first of four, values) for every four entries, a wave's stripes one after the other
         for (int b0 = w; b0 < p.stripes; b0 += AT * kWaves) {
@@ -893,12 +899,15 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
 int launch_sample(trhip_ctx *ctx, const void *logits, int io, int64_t stride, int64_t rows, int64_t vocab, const float *temperature,
                   const int *top_k, const float *top_p, const float *min_p, const float *u, int *token, float *logprob) {
     const int64_t cus = ctx->sm_count > 0 ? ctx->sm_count : 256, stripes = (vocab + kStripe - 1) / kStripe, esize = io == TRHIP_F32 ? 4 : 2;
-    // stripes a wave: few for few rows, so that they lie on many CUs
+    // stripes a wave: few for few rows, so that they lie on many CUs (16 x 151936: twice as many workgroups, four a wave, 14.3 us without a
+    // filter, eight 15.7), many for many, whose workgroups' entries and bins are fewer (256 x 128256, top_k 50: eight 44.6 us, four 48.4)
     constexpr int WAVES = kRead / 64;
     int64_t each = 1;
     auto groups_of = [&](int64_t j) { return (stripes + WAVES * j - 1) / (WAVES * j); };
     while (each < 8 && rows * groups_of(each) > 2 * cus) each *= 2;
-    while (each < 8 && groups_of(each) > 32) each *= 2;  // (a workgroup's share of a row's largest entries has a part that does not shrink)
+    // (a workgroup's share of a row's largest entries has a part that does not shrink: 1 x 128256 on 63 workgroups leaves too many of k 293
+    // to sort, 119 us against 31; on 16 it takes 11.3 without a filter against 10.0)
+    while (each < 8 && groups_of(each) > 32) each *= 2;
     const int64_t groups = groups_of(each);  // (at most 1024: one a thread of the second launch)
     const double mean = (double)kMost / 2 / (double)groups;
     int64_t room = (int64_t)(mean + 3.0 * __builtin_sqrt(mean) + 4.0) * 3 / 2 + 16;
