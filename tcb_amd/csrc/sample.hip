@@ -14,9 +14,9 @@
 // Weights and their sums are in 64 bits, since one border among a hundred thousand has to be met: e^x by a table of 64 powers and a
 // polynomial of degree 5.
 //
-// 1 x 128256, fp32: 10 us without a filter, 16 with top_k 50, 18 with top_p .85 (two launches, the second one's chain of steps by one workgroup);
-// a flat row of which thousands are kept 104, by one CU that reads the row twice more. 256 x 128256: 33 us for the largest (4 TB/s), 54 without a
-// filter, 45 with top_k 50, 87 with top_p .85, where the bins' atomics in LDS bound the first launch.
+// 1 x 128256, fp32: 10 us without a filter, 13 with top_k 50, 17 with top_p .85 (two launches, the second one's chain of steps by one workgroup);
+// a flat row of which thousands are kept 102, by one CU that reads the row twice more. 256 x 128256: 34 us for the largest (4 TB/s), 54 without a
+// filter, 42 with top_k 50, 87 with top_p .85, where the bins' atomics in LDS bound the first launch.
 #include "trhip_internal.hpp"
 
 namespace trhip {
@@ -154,9 +154,9 @@ __device__ __forceinline__ Setting setting_of(const SampleArgs &p, int r) {
 }
 // How many entries of the whole row its workgroups should cover, and a workgroup's share of them: the mean, three standard deviations of
 // entries that lie anywhere, and four. (Four and six left no room for k 293 of 1 x 128256, 32 workgroups, in the 1024 that are sorted:
-// 112 us by reading again, 31 so.)
+// 112 us by reading again, 23 so.)
 // Without top_k the run of top_p is unknown: 128 entries (with 64, 256 x 128256 of top_p .95 take 144 us against 105, with 256, 1 x 128256 takes
-// 35 against 32).
+// 35 against 32 then).
 constexpr int kCover = 128;
 __device__ __forceinline__ int share_of(int n, int groups) {
     const float m = (float)n * __builtin_amdgcn_rcpf((float)groups);
@@ -395,22 +395,63 @@ __device__ __forceinline__ int last_of(bool is, Lds &s) {
     return (int)all_max(m ? (threadIdx.x & ~63) + 64 - __builtin_clzll(m) : 0, s) - 1;
 }
 
-// Sorts s.sorted[0 .. n), padded to a power of two with 0 (falling) or ~0: largest first, or smallest.
+// The value of lane ^ J.
+template <int J> __device__ __forceinline__ uint32_t across(uint32_t v) {
+    if constexpr (J == 1) return moved<0xB1, 0xF>(v);        // quads 1 0 3 2
+    else if constexpr (J == 2) return moved<0x4E, 0xF>(v);   // 2 3 0 1
+    else if constexpr (J == 4) return moved<0x1B, 0xF>(moved<0x141, 0xF>(v));  // eights the other way round, then quads
+    else if constexpr (J == 8) return moved<0x128, 0xF>(v);  // rows of sixteen by eight
+    else {
+        const auto s = J == 16 ? __builtin_amdgcn_permlane16_swap(v, v, false, false) : __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return threadIdx.x & J ? s[0] : s[1];
+    }
+}
+__device__ __forceinline__ void order(unsigned long long &v, unsigned long long o, bool larger) {
+    const bool is = o > v;
+    v = is == larger ? o : v;
+}
+// One step of a bitonic sort between lanes: blocks of k fall where `falling` (this thread's block) holds.
+template <int J> __device__ __forceinline__ void step(unsigned long long &v, bool falling) {
+    const unsigned long long o = ((unsigned long long)across<J>((uint32_t)(v >> 32)) << 32) | across<J>((uint32_t)v);
+    order(v, o, ((threadIdx.x & J) == 0) == falling);
+}
+
+// The steps of blocks of k that stay within a wave.
+__device__ __forceinline__ void steps(unsigned long long &v, int k, bool falling) {
+    if (k >= 64) step<32>(v, falling);
+    if (k >= 32) step<16>(v, falling);
+    if (k >= 16) step<8>(v, falling);
+    if (k >= 8) step<4>(v, falling);
+    if (k >= 4) step<2>(v, falling);
+    step<1>(v, falling);
+}
+// The wave's 64 values in order.
+__device__ __forceinline__ void wave_sort(unsigned long long &v, bool falling) {
+#pragma unroll
+    for (int k = 2; k <= 64; k <<= 1) steps(v, k, ((threadIdx.x & 63 & k) == 0) == falling);
+}
+
+// Sorts s.sorted[0 .. n), padded to a power of two with 0 (falling) or ~0: largest first, or smallest. A thread has an entry; steps
+// within a wave move it between lanes, only those between waves go through LDS (10 of 55 for 1024 entries: 9 us with all of them).
 __device__ __forceinline__ void sort(Lds &s, int n, bool falling) {
+    static_assert(kEnd == kMost, "an entry a thread");
+    const int tid = threadIdx.x;
     int n2 = 2;
     while (n2 < n) n2 <<= 1;
     __syncthreads();
-    for (int i = n + threadIdx.x; i < n2; i += kEnd) s.sorted[i] = falling ? 0 : ~0ull;
-    for (int k = 2; k <= n2; k <<= 1)
-        for (int j = k >> 1; j; j >>= 1) {
+    unsigned long long v = tid < n ? s.sorted[tid] : falling ? 0 : ~0ull;
+    for (int k = 2; k <= n2; k <<= 1) {
+        const bool falls = ((tid & k) == 0) == falling;
+        for (int j = k >> 1; j >= 64; j >>= 1) {
             __syncthreads();
-            if ((int)threadIdx.x < n2 / 2) {
-                const int i = threadIdx.x, a = 2 * i - (i & (j - 1)), b = a + j;
-                const unsigned long long x = s.sorted[a], y = s.sorted[b];
-                const bool down = ((a & k) == 0) == falling;
-                if (down ? x < y : x > y) s.sorted[a] = y, s.sorted[b] = x;
-            }
+            if (tid < n2) s.sorted[tid] = v;
+            __syncthreads();
+            if (tid < n2) order(v, s.sorted[tid ^ j], ((tid & j) == 0) == falls);
         }
+        if ((tid & ~63) < n2) steps(v, k, falls);
+    }
+    __syncthreads();
+    if (tid < n2) s.sorted[tid] = v;
     __syncthreads();
 }
 
@@ -512,16 +553,7 @@ __device__ __forceinline__ bool top64(const SampleArgs &p, int r, const Weight &
     }
     __builtin_amdgcn_wave_barrier();
     unsigned long long e = lane < count ? some[lane] : 0;
-    // to its rank
-    int rank = 0;
-    for (int i = 0; i < count; i++) {
-        const unsigned long long o = ((unsigned long long)of_lane((uint32_t)(e >> 32), i) << 32) | of_lane((uint32_t)e, i);
-        rank += o > e;
-    }
-    __builtin_amdgcn_wave_barrier();
-    if (lane < count) some[rank] = e;
-    __builtin_amdgcn_wave_barrier();
-    e = lane < count ? some[lane] : 0;
+    wave_sort(e, true);
     const uint32_t key = (uint32_t)(e >> 32), index = ~(uint32_t)e;
     const bool in = lane < count && (st.k == 0 || lane < st.k);
     const double w = in ? wt(key) : 0.0, incl = running(w), before = before_lane(incl), sum = of_lane(incl, 63);
@@ -535,19 +567,14 @@ __device__ __forceinline__ bool top64(const SampleArgs &p, int r, const Weight &
         if (kept > certain || (kept == certain && kept != st.k)) return false;  // (the run may go on past what is here)
         if (st.k > 0 && st.tp < 1.0f && certain < st.k) return false;           // (nor is the sum certain)
     }
-    // the running sum by index, of each kept entry: over the ones of no larger index
-    double run = 0, kept_sum = 0;
-    for (int i = 0; i < kept; i++) {
-        const double y = of_lane(w, i);
-        run += of_lane(index, i) <= index ? y : 0.0;
-        kept_sum += y;
-    }
-    const double goal_u = st.u * kept_sum;
-    // the lowest index that is over the goal, or the highest that has weight
-    const bool over = lane < kept && run > goal_u, has = lane < kept && w > 0;
-    const uint32_t a = ~wave_max(over ? ~index : 0u), b = wave_max(has ? index + 1 : 0u) - 1;
-    const uint32_t token = __ballot(over) ? a : b;
-    if (lane < kept && index == token) result(p, r, (int)token, w, kept_sum);
+    // the kept ones by index, and their running sum
+    unsigned long long by = lane < kept ? ((unsigned long long)index << 32) | (uint32_t)lane : ~0ull;
+    wave_sort(by, false);
+    const double v = __shfl(w, (int)((uint32_t)by & 63));
+    const double y = lane < kept ? v : 0.0, run = running(y), kept_sum = of_lane(run, 63);
+    // the first that is over the goal, or the last that has weight
+    const uint64_t over = __ballot(run > st.u * kept_sum), has = __ballot(y > 0);
+    if (lane == (over ? __builtin_ctzll(over) : 63 - __builtin_clzll(has))) result(p, r, (int)(by >> 32), y, kept_sum);
     return true;
 }
 
@@ -900,13 +927,13 @@ int launch_sample(trhip_ctx *ctx, const void *logits, int io, int64_t stride, in
                   const int *top_k, const float *top_p, const float *min_p, const float *u, int *token, float *logprob) {
     const int64_t cus = ctx->sm_count > 0 ? ctx->sm_count : 256, stripes = (vocab + kStripe - 1) / kStripe, esize = io == TRHIP_F32 ? 4 : 2;
     // stripes a wave: few for few rows, so that they lie on many CUs (16 x 151936: twice as many workgroups, four a wave, 14.3 us without a
-    // filter, eight 15.7), many for many, whose workgroups' entries and bins are fewer (256 x 128256, top_k 50: eight 44.6 us, four 48.4)
+    // filter, eight 15.7), many for many, whose workgroups' entries and bins are fewer (256 x 128256, top_k 50: eight 45 us, four 48)
     constexpr int WAVES = kRead / 64;
     int64_t each = 1;
     auto groups_of = [&](int64_t j) { return (stripes + WAVES * j - 1) / (WAVES * j); };
     while (each < 8 && rows * groups_of(each) > 2 * cus) each *= 2;
     // (a workgroup's share of a row's largest entries has a part that does not shrink: 1 x 128256 on 63 workgroups leaves too many of k 293
-    // to sort, 119 us against 31; on 16 it takes 11.3 without a filter against 10.0)
+    // to sort, 119 us against 23; on 16 it takes 11.3 without a filter against 10.0)
     while (each < 8 && groups_of(each) > 32) each *= 2;
     const int64_t groups = groups_of(each);  // (at most 1024: one a thread of the second launch)
     const double mean = (double)kMost / 2 / (double)groups;
