@@ -358,8 +358,8 @@ int trhip_kv4_read(trhip_ctx *ctx, const trhip_kv4 *kv, int64_t tokens, void *k,
  * keys may be opened, as trhip_attn's; else to f16 for bf16 results and to two f16 numbers (2^-21) for f16 ones. Where the hint allows requests of more
  * than 96 rows, their keys are opened into the context's workspace in 16 bits
  * (exactly, where trhip_kv4_append wrote the scales, else rounded once): as many times max_pages pages (2 * page * heads * dim
- * bytes a plane) as the tokens can make such requests, if that is no more than 2 GiB a plane; beyond it, or with a hint that is too
- * small, they are read as they are, which takes up to five times as long. */
+ * bytes a plane) as the tokens can make such requests, if that is no more than 2 GiB a plane; beyond it, with a hint that is too
+ * small (both take up to five times as long) and in small calls they are read as they are. */
 int trhip_kv4_attn(trhip_ctx *ctx, const trhip_kv4 *kv, const void *q, int type, int64_t q_stride, void *out, int64_t out_stride,
                    int64_t tokens, int heads, int64_t nreq, const int32_t *q_start, const int32_t *kv_len,
                    const int32_t *table, int64_t max_pages, int64_t max_new, int64_t window, int64_t sinks, float scale);

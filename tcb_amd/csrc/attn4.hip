@@ -34,6 +34,12 @@ typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 // Bytes of a plane of opened keys at most: with both a seventieth of the memory. Where the keys of long requests are opened first, a prompt of
 // 8192 tokens takes 525 us, read as they are 1278; 8 prompts of up to 901 beside 32 tokens, window 1000: 87 and 105.
 constexpr int64_t kMostImage = (int64_t)2 << 30;
+// Calls so small that the two launches more and the other kernel's long tiles would not pay, by what the kernel of few rows has to do at most:
+// its tiles times the keys that one sees, a tile's start and end being as long as some 136 keys, times the elements of a head. A prompt of
+// 128 tokens 7.5 us against 22 with its keys opened, 6 of up to 523 behind a window of 21 11 against 57, 4 of 128 behind 1000 keys 19 against
+// 40; beyond it 1 of 1024 44 against 38, 1 of 2000 behind a window of 100 48 against 38, 64 tokens behind 8192 keys 54 against 47.
+constexpr double kSmall = 0x1p20 * 128;
+constexpr int kTileKeys = 136;
 // kLeast, kOver: blocks of a piece at least and what a piece costs beside them, in blocks; half and twice of either made no difference.
 constexpr int kWaves = 4, kBlock = 32, kLeast = 8, kOver = 6;
 
@@ -486,8 +492,10 @@ int launch_kv4_attn(trhip_ctx *ctx, const trhip_kv4 *kv, const AttnCall &c, int 
     // Requests of more than kTokMost rows: their keys go to the workspace in 16 bits and the 16-bit cache's kernel of many rows takes
     // them, where the workspace may hold the longest ones that the sizes allow. Which there are is known only from the hint.
     const int64_t most_long = c.tokens * p.group / (kTokMost + 1), longs = most_long < c.nreq ? most_long : c.nreq;
+    const double cap = (double)c.max_pages * kv->page, window = (double)c.window + (double)c.sinks + 16, seen = c.window > 0 && window < cap ? window : cap;
+    const double tiles = ((double)c.tokens * p.group / 16 + (double)c.nreq) * kv->heads;
     const double image_bytes = (double)longs * (double)c.max_pages * (double)p.page_bytes * (32.0 / 9.0);
-    const bool image = most_new * p.group > kTokMost && longs > 0 && longs < 65536 && p.kv_heads < 65536 && c.max_pages > 0 && image_bytes <= (double)kMostImage &&
+    const bool image = most_new * p.group > kTokMost && tiles * (seen + kTileKeys) * kv->dim > kSmall && longs > 0 && longs < 65536 && p.kv_heads < 65536 && c.max_pages > 0 && image_bytes <= (double)kMostImage &&
                        (double)c.nreq * (double)c.max_pages <= (double)(kMostImage / 4);
     if (image) {
         const int64_t plane = (longs * c.max_pages * (p.page_bytes / 9 * 32) + 255) & ~(int64_t)255, tables = c.nreq * c.max_pages * 4;

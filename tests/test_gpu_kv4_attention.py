@@ -56,8 +56,14 @@ class Batch:
     def planes(self):
         return [torch.from_numpy(K4.pack(c, d, w)).to(DEV) for c, d, w in zip(self.codes, self.scales, (False, True))]
 
-    def run(self, tb, window=0, sinks=0, scale=None, max_new=None, pad=0, shift=0, out_pad=0, out_shift=0):
-        """The operator's rows as float32 [tokens, heads, dim]; pad, shift: elements between rows and in front."""
+    def wide_table(self):
+        tiles = (self.tokens * self.heads // self.kv_heads // 16 + len(self.kv)) * self.kv_heads
+        most = max(self.most, 2 ** 27 // (tiles * self.dim * self.page) + 2)
+        return np.concatenate([self.table, np.full((len(self.kv), most - self.most), -7, np.int32)], 1)
+
+    def run(self, tb, window=0, sinks=0, scale=None, max_new=None, pad=0, shift=0, out_pad=0, out_shift=0, wide=False):
+        """The operator's rows as float32 [tokens, heads, dim]; pad, shift: elements between rows and in front; wide: a table so wide that
+        the call counts as a large one, whose long requests' keys are opened first."""
         width = self.heads * self.dim
         q = torch.zeros(shift + self.tokens * (width + pad) + 8, dtype=TORCH[self.dtype], device=DEV)
         rows = q[shift:shift + self.tokens * (width + pad)].view(self.tokens, width + pad)
@@ -65,12 +71,13 @@ class Batch:
         out = torch.full((out_shift + self.tokens * (width + out_pad) + 8,), 7.0, dtype=TORCH[self.dtype], device=DEV)
         k, v = self.planes()
         start, lens = torch.from_numpy(self.start).to(DEV), torch.tensor(self.kv, dtype=torch.int32, device=DEV)
-        table = torch.from_numpy(self.table).to(DEV)
+        table = self.wide_table() if wide else self.table
+        most, table = table.shape[1], torch.from_numpy(table).to(DEV)
         kv = tcb_amd.KV4Cache(k.shape[0], self.page, self.kv_heads, self.dim, k.data_ptr(), v.data_ptr())
         max_new = max(self.new) if max_new is None else max_new
         torch.cuda.synchronize()
         tb.KV4Attention(kv, q.data_ptr() + 2 * shift, CODE[self.dtype], width + pad, out.data_ptr() + 2 * out_shift, width + out_pad, self.tokens, self.heads,
-                        len(self.kv), start.data_ptr(), lens.data_ptr(), table.data_ptr(), self.most, max_new=max_new, window=window, sinks=sinks, scale=scale)
+                        len(self.kv), start.data_ptr(), lens.data_ptr(), table.data_ptr(), most, max_new=max_new, window=window, sinks=sinks, scale=scale)
         tb.ctx.sync()
         whole = out[out_shift:out_shift + self.tokens * (width + out_pad)].view(self.tokens, width + out_pad)
         assert (whole[:, width:] == 7.0).all() and (out[:out_shift] == 7.0).all() and (out[out_shift + whole.numel():] == 7.0).all()
@@ -89,8 +96,11 @@ class Batch:
             tols.append(K4.bound(self.dtype, self.dim, m, n * (self.heads // self.kv_heads) > 96, o, spread, reach, largest))
         return np.concatenate(outs), np.concatenate(tols)
 
-    def check(self, tb, window=0, sinks=0, scale=None, **how):
-        got = self.run(tb, window, sinks, scale, **how)
+    def check(self, tb, window=0, sinks=0, scale=None, wide=False, **how):
+        """Twice, where there are long requests: as a small call and as a large one."""
+        if not wide and not window and max(self.new) * self.heads // self.kv_heads > 96:
+            self.check(tb, window, sinks, scale, True, **how)
+        got = self.run(tb, window, sinks, scale, wide=wide, **how)
         want, tol = self.want(window, sinks, scale)
         off = np.abs(got - want) - tol
         assert np.isfinite(want).all()
@@ -165,16 +175,43 @@ def test_windows(backend, dtype, window, sinks):
     assert (np.abs(b2 - want) <= tol).all()
 
 
+@pytest.mark.parametrize("dtype,window,sinks", [("bf16", 1, 0), ("f16", 33, 5), ("bf16", 100, 0), ("f16", 100, 70), ("bf16", 500, 17), ("f16", 2000, 4)])
+def test_windows_of_large_calls(backend, dtype, window, sinks):
+    """Windows over prompts whose keys are opened first (some of their tokens are compared). What no token of a request sees is not finite, and
+    page entries there are out of range."""
+    new, lens = [1300, 1, 900, 1300, 40], [1300, 50, 1500, 2205, 90]
+    b = Batch(dtype, 32, 8, 128, 16, new, lens, seed=window)
+    clean = [c.copy() for c in b.scales]
+    table = b.table.copy()
+    for i, (n, m) in enumerate(zip(new, lens)):
+        for j in range(sinks, max(m - n - window + 1, 0)):
+            for d in b.scales:
+                d[table[i, j // 16], :, j % 16] = np.float16("nan")
+        for j in range(-(-sinks // 16), max(m - n - window + 1, 0) // 16):
+            b.table[i, j] = 2 ** 31 - 1 - j
+    got = b.run(backend, window, sinks)
+    b.scales, b.table = clean, table
+    k, v = b.values()
+    for i, (n, m) in enumerate(zip(new, lens)):
+        kk, vv = (R.rows_of(c, table[i], m, 16) for c in (k, v))
+        for t in sorted({0, min(1, n - 1), max(n - 2, 0), n - 1, window % n, (window + 1) % n} | set(range(7, n, 211))):
+            q = b.q[b.start[i] + t:b.start[i] + t + 1].float().numpy()
+            o, spread, reach = R.attend(q, kk, vv, m - n + t, 128 ** -0.5, window, sinks)
+            tol = K4.bound(dtype, 128, m, n * 4 > 96, o, spread, reach, np.abs(np.nan_to_num(vv)).max())
+            assert (np.abs(got[b.start[i] + t] - o[0]) <= tol[0]).all(), (i, t)
+
+
 def test_tokens_that_see_nothing(backend):
     """More tokens than keys: the first rows are zeros. Requests without tokens, without keys."""
     for new, kv in [([3, 1], [2, 0]), ([40, 0, 2], [5, 9, 0]), ([200], [100]), ([1], [-4])]:
-        got = Batch("bf16", 8, 2, 64, 16, new, kv).run(backend)
         want, tol = Batch("bf16", 8, 2, 64, 16, new, [max(n, 0) for n in kv]).want()
-        assert (np.abs(got - want) <= tol).all()
-        at = 0
-        for n, m in zip(new, kv):
-            assert (got[at:at + max(0, n - max(m, 0))] == 0).all()
-            at += n
+        for wide in (False, True):
+            got = Batch("bf16", 8, 2, 64, 16, new, kv).run(backend, wide=wide)
+            assert (np.abs(got - want) <= tol).all()
+            at = 0
+            for n, m in zip(new, kv):
+                assert (got[at:at + max(0, n - max(m, 0))] == 0).all()
+                at += n
 
 
 def test_rows_outside_every_request(backend):
@@ -184,10 +221,12 @@ def test_rows_outside_every_request(backend):
         want, tol = c.want()
         c.table, c.kv = c.table[[0, 2]], [c.kv[0], c.kv[2]]
         c.start = np.array([0, 2, 2 + n + 2], np.int32)  # the second request takes the tokens in between as its own first ones
-        off = np.abs(c.run(backend) - want) - tol  # (its last two tokens see what they saw, by another kernel where there are many)
-        assert off[:2].max() <= 0 and off[-2:].max() <= 0
+        for wide in (False, True):
+            off = np.abs(c.run(backend, wide=wide) - want) - tol  # (its last two tokens see what they saw, by another kernel where there are many)
+            assert off[:2].max() <= 0 and off[-2:].max() <= 0
         c.table, c.kv, c.start = c.table[:1], c.kv[:1], np.array([0, 2], np.int32)
-        assert (c.run(backend)[2:] == 7).all()
+        for wide in (False, True):
+            assert (c.run(backend, wide=wide)[2:] == 7).all()
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
@@ -211,14 +250,15 @@ def test_pages_out_of_range(backend):
             b.codes[i], b.scales[i] = b.codes[i][:-1], b.scales[i][:-1]
         for bad in (z, -1, 2 ** 31 - 1, -2 ** 31):
             b.table[0, 2] = b.table[1, 0] = bad
-            assert (np.abs(b.run(backend) - want) <= tol).all()
+            for wide in (False, True):
+                assert (np.abs(b.run(backend, wide=wide) - want) <= tol).all()
 
 
 @pytest.mark.parametrize("new,kv", [([1, 1, 1], [70, 40, 333]), ([30, 1, 5], [70, 40, 333]), ([300, 1, 120], [350, 40, 120])])
 def test_blocks_that_are_not_finite(backend, new, kv):
     """A value's block with scale NaN or Inf: NaN in its elements for every token that sees it, nothing for the others; a key's: the whole
     row of the heads that read it."""
-    for window, sinks in ((0, 0), (50, 3)):
+    for window, sinks, wide in ((0, 0, False), (0, 0, True), (50, 3, False)):
         for which in range(2):
             b = Batch("bf16", 8, 2, 96, 16, new, kv, seed=4)
             hit = []
@@ -231,7 +271,7 @@ def test_blocks_that_are_not_finite(backend, new, kv):
                     if R.visible(kv[i] - new[i] + t, j, window, sinks):
                         a = slice(None) if which == 0 else slice(32 * block, 32 * block + 32)
                         want[b.start[i] + t, 4 * head:4 * head + 4, a] = True
-            got = b.run(backend, window, sinks)
+            got = b.run(backend, window, sinks, wide=wide)
             assert np.array_equal(np.isnan(got), want) and not np.isinf(got).any()
             for i, j, head, block in hit:
                 b.scales[which][b.table[i, j // 16], head, j % 16, block] = 0
@@ -248,7 +288,7 @@ def test_scales_that_append_does_not_write(backend, dtype):
     b = Batch(dtype, 8, 2, 96, 32, [1, 3, 40, 130], [70, 333, 300, 513], seed=21, size=0.5)
     rng = np.random.default_rng(2)
     b.scales = [np.where(np.isnan(d), d, (d.astype(np.float64) * (1 + rng.random(d.shape) / 16)).astype(np.float16)) for d in b.scales]
-    got, (want, tol) = b.run(backend), b.want()
+    want, tol = b.want()
     k, v = b.values()
     for i, (n, m) in enumerate(zip(b.new, b.kv)):
         if n * 4 > 96:
@@ -256,7 +296,8 @@ def test_scales_that_append_does_not_write(backend, dtype):
             _, spread, reach = R.attend(b.q[b.start[i]:b.start[i + 1]].float().numpy(), kk, vv, m - n, b.dim ** -0.5)
             half = K4.HALF[dtype]
             tol[b.start[i]:b.start[i + 1]] += (1 + half) * half * spread * (1 + 2 * reach)
-    assert (np.abs(got - want) <= tol).all()
+    for wide in (False, True):
+        assert (np.abs(b.run(backend, wide=wide) - want) <= tol).all()
 
 
 def test_sizes_of_values(backend):
@@ -305,13 +346,15 @@ def test_far_scores(backend):
             for scale in (1e-20, 1e-3, 1.0, 30.0):
                 b = Batch(dtype, 4, 1, 64, 16, [new], [300], seed=9)
                 want, _ = b.want(scale=scale)
-                got = b.run(backend, scale=scale)
                 _, tol = b.want(scale=scale)
-                assert (np.abs(got - want) <= np.minimum(tol, 50)).all()
+                for wide in (False, True):
+                    assert (np.abs(b.run(backend, scale=scale, wide=wide) - want) <= np.minimum(tol, 50)).all()
             b = Batch(dtype, 4, 1, 64, 16, [new], [300], seed=10)
             b.q = (b.q.float() * 1000).to(TORCH[dtype])
-            got, (want, tol) = b.run(backend), b.want()
-            assert np.isfinite(got).all() and (np.abs(got - want) <= np.minimum(tol, 50)).all()
+            want, tol = b.want()
+            for wide in (False, True):
+                got = b.run(backend, wide=wide)
+                assert np.isfinite(got).all() and (np.abs(got - want) <= np.minimum(tol, 50)).all()
 
 
 def test_q_of_any_size(backend):
@@ -329,11 +372,11 @@ def test_q_of_any_size(backend):
 
 def test_q_that_is_not_finite(backend):
     """A NaN in a row of q is NaN in that head's row, and nowhere else."""
-    for new, kv in (([2, 1], [50, 20]), ([60, 1], [70, 20])):
+    for new, kv, wide in (([2, 1], [50, 20], False), ([60, 1], [70, 20], False), ([60, 1], [70, 20], True)):
         b = Batch("bf16", 8, 2, 64, 16, new, kv, seed=12)
-        clean = b.run(backend)
+        clean = b.run(backend, wide=wide)
         b.q[1, 3, 5] = float("nan")
-        got = b.run(backend)
+        got = b.run(backend, wide=wide)
         want = np.zeros(got.shape, bool)
         want[1, 3] = True
         assert np.array_equal(np.isnan(got), want) and np.array_equal(got[~want], clean[~want])
@@ -365,22 +408,26 @@ def test_starts_and_lengths_of_any_kind(backend):
     """Starts out of order, negative, past the tokens; lengths past the table: nothing is read or written out of range."""
     b = Batch("bf16", 8, 2, 64, 16, [1, 4, 9, 150], [40, 60, 9, 160], seed=14, poison=False)
     b.table = np.where(b.table < 0, 0, b.table)
-    good, start, kv = b.run(backend), b.start.copy(), list(b.kv)
-    for bad in ([0, -5, 400, 3, 164], [164, 14, 5, 1, 0], [2 ** 31 - 1, -2 ** 31, 7, 0, 2 ** 31 - 1], [0, 164, 0, 164, 0]):
-        b.start = np.array(bad, np.int32)
-        b.run(backend)
-    b.start, b.kv = start, [2 ** 31 - 1, -2 ** 31, 10 ** 6, 161]
-    b.run(backend)
-    b.kv = kv
-    assert np.array_equal(b.run(backend), good)
+    start, kv = b.start.copy(), list(b.kv)
+    for wide in (False, True):
+        good = b.run(backend, wide=wide)
+        for bad in ([0, -5, 400, 3, 164], [164, 14, 5, 1, 0], [2 ** 31 - 1, -2 ** 31, 7, 0, 2 ** 31 - 1], [0, 164, 0, 164, 0]):
+            b.start = np.array(bad, np.int32)
+            b.run(backend, wide=wide)
+        b.start, b.kv = start, [2 ** 31 - 1, -2 ** 31, 10 ** 6, 161]
+        b.run(backend, wide=wide)
+        b.kv = kv
+        assert np.array_equal(b.run(backend, wide=wide), good)
 
 
 def test_captured(backend):
     """A replayed graph follows lengths, starts, tables and rows, with other work and another graph of the same context in between."""
     lib = _lib.lib()
     graphs = []
-    for new, kv in (([1] * 6, [100, 7, 33, 1, 900, 64]), ([120, 1, 7], [130, 40, 300])):
+    for new, kv, wide in (([1] * 6, [100, 7, 33, 1, 900, 64], False), ([120, 1, 7], [130, 40, 300], False), ([120, 1, 7], [130, 40, 300], True)):
         b = Batch("bf16", 8, 2, 128, 16, new, kv, seed=15)
+        b.table = b.wide_table() if wide else b.table
+        b.most = b.table.shape[1]
         k, v = b.planes()
         q = torch.zeros((b.tokens, 8 * 128), dtype=torch.bfloat16, device=DEV)
         out = torch.zeros_like(q)
@@ -423,8 +470,8 @@ def test_two_contexts_at_once():
         try:
             b = Batch("bf16", 8, 2, 128, 16, [1, 1, 50, 130], [3000, 70, 60, 700], seed=seed)
             want, tol = b.want()
-            for _ in range(10):
-                if not (np.abs(b.run(tb) - want) <= tol).all():
+            for i in range(10):
+                if not (np.abs(b.run(tb, wide=i % 2 == 0) - want) <= tol).all():
                     wrong.append(seed)
         except Exception as e:  # (a thread's exception is not seen otherwise)
             wrong.append(e)
@@ -436,9 +483,10 @@ def test_two_contexts_at_once():
 
 def test_same_bits_every_time(backend):
     b = Batch("f16", 8, 2, 128, 16, [1, 1, 30, 1], [9000, 70, 60, 2000], seed=16)
-    first = b.run(backend)
-    for _ in range(5):
-        assert np.array_equal(b.run(backend), first)
+    for wide in (False, True):
+        first = b.run(backend, wide=wide)
+        for _ in range(5):
+            assert np.array_equal(b.run(backend, wide=wide), first)
 
 
 def test_refusals(backend):
