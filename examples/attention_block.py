@@ -1,5 +1,5 @@
 """A quantized attention block over a paged key/value cache: a layer's products with the cache and the attention between the merged
-q/k/v product and the output projection (no rotation of q and k by position: a model that has one applies it there).
+q/k/v product and the output projection (no rotation of q and k by position: a model that has one applies it there, with Rope).
 
 A few chats are served together. Their prompts come in at once, then each step brings a token of every chat (and another
 chat's prompt in between). All of it goes through the same four calls a step: page tables from the lengths, the quantized
