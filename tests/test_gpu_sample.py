@@ -1,6 +1,7 @@
 """Sampling (trhip_sample) against the definition in 64 bits."""
 import ctypes
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -312,6 +313,26 @@ def test_captured(backend):
             assert close or got[r] == want
         check(backend, zipf(40, 9000, i), [0.5] * 40)
     assert lib.trhip_graph_destroy(g) == 0
+
+
+def test_two_contexts_at_once():
+    """Two contexts on two threads, each with its own workspaces."""
+    x, wrong = zipf(24, 50257, 3), []
+    t, k, p, low, u = settings(24, 17)
+    want = [choose(x[r].double().numpy(), *(float(np.float32(a[r])) if a is not k else a[r] for a in (t, k, p, low, u))) for r in range(24)]
+
+    def work():
+        tb = tcb_amd.QuantBackend(0)
+        try:
+            for _ in range(8):
+                token, _ = sample(tb, x, u, t, k, p, low)
+                wrong.extend(r for r in range(24) if not want[r][2] and token[r] != want[r][0])
+        except Exception as e:  # (a thread's exception is not seen otherwise)
+            wrong.append(e)
+        tb.close()
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    [a.start() for a in threads], [a.join() for a in threads]
+    assert not wrong
 
 
 def test_refusals(backend):
