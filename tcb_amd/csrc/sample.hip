@@ -177,6 +177,11 @@ __device__ __forceinline__ int bin_of(uint32_t k, float per) {
 // power of two is 96 ln 2 = 66.54 bins; 984 / 65536 is 1 / 66.6.
 __device__ __forceinline__ int bin_exponent(int b) { return b < 2 ? 0 : ((b - 1) * 984) >> 16; }
 
+// The nearest whole number of one up to 2^51 (the sum's last bits; a conversion is twelve instructions).
+__device__ __forceinline__ unsigned long long whole(double x) {
+    return (unsigned long long)__double_as_longlong(x + 0x1p52) - 0x4330000000000000ull;
+}
+
 // Inclusive sums over the wave's lanes, in six lane moves (row_shr 1, 2, 4, 8, then row_bcast 15 and 31).
 template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t moved(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
@@ -272,7 +277,7 @@ template <int J> __global__ __launch_bounds__(kRead) void sample_read(const Samp
 #pragma unroll
                 for (int v = 0; v < 4; v++) {
                     const int b = first - bin_of(key[j][v], per);
-                    if (key[j][v] != 0 && (uint32_t)b < (uint32_t)kBins) atomicAdd(&s_bins[b], (unsigned long long)rint(ldexp(y[v], 48 + bin_exponent(b))));
+                    if (key[j][v] != 0 && (uint32_t)b < (uint32_t)kBins) atomicAdd(&s_bins[b], whole(ldexp(y[v], 48 + bin_exponent(b))));
                 }
             }
             const double sum = wave_sum((y[0] + y[1]) + (y[2] + y[3]));
@@ -693,7 +698,7 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
     // ---- read again: what is kept are the entries above `cut`, and of that value those up to index `last`; of weights from low up ----
     float cut = -3.4028234663852886e38f;
     int last = 0x7FFFFFFF;
-    int bits = 62;
+    int bits = 51;  // of a weight of 1 (whole()), so that the sum of all fits 62
     while ((p.vocab - 1) >> (62 - bits)) bits--;
     const double unit = __longlong_as_double((long long)(1023 + bits) << 52);
     constexpr int AT = 2;  // (four: registers spill, 256 x 128256 with flat rows among them 187 us against 180)
@@ -833,7 +838,7 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
                     if (f[v] >= from && f[v] <= to && kept_at(f[v], i + v)) {
                         const uint32_t k = key_of(f[v]);
                         const int q = (int)sub(k);
-                        atomicAdd(&s.bins[q], weigh ? (unsigned long long)rint(ldexp(wt(k), bits + finer[q])) : 1ull);
+                        atomicAdd(&s.bins[q], weigh ? whole(ldexp(wt(k), bits + finer[q])) : 1ull);
                     }
             });
             __syncthreads();
