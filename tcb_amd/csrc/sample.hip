@@ -9,14 +9,15 @@
 // entry; with one it takes the entries that the workgroups left (some hundreds), cuts the run that is kept, and walks it by index. The
 // workgroups' shares are what a row whose large entries lie anywhere needs with room to spare; whether they are complete is checked, and a row
 // where they are not (a flat one, of which thousands are kept, or one whose largest entries lie in few stripes) is read again, a few
-// times: the bin in which the run ends is opened until its entries can be sorted, then all stripes are weighed.
+// times: the bin in which the run ends is opened until its entries can be sorted (at once, where its weight says that they are few), then all
+// stripes are weighed.
 //
 // Weights and their sums are in 64 bits, since one border among a hundred thousand has to be met: e^x by a table of 64 powers and a
 // polynomial of degree 5.
 //
 // 1 x 128256, fp32: 10 us without a filter, 13 with top_k 50, 17 with top_p .85 (two launches, the second one's chain of steps by one workgroup);
-// a flat row of which thousands are kept 102, by one CU that reads the row twice more. 256 x 128256: 34 us for the largest (4 TB/s), 54 without a
-// filter, 42 with top_k 50, 87 with top_p .85, where the bins' atomics in LDS bound the first launch.
+// a flat row of which thousands are kept 91, by one CU that reads the row once more. 256 x 128256: 34 us for the largest (4 TB/s), 54 without a
+// filter, 42 with top_k 50, 84 with top_p .85, where the bins' atomics in LDS bound the first launch.
 #include "trhip_internal.hpp"
 
 namespace trhip {
@@ -711,6 +712,39 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
             for (int a = 0; a < AT; a++) use((b0 + a * kWaves) * kStripe + 4 * lane, f[a]);
         }
     };
+    const double low = (double)st.low;
+    auto weigh_at = [&](float f, int i) {
+        const double y = wt.of(kept_at(f, i) ? f : __builtin_nanf(""));
+        return y >= low ? y : 0.0;
+    };
+    auto set_mass = [&](int i, double y) { __hip_atomic_store(p.mass + (int64_t)r * p.stripes + i, y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    auto mass_of = [&](int i) { return __hip_atomic_load(p.mass + (int64_t)r * p.stripes + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    // This wave's entries with `is` to s.sorted, as far as there is room; s.small[3] counts them.
+    auto collect = [&](int i, const float (&f)[4], const bool (&is)[4]) {
+        uint32_t n = 0;
+#pragma unroll
+        for (int v = 0; v < 4; v++) n += is[v];
+        const uint32_t incl = running(n);
+        uint32_t base = 0;
+        if (lane == 63 && incl != 0) base = atomicAdd(&s.small[3], incl);
+        uint32_t at = of_lane(base, 63) + (incl - n);
+#pragma unroll
+        for (int v = 0; v < 4; v++)
+            if (is[v]) {
+                if (at < kMost) s.sorted[at] = ((unsigned long long)key_of(f[v]) << 32) | (uint32_t)~(i + v);
+                at++;
+            }
+    };
+    // Of the `inside` entries in s.sorted, where those before them weigh `above`: how many the run takes. In order afterwards.
+    auto take = [&](int inside, bool weigh, double above, double goal) {
+        sort(s, inside, true);
+        const unsigned long long e = tid < inside ? s.sorted[tid] : 0;
+        const double y = tid < inside ? (weigh ? wt((uint32_t)(e >> 32)) * unit : 1.0) : 0.0;
+        double sum;
+        const double run = above + before_me(y, s.wave, sum);
+        // up to the last entry before which the goal has not been reached
+        return last_of(tid < inside && (run < goal || (tid == 0 && above == 0)), s) + 1;
+    };
     auto finite = [](uint32_t k) { return k < 0x00800000u ? -3.4028234663852886e38f : of_key(k); };  // the smallest value of key k or above
     for (int phase = 0; phase < 2; phase++) {
         if (phase == 0 ? st.k == 0 : st.tp >= 1.0f) continue;
@@ -718,6 +752,7 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
         double goal = st.k;
         uint32_t lo = 1, hi = top;  // the keys among which the run ends
         double above = 0;           // entries, or weight in units, above them
+        double expected = weigh ? st.k : p.vocab;  // entries among them, at least where it is more than can be sorted
         if (weigh && st.k == 0) {   // from the workgroups' bins
             const float per = bins_a_unit(st.t);
             const int first = bin_of(top, per);
@@ -755,6 +790,7 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
                 const bool second = t == kEnd || !(mine[0] > 0 && run + mine[0] >= goal);
                 s.small[2] = (uint32_t)(2 * tid + second);
                 s.sum = t == kEnd ? 0.0 : second ? run + mine[0] : run;
+                s.wave[0] = second ? mine[1] : mine[0];
             }
             __syncthreads();
             const int bin = first - (int)s.small[2];
@@ -774,6 +810,8 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
                 hi = from_bin(bin + 1) - 1;
                 if (hi < lo) hi = lo;
             }
+            expected = t < kEnd ? s.wave[0] / (wt(hi < top ? hi : top) * unit) : p.vocab;
+            __syncthreads();
         } else if (weigh) {
             double sum = 0, all;
             each([&](int i, const float (&f)[4]) {
@@ -786,29 +824,66 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
             lo = key_of(cut);
         }
         int inside = 0;
-        for (;;) {
-            // how many they are, and the first of them
-            const float from = finite(lo), to = of_key(hi == 0x7FFFFFFFu ? hi - 1 : hi);  // (that key would be -0, which has 0's)
+        if (weigh && st.k == 0 && expected <= kMost) {
+            // the bin's entries, and at once the stripes' weights above them; if the bin can be sorted, its kept entries are added (1 x 128256,
+            // top_p .95: 91 us against 101)
+            const float from = finite(lo), to = of_key(hi == 0x7FFFFFFFu ? hi - 1 : hi);
             if (tid == 0) s.small[3] = 0;
             __syncthreads();
             each([&](int i, const float (&f)[4]) {
                 bool is[4], some = false;
+                double sum = 0;
+#pragma unroll
+                for (int v = 0; v < 4; v++) {
+                    is[v] = f[v] >= from && f[v] <= to, some = some || is[v];
+                    const double y = wt.of(f[v] > to ? f[v] : __builtin_nanf(""));
+                    sum += y >= low ? y : 0.0;
+                }
+                sum = wave_sum(sum);
+                if (lane == 0 && i < p.vocab) set_mass(i / kStripe, sum);
+                if (__any(some)) collect(i, f, is);
+            });
+            __builtin_amdgcn_s_waitcnt(0);
+            __syncthreads();
+            inside = (int)s.small[3];
+            if (inside <= kMost) {
+                const int n = take(inside, true, above, goal);
+                const unsigned long long e = s.sorted[tid < n ? tid : 0], e_last = s.sorted[n > 0 ? n - 1 : 0];
+                cut = n > 0 ? of_key((uint32_t)(e_last >> 32)) : to;
+                last = n > 0 ? (int)~(uint32_t)e_last : -1;
+                double *weights = reinterpret_cast<double *>(s.bins);
+                const double y = tid < n ? wt((uint32_t)(e >> 32)) : 0.0;
+                weights[tid] = y >= low ? y : 0.0;
+                __syncthreads();
+                if (tid < n) s.sorted[tid] = ((unsigned long long)(uint32_t)~(uint32_t)e << 32) | (uint32_t)tid;
+                sort(s, n, false);
+                auto stripe_of = [&](int i) { return (int)(s.sorted[i] >> 32) / kStripe; };
+                if (tid < n && (tid == 0 || stripe_of(tid) != stripe_of(tid - 1))) {
+                    double sum = 0;
+                    for (int i = tid; i < n && stripe_of(i) == stripe_of(tid); i++) sum += weights[(uint32_t)s.sorted[i]];
+                    set_mass(stripe_of(tid), mass_of(stripe_of(tid)) + sum);
+                }
+                __builtin_amdgcn_s_waitcnt(0);
+                __syncthreads();
+                return by_stripes(p, r, x, st.u, s, mass_of, [&](uint32_t key, uint32_t i) { return weigh_at(of_key(key), (int)i); });
+            }
+            __syncthreads();
+        }
+        // (more than can be sorted, surely: straight to the bins)
+        bool many = expected > kMost && lo < hi;
+        for (;; many = false) {
+            // how many they are, and the first of them
+            const float from = finite(lo), to = of_key(hi == 0x7FFFFFFFu ? hi - 1 : hi);  // (that key would be -0, which has 0's)
+            if (tid == 0) s.small[3] = many ? kMost + 1 : 0;
+            __syncthreads();
+            if (!many) each([&](int i, const float (&f)[4]) {
+                bool is[4], some = false;
 #pragma unroll
                 for (int v = 0; v < 4; v++) is[v] = f[v] >= from && f[v] <= to, some = some || is[v];
                 if (!__any(some)) return;
-                uint32_t n = 0;
 #pragma unroll
-                for (int v = 0; v < 4; v++) is[v] = is[v] && kept_at(f[v], i + v), n += is[v];
-                const uint32_t incl = running(n);
-                uint32_t base = 0;
-                if (lane == 63 && incl != 0) base = atomicAdd(&s.small[3], incl);
-                uint32_t at = of_lane(base, 63) + (incl - n);
-#pragma unroll
-                for (int v = 0; v < 4; v++)
-                    if (is[v]) {
-                        if (at < kMost) s.sorted[at] = ((unsigned long long)key_of(f[v]) << 32) | (uint32_t)~(i + v);
-                        at++;
-                    }
+                for (int v = 0; v < 4; v++) is[v] = is[v] && kept_at(f[v], i + v);
+                collect(i, f, is);
             });
             __syncthreads();
             inside = (int)s.small[3];
@@ -862,16 +937,10 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
             __syncthreads();
         }
         if (inside <= kMost) {
-            sort(s, inside, true);
-            const unsigned long long e = tid < inside ? s.sorted[tid] : 0;
-            const double y = tid < inside ? (weigh ? wt((uint32_t)(e >> 32)) * unit : 1.0) : 0.0;
-            double sum;
-            const double run = above + before_me(y, s.wave, sum);
-            // the last entry before which the goal has not been reached
-            const int t = last_of(tid < inside && (run < goal || (tid == 0 && above == 0)), s);
-            const unsigned long long e_last = s.sorted[t >= 0 ? t : 0];
-            cut = t >= 0 ? of_key((uint32_t)(e_last >> 32)) : of_key(hi);
-            last = t >= 0 ? (int)~(uint32_t)e_last : -1;  // (none of these: what is above them)
+            const int n = take(inside, weigh, above, goal);
+            const unsigned long long e_last = s.sorted[n > 0 ? n - 1 : 0];
+            cut = n > 0 ? of_key((uint32_t)(e_last >> 32)) : of_key(hi);
+            last = n > 0 ? (int)~(uint32_t)e_last : -1;  // (none of these: what is above them)
         } else {
             // one key many times: as many as it takes, by index
             double n = weigh ? ceil((goal - above) / (wt(lo) * unit)) : goal - above;
@@ -902,12 +971,6 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
         __syncthreads();
     }
     // the stripes' weights
-    const double low = (double)st.low;
-    auto weigh_at = [&](float f, int i) {
-        const double y = wt.of(kept_at(f, i) ? f : __builtin_nanf(""));
-        return y >= low ? y : 0.0;
-    };
-    double *to = p.mass + (int64_t)r * p.stripes;
     each([&](int i, const float (&f)[4]) {
         bool some = false;
 #pragma unroll
@@ -918,12 +981,11 @@ __global__ __launch_bounds__(kEnd) void sample_end(const SampleArgs p) {
             for (int v = 0; v < 4; v++) sum += weigh_at(f[v], i + v);
             sum = wave_sum(sum);
         }
-        if (lane == 0 && i < p.vocab) __hip_atomic_store(to + i / kStripe, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (lane == 0 && i < p.vocab) set_mass(i / kStripe, sum);
     });
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    by_stripes(p, r, x, st.u, s, [&](int i) { return __hip_atomic_load(to + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); },
-               [&](uint32_t key, uint32_t i) { return weigh_at(of_key(key), (int)i); });
+    by_stripes(p, r, x, st.u, s, mass_of, [&](uint32_t key, uint32_t i) { return weigh_at(of_key(key), (int)i); });
 }
 
 }  // namespace

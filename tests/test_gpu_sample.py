@@ -133,6 +133,25 @@ def test_flat_rows(backend, vocab):
         check(backend, x.to(torch.bfloat16), u, k=[3 + 97 * i for i in range(16)], p=[0.99] * 16)
 
 
+def test_ties_at_the_cut_of_top_k(backend):
+    """Large entries in few stripes and many equal ones at the border of top_k, then top_p among them: the lowest indexes of the equal ones."""
+    g, vocab, rows = torch.Generator().manual_seed(12), 60000, 24
+    x = torch.randn((rows, vocab), generator=g)
+    for r in range(rows):
+        at = 256 * (r * 7 % 200)
+        x[r, at:at + 700] = 5 + torch.rand(700, generator=g)  # more in a workgroup than its share
+        x[r, torch.randperm(vocab, generator=g)[:3000]] = 4.5
+    x[:, 0] = 9
+    k, p = [300 + 60 * r for r in range(rows)], [0.5 + 0.02 * r for r in range(rows)]
+    u = torch.rand(rows, generator=g).tolist()
+    check(backend, x, u, k=k)
+    check(backend, x, u, k=k, p=p)
+    check(backend, x, u, k=k, p=[0.999] * rows, low=[0.001 * r for r in range(rows)])
+    check(backend, x, u, p=p)
+    check(backend, x.bfloat16(), u, k=k, p=p)
+    check(backend, x.bfloat16(), u, p=p)
+
+
 def test_around_zero(backend):
     """Cuts at -0, 0 and the smallest numbers, many of each; and rows of nothing but negative or positive values."""
     g = torch.Generator().manual_seed(4)
