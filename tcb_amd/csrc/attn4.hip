@@ -15,9 +15,9 @@
 // The weights p s stand in f16, in one term for bf16 results (their rounding of 2^-12 is a sixteenth of the result's) and in two
 // for f16 ones. So that they neither overflow nor vanish, the softmax's reference includes the largest scale the wave has met.
 //
-// A wave copies its next pieces into LDS while it works (two blocks ahead; loads into registers instead: 64 x 8192 tokens 119 us against 97 at
-// that step). What bounds it is its instructions beside the bytes: 64 tokens of 32 heads on 8 of 128, up to 8192 keys, bf16: 77 to 82 us
-// (3.7 to 3.9 TB/s of codes and scales), vector units busy half the time, matrix units a twelfth. A token over 131071 keys, f16: 46 to 48 us;
+// A wave copies its next block's pieces into LDS while it works on one in registers (loads into registers instead: 64 x 8192 tokens 119 us
+// against 97 at that step; copies two blocks ahead 77 against 75, with heads of 64 47 against 43). What bounds it is its instructions beside the bytes: 64 tokens of 32 heads on 8 of 128, up to 8192 keys, bf16: 75 to 81 us
+// (3.8 to 4.0 TB/s of codes and scales), vector units busy half the time, matrix units a twelfth. A token over 131071 keys, f16: 45 to 48 us;
 // over 300 keys: 8.7, most of it the chain of one block after the other.
 #include "attn4_image.hpp"
 #include "attn_plan.hpp"
@@ -54,10 +54,9 @@ template <int NG> struct Shape4 {
     static constexpr int BYTES_IN = 288 * NG, WHOLE = BYTES_IN / 1024, TAIL = BYTES_IN % 1024, COPIES = WHOLE + (TAIL > 0);
     static constexpr int PIECE = WHOLE * 1024 + (TAIL == 0 ? 0 : TAIL <= 256 ? 256 : 1024);
     static constexpr int SLOT = 4 * PIECE;  // a block's two pieces of keys and two of values
-    static constexpr int SLOTS = 2;
     static constexpr int OSTRIDE = DIM + 4;  // floats between rows of a wave's results
-    static constexpr int RING = SLOTS * SLOT, OUT = ROWS * (OSTRIDE * 4 + 8);
-    static constexpr int WAVE = RING > OUT ? RING : OUT;
+    static constexpr int OUT = ROWS * (OSTRIDE * 4 + 8);
+    static constexpr int WAVE = SLOT > OUT ? SLOT : OUT;
     static constexpr int BYTES = kWaves * WAVE;
 };
 
@@ -202,7 +201,7 @@ template <int NG, bool BF> __global__ __launch_bounds__(64 * kWaves, per_cu(NG))
         x.bytes = (uint32_t)(9 * S::DIM) & ~(uint32_t)((int)x.hi >> 31);
         return x;
     };
-    const uint32_t ring = lds_addr(lds) + w * S::WAVE, voff = 16 * lane, voff4 = 4 * lane;
+    const uint32_t slot = lds_addr(lds) + w * S::WAVE, voff = 16 * lane, voff4 = 4 * lane;
     auto copy = [&](const uint8_t *plane, const Where &at, uint32_t to) {
         const dma_rsrc d = dma_desc(plane + (int64_t)(((uint64_t)at.hi << 32) | at.lo), at.bytes);
 #pragma unroll
@@ -211,18 +210,16 @@ template <int NG, bool BF> __global__ __launch_bounds__(64 * kWaves, per_cu(NG))
             else dma4(d, to + 1024 * i, voff4, 1024 * i);
         }
     };
-    // Copies in flight behind the ones of a block's keys (or values): those of its values, and of SLOTS - 1 blocks.
-    constexpr int AHEAD = 4 * S::COPIES * S::SLOTS - 2 * S::COPIES;
+    // Copies in flight behind the ones of a block's keys (or values): those of its values (or of the next block's keys).
+    constexpr int AHEAD = 2 * S::COPIES;
     place(0);
+    {
+        const Where at[2] = {where_of(0, 0), where_of(0, 1)};
 #pragma unroll
-    for (int i = 0; i < S::SLOTS; i++) {
-        const Where at[2] = {where_of(i, 0), where_of(i, 1)};
+        for (int h = 0; h < 2; h++) copy(p.k, at[h], slot + h * S::PIECE);
 #pragma unroll
-        for (int h = 0; h < 2; h++) copy(p.k, at[h], ring + i * S::SLOT + h * S::PIECE);
-#pragma unroll
-        for (int h = 0; h < 2; h++) copy(p.v, at[h], ring + i * S::SLOT + (2 + h) * S::PIECE);
+        for (int h = 0; h < 2; h++) copy(p.v, at[h], slot + (2 + h) * S::PIECE);
     }
-    uint32_t slot = ring;
 
     Open8 open8;
     open8.init();
@@ -235,7 +232,7 @@ template <int NG, bool BF> __global__ __launch_bounds__(64 * kWaves, per_cu(NG))
     int tl = -24;                // the values' scales met so far are at most 2^tl,
     uint32_t limit = 0x0001u;    // in f16
 
-    int turn = S::SLOTS;  // the wave's block whose copies are next
+    int turn = 1;  // the wave's block whose copies are next
     for (int b = b0 + w; b < b1; b += kWaves, turn++) {
         const int t = key_of(b);
         if ((turn & 31) == 0) place(turn);
@@ -273,7 +270,6 @@ template <int NG, bool BF> __global__ __launch_bounds__(64 * kWaves, per_cu(NG))
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the values' part has been read
 #pragma unroll
         for (int h = 0; h < 2; h++) copy(p.v, next[h], slot + (2 + h) * S::PIECE);
-        slot = slot + S::SLOT == ring + S::RING ? ring : slot + S::SLOT;
         const bool all = t + kBlock - 1 <= hi_min && (t >= lo_max || t + kBlock <= p.sinks);
         if (__any(big > limit)) {
             uint32_t finite = big;
