@@ -231,7 +231,7 @@ template <int NG, bool BF> __global__ __launch_bounds__(64 * kWaves, per_cu(NG))
 #pragma unroll
     for (int g = 0; g < NG; g++) A.o[g][0] = A.o[g][1] = (f4){0, 0, 0, 0};
     int tl = -24;                // the values' scales met so far are at most 2^tl,
-    uint32_t limit = 0x0001u;    // in f16
+    uint32_t limit = 0x0001u;    // in f16, below infinity's bits
 
     int turn = 1;  // the wave's block whose copies are next
     for (int b = b0 + w; b < b1; b += kWaves, turn++) {
@@ -305,7 +305,7 @@ template <int NG, bool BF> __global__ __launch_bounds__(64 * kWaves, per_cu(NG))
                 const uint32_t u = uni(__float_as_uint(top));
                 const int to = (int)(u >> 23) - 127 + ((u & 0x7FFFFFu) != 0), by = to - tl;
                 tl = to;
-                limit = __builtin_bit_cast(uint16_t, (_Float16)ldexpf(1.0f, tl));
+                limit = tl > 15 ? 0x7BFFu : __builtin_bit_cast(uint16_t, (_Float16)ldexpf(1.0f, tl));
                 const float less = ldexpf(1.0f, -by);
                 A.m += (float)by;
                 A.most += (float)by;
