@@ -13,7 +13,7 @@
 //   to f16's upper end.
 //   O^T += V^T P^T: the value's scale goes to the weight, w = p s (there is one product a block of 32 elements).
 // The weights p s stand in f16, in one term for bf16 results (their rounding of 2^-12 is a sixteenth of the result's) and in two
-// for f16 ones. So that they neither overflow nor vanish, the softmax's reference includes the largest scale the wave has met.
+// for f16 ones. So that they neither overflow nor vanish, the softmax's reference includes the largest scale the row has seen.
 //
 // A wave copies its next block's pieces into LDS while it works on one in registers (loads into registers instead: 64 x 8192 tokens 119 us
 // against 97 at that step; copies two blocks ahead 77 against 75, with heads of 64 47 against 43). What bounds it is its instructions beside the bytes: 64 tokens of 32 heads on 8 of 128, up to 8192 keys, bf16: 75 to 81 us
@@ -230,8 +230,8 @@ template <int NG, bool BF> __global__ __launch_bounds__(64 * kWaves, per_cu(NG))
     A.far = false;
 #pragma unroll
     for (int g = 0; g < NG; g++) A.o[g][0] = A.o[g][1] = (f4){0, 0, 0, 0};
-    int tl = -24;                // the values' scales met so far are at most 2^tl,
-    uint32_t limit = 0x0001u;    // in f16, below infinity's bits
+    int tl = -24;              // the scales of the values that this lane's row has seen are at most 2^tl,
+    uint32_t limit = 0x0001u;  // in f16, below infinity's bits: of the row that has seen the smallest
 
     int turn = 1;  // the wave's block whose copies are next
     for (int b = b0 + w; b < b1; b += kWaves, turn++) {
@@ -273,39 +273,51 @@ template <int NG, bool BF> __global__ __launch_bounds__(64 * kWaves, per_cu(NG))
         for (int h = 0; h < 2; h++) copy(p.v, next[h], slot + (2 + h) * S::PIECE);
         const bool all = t + kBlock - 1 <= hi_min && (t >= lo_max || t + kBlock <= p.sinks);
         if (__any(big > limit)) {
-            uint32_t finite = big;
+            // (The pieces come whole, and what a place that a row does not see holds must not reach the row, its scale's size neither: beside
+            // a hidden scale of 7936 the largest weight times a scale of 2^-10 would stand as low as 2^-16, where f16's step is 2^-24.)
+            auto seen = [&](int i) {
+                const int key = t + 16 * (i >> 2) + 4 * quarter + (i & 3);
+                return key <= my_hi && (key >= my_lo || key < p.sinks);
+            };
             if (__any(big >= 0x7C00u)) {
-                finite = 0;
 #pragma unroll
                 for (int g = 0; g < NG; g++) {
                     bool bad = false;
 #pragma unroll
-                    for (int h = 0; h < 2; h++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            uint32_t &d = v[h].scales[2 * g + (i >> 1)];
-                            const int sh = 16 * (i & 1);
-                            const uint32_t u = d >> sh & 0x7FFFu;
-                            if (u < 0x7C00u) {
-                                finite = finite > u ? finite : u;
-                            } else {  // it reaches the rows that see it, and no other
-                                const int key = t + 16 * h + 4 * quarter + i;
-                                bad = bad || (key <= my_hi && (key >= my_lo || key < p.sinks));
-                                d &= ~(0xFFFFu << sh);
-                            }
+                    for (int i = 0; i < 8; i++) {
+                        uint32_t &d = v[i >> 2].scales[2 * g + ((i & 3) >> 1)];
+                        const int sh = 16 * (i & 1);
+                        if ((d >> sh & 0x7FFFu) >= 0x7C00u) {
+                            bad = bad || seen(i);
+                            d &= ~(0xFFFFu << sh);
                         }
+                    }
                     const float nan = row_max(bad ? 1.0f : 0.0f) > 0.0f ? __builtin_nanf("") : 0.0f;
                     A.o[g][0] += nan;
                     A.o[g][1] += nan;
                 }
             }
+            uint32_t finite = 0;  // the largest that this lane's row sees of its eight places
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                uint32_t u = 0;
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    const uint32_t d = v[i >> 2].scales[2 * g + ((i & 3) >> 1)] >> (16 * (i & 1)) & 0x7FFFu;
+                    u = u > d ? u : d;
+                }
+                u = all || seen(i) ? u : 0;
+                finite = finite > u ? finite : u;
+            }
             // (f16's bits as fp32's: exact, subnormal ones too)
-            const float top = __uint_as_float(__builtin_amdgcn_readlane(scan64((int)(finite << 13), 0, [](int a, int b) { return a > b ? a : b; }), 63)) * 0x1p112f;
-            if (uni(__float_as_uint(top)) > __float_as_uint(ldexpf(1.0f, tl))) {
-                const uint32_t u = uni(__float_as_uint(top));
-                const int to = (int)(u >> 23) - 127 + ((u & 0x7FFFFFu) != 0), by = to - tl;
+            const float top = row_max(__uint_as_float(finite << 13) * 0x1p112f);
+            const bool more = top > ldexpf(1.0f, tl);
+            if (__any(more)) {
+                const uint32_t u = __float_as_uint(top);
+                const int to = more ? (int)(u >> 23) - 127 + ((u & 0x7FFFFFu) != 0) : tl, by = to - tl;
                 tl = to;
-                limit = tl > 15 ? 0x7BFFu : __builtin_bit_cast(uint16_t, (_Float16)ldexpf(1.0f, tl));
+                const int least = __builtin_amdgcn_readlane(scan64(tl, 0x7FFF, [](int a, int b) { return a < b ? a : b; }), 63);
+                limit = least > 15 ? 0x7BFFu : __builtin_bit_cast(uint16_t, (_Float16)ldexpf(1.0f, least));
                 const float less = ldexpf(1.0f, -by);
                 A.m += (float)by;
                 A.most += (float)by;
