@@ -297,20 +297,28 @@ template <int NG, bool BF> __global__ __launch_bounds__(64 * kWaves, per_cu(NG))
                     A.o[g][1] += nan;
                 }
             }
-            uint32_t finite = 0;  // the largest that this lane's row sees of its eight places
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                uint32_t u = 0;
-#pragma unroll
-                for (int g = 0; g < NG; g++) {
-                    const uint32_t d = v[i >> 2].scales[2 * g + ((i & 3) >> 1)] >> (16 * (i & 1)) & 0x7FFFu;
-                    u = u > d ? u : d;
-                }
-                u = all || seen(i) ? u : 0;
-                finite = finite > u ? finite : u;
-            }
+            // The largest that the row sees: of all places, or of the eight that this lane has the row's scores of.
             // (f16's bits as fp32's: exact, subnormal ones too)
-            const float top = row_max(__uint_as_float(finite << 13) * 0x1p112f);
+            uint32_t finite = big;
+            if (!all || __any(big >= 0x7C00u)) {
+                finite = 0;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    uint32_t u = 0;
+#pragma unroll
+                    for (int g = 0; g < NG; g++) {
+                        const uint32_t d = v[i >> 2].scales[2 * g + ((i & 3) >> 1)] >> (16 * (i & 1)) & 0x7FFFu;
+                        u = u > d ? u : d;
+                    }
+                    u = seen(i) ? u : 0;
+                    finite = finite > u ? finite : u;
+                }
+                finite = __float_as_uint(row_max(__uint_as_float(finite << 13) * 0x1p112f));
+            } else {
+                finite = __builtin_amdgcn_readlane(scan64((int)finite, 0, [](int a, int b) { return a > b ? a : b; }), 63);
+                finite = __float_as_uint(__uint_as_float(finite << 13) * 0x1p112f);
+            }
+            const float top = __uint_as_float(finite);
             const bool more = top > ldexpf(1.0f, tl);
             if (__any(more)) {
                 const uint32_t u = __float_as_uint(top);
