@@ -150,7 +150,8 @@ __device__ __forceinline__ Setting setting_of(const SampleArgs &p, int r) {
     if (!(s.low > 0.0f)) s.low = 0.0f;
     if (s.low > 1.0f) s.low = 1.0f;
     const float u = p.u[r];
-    s.u = u >= 0.0f ? (double)u : 0.0;
+    // (from 1 up infinite: no sum exceeds a goal of that, while the sum of all can differ from a running sum's end by a rounding)
+    s.u = u >= 1.0f ? (double)__builtin_inff() : u >= 0.0f ? (double)u : 0.0;
     return s;
 }
 // How many entries of the whole row its workgroups should cover, and a workgroup's share of them: the mean, three standard deviations of
