@@ -467,10 +467,13 @@ __device__ __forceinline__ void result(const SampleArgs &p, int r, int token, do
     if (p.logprob) p.logprob[r] = (float)log(w / total);
 }
 
-// The entry of stripe `at` (keys k, four a lane) in which the goal falls, the weights before the stripe being `before`; by one wave.
+// The entry of stripe `at` in which the goal falls, the weights before the stripe being `before`; by one wave. False: no entry of it has
+// weight.
 template <class F>
-__device__ __forceinline__ void last_stripe(const SampleArgs &p, int r, int at, double before, double goal, double total, const uint32_t (&k)[4], F weight) {
+__device__ __forceinline__ bool last_stripe(const SampleArgs &p, int r, const Row &x, int at, double before, double goal, double total, F weight) {
     const int lane = threadIdx.x & 63;
+    uint32_t k[4];
+    x.keys4(at * kStripe + 4 * lane, k);
     double y[4], sum = 0;
 #pragma unroll
     for (int v = 0; v < 4; v++) y[v] = weight(k[v], (uint32_t)(at * kStripe + 4 * lane + v)), sum += y[v];
@@ -483,14 +486,16 @@ __device__ __forceinline__ void last_stripe(const SampleArgs &p, int r, int at, 
         if (y[v] > 0 && run > goal && found < 0) found = v, chosen = y[v];
     }
     const uint64_t over = __ballot(found >= 0), some = __ballot(last >= 0);
-    const int src = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : 0;
+    if (some == 0) return false;
+    const int src = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
     if (lane == src) result(p, r, at * kStripe + 4 * lane + (over ? found : last), over ? chosen : final, total);
+    return true;
 }
 
 // The entry in which u falls among stripes of these weights: mass(i), in one order for every call, and weight(key, index) of their entries.
 template <class M, class F>
 __device__ __forceinline__ void by_stripes(const SampleArgs &p, int r, const Row &x, double u, Lds &s, M mass, F weight) {
-    const int tid = threadIdx.x, lane = tid & 63;
+    const int tid = threadIdx.x;
     const int each = (p.stripes + kEnd - 1) / kEnd, s0 = tid * each < p.stripes ? tid * each : p.stripes, s1 = s0 + each < p.stripes ? s0 + each : p.stripes;
     double sum = 0, total;
     for (int i = s0; i < s1; i++) sum += mass(i);
@@ -513,10 +518,11 @@ __device__ __forceinline__ void by_stripes(const SampleArgs &p, int r, const Row
     }
     __syncthreads();
     if (tid >= 64) return;
-    const int at = (int)s.small[0];
-    uint32_t k[4];
-    x.keys4(at * kStripe + 4 * lane, k);
-    last_stripe(p, r, at, s.sum, goal, total, k, weight);
+    // A stripe's weight is relative to its workgroup's largest logit, and may be there where each of its entries' is below 2^-1074, which is
+    // 0: then the entry is in the next stripe that has one with weight (the goal is 0: the first of all), or in the one before (the last).
+    // The largest logit's is on that side.
+    for (int at = (int)s.small[0]; at >= 0 && at < p.stripes; at += none ? -1 : 1)
+        if (last_stripe(p, r, x, at, s.sum, goal, total, weight)) return;
 }
 
 // A filtered row whose kept run is among its largest 64 entries, by one wave: those that a threshold leaves of the n in s.sorted.
