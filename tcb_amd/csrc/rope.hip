@@ -3,6 +3,7 @@
 // A workgroup takes one or four tokens and some of their heads: first the sines and cosines of the tokens' pairs, once for all heads, into
 // LDS, then the heads, 16 bytes a load. Every element moves once in and once out, which is what bounds it: 8192 tokens of 40 heads of 128 in bf16
 // take 38 us (4.4 TB/s), 16 tokens 4.6, a launch. (Angles by every head anew, 64-bit arithmetic each: 72 us.)
+#include "rope.hpp"
 #include "trhip_internal.hpp"
 
 #include <cmath>
@@ -26,12 +27,11 @@ struct RopeArgs {
 };
 
 // Sine and cosine of `turns` whole turns. The turns are reduced to a quarter in 64 bits, the rest y (|y| <= 1/8 turn) goes through the
-// Taylor series of x = 2 pi y, |x| <= pi / 4: what they leave out is below 2^-28, so fp32's own roundings are what is off.
+// series of x = 2 pi y, |x| <= pi / 4: what they leave out is below 2^-29, so fp32's own roundings are what is off.
 __device__ __forceinline__ float2 cos_sin(double turns) {
     const double q = 4.0 * (turns - rint(turns)), k = rint(q);
     const float x = (float)(q - k) * 1.57079632679f, z = x * x;
-    const float s = fmaf(z * x, fmaf(z, fmaf(z, fmaf(z, 2.7557319e-6f, -1.98412698e-4f), 8.33333333e-3f), -1.66666667e-1f), x);
-    const float c = fmaf(z, fmaf(z, fmaf(z, fmaf(z, 2.48015873e-5f, -1.38888889e-3f), 4.16666667e-2f), -0.5f), 1.0f);
+    const float s = rope_sin(x, z), c = rope_cos(z);
     const int n = (int)k & 3;
     const float a = n & 1 ? s : c, b = n & 1 ? c : s;
     return make_float2(n == 1 || n == 2 ? -a : a, n >= 2 ? -b : b);
