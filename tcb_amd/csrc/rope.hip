@@ -11,8 +11,7 @@
 namespace trhip {
 namespace {
 
-constexpr int kMostPairs = 256, kThreads = 256;
-constexpr int64_t kMostTokens = (int64_t)1 << 24;  // of a launch, which may have 2^32 threads
+constexpr int kMostPairs = 256, kThreads = kRopeThreads;
 
 struct RopeArgs {
     const void *x;
@@ -155,9 +154,9 @@ template <int IO, bool WIDE, int TOKENS> __global__ __launch_bounds__(kThreads) 
     }
 }
 
-template <int IO, bool WIDE> void launch(trhip_ctx *ctx, const RopeArgs &p, bool four, unsigned splits) {
-    if (four) hipLaunchKernelGGL((rope_kernel<IO, WIDE, 4>), dim3((unsigned)((p.tokens + 3) / 4), splits), dim3(kThreads), 0, ctx->stream, p);
-    else hipLaunchKernelGGL((rope_kernel<IO, WIDE, 1>), dim3((unsigned)p.tokens, splits), dim3(kThreads), 0, ctx->stream, p);
+template <int IO, bool WIDE> void launch(trhip_ctx *ctx, const RopeArgs &p, bool four, unsigned groups, unsigned splits) {
+    if (four) hipLaunchKernelGGL((rope_kernel<IO, WIDE, 4>), dim3(groups, splits), dim3(kThreads), 0, ctx->stream, p);
+    else hipLaunchKernelGGL((rope_kernel<IO, WIDE, 1>), dim3(groups, splits), dim3(kThreads), 0, ctx->stream, p);
 }
 
 }  // namespace
@@ -191,16 +190,17 @@ int launch_rope(trhip_ctx *ctx, const trhip_rope_spec &spec, const void *x, int6
     }
     p.each = (int)((heads + splits - 1) / splits);
     const unsigned s = (unsigned)((heads + p.each - 1) / p.each);
-    for (int64_t t = 0; t < tokens; t += kMostTokens) {
-        p.tokens = (int)(tokens - t < kMostTokens ? tokens - t : kMostTokens);
-        if (io == TRHIP_F32) wide ? launch<TRHIP_F32, true>(ctx, p, four, s) : launch<TRHIP_F32, false>(ctx, p, four, s);
-        else if (io == TRHIP_F16) wide ? launch<TRHIP_F16, true>(ctx, p, four, s) : launch<TRHIP_F16, false>(ctx, p, four, s);
-        else wide ? launch<TRHIP_BF16, true>(ctx, p, four, s) : launch<TRHIP_BF16, false>(ctx, p, four, s);
+    for (int64_t t = 0; t < tokens; t += kRopeTokens) {
+        const RopeLaunch l = rope_launch(tokens - t, four ? 4 : 1);
+        p.tokens = l.tokens;
+        if (io == TRHIP_F32) wide ? launch<TRHIP_F32, true>(ctx, p, four, l.groups, s) : launch<TRHIP_F32, false>(ctx, p, four, l.groups, s);
+        else if (io == TRHIP_F16) wide ? launch<TRHIP_F16, true>(ctx, p, four, l.groups, s) : launch<TRHIP_F16, false>(ctx, p, four, l.groups, s);
+        else wide ? launch<TRHIP_BF16, true>(ctx, p, four, l.groups, s) : launch<TRHIP_BF16, false>(ctx, p, four, l.groups, s);
         const int st = launch_check(ctx, "rope");
         if (st != TRHIP_OK) return st;
-        p.x = static_cast<const char *>(p.x) + kMostTokens * x_stride * size;
-        p.out = static_cast<char *>(p.out) + kMostTokens * out_stride * size;
-        p.pos += kMostTokens;
+        p.x = static_cast<const char *>(p.x) + kRopeTokens * x_stride * size;
+        p.out = static_cast<char *>(p.out) + kRopeTokens * out_stride * size;
+        p.pos += kRopeTokens;
     }
     return TRHIP_OK;
 }

@@ -1,5 +1,7 @@
-// rope.hpp -- what of the rotary positions needs no device: the series of sine and cosine (for tests also in 64 bits).
+// rope.hpp -- what of the rotary positions needs no device: the series of sine and cosine (for tests also in 64 bits), the sizes of launches.
 #pragma once
+
+#include <cstdint>
 
 #if defined(__HIPCC__)
 #include <hip/hip_runtime.h>
@@ -21,6 +23,19 @@ template <class T> ROPE_BOTH T rope_sin(T x, T z) {
 template <class T> ROPE_BOTH T rope_cos(T z) {
     const T y = rope_fma(z, rope_fma(z, rope_fma(z, T(-2.7557319e-7), T(2.48015873e-5)), T(-1.38888889e-3)), T(4.16666667e-2));
     return rope_fma(z, rope_fma(z, y, T(-0.5)), T(1));
+}
+
+// A launch of the first of `left` tokens, `each` (one or four) a workgroup. Workgroups times threads has to stay below 2^32, so a launch has
+// 2^23 tokens at most, a multiple of four, and 2^31 threads.
+constexpr int kRopeThreads = 256;
+constexpr int64_t kRopeTokens = (int64_t)1 << 23;
+struct RopeLaunch {
+    int tokens;
+    unsigned groups;
+};
+inline RopeLaunch rope_launch(int64_t left, int each) {
+    const int tokens = (int)(left < kRopeTokens ? left : kRopeTokens);
+    return {tokens, (unsigned)((tokens + each - 1) / each)};
 }
 
 }  // namespace trhip
