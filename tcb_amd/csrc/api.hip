@@ -1189,7 +1189,7 @@ int trhip_rope(trhip_ctx *ctx, const trhip_rope_spec *spec, const void *x, int64
         pairs += spec->pairs[a];
     }
     if (spec->flags & ~(TRHIP_ROPE_NEIGHBOURS | TRHIP_ROPE_DEALT | TRHIP_ROPE_LADDERS)) return bad("unknown flags");
-    if (!(spec->base > 0.0) || spec->base > 1e300) return bad("the base must be positive and finite");
+    if (!(spec->base > 0.0) || spec->base > 1.7976931348623157e308) return bad("the base must be positive and finite");
     if (reinterpret_cast<uintptr_t>(spec->factors) % 4) return bad("factors are not aligned to their type");
     if (tokens < 0) return bad("negative size");
     if (bad_type(type)) return bad("bad element type");

@@ -1,8 +1,10 @@
 """Rotary positions at the ends of what a call may have."""
+import numpy as np
 import pytest
 import torch
 
 import tcb_amd
+from test_gpu_rope import check
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -31,3 +33,9 @@ def test_more_tokens_than_a_launch_has_one_by_one(backend):
         # half a step of f16, and the arithmetic's 2^-20 of values of up to 10
         got = rows[a:a + m].double().view(m, heads, dim)
         assert ((got - want).abs() <= 2.0 ** -11 * want.abs() + 10 * 2.0 ** -20 + 2.0 ** -25).all(), a
+
+
+@pytest.mark.parametrize("base", [1e301, np.finfo(np.float64).max])
+def test_the_largest_bases(backend, base):
+    """Any finite base is one."""
+    check(backend, "f32", 33, 2, 64, [32], float(base), pos=torch.arange(33, dtype=torch.int32).view(1, -1) * 977)
