@@ -6,6 +6,7 @@
 // an element took 23), out 11.5 (3.7 TB/s). Tokens one by one, whose value codes are written as bytes: in and out 140 us against 29.
 #include "attn_common.hpp"
 #include "kv4.hpp"
+#include "kv4_runs.hpp"
 
 namespace trhip {
 namespace {
@@ -14,22 +15,10 @@ struct Kv4Args {
     uint8_t *kc, *vc;
     int page_log2, heads, dim;
     int64_t places, stride;
-    int tokens, wide, run;  // wide: rows are aligned to 16 bytes; run: tokens of a workgroup
+    uint32_t tokens, run;  // run: tokens of a workgroup
+    int wide;              // rows are aligned to 16 bytes
     const int *slots;
 };
-
-// The token's slot and how many tokens the workgroup of token t takes: 4 where t is the first of four in a row from a multiple of four,
-// 0 where an earlier workgroup takes it.
-__device__ __forceinline__ int together(const Kv4Args &p, int t, int64_t &slot) {
-    slot = p.slots[t];
-    if ((uint64_t)slot >= (uint64_t)p.places) return 0;
-    const int at = (int)(slot & 3), first = t - at;
-    if (first < 0 || first + 3 >= p.tokens) return 1;
-    bool row = true;
-#pragma unroll
-    for (int i = 0; i < 4; i++) row = row && (int64_t)p.slots[first + i] == slot - at + i;
-    return !row ? 1 : at == 0 ? 4 : 0;
-}
 
 template <int CTRL> __device__ __forceinline__ uint32_t quad(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
@@ -226,10 +215,10 @@ template <int IO, bool APPEND> __global__ __launch_bounds__(256, APPEND || IO !=
     const bool value = x >= row;
     const int y = value ? x - row : x, head = y / (4 * blocks), e = y - head * (4 * blocks), b = e >> 2, q = e & 3;
     // (a workgroup a token would leave all work to every fourth, and workgroups are dealt to the XCDs in turn: two of eight would do it)
-    for (int t0 = blockIdx.y * p.run; t0 < p.tokens; t0 += gridDim.y * p.run)
-    for (int t = t0; t < t0 + p.run && t < p.tokens; t++) {
+    for (uint32_t t0 = blockIdx.y * p.run; t0 < p.tokens; t0 = kv4_next(t0, gridDim.y, p.run))
+    for (uint32_t t = t0; t < t0 + p.run && t < p.tokens; t++) {
         int64_t slot;
-        const int n = together(p, t, slot);
+        const int n = kv4_together(p.slots, p.tokens, p.places, t, slot);
         if (n == 0 || x >= 2 * row) continue;
         const Kv4Place at = kv4_place(slot, p.page_log2, p.heads, head, p.dim);
         uint8_t *piece = (value ? p.vc : p.kc) + at.piece;
@@ -250,12 +239,12 @@ int launch(trhip_ctx *ctx, const trhip_kv4 *kv, int64_t tokens, void *k, void *v
     const int64_t size = io == TRHIP_F32 ? 4 : 2;
     const bool wide = reinterpret_cast<uintptr_t>(k) % 16 == 0 && reinterpret_cast<uintptr_t>(v) % 16 == 0 && stride * size % 16 == 0;
     // (8192 tokens: in 15.8 us, with one token a workgroup 34; few tokens go faster on a workgroup each, 6.0 us against 6.2)
-    const int run = tokens >= 256 ? 4 : 1;
+    const uint32_t run = tokens >= 256 ? 4 : 1;
     const Kv4Args p = {static_cast<uint8_t *>(kv->k), static_cast<uint8_t *>(kv->v), __builtin_ctz((unsigned)kv->page), kv->heads, kv->dim,
-                       kv->pages * kv->page, stride, (int)tokens, wide, run, slots};
+                       kv->pages * kv->page, stride, (uint32_t)tokens, run, wide, slots};
     const int eights = kv->heads * kv->dim / 4, threads = eights >= 256 ? 256 : (eights + 63) / 64 * 64;
     const int64_t y = (tokens + run - 1) / run;
-    const dim3 grid((unsigned)((eights + threads - 1) / threads), (unsigned)(y < 65535 ? y : 65535));
+    const dim3 grid((unsigned)((eights + threads - 1) / threads), (unsigned)(y < kKv4Groups ? y : kKv4Groups));
     if (io == TRHIP_F32) hipLaunchKernelGGL((kv4_rows_kernel<TRHIP_F32, APPEND>), grid, dim3(threads), 0, ctx->stream, p, k, v);
     else if (io == TRHIP_F16) hipLaunchKernelGGL((kv4_rows_kernel<TRHIP_F16, APPEND>), grid, dim3(threads), 0, ctx->stream, p, k, v);
     else hipLaunchKernelGGL((kv4_rows_kernel<TRHIP_BF16, APPEND>), grid, dim3(threads), 0, ctx->stream, p, k, v);
