@@ -358,8 +358,9 @@ int trhip_kv4_read(trhip_ctx *ctx, const trhip_kv4 *kv, int64_t tokens, void *k,
  * keys may be opened, as trhip_attn's; else to f16 for bf16 results and to two f16 numbers (2^-21) for f16 ones. Where the hint allows requests of more
  * than 96 rows, their keys are opened into the context's workspace in 16 bits
  * (exactly, where trhip_kv4_append wrote the scales, else rounded once): as many times max_pages pages (2 * page * heads * dim
- * bytes a plane) as the tokens can make such requests, if that is no more than 2 GiB a plane; beyond it, with a hint that is too
- * small (both take up to five times as long) and in small calls they are read as they are. */
+ * bytes a plane) as the tokens can make such requests, if that is no more than 2 GiB a plane; beyond it, where the device has no memory for it,
+ * with a hint that is too small (all of these take up to five times as long) and in small calls they are read as they are. The context
+ * keeps that workspace: both planes, 4 bytes for each of nreq * max_pages page numbers (up to 2 GiB), and a quarter more. */
 int trhip_kv4_attn(trhip_ctx *ctx, const trhip_kv4 *kv, const void *q, int type, int64_t q_stride, void *out, int64_t out_stride,
                    int64_t tokens, int heads, int64_t nreq, const int32_t *q_start, const int32_t *kv_len,
                    const int32_t *table, int64_t max_pages, int64_t max_new, int64_t window, int64_t sinks, float scale);
@@ -421,9 +422,11 @@ int trhip_rows_plan(int dtype, int64_t M, int64_t N, int64_t K, int cus, int64_t
  * TRHIP_KNOB_KL_GRID: at least a workgroups for the K-across-lanes fast GEMV (its rows dealt over more, shorter row groups); TRHIP_KNOB_ROWS: exact products of more
  * than 16 activation rows (a, b, c) = (1: a row block's K chunks in one workgroup, 2: in slices where there are
  * enough of them; activation rows a pass, 16 or 32; workgroups its passes are dealt over); TRHIP_KNOB_FAST_GEMM: fast
- * mode of more than 16 rows, a = 1: always the f16 / bf16 matrix-core kernel (K of 256 up), 2: never. */
+ * mode of more than 16 rows, a = 1: always the f16 / bf16 matrix-core kernel (K of 256 up), 2: never; TRHIP_KNOB_WORKSPACE: MiB
+ * a that each of the context's workspaces may grow to; a call that needs more finds no memory, as on a device that is full. */
 enum { TRHIP_KNOB_KL = 1, TRHIP_KNOB_FAST_Q4K = 2, TRHIP_KNOB_EXACT_ROWS = 3, TRHIP_KNOB_EXACT_LANES = 4,
-       TRHIP_KNOB_ACTQ_TM = 5, TRHIP_KNOB_ROWS16 = 6, TRHIP_KNOB_KL_GRID = 7, TRHIP_KNOB_ROWS = 8, TRHIP_KNOB_FAST_GEMM = 9 };
+       TRHIP_KNOB_ACTQ_TM = 5, TRHIP_KNOB_ROWS16 = 6, TRHIP_KNOB_KL_GRID = 7, TRHIP_KNOB_ROWS = 8, TRHIP_KNOB_FAST_GEMM = 9,
+       TRHIP_KNOB_WORKSPACE = 10 };
 int trhip_set_launch_shape(trhip_ctx *ctx, int knob, int a, int b, int c, int d);
 
 #ifdef __cplusplus

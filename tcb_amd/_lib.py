@@ -95,7 +95,7 @@ Q8, Q4, Q4K, Q6K = 1, 2, 3, 4
 MODE_EXACT, MODE_FAST = 0, 1
 F32, F16, BF16 = 0, 1, 2
 ROPE_NEIGHBOURS, ROPE_DEALT, ROPE_LADDERS = 1, 2, 4
-KNOB_KL, KNOB_FAST_Q4K, KNOB_EXACT_ROWS, KNOB_EXACT_LANES, KNOB_ACTQ_TM, KNOB_ROWS16, KNOB_KL_GRID, KNOB_ROWS, KNOB_FAST_GEMM = range(1, 10)
+KNOB_KL, KNOB_FAST_Q4K, KNOB_EXACT_ROWS, KNOB_EXACT_LANES, KNOB_ACTQ_TM, KNOB_ROWS16, KNOB_KL_GRID, KNOB_ROWS, KNOB_FAST_GEMM, KNOB_WORKSPACE = range(1, 11)
 
 
 def load(path=LIB_PATH):

@@ -50,6 +50,10 @@ void *grow(trhip_ctx *ctx, void *&buf, size_t &have, size_t bytes, int *status) 
         *status = fail(ctx, TRHIP_ERR_INVALID, "workspace must be sized by an eager call before graph capture");
         return nullptr;
     }
+    if (ctx->ws_most > 0 && bytes > ((size_t)ctx->ws_most << 20)) {
+        *status = fail(ctx, TRHIP_ERR_OOM, "workspace of more than TRHIP_KNOB_WORKSPACE allows");
+        return nullptr;
+    }
     // Growing: earlier work on the stream may still read the old buffer.
     hipError_t e = hipStreamSynchronize(ctx->stream);
     if (e != hipSuccess) { *status = hip_fail(ctx, e, "workspace sync"); return nullptr; }
@@ -61,7 +65,12 @@ void *grow(trhip_ctx *ctx, void *&buf, size_t &have, size_t bytes, int *status) 
     have = 0;
     size_t want = bytes < (size_t)(1 << 20) ? (size_t)(1 << 20) : bytes + bytes / 4;
     e = hipMalloc(&buf, want);
-    if (e != hipSuccess) { buf = nullptr; *status = hip_fail(ctx, e, "workspace alloc"); return nullptr; }
+    if (e != hipSuccess) {
+        (void)hipGetLastError();  // (or the next launch's check would take it for its own)
+        buf = nullptr;
+        *status = hip_fail(ctx, e, "workspace alloc");
+        return nullptr;
+    }
     have = want;
     return buf;
 }
@@ -667,6 +676,10 @@ int trhip_set_launch_shape(trhip_ctx *ctx, int knob, int a, int b, int c, int d)
         if (!(reset || ((a == 1 || a == 2) && !b && !c && !d)))
             return fail(ctx, TRHIP_ERR_INVALID, "set_launch_shape: fast kernel of many rows takes 1 (always) or 2 (never)");
         ctx->force_fast_gemm = a;
+        return TRHIP_OK;
+    case TRHIP_KNOB_WORKSPACE:
+        if (!(reset || (a >= 1 && !b && !c && !d))) return fail(ctx, TRHIP_ERR_INVALID, "set_launch_shape: workspaces take 1 MiB and more");
+        ctx->ws_most = a;
         return TRHIP_OK;
     case TRHIP_KNOB_ROWS16:
         if (!(reset || ((a == 1 || a == 2) && b >= 1 && b <= 64 && !c && !d)))

@@ -512,13 +512,21 @@ int launch_kv4_attn(trhip_ctx *ctx, const trhip_kv4 *kv, const AttnCall &c, int 
     const double cap = (double)c.max_pages * kv->page, window = (double)c.window + (double)c.sinks + 16, seen = c.window > 0 && window < cap ? window : cap;
     const double tiles = ((double)c.tokens * p.group / 16 + (double)c.nreq) * kv->heads;
     const double image_bytes = (double)longs * (double)c.max_pages * (double)p.page_bytes * (32.0 / 9.0);
-    const bool image = most_new * p.group > kTokMost && tiles * (seen + kTileKeys) * kv->dim > kSmall && longs > 0 && longs < 65536 && p.kv_heads < 65536 && c.max_pages > 0 && image_bytes <= (double)kMostImage &&
+    bool image = most_new * p.group > kTokMost && tiles * (seen + kTileKeys) * kv->dim > kSmall && longs > 0 && longs < 65536 && p.kv_heads < 65536 && c.max_pages > 0 && image_bytes <= (double)kMostImage &&
                        (double)c.nreq * (double)c.max_pages <= (double)(kMostImage / 4);
+    const int64_t plane = image ? (longs * c.max_pages * (p.page_bytes / 9 * 32) + 255) & ~(int64_t)255 : 0, tables = image ? c.nreq * c.max_pages * 4 : 0;
+    uint8_t *room = nullptr;
+    // (no memory for it: the kernel of few rows takes all requests, and does so in a capture behind such a call)
+    if (image && ctx->no_room && (size_t)(2 * plane + tables) >= ctx->no_room && capturing(ctx)) image = false;
     if (image) {
-        const int64_t plane = (longs * c.max_pages * (p.page_bytes / 9 * 32) + 255) & ~(int64_t)255, tables = c.nreq * c.max_pages * 4;
         int st = TRHIP_OK;
-        uint8_t *room = static_cast<uint8_t *>(workspace2(ctx, (size_t)(2 * plane + tables), &st));
-        if (!room) return st;
+        room = static_cast<uint8_t *>(workspace2(ctx, (size_t)(2 * plane + tables), &st));
+        if (!room && st != TRHIP_ERR_OOM) return st;
+        image = room != nullptr;
+        ctx->no_room = image ? 0 : (size_t)(2 * plane + tables);
+    }
+    if (image) {
+        int st = TRHIP_OK;
         const Image4 im = {p.k, p.v, reinterpret_cast<uint16_t *>(room), reinterpret_cast<uint16_t *>(room + plane), reinterpret_cast<int *>(room + 2 * plane),
                            p.q_start, p.kv_len, p.table, p.max_pages, p.npages, p.nreq, p.tokens, p.group, p.kv_heads, p.dim, p.page_log2, kTokMost,
                            p.window, p.sinks, io == TRHIP_BF16};

@@ -331,6 +331,7 @@ struct trhip_ctx {
     // (the merged gate_up output of trhip_gemm_q_swiglu).
     void *ws2 = nullptr;
     size_t ws2_bytes = 0;
+    size_t no_room = 0;  // bytes for opened keys that there was no memory for (launch_kv4_attn), 0 once there was
     // A third for the fp32 copies of 16-bit activations and outputs (trhip_gemm_q_typed), which live across the call
     // of the fp32 operator that uses the others.
     void *ws3 = nullptr;
@@ -365,6 +366,7 @@ struct trhip_ctx {
     int force_actq_slices = 0;  // act-quant MFMA K slices, fast mode (0: built-in)
     int force_rows16 = 0;       // batched-decode q4_k kernel: 100 tiles per wave + K slices
     int force_rows[3] = {};     // exact M > 16 plan: 1 whole / 2 in slices, activation rows a pass, workgroups (0: built-in)
+    int ws_most = 0;            // MiB that a workspace may have (0: whatever there is)
     int force_fast_gemm = 0;    // fast mode of more than 16 rows: 1 fastg.hip, 2 the other kernels (0: built-in)
     // Arrival counters of kernels whose K slices are summed by the workgroup that finishes a row tile last
     // (rows16.hip): kArrivalSlots zeroed words, each returned to zero by that workgroup.
