@@ -352,7 +352,8 @@ int trhip_kv4_append(trhip_ctx *ctx, const trhip_kv4 *kv, int64_t tokens, const 
 int trhip_kv4_read(trhip_ctx *ctx, const trhip_kv4 *kv, int64_t tokens, void *k, void *v, int type, int64_t stride,
                    const int32_t *slots);
 
-/* trhip_attn over the 4-bit cache: same masks, tables, lengths, hints and limits. q and out are of `type` (TRHIP_F16 or TRHIP_BF16).
+/* trhip_attn over the 4-bit cache: same masks, tables, lengths, hints and limits; beside them, tokens * heads / 16 + nreq * kv->heads, the tiles
+ * of rows, must be below 2^24 where requests are read as they are. q and out are of `type` (TRHIP_F16 or TRHIP_BF16).
  * A block whose scale is not finite reads as NaN where a token sees it: in its elements of the result as a value, in the whole row
  * of the head as a key. What a token's mask hides never reaches it. Weights are rounded: in requests of more than 96 rows, where their
  * keys may be opened, as trhip_attn's; else to f16 for bf16 results and to two f16 numbers (2^-21) for f16 ones. Where the hint allows requests of more

@@ -525,6 +525,13 @@ int launch_kv4_attn(trhip_ctx *ctx, const trhip_kv4 *kv, const AttnCall &c, int 
         image = room != nullptr;
         ctx->no_room = image ? 0 : (size_t)(2 * plane + tables);
     }
+    p.row_lo = 0;
+    p.row_hi = image ? kTokMost : kAnyRows;
+    const int rows = 16;
+    p.target = cus * per_cu(kv->dim / 32);
+    const int64_t grid = plan_items(p, c, rows, kBlock, kLeast);
+    // (workgroups times threads has to stay below 2^32)
+    if (grid >= ((int64_t)1 << 32) / (64 * kWaves)) return fail(ctx, TRHIP_ERR_INVALID, "kv4_attn: too many rows");
     if (image) {
         int st = TRHIP_OK;
         const Image4 im = {p.k, p.v, reinterpret_cast<uint16_t *>(room), reinterpret_cast<uint16_t *>(room + plane), reinterpret_cast<int *>(room + 2 * plane),
@@ -539,12 +546,6 @@ int launch_kv4_attn(trhip_ctx *ctx, const trhip_kv4 *kv, const AttnCall &c, int 
         st = launch_attn(ctx, &open, lc);
         if (st != TRHIP_OK) return st;
     }
-    p.row_lo = 0;
-    p.row_hi = image ? kTokMost : kAnyRows;
-    const int rows = 16;
-    p.target = cus * per_cu(kv->dim / 32);
-    const int64_t grid = plan_items(p, c, rows, kBlock, kLeast);
-    if (grid >= ((int64_t)1 << 31)) return fail(ctx, TRHIP_ERR_INVALID, "kv4_attn: too many rows");
     int st = TRHIP_OK;
     float *ws = static_cast<float *>(workspace(ctx, (size_t)p.part_slots * rows * (kv->dim + 2) * sizeof(float), &st));
     if (!ws) return st;
