@@ -173,7 +173,9 @@ template <int NG, bool BF> __global__ __launch_bounds__(64 * kWaves, per_cu(NG))
         int e = 141 - (int)(__float_as_uint(top) >> 23);
         e = e > 126 ? 126 : e;
         const float up = __uint_as_float((uint32_t)(e + 127) << 23);
-        sc = ldexpf(p.scale, -e);
+        // (finite, while scores that fp32 holds can need more, from small keys: infinity times a difference of 0 would be NaN, and such scores
+        // are so far apart that a smaller factor leaves one key all the weight too)
+        sc = fminf(ldexpf(p.scale, -e), 3.4028234663852886e38f);
 #pragma unroll
         for (int g = 0; g < NG; g++) {
             each(g, [&](int i, float a, float b) { q[g][i] = __builtin_bit_cast(uint32_t, (h2){(_Float16)(a * up), (_Float16)(b * up)}); });
