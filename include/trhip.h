@@ -317,14 +317,16 @@ typedef struct trhip_rope_spec {
 /* Turns `heads` heads of dim elements, one behind the other in each token's row, x + t * x_stride to out + t * out_stride
  * (type: TRHIP_F32, TRHIP_F16 or TRHIP_BF16; strides in elements). q and k heads that lie next to each other in a merged
  * product's rows are one call. out may be x, with the same stride; else the rows must not overlap. pos: int32 [axes][tokens]
- * on the device, pos_stride elements between axes; any value. Angles are reduced in 64 bits, so that they are as good far from 0
- * as near; sines, cosines and products are in fp32, out is rounded once. dim: an even number up to 1024. */
+ * on the device, pos_stride elements between axes; any value. Angles are taken and reduced in 64 bits, off
+ * by 2^-51 of their size at most, which passes fp32's roundings from some 2^27 radians on (2^-20 at 2^31); sines, cosines and products are in
+ * fp32, out is rounded once. dim: an even number up to 1024; heads: up to 65536. */
 int trhip_rope(trhip_ctx *ctx, const trhip_rope_spec *spec, const void *x, int64_t x_stride, void *out, int64_t out_stride,
                int type, int64_t tokens, int heads, int dim, const int32_t *pos, int64_t pos_stride);
 
 /* ---- The paged key/value cache in 4 bits ---------------------------------------------------------------------------------
  * 4.5 bits an element instead of 16: 32 consecutive elements of a head's row are a block of 4-bit codes c with one f16 scale d,
- * and element i stands for (c_i - 8) * d. Page tables, slots and lengths are those of the 16-bit cache (trhip_page_tables).
+ * and element i stands for (c_i - 8) * d. Page tables, slots and lengths are those of the 16-bit cache (trhip_page_tables). There is no
+ * trhip_attn_shared over this cache: requests whose tables name the same pages read them once each.
  * page: a power of two from 16 to 4096; dim: a multiple of 32 up to 256. A plane (k, v: 16-byte aligned) is
  * pages * heads * page * dim * 9 / 16 bytes: [pages][heads][page / 16] pieces of sixteen places, each 8 * dim bytes of codes and then
  * 16 * dim / 32 scales, in the order in which the attention multiplies them. In a piece, with B = dim / 32 and the place r:
@@ -356,9 +358,11 @@ int trhip_kv4_read(trhip_ctx *ctx, const trhip_kv4 *kv, int64_t tokens, void *k,
  * of rows, must be below 2^24 where requests are read as they are. q and out are of `type` (TRHIP_F16 or TRHIP_BF16).
  * A block whose scale is not finite reads as NaN where a token sees it: in its elements of the result as a value, in the whole row
  * of the head as a key. What a token's mask hides never reaches it. Weights are rounded: in requests of more than 96 rows, where their
- * keys may be opened, as trhip_attn's; else to f16 for bf16 results and to two f16 numbers (2^-21) for f16 ones. Where the hint allows requests of more
+ * keys may be opened, as trhip_attn's; else, times their value's scale, to f16 for bf16 results and to two f16 numbers (2^-21) for f16 ones, and
+ * where that is small by 2^-30 of the largest value that the token sees (so values below some 2^-20 of the largest keep fewer bits). Scores have
+ * to fit fp32. Where the hint allows requests of more
  * than 96 rows, their keys are opened into the context's workspace in 16 bits
- * (exactly, where trhip_kv4_append wrote the scales, else rounded once): as many times max_pages pages (2 * page * heads * dim
+ * (exactly, where trhip_kv4_append wrote the scales, else rounded once, in f16 past 65504 to an infinity): as many times max_pages pages (2 * page * heads * dim
  * bytes a plane) as the tokens can make such requests, if that is no more than 2 GiB a plane; beyond it, where the device has no memory for it,
  * with a hint that is too small (all of these take up to five times as long) and in small calls they are read as they are. The context
  * keeps that workspace: both planes, 4 bytes for each of nreq * max_pages page numbers (up to 2 GiB), and a quarter more. */
@@ -374,10 +378,10 @@ int trhip_kv4_attn(trhip_ctx *ctx, const trhip_kv4 *kv, const void *q, int type,
  *   of those the shortest run whose weights reach top_p of their sum (1 and above, NaN: all; 0 and below: the first),
  *   of those the ones of at least min_p times the largest weight (0 and below, NaN: all; 1 and above: the largest),
  * so the first is always kept. token[r] is the first kept index at which the running sum of kept weights, by index, exceeds u
- * times their sum (u of 1 and above: the last kept one whose weight is not 0; below 0 and NaN: as 0); logprob[r] (may be null) the logarithm of its weight in
+ * times their sum (u of 1 and above: the last kept one whose weight is not 0, where 64 bits hold it, from e^-745 on; below 0 and NaN: as 0); logprob[r] (may be null) the logarithm of its weight in
  * their sum. A temperature of 0, below, or NaN takes the largest logit (logprob 0). -Inf and NaN are never taken; where there is
  * +Inf, only entries of +Inf have weight (each the same). A row with nothing else has token -1 and logprob NaN. Weights and sums are in 64 bits, so
- * the token is the definition's unless u lies within some 1e-13 of a border. vocab: up to 2^24. */
+ * the token is the definition's unless u lies within some 1e-13 of a border. vocab: up to 2^24; rows: up to 2^20. */
 int trhip_sample(trhip_ctx *ctx, const void *logits, int type, int64_t stride, int64_t rows, int64_t vocab,
                  const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p, const float *u,
                  int32_t *token, float *logprob);

@@ -2,8 +2,8 @@
 //
 // A workgroup takes a token, or the four tokens of four places in a row (a quarter of a piece), whose value codes share dwords: written
 // together they are dwords, by themselves bytes. A lane has eight elements of each token's row, four lanes a block. Every element moves
-// once, so bytes bound it; of few tokens it is a launch. 8192 tokens of 8 heads of 128, bf16: in 15.3 us (2.8 TB/s; 18 vector instructions
-// an element took 23), out 11.5 (3.7 TB/s). Tokens one by one, whose value codes are written as bytes: in and out 140 us against 29.
+// once, so bytes bound it; of few tokens it is a launch. 8192 tokens of 8 heads of 128, bf16, what is read in the last cache: in 15.3 us (2.8 TB/s; 18
+// vector instructions an element took 23), out 12.2 (3.5 TB/s); from memory 16.0 and 15.6, in fp32 23 (3.3 TB/s) and 27. Tokens one by one, whose value codes are written as bytes: in and out 140 us against 29.
 #include "attn_common.hpp"
 #include "kv4.hpp"
 #include "kv4_runs.hpp"
@@ -208,7 +208,7 @@ __device__ __forceinline__ void read_rows(const Kv4Args &p, void *dst, const uin
 
 // APPEND: rows k, v into the cache; else out of it.
 // (Registers for eight waves a SIMD hold 8192 tokens at once, in 15.3 us against 15.8 with seven waves, in and out by other inputs each time 27.5 against
-// 29.2; rows out to fp32 would spill more than that gives, 26.7 us against 18.8.)
+// 29.2; rows out to fp32 would spill more than that gives, 26.7 us against 18.8, both with the codes in the last cache.)
 template <int IO, bool APPEND> __global__ __launch_bounds__(256, APPEND || IO != TRHIP_F32 ? 8 : 5) void kv4_rows_kernel(const Kv4Args p, void *k, void *v) {
     const int blocks = p.dim >> 5, row = 4 * p.heads * blocks;  // eights of a row
     const int x = blockIdx.x * blockDim.x + threadIdx.x;

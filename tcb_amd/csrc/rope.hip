@@ -2,7 +2,8 @@
 //
 // A workgroup takes one or four tokens and some of their heads: first the sines and cosines of the tokens' pairs, once for all heads, into
 // LDS, then the heads, 16 bytes a load. Every element moves once in and once out, which is what bounds it: 8192 tokens of 40 heads of 128 in bf16
-// take 38 us (4.4 TB/s), 16 tokens 4.6, a launch. (Angles by every head anew, 64-bit arithmetic each: 72 us.)
+// take 35 us from memory (4.8 TB/s; three axes and factors 38), in place 36.5, in fp32 63 (5.3 TB/s); 16 tokens 4.8, a launch. (Angles by every head
+// anew, 64-bit arithmetic each: 72 us.)
 #include "rope.hpp"
 #include "trhip_internal.hpp"
 
@@ -177,8 +178,8 @@ int launch_rope(trhip_ctx *ctx, const trhip_rope_spec &spec, const void *x, int6
     const auto whole = [&](int64_t bytes) { return bytes % 16 == 0; };
     const bool wide = whole(reinterpret_cast<uintptr_t>(x)) && whole(reinterpret_cast<uintptr_t>(out)) && (tokens == 1 || (whole(x_stride * size) && whole(out_stride * size))) &&
                       whole((int64_t)dim * size) && whole((int64_t)p.pairs * size);
-    // Four tokens a workgroup where there are many whose items do not fill one (8192 tokens of 10 heads of 128: 10.5 us against 14.5 with one;
-    // of 40 heads 29.1 against 27.7); of few tokens the heads are dealt out, an item a thread (a token of 128 heads, fp32: 4.4 against 5.0).
+    // Four tokens a workgroup where there are many whose items do not fill one (8192 tokens of 10 heads of 128, the same rows each time, which
+    // the last cache holds: 10.5 us against 14.5 with one; of 40 heads, which do, 29.1 against 27.7); of few tokens the heads are dealt out, an item a thread (a token of 128 heads, fp32: 4.4 against 5.0).
     const int64_t cus = ctx->sm_count > 0 ? ctx->sm_count : 256;
     const int per = wide ? p.pairs / n + (p.copy ? (dim - 2 * p.pairs) / n : 0) : p.pairs + (p.copy ? dim - 2 * p.pairs : 0);
     const bool four = tokens >= 16 * cus && heads * per <= kThreads;

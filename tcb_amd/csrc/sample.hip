@@ -15,9 +15,11 @@
 // Weights and their sums are in 64 bits, since one border among a hundred thousand has to be met: e^x by a table of 64 powers and a
 // polynomial of degree 5.
 //
-// 1 x 128256, fp32: 10 us without a filter, 13 with top_k 50, 17 with top_p .85 (two launches, the second one's chain of steps by one workgroup);
-// a flat row of which thousands are kept 91, by one CU that reads the row once more. 256 x 128256: 34 us for the largest (4 TB/s), 54 without a
-// filter, 42 with top_k 50, 84 with top_p .85, where the bins' atomics in LDS bound the first launch.
+// 1 x 128256, fp32: 10 us without a filter, 13 with top_k 50, 16 with top_p .85 (two launches, the second one's chain of steps by one workgroup);
+// a flat row of which thousands are kept 91 to 94, by one CU that reads the row once more. 256 x 128256, from memory: 37 us for the largest, 53 without
+// a filter, 45 with top_k 50, 84 with top_p .85 of peaked rows and 148 where some keep thousands. In the first launch 32 (4.2 TB/s), 51 (a 64-bit
+// exponential of every logit), 41 (the threshold, after all of a workgroup's loads), 87 (bins in LDS by 64-bit atomics); the second takes 6 to 7,
+// and 70 of those 148.
 #include "trhip_internal.hpp"
 
 namespace trhip {
