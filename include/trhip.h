@@ -378,7 +378,8 @@ int trhip_kv4_attn(trhip_ctx *ctx, const trhip_kv4 *kv, const void *q, int type,
  *   of those the shortest run whose weights reach top_p of their sum (1 and above, NaN: all; 0 and below: the first),
  *   of those the ones of at least min_p times the largest weight (0 and below, NaN: all; 1 and above: the largest),
  * so the first is always kept. token[r] is the first kept index at which the running sum of kept weights, by index, exceeds u
- * times their sum (u of 1 and above: the last kept one whose weight is not 0, where 64 bits hold it, from e^-745 on; below 0 and NaN: as 0); logprob[r] (may be null) the logarithm of its weight in
+ * times their sum (u of 1 and above: the last kept one whose weight is not 0, where 64 bits hold it, from e^-745 on; below 0 and NaN: as 0);
+ * logprob[r] (may be null) the logarithm of its weight in
  * their sum. A temperature of 0, below, or NaN takes the largest logit (logprob 0). -Inf and NaN are never taken; where there is
  * +Inf, only entries of +Inf have weight (each the same). A row with nothing else has token -1 and logprob NaN. Weights and sums are in 64 bits, so
  * the token is the definition's unless u lies within some 1e-13 of a border. vocab: up to 2^24; rows: up to 2^20. */

@@ -3,7 +3,8 @@
 // A workgroup takes a token, or the four tokens of four places in a row (a quarter of a piece), whose value codes share dwords: written
 // together they are dwords, by themselves bytes. A lane has eight elements of each token's row, four lanes a block. Every element moves
 // once, so bytes bound it; of few tokens it is a launch. 8192 tokens of 8 heads of 128, bf16, what is read in the last cache: in 15.3 us (2.8 TB/s; 18
-// vector instructions an element took 23), out 12.2 (3.5 TB/s); from memory 16.0 and 15.6, in fp32 23 (3.3 TB/s) and 27. Tokens one by one, whose value codes are written as bytes: in and out 140 us against 29.
+// vector instructions an element took 23), out 12.2 (3.5 TB/s); from memory 16.0 and 15.6, in fp32 23 (3.3 TB/s) and 27. Tokens one by one, whose
+// value codes are written as bytes: in and out 140 us against 29.
 #include "attn_common.hpp"
 #include "kv4.hpp"
 #include "kv4_runs.hpp"

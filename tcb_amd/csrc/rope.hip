@@ -179,7 +179,8 @@ int launch_rope(trhip_ctx *ctx, const trhip_rope_spec &spec, const void *x, int6
     const bool wide = whole(reinterpret_cast<uintptr_t>(x)) && whole(reinterpret_cast<uintptr_t>(out)) && (tokens == 1 || (whole(x_stride * size) && whole(out_stride * size))) &&
                       whole((int64_t)dim * size) && whole((int64_t)p.pairs * size);
     // Four tokens a workgroup where there are many whose items do not fill one (8192 tokens of 10 heads of 128, the same rows each time, which
-    // the last cache holds: 10.5 us against 14.5 with one; of 40 heads, which do, 29.1 against 27.7); of few tokens the heads are dealt out, an item a thread (a token of 128 heads, fp32: 4.4 against 5.0).
+    // the last cache holds: 10.5 us against 14.5 with one; of 40 heads, which do, 29.1 against 27.7); of few tokens the heads are dealt out, an
+    // item a thread (a token of 128 heads, fp32: 4.4 against 5.0).
     const int64_t cus = ctx->sm_count > 0 ? ctx->sm_count : 256;
     const int per = wide ? p.pairs / n + (p.copy ? (dim - 2 * p.pairs) / n : 0) : p.pairs + (p.copy ? dim - 2 * p.pairs : 0);
     const bool four = tokens >= 16 * cus && heads * per <= kThreads;
