@@ -382,7 +382,8 @@ int trhip_kv4_attn(trhip_ctx *ctx, const trhip_kv4 *kv, const void *q, int type,
  * logprob[r] (may be null) the logarithm of its weight in
  * their sum. A temperature of 0, below, or NaN takes the largest logit (logprob 0). -Inf and NaN are never taken; where there is
  * +Inf, only entries of +Inf have weight (each the same). A row with nothing else has token -1 and logprob NaN. Weights and sums are in 64 bits, so
- * the token is the definition's unless u lies within some 1e-13 of a border. vocab: up to 2^24; rows: up to 2^20. */
+ * the token is the definition's unless u, or what top_p or min_p asks for, lies within some 1e-13 of a border (with a min_p of 1, weights that
+ * close to the largest are kept too). vocab: up to 2^24; rows: up to 2^20. */
 int trhip_sample(trhip_ctx *ctx, const void *logits, int type, int64_t stride, int64_t rows, int64_t vocab,
                  const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p, const float *u,
                  int32_t *token, float *logprob);
